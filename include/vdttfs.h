@@ -510,6 +510,111 @@ int vdttfs_culif_net_count(vdttfs_culif_net* net, const float* d_data, uint64_t*
 int vdttfs_stepnet_create_culif(vdttfs_ctx* ctx, const vdttfs_culif_layer* layers, int n_layers, int B,
                                 vdttfs_stepnet** out);
 
+/* ---- dense and conditional heads in 8-bit integers ---------------------- */
+/* No counterpart in the reference, which has no layer but the spiking ones.
+ * A spike map is an activation of few bits (an arrival bin), so the dense twin
+ * of a layer, a head on a spiking trunk, or experts of which each sample takes
+ * a few, are products of 8-bit codes with a float scale for each row (a sample
+ * or token) and for each output channel.
+ *
+ * Matrices are row-major with a leading dimension in elements, >= the columns;
+ * a row's elements are contiguous.  Codes need no alignment (rows that start
+ * on 16 bytes are read fastest), floats that of their type.  Outputs must not
+ * overlap inputs.  Calls are stream-ordered on the context's stream; scratch
+ * is the context's and grows on demand: under stream capture a call that needs
+ * more than an earlier one made fails with VDTTFS_E_UNSUPPORTED, so run it
+ * once before capturing it. */
+/* Element types.  TIMES, an input only: float spike times as the engine's maps
+ * hold them, under the context's T and tfs. */
+#define VDTTFS_ELEM_F32   0
+#define VDTTFS_ELEM_BF16  1
+#define VDTTFS_ELEM_F16   2
+#define VDTTFS_ELEM_TIMES 3
+/* Activations: v, max(v, 0) (NaN stays), v / (1 + exp(-v)). */
+#define VDTTFS_ACT_NONE 0
+#define VDTTFS_ACT_RELU 1
+#define VDTTFS_ACT_SILU 2
+#define VDTTFS_I8_MAX_K 131071  /* 128 * 128 * K stays below 2^31 */
+
+/* Rows to codes.  Floats: s = max|x| / 127, q = x / s rounded to the nearest
+ * whole number (half to even, within [-127, 127]); both divisions in 32-bit
+ * floats.  A row of zeros has s = 0 and codes 0; a row with an infinity or a
+ * NaN has s = NaN and codes 0, so that products with it are NaN.  Spike times:
+ * with b the arrival bin and L = min(T, 127), q = (T - b) * L / T rounded (for
+ * T <= 127 exactly T - b), 0 where nothing arrives inside the window, and
+ * s = 1 / L: a linear encoding's pixel value x = (T - b) / T is q * s.
+ * d_q int8 [rows][ldq], d_scale float [rows]. */
+int vdttfs_quant_rows(vdttfs_ctx* ctx, const void* d_x, int elem, int64_t ldx, int64_t rows, int cols,
+                      int8_t* d_q, int64_t ldq, float* d_scale);
+/* An FC kernel in the reference layout, float [C_in][C_out] as the weights
+ * blob holds it, to the products' layout: codes [C_out][ldw] and a scale for
+ * each output channel, each channel quantised as quant_rows does a row. */
+int vdttfs_quant_kernel(vdttfs_ctx* ctx, const float* d_kernel, int C_in, int C_out, int8_t* d_w, int64_t ldw,
+                        float* d_ch_scale);
+/* out[m][n] = act(sum_k q[m][k] * w[n][k] * row_scale[m] * ch_scale[n] + bias[n]),
+ * the sum exact in 32-bit integers, the scales applied in this order in 32-bit
+ * floats and rounded once to out_elem (F32, BF16 or F16).  d_bias may be NULL.
+ * Any int8 values, -128 too; K <= VDTTFS_I8_MAX_K. */
+int vdttfs_i8_matmul(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const int8_t* d_q, int64_t ldq,
+                     const float* d_row_scale, const int8_t* d_w, int64_t ldw, const float* d_ch_scale,
+                     const float* d_bias, int act, int64_t M, int N, int K);
+/* quant_rows of d_x (any element type), then i8_matmul: the same results. */
+int vdttfs_i8_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const void* d_x, int x_elem,
+                     int64_t ldx, const int8_t* d_w, int64_t ldw, const float* d_ch_scale, const float* d_bias,
+                     int act, int64_t M, int N, int K);
+
+/* Routing of rows to experts from their logits (F32, BF16 or F16 [M][ld]).
+ * An expert can be chosen where its logit is above -inf (NaN is not) and, with
+ * d_row_mask (uint8 [M], NULL: every row), the row's byte is not 0.  Scores p
+ * over those experts: softmax, exp(l - max) / sum, or sigmoid,
+ * 1 / (1 + exp(-l)).  The choice goes by c = p + d_bias (float [E], NULL: p
+ * itself; a bias of -inf or NaN takes the expert out).  With groups > 1 the E
+ * experts are `groups` runs of neighbours; a run is worth the sum of its
+ * group_top (1 or 2) largest c, and only the top_groups best runs stay.
+ * d_idx [M][top_k] receives the experts of largest c, largest first, ties to
+ * the lowest index, -1 where none is left; d_weight [M][top_k] their p (0
+ * where idx is -1), divided by their sum where renorm != 0 and the sum is above
+ * 0, times scale.  d_count (int32 [E], NULL: not counted) receives how many
+ * entries of d_idx name each expert.  E <= 1024, top_k <= min(E, 64),
+ * groups <= 64 and a divisor of E, M * top_k < 2^31. */
+#define VDTTFS_SCORE_SOFTMAX 0
+#define VDTTFS_SCORE_SIGMOID 1
+typedef struct vdttfs_route_opts {
+    int32_t n_experts, top_k, score;
+    int32_t groups, top_groups, group_top;  /* 1, 1, 1: no groups */
+    int32_t renorm;
+    float   scale;
+} vdttfs_route_opts;
+int vdttfs_route(vdttfs_ctx* ctx, int32_t* d_idx, float* d_weight, int32_t* d_count, const void* d_logits,
+                 int elem, int64_t ld, const float* d_bias, const uint8_t* d_row_mask, int64_t M,
+                 const vdttfs_route_opts* opts);
+
+/* A layer of experts, each two products with a quantisation between them.  For
+ * row m and each slot j with e = idx[m][j] in [0, n_experts) (others are
+ * skipped):
+ *   u = i8_linear(x[m], w1[e], s1[e], b1[e])   (2 * d_hidden channels if gated)
+ *   h = act(u), or act(u[:d_hidden]) * u[d_hidden:] if gated
+ *   z = i8_linear(h, w2[e], s2[e], b2[e])
+ * and out[m] = sum_j weight[m][j] * z_j, summed in the order of the slots in
+ * 32-bit floats; a row whose slots are all skipped is 0.  Device pointers, all
+ * dense: w1 [E][H][d_in], s1 and b1 [E][H] with H = d_hidden or 2 * d_hidden,
+ * w2 [E][d_out][d_hidden], s2 and b2 [E][d_out]; b1 and b2 may be NULL.
+ * With a BF16 out the weighted products of the slots may pass through BF16
+ * before their sum.  n_experts <= 1024, top_k <= 64, M * top_k < 2^31. */
+typedef struct vdttfs_expert_layer {
+    int32_t n_experts, d_in, d_hidden, d_out;
+    int32_t act, gated;
+    const int8_t* w1;
+    const float*  s1;
+    const float*  b1;
+    const int8_t* w2;
+    const float*  s2;
+    const float*  b2;
+} vdttfs_expert_layer;
+int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const void* d_x, int x_elem,
+                   int64_t ldx, const int32_t* d_idx, const float* d_weight, int64_t M, int top_k,
+                   const vdttfs_expert_layer* layer);
+
 /* ---- gather-roof probe (measurement; no reference counterpart) --------- */
 /* The integrator's weight-gather pattern alone: `waves` waves each stream
  * n_ev wave-uniform random row offsets (scalar loads, 8 per group) and issue

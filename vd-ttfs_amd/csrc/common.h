@@ -42,6 +42,10 @@ struct vdttfs_ctx {
     size_t split_bytes;
     bool split_captured;
     std::vector<void*> split_kept;
+    // scratch of the 8-bit heads, kept as split_buf is
+    void* head_buf;
+    size_t head_bytes;
+    bool head_captured;
     bool named_skip;  // a split call could not size its named plan's scratch too
     unsigned long long* d_counters;  // kCounterStripes x 4 u64 (summed on the host)
     hipEvent_t timer[2];             // vdttfs_timer_begin/end (created on first use)

@@ -1,0 +1,44 @@
+// Element types of the 8-bit heads: loads, stores and activations.
+#pragma once
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+
+#include "vdttfs.h"
+
+namespace vdttfs {
+
+__device__ __forceinline__ float bf16_to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+
+// Round to nearest even; NaN stays NaN.
+__device__ __forceinline__ uint16_t f32_to_bf16(float v) {
+    const uint32_t u = __float_as_uint(v);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
+    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+
+__device__ __forceinline__ float f16_to_f32(uint16_t v) { return __half2float(__ushort_as_half(v)); }
+__device__ __forceinline__ uint16_t f32_to_f16(float v) { return __half_as_ushort(__float2half_rn(v)); }
+
+template <int ELEM>
+__device__ __forceinline__ float load_elem(const void* p, int64_t i) {
+    if constexpr (ELEM == VDTTFS_ELEM_BF16) return bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
+    else if constexpr (ELEM == VDTTFS_ELEM_F16) return f16_to_f32(static_cast<const uint16_t*>(p)[i]);
+    else return static_cast<const float*>(p)[i];
+}
+
+__device__ __forceinline__ void store_elem(void* p, int64_t i, float v, int elem) {
+    if (elem == VDTTFS_ELEM_F32) static_cast<float*>(p)[i] = v;
+    else static_cast<uint16_t*>(p)[i] = elem == VDTTFS_ELEM_BF16 ? f32_to_bf16(v) : f32_to_f16(v);
+}
+
+// silu with the library's exp and an IEEE division: what is quantised again
+// may not depend on which product kernel made it.
+__device__ __forceinline__ float apply_act(float v, int act) {
+    if (act == VDTTFS_ACT_RELU) return v < 0.0f ? 0.0f : v;
+    if (act == VDTTFS_ACT_SILU) return v / (1.0f + expf(-v));
+    return v;
+}
+
+}  // namespace vdttfs

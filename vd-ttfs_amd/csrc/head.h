@@ -1,0 +1,64 @@
+// Internal declarations of the 8-bit heads: quantisation, products of codes,
+// routing and experts (vdttfs_quant_rows ... vdttfs_experts).
+#pragma once
+
+#include "common.h"
+
+namespace vdttfs {
+
+// A product of codes.  A: activations [rows][lda], B: weights [channels][ldb].
+// Grouped (tiles != nullptr): row tile t belongs to expert tiles[t].x, starts
+// at sorted row tiles[t].y and ends before tiles[t].z; the A row of sorted row
+// i is a_rows[i] (i itself if null), its output row o_rows[i] (i if null).
+struct I8Args {
+    const int8_t* A;
+    int64_t lda;
+    const float* sa;  // per A row
+    const int8_t* B;
+    int64_t ldb;
+    const float* sb;    // per channel
+    const float* bias;  // per channel, nullable
+    void* out;
+    int64_t ldo;
+    int64_t M;  // rows (grouped: unused)
+    int N, K;   // N: output columns; gated products read 2 * N channels
+    int act, out_elem;
+    const int4* tiles;
+    const int* n_tiles;
+    const int* a_rows;
+    const int* o_rows;
+    int64_t b_stride;  // codes of one expert's B
+    int s_stride;      // channels of one expert
+    int max_tiles;     // bound on *n_tiles
+};
+
+// Rows to codes; columns [cols, ldq_zero) of each row get 0.
+int launch_quant_rows(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int64_t rows, int cols, int8_t* q,
+                      int64_t ldq, int cols_zero, float* scale);
+int launch_quant_kernel(vdttfs_ctx* ctx, const float* kernel, int c_in, int c_out, int8_t* w, int64_t ldw,
+                        float* scale);
+// bm: rows of a tile of a grouped product (i8_tile_rows of the same call)
+int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a);
+int launch_i8_grouped(vdttfs_ctx* ctx, const I8Args& a, bool gated, int bm);
+int i8_tile_rows(int64_t pairs, int n_experts);
+
+int launch_route(vdttfs_ctx* ctx, int32_t* idx, float* wt, int32_t* count, const void* logits, int elem, int64_t ld,
+                 const float* bias, const uint8_t* row_mask, int64_t M, const vdttfs_route_opts& o);
+
+// The pairs (row, slot) sorted by expert.  pair[i]: row * top_k + slot of
+// sorted row i, row[i]: its row; tiles as in I8Args with bm rows each.
+struct Dispatch {
+    int* pair;
+    int* row;
+    int4* tiles;
+    int* n_tiles;
+    int* hist;  // [blocks][n_experts] and scratch of the sort
+};
+int dispatch_blocks(int64_t pairs);
+int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_k, int n_experts, int bm,
+                    const Dispatch& d);
+// out[m] = sum over slots of weight * z[m * top_k + slot]
+int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const float* z, const int32_t* idx,
+                   const float* wt, int64_t M, int N, int top_k, int n_experts);
+
+}  // namespace vdttfs

@@ -31,6 +31,10 @@ STEP_T1, STEP_T2, STEP_T3 = 1, 2, 3
 PATH_AUTO, PATH_BINS, PATH_DENSE, PATH_FUSED, PATH_REG, PATH_WINDOW = 0, 1, 2, 3, 4, 5
 ROUTE_PLAN, ROUTE_SPLIT, ROUTE_LISTS, ROUTE_PIXEL = 0, 1, 2, 3
 POOL_FUSE_OFF, POOL_FUSE_ALL, POOL_FUSE_AUTO = 0, 1, 2
+ELEM_F32, ELEM_BF16, ELEM_F16, ELEM_TIMES = 0, 1, 2, 3
+ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+I8_MAX_K = 131071
 
 
 class VdttfsError(RuntimeError):
@@ -123,6 +127,36 @@ class CulifLayer(C.Structure):
     ]
 
 
+class RouteOpts(C.Structure):
+    _fields_ = [
+        ("n_experts", C.c_int32),
+        ("top_k", C.c_int32),
+        ("score", C.c_int32),
+        ("groups", C.c_int32),
+        ("top_groups", C.c_int32),
+        ("group_top", C.c_int32),
+        ("renorm", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
+class ExpertLayer(C.Structure):
+    _fields_ = [
+        ("n_experts", C.c_int32),
+        ("d_in", C.c_int32),
+        ("d_hidden", C.c_int32),
+        ("d_out", C.c_int32),
+        ("act", C.c_int32),
+        ("gated", C.c_int32),
+        ("w1", C.c_void_p),
+        ("s1", C.c_void_p),
+        ("b1", C.c_void_p),
+        ("w2", C.c_void_p),
+        ("s2", C.c_void_p),
+        ("b2", C.c_void_p),
+    ]
+
+
 _vp = C.c_void_p
 _i = C.c_int
 _i64 = C.c_int64
@@ -208,6 +242,12 @@ SIGNATURES = {
     "vdttfs_culif_net_set_timing": [_vp, _i],
     "vdttfs_culif_net_read_timing": [_vp, C.POINTER(C.c_double), C.POINTER(_i64)],
     "vdttfs_culif_net_count": [_vp, _vp, _u64p, _u64p, _u64p, _u64p],
+    "vdttfs_quant_rows": [_vp, _vp, _i, _i64, _i64, _i, _vp, _i64, _vp],
+    "vdttfs_quant_kernel": [_vp, _vp, _i, _i, _vp, _i64, _vp],
+    "vdttfs_i8_matmul": [_vp, _vp, _i, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i, _i64, _i, _i],
+    "vdttfs_i8_linear": [_vp, _vp, _i, _i64, _vp, _i, _i64, _vp, _i64, _vp, _vp, _i, _i64, _i, _i],
+    "vdttfs_route": [_vp, _vp, _vp, _vp, _vp, _i, _i64, _vp, _vp, _i64, C.POINTER(RouteOpts)],
+    "vdttfs_experts": [_vp, _vp, _i, _i64, _vp, _i, _i64, _vp, _vp, _i64, _i, C.POINTER(ExpertLayer)],
     "vdttfs_timer_begin": [_vp],
     "vdttfs_timer_end": [_vp, C.POINTER(C.c_double)],
     "vdttfs_probe_gather": [_vp, _i, _i64, _i, _i64, _i, C.POINTER(C.c_double)],

@@ -19,7 +19,9 @@ from ._lib import (Consts, CulifLayer, LayerDesc, VdttfsError, check, lib, INF_T
                    READOUT_ARGMIN, READOUT_ARGMAX, CULIF_RAW_CONV, CULIF_CONV, CULIF_POOL,
                    CULIF_FC_REC, CULIF_FC, STEP_T1, STEP_T2, STEP_T3, LayerPlan, PATH_AUTO, PATH_BINS, PATH_DENSE,
                    PATH_FUSED, PATH_REG, PATH_WINDOW, ROUTE_PLAN, ROUTE_SPLIT, ROUTE_LISTS,
-                   ROUTE_PIXEL, POOL_FUSE_OFF, POOL_FUSE_ALL, POOL_FUSE_AUTO)
+                   ROUTE_PIXEL, POOL_FUSE_OFF, POOL_FUSE_ALL, POOL_FUSE_AUTO, RouteOpts, ExpertLayer,
+                   ELEM_F32, ELEM_BF16, ELEM_F16, ELEM_TIMES, ACT_NONE, ACT_RELU, ACT_SILU, SCORE_SOFTMAX,
+                   SCORE_SIGMOID)
 
 
 def _ptr(a: np.ndarray) -> C.c_void_p:
@@ -258,12 +260,57 @@ class Context:
     def readout_argmin_first(self, d_out, B, Cc, d_pred):
         check(lib().vdttfs_readout_argmin_first(self.handle, d_out.ptr, B, Cc, d_pred.ptr))
 
+    # 8-bit heads (vdttfs_quant_rows ...): arguments are anything with the
+    # device pointer in .ptr, optional ones None
+    def quant_rows(self, d_x, elem, ldx, rows, cols, d_q, ldq, d_scale):
+        """Rows of floats or spike times to 8-bit codes with a scale each (vdttfs_quant_rows)."""
+        check(lib().vdttfs_quant_rows(self.handle, d_x.ptr, elem, ldx, rows, cols, d_q.ptr, ldq, d_scale.ptr))
+
+    def quant_kernel(self, d_kernel, C_in, C_out, d_w, ldw, d_ch_scale):
+        """A float [C_in][C_out] FC kernel to codes [C_out][ldw] and channel scales (vdttfs_quant_kernel)."""
+        check(lib().vdttfs_quant_kernel(self.handle, d_kernel.ptr, C_in, C_out, d_w.ptr, ldw, d_ch_scale.ptr))
+
+    def i8_matmul(self, d_out, out_elem, ldo, d_q, ldq, d_row_scale, d_w, ldw, d_ch_scale, d_bias, act, M, N, K):
+        """act(codes x codes * row scale * channel scale + bias) (vdttfs_i8_matmul)."""
+        check(lib().vdttfs_i8_matmul(self.handle, d_out.ptr, out_elem, ldo, d_q.ptr, ldq, d_row_scale.ptr, d_w.ptr,
+                                     ldw, d_ch_scale.ptr, d_bias.ptr if d_bias is not None else None, act, M, N, K))
+
+    def i8_linear(self, d_out, out_elem, ldo, d_x, x_elem, ldx, d_w, ldw, d_ch_scale, d_bias, act, M, N, K):
+        """quant_rows of d_x, then i8_matmul, in one call (vdttfs_i8_linear)."""
+        check(lib().vdttfs_i8_linear(self.handle, d_out.ptr, out_elem, ldo, d_x.ptr, x_elem, ldx, d_w.ptr, ldw,
+                                     d_ch_scale.ptr, d_bias.ptr if d_bias is not None else None, act, M, N, K))
+
+    def route(self, d_idx, d_weight, d_count, d_logits, elem, ld, d_bias, d_row_mask, M, E, top_k,
+              score=SCORE_SOFTMAX, groups=1, top_groups=1, group_top=1, renorm=False, scale=1.0):
+        """The experts of each row and their weights from router logits (vdttfs_route)."""
+        o = RouteOpts(E, top_k, score, groups, top_groups, group_top, int(renorm), scale)
+        check(lib().vdttfs_route(self.handle, d_idx.ptr, d_weight.ptr, d_count.ptr if d_count is not None else None,
+                                 d_logits.ptr, elem, ld, d_bias.ptr if d_bias is not None else None,
+                                 d_row_mask.ptr if d_row_mask is not None else None, M, C.byref(o)))
+
+    def experts(self, d_out, out_elem, ldo, d_x, x_elem, ldx, d_idx, d_weight, M, top_k, weights):
+        """Each row's experts applied and summed by weight (vdttfs_experts)."""
+        check(lib().vdttfs_experts(self.handle, d_out.ptr, out_elem, ldo, d_x.ptr, x_elem, ldx, d_idx.ptr,
+                                   d_weight.ptr, M, top_k, C.byref(weights.c)))
+
     def launch_pool(self, d_in, d_out, H_in, W_in, Cc, B):
         check(lib().vdttfs_launch_pool_sync(self.handle, d_in.ptr, d_out.ptr, H_in, W_in, Cc, B))
 
     def launch_fc_vmem(self, d_in, d_out, C_in, C_out, d_kernel, d_bias, d_alpha, B):
         check(lib().vdttfs_launch_fc_vmem_sync(self.handle, d_in.ptr, d_out.ptr, C_in, C_out,
                                                d_kernel.ptr, d_bias.ptr, d_alpha.ptr, B))
+
+
+class ExpertWeights:
+    """Device weights of a layer of experts (vdttfs_expert_layer): codes w1
+    [E][H][d_in] and w2 [E][d_out][d_hidden] with channel scales s1, s2 and
+    optional biases b1, b2; H is d_hidden, or 2 * d_hidden (gate rows, then up
+    rows) where gated.  Keeps the buffers it was given alive."""
+
+    def __init__(self, n_experts, d_in, d_hidden, d_out, act, gated, w1, s1, b1, w2, s2, b2):
+        self.buffers = (w1, s1, b1, w2, s2, b2)
+        self.c = ExpertLayer(n_experts, d_in, d_hidden, d_out, act, int(gated),
+                             *[b.ptr if b is not None else None for b in self.buffers])
 
 
 @dataclass
