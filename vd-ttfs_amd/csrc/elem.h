@@ -1,8 +1,6 @@
 // Element types of the 8-bit heads: loads, stores and activations.
 #pragma once
 
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
 #include "vdttfs.h"
@@ -11,15 +9,19 @@ namespace vdttfs {
 
 __device__ __forceinline__ float bf16_to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 
-// Round to nearest even; NaN stays NaN.
-__device__ __forceinline__ uint16_t f32_to_bf16(float v) {
-    const uint32_t u = __float_as_uint(v);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
+// Both round to nearest even; NaN stays NaN.
+__device__ __forceinline__ uint16_t f32_to_bf16(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
+__device__ __forceinline__ float f16_to_f32(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
+__device__ __forceinline__ uint16_t f32_to_f16(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
 
-__device__ __forceinline__ float f16_to_f32(uint16_t v) { return __half2float(__ushort_as_half(v)); }
-__device__ __forceinline__ uint16_t f32_to_f16(float v) { return __half_as_ushort(__float2half_rn(v)); }
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// Two values of a 16-bit type in one word.
+__device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
+    if (bf16) return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+    return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+}
 
 template <int ELEM>
 __device__ __forceinline__ float load_elem(const void* p, int64_t i) {

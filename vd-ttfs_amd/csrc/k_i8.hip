@@ -18,11 +18,121 @@ struct __attribute__((packed, aligned(1))) Bytes16 {
 // have any alignment (gfx950 loads 16 bytes from any address).
 __device__ __forceinline__ v4i load16(const int8_t* p, int valid) {
     if (valid >= 16) return reinterpret_cast<const Bytes16*>(p)->v;
-    v4i r = {0, 0, 0, 0};
+    uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+    for (int i = 0; i < valid; ++i) {
+        const uint64_t b = (uint64_t)(uint8_t)p[i] << (8 * (i & 7));
+        if (i < 8) lo |= b;
+        else hi |= b;
+    }
+    return v4i{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+}
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+// v[0..3] of p, zero past the first n_ok
+__device__ __forceinline__ v4f take4(const float* p, int n_ok) {
+    v4f r;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (i < valid) r[i >> 2] |= (int)(uint32_t)(uint8_t)p[i] << (8 * (i & 3));
+    for (int e = 0; e < 4; ++e) r[e] = e < n_ok ? p[e] : 0.0f;
     return r;
+}
+
+// A wave's sums to its outputs.  A lane's four sums of a fragment are row
+// m = lane & 15, channels (lane >> 4) * 4 + 0..3; stored from there, a wave
+// would write 32 bytes of each of 16 rows at a time, and whole-chip stores
+// then ran at 1 TB/s (64 of the 170 us of 8192 x 4096 x 4096).  So 16 rows at
+// a time pass through the wave's own part of LDS (stage) and leave as 16
+// bytes a lane, a row's outputs together.  m0: the wave's first row; wn: its
+// first channel in the tile.
+template <int FM, int FN, bool GATED>
+struct Stage {
+    static constexpr int kCols = GATED ? FN * 8 : FN * 16;  // outputs of a row
+    static constexpr int kRow = kCols + 4;                  // floats from row to row
+    static constexpr int kBytes = 16 * kRow * 4;
+};
+template <int FM, int FN, bool GATED, bool GROUPED>
+__device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][FN], int64_t m0, int64_t m_end, int n0,
+                                         int wn, const float* sb, const float* bias, float* stage) {
+    typedef Stage<FM, FN, GATED> S;
+    const int lane = lane_id();
+    const int nw = n0 + (GATED ? wn / 2 : wn);  // the wave's first output column
+    const int size = p.out_elem == VDTTFS_ELEM_F32 ? 4 : 2;
+    const bool bf16 = p.out_elem == VDTTFS_ELEM_BF16;
+    const bool vec = nw + S::kCols <= p.N && ((p.ldo * size) & 15) == 0 &&
+                     (((uintptr_t)p.out + (size_t)nw * size) & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int64_t mi = m0 + i * 16;
+        if (mi >= m_end) break;
+        const int64_t m = mi + (lane & 15) < m_end ? mi + (lane & 15) : m_end - 1;
+        const float sa = p.sa[GROUPED && p.a_rows ? p.a_rows[m] : m];
+#pragma unroll
+        for (int j = 0; j < FN; j += GATED ? 2 : 1) {
+            const int c = (GATED ? j * 8 : j * 16) + (lane >> 4) * 4;  // column of the wave's outputs
+            const int n = nw + c, n_ok = p.N - n;
+            const v4f s = take4(sb + n, n_ok);
+            v4f v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * sa * s[e];
+            if (bias) {
+                const v4f b = take4(bias + n, n_ok);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += b[e];
+            }
+            if (p.act == VDTTFS_ACT_RELU) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = apply_act(v[e], VDTTFS_ACT_RELU);
+            } else if (p.act == VDTTFS_ACT_SILU) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = apply_act(v[e], VDTTFS_ACT_SILU);
+            }
+            if constexpr (GATED) {
+                const v4f s2 = take4(sb + p.N + n, n_ok);
+                v4f u;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[e] = (float)acc[i][j + 1][e] * sa * s2[e];
+                if (bias) {
+                    const v4f b = take4(bias + p.N + n, n_ok);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) u[e] += b[e];
+                }
+                v *= u;
+            }
+            *reinterpret_cast<v4f*>(stage + (lane & 15) * S::kRow + c) = v;
+        }
+        wave_sync();
+        if (vec && size == 2) {
+            constexpr int kLanes = S::kCols / 8;  // lanes of a row
+#pragma unroll
+            for (int r = 0; r < 16; r += 64 / kLanes) {
+                const int row = r + lane / kLanes, c = lane % kLanes * 8;
+                if (row >= 16 || mi + row >= m_end) continue;
+                const float* f = stage + row * S::kRow + c;
+                const v4f x = *reinterpret_cast<const v4f*>(f), y = *reinterpret_cast<const v4f*>(f + 4);
+                const int64_t o = (GROUPED && p.o_rows ? p.o_rows[mi + row] : mi + row) * p.ldo + nw + c;
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + o) = make_uint4(
+                    pack2(x[0], x[1], bf16), pack2(x[2], x[3], bf16), pack2(y[0], y[1], bf16), pack2(y[2], y[3], bf16));
+            }
+        } else if (vec) {
+            constexpr int kLanes = S::kCols / 4;
+#pragma unroll
+            for (int r = 0; r < 16; r += 64 / kLanes) {
+                const int row = r + lane / kLanes, c = lane % kLanes * 4;
+                if (row >= 16 || mi + row >= m_end) continue;
+                const int64_t o = (GROUPED && p.o_rows ? p.o_rows[mi + row] : mi + row) * p.ldo + nw + c;
+                *reinterpret_cast<v4f*>(static_cast<float*>(p.out) + o) =
+                    *reinterpret_cast<const v4f*>(stage + row * S::kRow + c);
+            }
+        } else {
+            const int c = lane % S::kCols;
+            for (int row = lane / S::kCols; row < 16 && mi + row < m_end; row += 64 / S::kCols) {
+                const int64_t o = (GROUPED && p.o_rows ? p.o_rows[mi + row] : mi + row) * p.ldo + nw + c;
+                if (nw + c < p.N) store_elem(p.out, o, stage[row * S::kRow + c], p.out_elem);
+            }
+        }
+        wave_sync();
+    }
 }
 
 constexpr int kBK = 128;  // codes of a row in one LDS tile
@@ -42,8 +152,10 @@ __global__ __launch_bounds__(WM* WN * 64) void k_i8_tile(I8Args p, int tiles_n) 
     constexpr int OUT_N = GATED ? BN / 2 : BN;         // output columns of a tile
     static_assert(NA * kT == BM * 8 && NB * kT == BN * 8, "chunks divide");
     static_assert(!GATED || FN % 2 == 0, "a wave holds gate and up");
-    __shared__ __align__(16) int8_t sA[BM * kBK];
-    __shared__ __align__(16) int8_t sB[BN * kBK];
+    __shared__ __align__(16) int8_t lds[(BM + BN) * kBK];
+    int8_t* sA = lds;
+    int8_t* sB = lds + BM * kBK;
+    static_assert(WM * WN * Stage<FM, FN, GATED>::kBytes <= (BM + BN) * kBK, "the outputs' stage fits");
 
     const int tile_m = blockIdx.x / tiles_n, tile_n = blockIdx.x % tiles_n;
     int64_t m0 = (int64_t)tile_m * BM, m_end = p.M;
@@ -129,34 +241,145 @@ __global__ __launch_bounds__(WM* WN * 64) void k_i8_tile(I8Args p, int tiles_n) 
         }
     }
 
-    // A lane's four sums of a fragment: row m = lane & 15, channels
-    // (lane >> 4) * 4 + 0..3.
+    __syncthreads();
+    epilogue<FM, FN, GATED, GROUPED>(p, acc, m0 + wm, m_end, n0, wn, sb, bias,
+                                     reinterpret_cast<float*>(lds) + wave * (Stage<FM, FN, GATED>::kBytes / 4));
+}
+
+// XCD-aware tile order: workgroups are handed to the eight XCDs in turn, so
+// every XCD gets a contiguous run of tiles; a run goes through bands of kBand
+// row tiles, column by column, so that the tiles in flight on an XCD share
+// their rows and channels in its L2.
+constexpr int kXcds = 8, kBand = 8;
+__device__ __forceinline__ void tile_of(int b, int blocks, int tiles_m, int tiles_n, int* tm, int* tn) {
+    const int per = blocks / kXcds, rest = blocks % kXcds, x = b % kXcds;
+    b = x * per + (x < rest ? x : rest) + b / kXcds;
+    const int band = b / (kBand * tiles_n), in = b % (kBand * tiles_n);
+    const int left = tiles_m - band * kBand;
+    const int h = left < kBand ? left : kBand;
+    *tm = band * kBand + in % h;
+    *tn = in / h;
+}
+
+typedef const __attribute__((address_space(1))) void* GlobalPtr;
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+// The large product: tiles go from memory to LDS directly (16 bytes a lane,
+// no registers between), the next tile's loads in flight while this one is
+// multiplied.  A wave-wide load fills 1 KiB of LDS, eight rows; lane i's chunk
+// lies at i % 8, so it fetches chunk (i % 8) ^ (row % 8) of its row: the same
+// bank order as above.  Needs 16-byte aligned rows; the last K % 128 codes go
+// through registers with zeros behind them.
+template <int BM, int BN, int WM, int WN, bool GATED, bool GROUPED>
+__global__ __launch_bounds__(WM* WN * 64) void k_i8_big(I8Args p, int tiles_m, int tiles_n) {
+    constexpr int kWavesB = WM * WN;
+    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+    constexpr int NA = BM / 8 / kWavesB, NB = BN / 8 / kWavesB;  // 1 KiB loads a wave issues
+    constexpr int OUT_N = GATED ? BN / 2 : BN;
+    static_assert(NA * kWavesB * 8 == BM && NB * kWavesB * 8 == BN, "loads divide");
+    __shared__ __align__(16) int8_t s0[(BM + BN) * kBK];
+    __shared__ __align__(16) int8_t s1[(BM + BN) * kBK];
+    static_assert(WM * WN * Stage<FM, FN, GATED>::kBytes <= (BM + BN) * kBK, "the outputs' stage fits");
+
+    int tile_m, tile_n;
+    tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, &tile_m, &tile_n);
+    int64_t m0 = (int64_t)tile_m * BM, m_end = p.M;
+    const int8_t* B = p.B;
+    const float* sb = p.sb;
+    const float* bias = p.bias;
+    if constexpr (GROUPED) {
+        if (tile_m >= *p.n_tiles) return;
+        const int4 t = p.tiles[tile_m];
+        m0 = t.y;
+        m_end = t.z;
+        B += (int64_t)t.x * p.b_stride;
+        sb += (int64_t)t.x * p.s_stride;
+        if (bias) bias += (int64_t)t.x * p.s_stride;
+    }
+    const int n0 = tile_n * OUT_N;
+    const int lane = lane_id(), wave = uniform(threadIdx.x >> 6);
+    const int r8 = lane >> 3, chunk = ((lane & 7) ^ r8) * 16;
+    auto a_row = [&](int i) __attribute__((always_inline)) {
+        int64_t m = m0 + (wave * NA + i) * 8 + r8;
+        if (m >= m_end) m = m_end - 1;  // a valid row, its products are not stored
+        if (GROUPED && p.a_rows) m = p.a_rows[m];
+        return p.A + m * p.lda + chunk;
+    };
+    auto b_row = [&](int i) __attribute__((always_inline)) {
+        const int c = (wave * NB + i) * 8 + r8;
+        int n = GATED ? n0 + (c >> 5) * 16 + (c & 15) : n0 + c;
+        if (n >= p.N) n = p.N - 1;
+        if (GATED && (c & 16)) n += p.N;
+        return B + (int64_t)n * p.ldb + chunk;
+    };
+    const int8_t* pa[NA];
+    const int8_t* pb[NB];
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int64_t m = m0 + wm + i * 16 + (lane & 15);
-        if (m >= m_end) continue;
-        const int64_t ar = GROUPED && p.a_rows ? p.a_rows[m] : m;
-        const float sa = p.sa[ar];
-        const int64_t orow = (GROUPED && p.o_rows ? p.o_rows[m] : m) * p.ldo;
+    for (int i = 0; i < NA; ++i) pa[i] = a_row(i);
 #pragma unroll
-        for (int j = 0; j < FN; j += GATED ? 2 : 1) {
-            const int c = wn + j * 16 + (lane >> 4) * 4;
-            const int n = n0 + (GATED ? (c >> 5) * 16 + (c & 15) : c);
+    for (int i = 0; i < NB; ++i) pb[i] = b_row(i);
+    const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+    v4i acc[FM][FN];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (n + e >= p.N) continue;
-                float v = (float)acc[i][j][e] * sa * sb[n + e];
-                if (bias) v += bias[n + e];
-                v = apply_act(v, p.act);
-                if constexpr (GATED) {
-                    float u = (float)acc[i][j + 1][e] * sa * sb[p.N + n + e];
-                    if (bias) u += bias[p.N + n + e];
-                    v *= u;
-                }
-                store_elem(p.out, orow + n + e, v, p.out_elem);
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+
+    auto fetch = [&](int8_t* s, int k0) __attribute__((always_inline)) {
+        if (k0 + kBK <= p.K) {
+#pragma unroll
+            for (int i = 0; i < NA; ++i)
+                __builtin_amdgcn_global_load_lds((GlobalPtr)(pa[i] + k0), (LdsPtr)(s + (wave * NA + i) * 1024), 16, 0,
+                                                 0);
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+                __builtin_amdgcn_global_load_lds((GlobalPtr)(pb[i] + k0),
+                                                 (LdsPtr)(s + BM * kBK + (wave * NB + i) * 1024), 16, 0, 0);
+        } else {
+            const int valid = p.K - k0 - chunk;
+#pragma unroll 1
+            for (int i = 0; i < NA + NB; ++i) {
+                const int8_t* from = i < NA ? a_row(i) : b_row(i - NA);
+                int8_t* to = s + (i < NA ? wave * NA + i : BM / 8 + wave * NB + i - NA) * 1024 + lane * 16;
+                *reinterpret_cast<v4i*>(to) = load16(from + k0, valid);
             }
         }
+    };
+    auto multiply = [&](const int8_t* s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const int c = ((kk * 4 + (lane >> 4)) ^ (lane & 7)) * 16;  // every fragment starts at a row of 8k
+            v4i fa[FM], fb[FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                fb[j] = *reinterpret_cast<const v4i*>(s + (BM + wn + j * 16 + (lane & 15)) * kBK + c);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+                fa[i] = *reinterpret_cast<const v4i*>(s + (wm + i * 16 + (lane & 15)) * kBK + c);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[j], fa[i], acc[i][j], 0, 0, 0);
+        }
+    };
+    // Two tiles a turn, each LDS array of its own: only then does the compiler
+    // see that the reads of one need not wait for the loads into the other.
+    if (p.K > 0) fetch(s0, 0);
+    __syncthreads();
+    int k0 = 0;
+    for (; k0 + kBK < p.K; k0 += 2 * kBK) {
+        fetch(s1, k0 + kBK);
+        multiply(s0);
+        __syncthreads();
+        if (k0 + 2 * kBK < p.K) fetch(s0, k0 + 2 * kBK);
+        multiply(s1);
+        __syncthreads();
     }
+    if (k0 < p.K) multiply(s0);
+    __syncthreads();
+    epilogue<FM, FN, GATED, GROUPED>(p, acc, m0 + wm, m_end, n0, wn, sb, bias,
+                                     reinterpret_cast<float*>(s0) + wave * (Stage<FM, FN, GATED>::kBytes / 4));
 }
 
 int check_grid(int64_t blocks) {
@@ -164,10 +387,21 @@ int check_grid(int64_t blocks) {
     return VDTTFS_OK;
 }
 
+bool aligned16(const I8Args& a) {
+    return (((uintptr_t)a.A | (uintptr_t)a.B | (uintptr_t)a.lda | (uintptr_t)a.ldb | (uintptr_t)a.b_stride) & 15) == 0;
+}
+
 }  // namespace
 
 int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
     if (a.M <= 0 || a.N <= 0) return VDTTFS_OK;
+    if (a.M >= 1024 && aligned16(a)) {
+        const int tm = (int)((a.M + 255) / 256), tn = (a.N + 255) / 256;
+        VD_TRY(check_grid((int64_t)tm * tn));
+        k_i8_big<256, 256, 2, 4, false, false><<<dim3((unsigned)(tm * tn)), 512, 0, ctx->stream>>>(a, tm, tn);
+        VD_HIP(hipGetLastError());
+        return VDTTFS_OK;
+    }
     const int tiles_n = (a.N + 63) / 64;
     const int64_t blocks = (a.M + 63) / 64 * tiles_n;
     VD_TRY(check_grid(blocks));
