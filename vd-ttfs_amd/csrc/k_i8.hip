@@ -5,6 +5,7 @@
 #include "elem.h"
 #include "head.h"
 #include "wave.h"
+#include <cstdlib>
 
 namespace vdttfs {
 namespace {
@@ -393,14 +394,28 @@ bool aligned16(const I8Args& a) {
 
 }  // namespace
 
+template <int BM, int BN, int WM, int WN>
+int run_big(vdttfs_ctx* ctx, const I8Args& a) {
+    const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
+    VD_TRY(check_grid(tm * tn));
+    k_i8_big<BM, BN, WM, WN, false, false>
+        <<<dim3((unsigned)(tm * tn)), WM * WN * 64, 0, ctx->stream>>>(a, (int)tm, (int)tn);
+    VD_HIP(hipGetLastError());
+    return VDTTFS_OK;
+}
+
 int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
     if (a.M <= 0 || a.N <= 0) return VDTTFS_OK;
-    if (a.M >= 1024 && aligned16(a)) {
-        const int tm = (int)((a.M + 255) / 256), tn = (a.N + 255) / 256;
-        VD_TRY(check_grid((int64_t)tm * tn));
-        k_i8_big<256, 256, 2, 4, false, false><<<dim3((unsigned)(tm * tn)), 512, 0, ctx->stream>>>(a, tm, tn);
-        VD_HIP(hipGetLastError());
-        return VDTTFS_OK;
+    static int tile = getenv("VD_TILE") ? atoi(getenv("VD_TILE")) : 0;
+    if (aligned16(a)) {
+        if (tile == 1 ) return run_big<256, 256, 2, 4>(ctx, a);
+        if (tile == 2) return run_big<128, 128, 2, 2>(ctx, a);
+        if (tile == 3) return run_big<64, 64, 2, 2>(ctx, a);
+        if (tile == 4) return run_big<32, 64, 2, 2>(ctx, a);
+        if (tile == 5) return run_big<64, 128, 2, 2>(ctx, a);
+        if (tile == 6) return run_big<128, 256, 2, 4>(ctx, a);
+        if (tile == 7) return run_big<256, 128, 4, 2>(ctx, a);
+        if (tile == 8) return run_big<32, 32, 2, 2>(ctx, a);
     }
     const int tiles_n = (a.N + 63) / 64;
     const int64_t blocks = (a.M + 63) / 64 * tiles_n;
@@ -410,25 +425,32 @@ int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
     return VDTTFS_OK;
 }
 
+// Rows of a grouped product's tiles: the largest that an expert's rows fill on
+// average.
 int i8_tile_rows(int64_t pairs, int n_experts) {
-    (void)pairs;
-    (void)n_experts;
-    return 64;
+    const int64_t mean = pairs / n_experts;
+    return mean >= 256 ? 256 : mean >= 96 ? 128 : 64;
+}
+
+template <int BM, int BN, int WM, int WN, bool GATED>
+int run_grouped(vdttfs_ctx* ctx, const I8Args& a) {
+    constexpr int kOut = GATED ? BN / 2 : BN;
+    const int64_t tn = (a.N + kOut - 1) / kOut, blocks = a.max_tiles * tn;
+    VD_TRY(check_grid(blocks));
+    if (aligned16(a))
+        k_i8_big<BM, BN, WM, WN, GATED, true>
+            <<<dim3((unsigned)blocks), WM * WN * 64, 0, ctx->stream>>>(a, a.max_tiles, (int)tn);
+    else
+        k_i8_tile<BM, BN, WM, WN, GATED, true><<<dim3((unsigned)blocks), WM * WN * 64, 0, ctx->stream>>>(a, (int)tn);
+    VD_HIP(hipGetLastError());
+    return VDTTFS_OK;
 }
 
 int launch_i8_grouped(vdttfs_ctx* ctx, const I8Args& a, bool gated, int bm) {
     if (a.max_tiles <= 0 || a.N <= 0) return VDTTFS_OK;
-    (void)bm;
-    const int out_n = gated ? 32 : 64;
-    const int tiles_n = (a.N + out_n - 1) / out_n;
-    const int64_t blocks = (int64_t)a.max_tiles * tiles_n;
-    VD_TRY(check_grid(blocks));
-    if (gated)
-        k_i8_tile<64, 64, 2, 2, true, true><<<dim3((unsigned)blocks), 256, 0, ctx->stream>>>(a, tiles_n);
-    else
-        k_i8_tile<64, 64, 2, 2, false, true><<<dim3((unsigned)blocks), 256, 0, ctx->stream>>>(a, tiles_n);
-    VD_HIP(hipGetLastError());
-    return VDTTFS_OK;
+    if (bm == 256) return gated ? run_grouped<256, 256, 2, 4, true>(ctx, a) : run_grouped<256, 256, 2, 4, false>(ctx, a);
+    if (bm == 128) return gated ? run_grouped<128, 128, 2, 2, true>(ctx, a) : run_grouped<128, 128, 2, 2, false>(ctx, a);
+    return gated ? run_grouped<64, 64, 2, 2, true>(ctx, a) : run_grouped<64, 64, 2, 2, false>(ctx, a);
 }
 
 }  // namespace vdttfs
