@@ -2,10 +2,11 @@
 //
 // out[m][n] = act(float(sum_k A[m][k] B[n][k]) * sa[m] * sb[n] + bias[n]), the
 // sum in 32-bit integers (v_mfma_i32_16x16x64_i8), so no order of k matters.
+#include <type_traits>
+
 #include "elem.h"
 #include "head.h"
 #include "wave.h"
-#include <cstdlib>
 
 namespace vdttfs {
 namespace {
@@ -126,10 +127,12 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
                     *reinterpret_cast<const v4f*>(stage + row * S::kRow + c);
             }
         } else {
-            const int c = lane % S::kCols;
-            for (int row = lane / S::kCols; row < 16 && mi + row < m_end; row += 64 / S::kCols) {
+#pragma unroll 1
+            for (int at = lane; at < 16 * S::kCols; at += 64) {
+                const int row = at / S::kCols, c = at % S::kCols;
+                if (mi + row >= m_end || nw + c >= p.N) continue;
                 const int64_t o = (GROUPED && p.o_rows ? p.o_rows[mi + row] : mi + row) * p.ldo + nw + c;
-                if (nw + c < p.N) store_elem(p.out, o, stage[row * S::kRow + c], p.out_elem);
+                store_elem(p.out, o, stage[row * S::kRow + c], p.out_elem);
             }
         }
         wave_sync();
@@ -265,22 +268,47 @@ __device__ __forceinline__ void tile_of(int b, int blocks, int tiles_m, int tile
 typedef const __attribute__((address_space(1))) void* GlobalPtr;
 typedef __attribute__((address_space(3))) void* LdsPtr;
 
-// The large product: tiles go from memory to LDS directly (16 bytes a lane,
-// no registers between), the next tile's loads in flight while this one is
-// multiplied.  A wave-wide load fills 1 KiB of LDS, eight rows; lane i's chunk
-// lies at i % 8, so it fetches chunk (i % 8) ^ (row % 8) of its row: the same
-// bank order as above.  Needs 16-byte aligned rows; the last K % 128 codes go
-// through registers with zeros behind them.
-template <int BM, int BN, int WM, int WN, bool GATED, bool GROUPED>
-__global__ __launch_bounds__(WM* WN * 64) void k_i8_big(I8Args p, int tiles_m, int tiles_n) {
-    constexpr int kWavesB = WM * WN;
+// The large product: tiles of BK codes a row go from memory to LDS directly
+// (16 bytes a lane, no registers between), S tiles deep: while one is
+// multiplied, the loads of the next S - 1 are in flight.  A wave-wide load
+// fills 1 KiB of LDS; the chunk that lies at place c of row r is chunk
+// c ^ swizzle(r), so that the 16 rows of a fragment come from all banks.
+// Needs 16-byte aligned rows; the last K % BK codes go through registers with
+// zeros behind them.
+template <int BK>
+__device__ __forceinline__ int swizzle(int row) {
+    return BK == 128 ? row & 7 : (row >> 2) & 3;
+}
+
+// Waits until at most N of the wave's loads are outstanding (LDS writes: none).
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4 | 0 << 8);
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <int BM, int BN, int WM, int WN, int BK, int S, bool GATED, bool GROUPED>
+__global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m, int tiles_n) {
+    constexpr int kW = WM * WN, kChunks = BK / 16, kRows = 64 / kChunks;  // rows of one 1 KiB load
     constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-    constexpr int NA = BM / 8 / kWavesB, NB = BN / 8 / kWavesB;  // 1 KiB loads a wave issues
+    constexpr int NA = BM / kRows / kW, NB = BN / kRows / kW, NL = NA + NB;  // loads of a wave and tile
     constexpr int OUT_N = GATED ? BN / 2 : BN;
-    static_assert(NA * kWavesB * 8 == BM && NB * kWavesB * 8 == BN, "loads divide");
-    __shared__ __align__(16) int8_t s0[(BM + BN) * kBK];
-    __shared__ __align__(16) int8_t s1[(BM + BN) * kBK];
-    static_assert(WM * WN * Stage<FM, FN, GATED>::kBytes <= (BM + BN) * kBK, "the outputs' stage fits");
+    constexpr int kTile = (BM + BN) * BK;
+    static_assert(NA * kW * kRows == BM && NB * kW * kRows == BN, "loads divide");
+    static_assert(S >= 2 && S <= 4 && (S - 2) * NL < 64, "stages");
+    constexpr int kStage = kW * Stage<FM, FN, GATED>::kBytes;
+    // an array for each stage: only then does the compiler see that reads of
+    // one need not wait for loads into another
+    __shared__ __align__(16) int8_t s0[kTile > kStage ? kTile : kStage];
+    __shared__ __align__(16) int8_t s1[kTile];
+    __shared__ __align__(16) int8_t s2[S > 2 ? kTile : 16];
+    __shared__ __align__(16) int8_t s3[S > 3 ? kTile : 16];
 
     int tile_m, tile_n;
     tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, &tile_m, &tile_n);
@@ -299,15 +327,15 @@ __global__ __launch_bounds__(WM* WN * 64) void k_i8_big(I8Args p, int tiles_m, i
     }
     const int n0 = tile_n * OUT_N;
     const int lane = lane_id(), wave = uniform(threadIdx.x >> 6);
-    const int r8 = lane >> 3, chunk = ((lane & 7) ^ r8) * 16;
+    const int lrow = lane / kChunks, chunk = ((lane % kChunks) ^ swizzle<BK>(lrow)) * 16;
     auto a_row = [&](int i) __attribute__((always_inline)) {
-        int64_t m = m0 + (wave * NA + i) * 8 + r8;
+        int64_t m = m0 + (wave * NA + i) * kRows + lrow;
         if (m >= m_end) m = m_end - 1;  // a valid row, its products are not stored
         if (GROUPED && p.a_rows) m = p.a_rows[m];
         return p.A + m * p.lda + chunk;
     };
     auto b_row = [&](int i) __attribute__((always_inline)) {
-        const int c = (wave * NB + i) * 8 + r8;
+        const int c = (wave * NB + i) * kRows + lrow;
         int n = GATED ? n0 + (c >> 5) * 16 + (c & 15) : n0 + c;
         if (n >= p.N) n = p.N - 1;
         if (GATED && (c & 16)) n += p.N;
@@ -326,58 +354,100 @@ __global__ __launch_bounds__(WM* WN * 64) void k_i8_big(I8Args p, int tiles_m, i
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = v4i{0, 0, 0, 0};
 
-    auto fetch = [&](int8_t* s, int k0) __attribute__((always_inline)) {
-        if (k0 + kBK <= p.K) {
-#pragma unroll
-            for (int i = 0; i < NA; ++i)
-                __builtin_amdgcn_global_load_lds((GlobalPtr)(pa[i] + k0), (LdsPtr)(s + (wave * NA + i) * 1024), 16, 0,
-                                                 0);
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-                __builtin_amdgcn_global_load_lds((GlobalPtr)(pb[i] + k0),
-                                                 (LdsPtr)(s + BM * kBK + (wave * NB + i) * 1024), 16, 0, 0);
-        } else {
-            const int valid = p.K - k0 - chunk;
-#pragma unroll 1
-            for (int i = 0; i < NA + NB; ++i) {
-                const int8_t* from = i < NA ? a_row(i) : b_row(i - NA);
-                int8_t* to = s + (i < NA ? wave * NA + i : BM / 8 + wave * NB + i - NA) * 1024 + lane * 16;
-                *reinterpret_cast<v4i*>(to) = load16(from + k0, valid);
-            }
-        }
+    const int tiles = p.K / BK;  // whole ones
+    auto fetch_one = [&](int8_t* s, int k0, int l) __attribute__((always_inline)) {
+        if (l < NA)
+            __builtin_amdgcn_global_load_lds((GlobalPtr)(pa[l] + k0), (LdsPtr)(s + (wave * NA + l) * 1024), 16, 0, 0);
+        else
+            __builtin_amdgcn_global_load_lds((GlobalPtr)(pb[l - NA] + k0),
+                                             (LdsPtr)(s + BM * BK + (wave * NB + l - NA) * 1024), 16, 0, 0);
     };
-    auto multiply = [&](const int8_t* s) __attribute__((always_inline)) {
+    auto k_of = [&](int t) __attribute__((always_inline)) {
+        return (t < tiles ? t : tiles - 1) * BK;  // past the end: loaded, not used
+    };
+    auto fetch = [&](int8_t* s, int t) __attribute__((always_inline)) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const int c = ((kk * 4 + (lane >> 4)) ^ (lane & 7)) * 16;  // every fragment starts at a row of 8k
-            v4i fa[FM], fb[FN];
+        for (int l = 0; l < NL; ++l) fetch_one(s, k_of(t), l);
+    };
+    // One tile multiplied, with the loads of another (k0 of it, to `next`)
+    // spread between: a wave that issues its loads in one go waits for the
+    // address unit, and its matrix instructions with it.  Each group is one row
+    // fragment against all channel fragments; fragments are read two groups
+    // (channels: one k step) ahead.
+    constexpr int KK = BK / 64, G = KK * FM, kSpread = S == 2 ? (G + 1) / 2 : G;
+    auto multiply = [&](auto with_loads, const int8_t* s, int8_t* next, int k0) __attribute__((always_inline)) {
+        const int r = lane & 15;
+        v4i fa[3], fb[2][FN];
+        auto read_a = [&](int g) __attribute__((always_inline)) {
+            const int c = ((g / FM * 4 + (lane >> 4)) ^ swizzle<BK>(r)) * 16;
+            fa[g % 3] = *reinterpret_cast<const v4i*>(s + (wm + g % FM * 16 + r) * BK + c);
+        };
+        auto read_b = [&](int kk, int j) __attribute__((always_inline)) {
+            const int c = ((kk * 4 + (lane >> 4)) ^ swizzle<BK>(r)) * 16;
+            fb[kk & 1][j] = *reinterpret_cast<const v4i*>(s + (BM + wn + j * 16 + r) * BK + c);
+        };
+        read_a(0);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) read_b(0, j);
+        if (G > 1) read_a(1);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int kk = g / FM, i = g % FM;
+            if (g + 2 < G) read_a(g + 2);
+            if (kk + 1 < KK) {
+#pragma unroll
+                for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j) read_b(kk + 1, j);
+            }
+            if constexpr (with_loads.value) {
+#pragma unroll
+                for (int l = 0; l < NL; ++l)
+                    if (l * kSpread / NL == g) fetch_one(next, k0, l);
+            }
 #pragma unroll
             for (int j = 0; j < FN; ++j)
-                fb[j] = *reinterpret_cast<const v4i*>(s + (BM + wn + j * 16 + (lane & 15)) * kBK + c);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-                fa[i] = *reinterpret_cast<const v4i*>(s + (wm + i * 16 + (lane & 15)) * kBK + c);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[j], fa[i], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[kk & 1][j], fa[g % 3], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // Two tiles a turn, each LDS array of its own: only then does the compiler
-    // see that the reads of one need not wait for the loads into the other.
-    if (p.K > 0) fetch(s0, 0);
-    __syncthreads();
-    int k0 = 0;
-    for (; k0 + kBK < p.K; k0 += 2 * kBK) {
-        fetch(s1, k0 + kBK);
-        multiply(s0);
-        __syncthreads();
-        if (k0 + 2 * kBK < p.K) fetch(s0, k0 + 2 * kBK);
-        multiply(s1);
-        __syncthreads();
+    // Tile t is in s; the loads of tile t + S - 1 go to `next`, whose tile
+    // every wave has read before the barrier.  No branch between loads and
+    // waits, so the number in flight is known everywhere and the compiler adds
+    // no waits of its own.
+    auto step = [&](const int8_t* s, int8_t* next, int t) __attribute__((always_inline)) {
+        wait_loads<(S - 2) * NL>();
+        barrier();
+        multiply(std::true_type{}, s, next, k_of(t + S - 1));
+    };
+    if (tiles > 0) {
+        fetch(s0, 0);
+        if (S > 2) fetch(s1, 1);
+        if (S > 3) fetch(s2, 2);
+        int t = 0;
+        for (; t + S <= tiles; t += S) {
+            step(s0, S == 2 ? s1 : S == 3 ? s2 : s3, t);
+            step(s1, s0, t + 1);
+            if (S > 2) step(s2, s1, t + 2);
+            if (S > 3) step(s3, s2, t + 3);
+        }
+        // the last tiles % S are in flight
+        wait_loads<0>();
+        barrier();
+        if (t < tiles) multiply(std::false_type{}, s0, s0, 0);
+        if (S > 2 && t + 1 < tiles) multiply(std::false_type{}, s1, s1, 0);
+        if (S > 3 && t + 2 < tiles) multiply(std::false_type{}, s2, s2, 0);
     }
-    if (k0 < p.K) multiply(s0);
+    if (tiles * BK < p.K) {
+        const int valid = p.K - tiles * BK - chunk;
+        __syncthreads();
+#pragma unroll 1
+        for (int i = 0; i < NL; ++i) {
+            const int8_t* from = i < NA ? a_row(i) : b_row(i - NA);
+            int8_t* to = s0 + (i < NA ? wave * NA + i : BM / kRows + wave * NB + i - NA) * 1024 + lane * 16;
+            *reinterpret_cast<v4i*>(to) = load16(from + tiles * BK, valid);
+        }
+        __syncthreads();
+        multiply(std::false_type{}, s0, s0, 0);
+    }
     __syncthreads();
     epilogue<FM, FN, GATED, GROUPED>(p, acc, m0 + wm, m_end, n0, wn, sb, bias,
                                      reinterpret_cast<float*>(s0) + wave * (Stage<FM, FN, GATED>::kBytes / 4));
@@ -394,51 +464,60 @@ bool aligned16(const I8Args& a) {
 
 }  // namespace
 
-template <int BM, int BN, int WM, int WN>
+template <int BM, int BN, int WM, int WN, int BK, int S>
 int run_big(vdttfs_ctx* ctx, const I8Args& a) {
     const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
     VD_TRY(check_grid(tm * tn));
-    k_i8_big<BM, BN, WM, WN, false, false>
+    k_i8_big<BM, BN, WM, WN, BK, S, false, false>
         <<<dim3((unsigned)(tm * tn)), WM * WN * 64, 0, ctx->stream>>>(a, (int)tm, (int)tn);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
 
-int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
-    if (a.M <= 0 || a.N <= 0) return VDTTFS_OK;
-    static int tile = getenv("VD_TILE") ? atoi(getenv("VD_TILE")) : 0;
-    if (aligned16(a)) {
-        if (tile == 1 ) return run_big<256, 256, 2, 4>(ctx, a);
-        if (tile == 2) return run_big<128, 128, 2, 2>(ctx, a);
-        if (tile == 3) return run_big<64, 64, 2, 2>(ctx, a);
-        if (tile == 4) return run_big<32, 64, 2, 2>(ctx, a);
-        if (tile == 5) return run_big<64, 128, 2, 2>(ctx, a);
-        if (tile == 6) return run_big<128, 256, 2, 4>(ctx, a);
-        if (tile == 7) return run_big<256, 128, 4, 2>(ctx, a);
-        if (tile == 8) return run_big<32, 32, 2, 2>(ctx, a);
-    }
-    const int tiles_n = (a.N + 63) / 64;
-    const int64_t blocks = (a.M + 63) / 64 * tiles_n;
+template <int BM, int BN>
+int run_tile(vdttfs_ctx* ctx, const I8Args& a) {
+    const int64_t tn = (a.N + BN - 1) / BN, blocks = (a.M + BM - 1) / BM * tn;
     VD_TRY(check_grid(blocks));
-    k_i8_tile<64, 64, 2, 2, false, false><<<dim3((unsigned)blocks), 256, 0, ctx->stream>>>(a, tiles_n);
+    k_i8_tile<BM, BN, 2, 2, false, false><<<dim3((unsigned)blocks), 256, 0, ctx->stream>>>(a, (int)tn);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
+}
+
+// Rows on 16 bytes take the tiles that go to LDS directly: the largest tile of
+// which there are enough to fill the chip, as below that a CU's time goes by
+// the number of steps in K, whatever the tile.  Measured (us, K last):
+//   8192x4096x4096: 256x256 128, 128x128 158, 64x128 187
+//   1536x8192x2048 (192 tiles of 256): 34, 39, 41;  2560x8192x2048 (320, so
+//   two rounds, the second a quarter full): 65, 60, 67
+//   1024x4096x4096 (256 of 128): 128x128 29, 64x128 27, 64x64 34
+//   256x4096x4096: 64x128 14.7, 64x64 10.4, 32x32 15.1;  64x4096x4096: 64x64
+//   10.0, 32x32 7.6;  333x1111x1003: 64x64 8.0, 32x32 4.9
+int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
+    if (a.M <= 0 || a.N <= 0) return VDTTFS_OK;
+    auto tiles = [&](int bm, int bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); };
+    if (!aligned16(a)) return tiles(64, 64) >= 192 ? run_tile<64, 64>(ctx, a) : run_tile<32, 32>(ctx, a);
+    const int64_t big = tiles(256, 256), rounds = (big + 255) / 256;
+    if (rounds == 1 ? big >= 160 : big * 10 >= rounds * 256 * 7) return run_big<256, 256, 2, 4, 128, 2>(ctx, a);
+    if (tiles(128, 128) >= 384) return run_big<128, 128, 2, 2, 128, 2>(ctx, a);
+    if (tiles(64, 128) >= 384) return run_big<64, 128, 2, 2, 128, 3>(ctx, a);
+    if (tiles(64, 64) >= 192) return run_big<64, 64, 2, 2, 128, 4>(ctx, a);
+    return run_big<32, 32, 2, 2, 128, 4>(ctx, a);
 }
 
 // Rows of a grouped product's tiles: the largest that an expert's rows fill on
 // average.
 int i8_tile_rows(int64_t pairs, int n_experts) {
     const int64_t mean = pairs / n_experts;
-    return mean >= 256 ? 256 : mean >= 96 ? 128 : 64;
+    return mean >= 256 ? 256 : mean >= 96 ? 128 : mean >= 40 ? 64 : 32;
 }
 
-template <int BM, int BN, int WM, int WN, bool GATED>
+template <int BM, int BN, int WM, int WN, int S, bool GATED>
 int run_grouped(vdttfs_ctx* ctx, const I8Args& a) {
     constexpr int kOut = GATED ? BN / 2 : BN;
     const int64_t tn = (a.N + kOut - 1) / kOut, blocks = a.max_tiles * tn;
     VD_TRY(check_grid(blocks));
     if (aligned16(a))
-        k_i8_big<BM, BN, WM, WN, GATED, true>
+        k_i8_big<BM, BN, WM, WN, 128, S, GATED, true>
             <<<dim3((unsigned)blocks), WM * WN * 64, 0, ctx->stream>>>(a, a.max_tiles, (int)tn);
     else
         k_i8_tile<BM, BN, WM, WN, GATED, true><<<dim3((unsigned)blocks), WM * WN * 64, 0, ctx->stream>>>(a, (int)tn);
@@ -446,11 +525,17 @@ int run_grouped(vdttfs_ctx* ctx, const I8Args& a) {
     return VDTTFS_OK;
 }
 
+template <bool GATED>
+int run_grouped_rows(vdttfs_ctx* ctx, const I8Args& a, int bm) {
+    if (bm == 256) return run_grouped<256, 256, 2, 4, 2, GATED>(ctx, a);
+    if (bm == 128) return run_grouped<128, 128, 2, 2, 2, GATED>(ctx, a);
+    if (bm == 64) return run_grouped<64, 64, 2, 2, 4, GATED>(ctx, a);
+    return run_grouped<32, 64, 2, 2, 4, GATED>(ctx, a);
+}
+
 int launch_i8_grouped(vdttfs_ctx* ctx, const I8Args& a, bool gated, int bm) {
     if (a.max_tiles <= 0 || a.N <= 0) return VDTTFS_OK;
-    if (bm == 256) return gated ? run_grouped<256, 256, 2, 4, true>(ctx, a) : run_grouped<256, 256, 2, 4, false>(ctx, a);
-    if (bm == 128) return gated ? run_grouped<128, 128, 2, 2, true>(ctx, a) : run_grouped<128, 128, 2, 2, false>(ctx, a);
-    return gated ? run_grouped<64, 64, 2, 2, true>(ctx, a) : run_grouped<64, 64, 2, 2, false>(ctx, a);
+    return gated ? run_grouped_rows<true>(ctx, a, bm) : run_grouped_rows<false>(ctx, a, bm);
 }
 
 }  // namespace vdttfs
