@@ -46,6 +46,7 @@ struct vdttfs_ctx {
     void* head_buf;
     size_t head_bytes;
     bool head_captured;
+    int* route_acc;  // routing's counters, 0 between calls
     bool named_skip;  // a split call could not size its named plan's scratch too
     unsigned long long* d_counters;  // kCounterStripes x 4 u64 (summed on the host)
     hipEvent_t timer[2];             // vdttfs_timer_begin/end (created on first use)

@@ -43,7 +43,11 @@ int launch_i8_grouped(vdttfs_ctx* ctx, const I8Args& a, bool gated, int bm);
 int i8_tile_rows(int64_t pairs, int n_experts);
 
 int launch_route(vdttfs_ctx* ctx, int32_t* idx, float* wt, int32_t* count, const void* logits, int elem, int64_t ld,
-                 const float* bias, const uint8_t* row_mask, int64_t M, const vdttfs_route_opts& o);
+                 const float* bias, const uint8_t* row_mask, int64_t M, const vdttfs_route_opts& o, int* acc);
+// Device memory that launch_route's counts pass through, 0 between calls;
+// calls of at most kRouteAlone rows do without.
+constexpr int kRouteAlone = 4;
+size_t route_acc_bytes();
 
 // The pairs (row, slot) sorted by expert.  pair[i]: row * top_k + slot of
 // sorted row i, row[i]: its row; tiles as in I8Args with bm rows each.

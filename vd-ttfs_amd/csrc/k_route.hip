@@ -14,17 +14,40 @@ constexpr int kSortPairs = 2048;  // pairs a workgroup of the sort takes
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
+// Another lane's value by a data-parallel-primitive move (no LDS trip).
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float dpp(float v) {
+    const int i = __float_as_int(v);
+    return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, ROWS, 0xf, false));
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140, kBcast15 = 0x142, kBcast31 = 0x143;
+
+// The wave's largest value, in every lane (scalar).
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-    return v;
+    v = fmaxf(v, dpp<kXor1>(v));
+    v = fmaxf(v, dpp<kXor2>(v));
+    v = fmaxf(v, dpp<kHalfMirror>(v));
+    v = fmaxf(v, dpp<kMirror>(v));
+    v = fmaxf(v, dpp<kBcast15, 0xa>(v));
+    v = fmaxf(v, dpp<kBcast31, 0xc>(v));
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
+    v += dpp<kXor1>(v);
+    v += dpp<kXor2>(v);
+    v += dpp<kHalfMirror>(v);
+    v += dpp<kMirror>(v);
+    float s = 0.0f;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+    for (int r = 0; r < 4; ++r) s += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), r * 16));
+    return s;
 }
+
+// exp and 1 / x of the scores, by the hardware's exp2 and reciprocal: relative
+// errors below (2 + |x|) 2^-23, equal inputs give equal scores.
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+__device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 
 struct RouteArgs {
     int32_t* idx;
@@ -37,13 +60,54 @@ struct RouteArgs {
     int64_t M;
     int E, k, score, groups, top_groups, group_top, renorm;
     float scale;
+    int* acc;  // [kReplicas][kMaxExperts] sums and the tickets, all 0 between calls; one workgroup: unused
 };
+
+// The workgroup's counts into the call's.  Adds to a few busy lines cost (65536
+// rows over 64 experts: 4096 workgroups add 40 us to the call, 1024 8 us), so
+// there are few workgroups, and sums go to one of kReplicas copies; the last
+// workgroup, told by tickets (one for each copy, and one for the copies), moves
+// them out and leaves zeros behind: no launch of its own to clear or to sum.
+// Whole numbers, so no order matters.
+constexpr int kReplicas = 8;
+__device__ __forceinline__ void finish_counts(const RouteArgs& a, const int* hist, int* last) {
+    __syncthreads();
+    if (gridDim.x == 1) {
+        for (int e = threadIdx.x; e < a.E; e += blockDim.x) a.count[e] = hist[e];
+        return;
+    }
+    const int copy = blockIdx.x % kReplicas;
+    int* mine = a.acc + copy * kMaxExperts;
+    int* tickets = a.acc + kReplicas * kMaxExperts;  // of each copy, then of the copies
+    for (int e = threadIdx.x; e < a.E; e += blockDim.x)
+        if (hist[e]) {
+            const int done = atomicAdd(&mine[e], hist[e]);
+            asm volatile("" ::"v"(done));  // wait for it: the ticket comes after every sum
+        }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int copies = gridDim.x < kReplicas ? gridDim.x : kReplicas;
+        const int blocks = (gridDim.x - copy + kReplicas - 1) / kReplicas;  // that add to this copy
+        bool all = atomicAdd(&tickets[copy], 1) == blocks - 1;
+        if (all) all = atomicAdd(&tickets[kReplicas], 1) == copies - 1;
+        *last = all;
+    }
+    __syncthreads();
+    if (!*last) return;
+    for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+        int n = 0;
+        for (int r = 0; r < kReplicas; ++r) n += atomicExch(&a.acc[r * kMaxExperts + e], 0);
+        a.count[e] = n;
+    }
+    if (threadIdx.x <= kReplicas) atomicExch(&tickets[threadIdx.x], 0);
+}
 
 // A wave per row, NPL neighbouring experts a lane: the largest value of the
 // wave is then first in index order at the first lane that holds it.
 template <int ELEM, int NPL>
 __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
     __shared__ int hist[kMaxExperts];
+    __shared__ int last;
     __shared__ float group_c[kWaves][64 * NPL];
     const int lane = lane_id(), wave = threadIdx.x >> 6;
     if (a.count) {
@@ -73,15 +137,15 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < NPL; ++i) {
-                p[i] = c[i] > neg_inf() ? (c[i] == mx ? 1.0f : expf(c[i] - mx)) : 0.0f;
+                p[i] = c[i] > neg_inf() ? (c[i] == mx ? 1.0f : fast_exp(c[i] - mx)) : 0.0f;
                 sum += p[i];
             }
-            sum = wave_sum(sum);
+            sum = 1.0f / wave_sum(sum);  // of a row without experts: not read
 #pragma unroll
-            for (int i = 0; i < NPL; ++i) p[i] = p[i] / sum;  // a row without experts is never read
+            for (int i = 0; i < NPL; ++i) p[i] *= sum;
         } else {
 #pragma unroll
-            for (int i = 0; i < NPL; ++i) p[i] = 1.0f / (1.0f + expf(-c[i]));
+            for (int i = 0; i < NPL; ++i) p[i] = fast_rcp(1.0f + fast_exp(-c[i]));
         }
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
@@ -89,54 +153,83 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
             c[i] = c[i] > neg_inf() && v > neg_inf() ? v : neg_inf();
         }
         if (a.groups > 1) {
-#pragma unroll
-            for (int i = 0; i < NPL; ++i) group_c[wave][lane * NPL + i] = c[i];
-            wave_sync();
+            // the group's value: g of lane 0..groups-1, or of every lane of it
             float t0 = neg_inf(), t1 = neg_inf();
-            if (lane < a.groups)
-                for (int i = 0; i < per; ++i) {
-                    const float v = group_c[wave][lane * per + i];
-                    t1 = fmaxf(t1, fminf(t0, v));
-                    t0 = fmaxf(t0, v);
-                }
-            wave_sync();
+            auto take = [&](float v) {
+                t1 = fmaxf(t1, fminf(t0, v));
+                t0 = fmaxf(t0, v);
+            };
+            const bool in_lanes = per % NPL == 0 && (per / NPL == 1 || per / NPL == 2 || per / NPL == 4 ||
+                                                     per / NPL == 8 || per / NPL == 16);
+            const int span = in_lanes ? per / NPL : 1;  // lanes of a group
+            auto merge = [&](float o0, float o1) {
+                t1 = fmaxf(fminf(t0, o0), fmaxf(t1, o1));
+                t0 = fmaxf(t0, o0);
+            };
+            if (in_lanes) {
+#pragma unroll
+                for (int i = 0; i < NPL; ++i) take(c[i]);
+                if (span > 1) merge(dpp<kXor1>(t0), dpp<kXor1>(t1));
+                if (span > 2) merge(dpp<kXor2>(t0), dpp<kXor2>(t1));
+                if (span > 4) merge(dpp<kHalfMirror>(t0), dpp<kHalfMirror>(t1));
+                if (span > 8) merge(dpp<kMirror>(t0), dpp<kMirror>(t1));
+            } else {
+#pragma unroll
+                for (int i = 0; i < NPL; ++i) group_c[wave][lane * NPL + i] = c[i];
+                wave_sync();
+                if (lane < a.groups)
+                    for (int i = 0; i < per; ++i) take(group_c[wave][lane * per + i]);
+                wave_sync();
+            }
             const float g = a.group_top == 2 && t1 > neg_inf() ? t0 + t1 : t0;
+            // a group stays if fewer than top_groups come before it
+            const int mine = in_lanes ? lane / span : lane;
             int rank = 0;
             for (int o = 0; o < a.groups; ++o) {
-                const float v = __shfl(g, o, 64);
-                rank += v > g || (v == g && o < lane) ? 1 : 0;
+                const float v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), o * span));
+                rank += v > g || (v == g && o < mine) ? 1 : 0;
             }
-            const uint64_t keep = __ballot(lane < a.groups && rank < a.top_groups);
+            const bool stays = rank < a.top_groups;
+            if (in_lanes) {
 #pragma unroll
-            for (int i = 0; i < NPL; ++i) {
-                const int e = lane * NPL + i;
-                if (e < a.E && !((keep >> (e / per)) & 1)) c[i] = neg_inf();
+                for (int i = 0; i < NPL; ++i)
+                    if (!stays) c[i] = neg_inf();
+            } else {
+                const uint64_t keep = __ballot(stays);
+#pragma unroll
+                for (int i = 0; i < NPL; ++i) {
+                    const int e = lane * NPL + i;
+                    if (e < a.E && !((keep >> (e / per)) & 1)) c[i] = neg_inf();
+                }
             }
         }
         int my_idx = -1;
         float my_w = 0.0f;
         for (int j = 0; j < a.k; ++j) {
-            float bv = neg_inf(), bp = 0.0f;
-            int bi = -1;
+            float bv = c[0];
 #pragma unroll
-            for (int i = 0; i < NPL; ++i)
-                if (c[i] > bv) {
-                    bv = c[i];
-                    bp = p[i];
-                    bi = lane * NPL + i;
-                }
+            for (int i = 1; i < NPL; ++i) bv = fmaxf(bv, c[i]);
             const float best = wave_max(bv);
             if (!(best > neg_inf())) break;
-            const int src = __builtin_ctzll(__ballot(bv == best));
-            const int e = __shfl(bi, src, 64);
-            const float w = __shfl(bp, src, 64);
+            const int src = __builtin_ctzll(__ballot(bv == best));  // the lowest index is in the first such lane
+            // that lane's first value equal to it leaves
+            int bi = 0;
+            float bp = 0.0f;
+            bool found = lane != src;
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) {
+                const bool hit = !found && c[i] == best;
+                bi = hit ? i : bi;
+                bp = hit ? p[i] : bp;
+                c[i] = hit ? neg_inf() : c[i];
+                found = found || hit;
+            }
+            const int e = src * NPL + __builtin_amdgcn_readlane(bi, src);
+            const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(bp), src));
             if (lane == j) {
                 my_idx = e;
                 my_w = w;
             }
-#pragma unroll
-            for (int i = 0; i < NPL; ++i)
-                if (lane * NPL + i == e) c[i] = neg_inf();
         }
         if (a.renorm) {
             const float sum = wave_sum(my_w);
@@ -148,23 +241,247 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
             if (a.count && my_idx >= 0) atomicAdd(&hist[my_idx], 1);
         }
     }
+    if (a.count) finish_counts(a, hist, &last);
+}
+
+// ---- four rows a wave -----------------------------------------------------------
+// A key orders the choice: the choice value as a double, whose low 29 bits a
+// 32-bit value leaves free, with the expert's index in them so that equal
+// values differ, the lower index above.  A maximum is then one instruction with
+// no second value to carry.
+constexpr double kNoKey = -1e300;  // not choosable
+__device__ __forceinline__ double make_key(float c, int e) {
+    // an infinite value goes as the largest finite one
+    const double d = (double)__builtin_amdgcn_fmed3f(c, -3.402823466e38f, 3.402823466e38f);
+    int hi = __double2hiint(d), lo = __double2loint(d);
+    lo |= (255 - e) ^ (hi >> 31 & 255);
+    const bool ok = c > neg_inf();
+    hi = ok ? hi : __double2hiint(kNoKey);
+    lo = ok ? lo : __double2loint(kNoKey);
+    return __hiloint2double(hi, lo);
+}
+__device__ __forceinline__ int key_expert(double key) {
+    return 255 - ((__double2loint(key) ^ __double2hiint(key) >> 31) & 255);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+    const int lo = __double2loint(v), hi = __double2hiint(v);
+    return __hiloint2double(__builtin_amdgcn_update_dpp(hi, hi, CTRL, 0xf, 0xf, false),
+                            __builtin_amdgcn_update_dpp(lo, lo, CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ double row16_max(double v) {
+    v = __builtin_fmax(v, dpp64<kXor1>(v));
+    v = __builtin_fmax(v, dpp64<kXor2>(v));
+    v = __builtin_fmax(v, dpp64<kHalfMirror>(v));
+    return __builtin_fmax(v, dpp64<kMirror>(v));
+}
+__device__ __forceinline__ float row16_maxf(float v) {
+    v = fmaxf(v, dpp<kXor1>(v));
+    v = fmaxf(v, dpp<kXor2>(v));
+    v = fmaxf(v, dpp<kHalfMirror>(v));
+    return fmaxf(v, dpp<kMirror>(v));
+}
+__device__ __forceinline__ float row16_sum(float v) {
+    v += dpp<kXor1>(v);
+    v += dpp<kXor2>(v);
+    v += dpp<kHalfMirror>(v);
+    return v + dpp<kMirror>(v);
+}
+
+// Sixteen lanes per row, NPL neighbouring experts a lane: each lane sorts its
+// keys once and gives up its first whenever that is the row's largest, so a
+// choice costs a maximum over 16 lanes and a shift, for four rows at a time.
+// Bound by these instructions: 65536 rows of 256 experts, 8 chosen of 4 groups
+// of 8, 38 us (floor by bytes 7); a wave per row with a search for every choice took
+// 80.  At most
+// kPop choices, and groups that are whole lanes.
+constexpr int kPop = 8;
+template <int ELEM, int NPL>
+__global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec) {
+    __shared__ int hist[256];
+    __shared__ int last;
+    const int lane = lane_id() & 15;
+    const int rows = blockDim.x / 16;
     if (a.count) {
+        for (int e = threadIdx.x; e < a.E; e += blockDim.x) hist[e] = 0;
         __syncthreads();
-        for (int e = threadIdx.x; e < a.E; e += kThreads) {
-            if (gridDim.x == 1)
-                a.count[e] = hist[e];
-            else if (hist[e])
-                atomicAdd(&a.count[e], hist[e]);
+    }
+    float bias[NPL];
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+        const int e = lane * NPL + i;
+        bias[i] = a.bias && e < a.E ? a.bias[e] : 0.0f;
+    }
+    const int64_t groups_of_rows = (a.M + rows - 1) / rows;
+    for (int64_t b = blockIdx.x; b < groups_of_rows; b += gridDim.x) {
+        const int64_t m = b * rows + threadIdx.x / 16;
+        const bool row = m < a.M && (!a.row_mask || a.row_mask[m] != 0);
+        float l[NPL];
+        if (row && vec && (lane + 1) * NPL <= a.E) {
+            if constexpr (ELEM == VDTTFS_ELEM_F32) {
+                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.logits) + m * a.ld) +
+                                  lane * (NPL / 4);
+#pragma unroll
+                for (int i = 0; i < NPL / 4; ++i) {
+                    const float4 v = p[i];
+                    l[4 * i] = v.x, l[4 * i + 1] = v.y, l[4 * i + 2] = v.z, l[4 * i + 3] = v.w;
+                }
+            } else {
+                const uint2* p = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.logits) + m * a.ld) +
+                                 lane * (NPL / 4);
+#pragma unroll
+                for (int i = 0; i < NPL / 4; ++i) {
+                    const uint2 v = p[i];
+                    const uint16_t h[4] = {(uint16_t)v.x, (uint16_t)(v.x >> 16), (uint16_t)v.y, (uint16_t)(v.y >> 16)};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        l[4 * i + q] = ELEM == VDTTFS_ELEM_BF16 ? bf16_to_f32(h[q]) : f16_to_f32(h[q]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) {
+                const int e = lane * NPL + i;
+                l[i] = row && e < a.E ? load_elem<ELEM>(a.logits, m * a.ld + e) : neg_inf();
+            }
+        }
+        float mx = neg_inf(), inv = 1.0f;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) {
+            l[i] = l[i] > neg_inf() ? l[i] : neg_inf();  // NaN: not choosable
+            mx = fmaxf(mx, l[i]);
+        }
+        float c[NPL];
+        if (a.score == VDTTFS_SCORE_SOFTMAX) {
+            mx = row16_maxf(mx);
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) {
+                const float x = fast_exp(l[i] - mx);
+                c[i] = l[i] == mx ? 1.0f : x;  // an infinity less itself is none
+                c[i] = l[i] > neg_inf() ? c[i] : 0.0f;
+                sum += c[i];
+            }
+            inv = 1.0f / row16_sum(sum);  // of a row without experts: not used
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) c[i] *= inv;
+        } else {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) c[i] = fast_rcp(1.0f + fast_exp(-l[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) {
+            const float v = c[i] + bias[i];
+            c[i] = l[i] > neg_inf() && v > neg_inf() ? v : neg_inf();
+        }
+        if (a.groups > 1) {
+            float t0 = neg_inf(), t1 = neg_inf();
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) {
+                t1 = fmaxf(t1, fminf(t0, c[i]));
+                t0 = fmaxf(t0, c[i]);
+            }
+            auto merge = [&](float o0, float o1) {
+                t1 = fmaxf(fminf(t0, o0), fmaxf(t1, o1));
+                t0 = fmaxf(t0, o0);
+            };
+            if (span > 1) merge(dpp<kXor1>(t0), dpp<kXor1>(t1));
+            if (span > 2) merge(dpp<kXor2>(t0), dpp<kXor2>(t1));
+            if (span > 4) merge(dpp<kHalfMirror>(t0), dpp<kHalfMirror>(t1));
+            if (span > 8) merge(dpp<kMirror>(t0), dpp<kMirror>(t1));
+            const float g = a.group_top == 2 && t1 > neg_inf() ? t0 + t1 : t0;
+            const int mine = lane / span;
+            int rank = 0;  // a group stays if fewer than top_groups come before it
+            for (int o = 0; o < a.groups; ++o) {
+                const float v = __shfl(g, o * span, 16);
+                rank += v > g || (v == g && o < mine) ? 1 : 0;
+            }
+            if (rank >= a.top_groups) {
+#pragma unroll
+                for (int i = 0; i < NPL; ++i) c[i] = neg_inf();
+            }
+        }
+        double key[NPL];
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) key[i] = make_key(c[i], lane * NPL + i);
+        // descending, by Batcher's odd-even merges (K. E. Batcher, "Sorting
+        // networks and their applications", 1968)
+#pragma unroll
+        for (int p = 1; p < NPL; p *= 2)
+#pragma unroll
+            for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+                for (int j = q % p; j + q < NPL; j += 2 * q)
+#pragma unroll
+                    for (int i = 0; i < q; ++i)
+                        if (i + j + q < NPL && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                            const double x = key[i + j], y = key[i + j + q];
+                            key[i + j] = __builtin_fmax(x, y);
+                            key[i + j + q] = __builtin_fmin(x, y);
+                        }
+        double mine = kNoKey;
+#pragma unroll
+        for (int j = 0; j < kPop; ++j) {
+            if (j < a.k) {
+                const double best = row16_max(key[0]);
+                const bool win = key[0] == best;  // one lane, but where nothing is left
+#pragma unroll
+                for (int i = 0; i + 1 < NPL && i + 1 < kPop - j; ++i) {
+                    const double up = key[i + 1], stay = key[i];
+                    key[i] = win ? up : stay;
+                }
+                if (NPL < kPop - j) {
+                    const double stay = key[NPL - 1];
+                    key[NPL - 1] = win ? kNoKey : stay;
+                }
+                mine = lane == j ? best : mine;
+            }
+        }
+        int e = -1;
+        float w = 0.0f;
+        if (mine > kNoKey) {
+            e = key_expert(mine);
+            const float v = load_elem<ELEM>(a.logits, m * a.ld + e);
+            w = a.score != VDTTFS_SCORE_SOFTMAX ? fast_rcp(1.0f + fast_exp(-v))
+                                                : (v == mx ? 1.0f : fast_exp(v - mx)) * inv;
+        }
+        if (a.renorm) {
+            const float sum = row16_sum(w);
+            w = sum > 0.0f ? w / sum : 0.0f;
+        }
+        if (m < a.M && lane < a.k) {
+            a.idx[m * a.k + lane] = e;
+            a.wt[m * a.k + lane] = w * a.scale;
+            if (a.count && e >= 0) atomicAdd(&hist[e], 1);
         }
     }
+    if (a.count) finish_counts(a, hist, &last);
 }
 
 __global__ void k_zero(int* p, int n) {
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) p[i] = 0;
 }
 
+// Four rows a wave where it can: up to 256 experts, 8 slots, and groups that
+// are a power of two of its lanes; else a wave per row.
 template <int ELEM>
-void route_npl(vdttfs_ctx* ctx, const RouteArgs& a, dim3 grid) {
+void route_elem(vdttfs_ctx* ctx, const RouteArgs& a) {
+    const int size = ELEM == VDTTFS_ELEM_F32 ? 4 : 2;
+    const int npl = a.E <= 64 ? 4 : a.E <= 128 ? 8 : 16, per = a.E / a.groups;
+    const int span = a.groups == 1 ? 16 : per % npl ? 0 : per / npl;
+    if (a.E <= 256 && a.k <= kPop && (span == 1 || span == 2 || span == 4 || span == 8 || span == 16)) {
+        // one workgroup a CU at most, of 16 waves where there are rows for them
+        const int threads = a.M > 4096 ? 1024 : kThreads;
+        const int64_t blocks = (a.M + threads / 16 - 1) / (threads / 16);
+        const dim3 grid((unsigned)(blocks < 256 ? blocks : 256));
+        const int vec = (((uintptr_t)a.logits | (uintptr_t)(a.ld * size)) & (4 * size - 1)) == 0;
+        if (npl == 4) k_route16<ELEM, 4><<<grid, threads, 0, ctx->stream>>>(a, span, vec);
+        else if (npl == 8) k_route16<ELEM, 8><<<grid, threads, 0, ctx->stream>>>(a, span, vec);
+        else k_route16<ELEM, 16><<<grid, threads, 0, ctx->stream>>>(a, span, vec);
+        return;
+    }
+    const int64_t blocks = (a.M + kWaves - 1) / kWaves;
+    const dim3 grid((unsigned)(blocks < 1024 ? blocks : 1024));
     if (a.E <= 64) k_route<ELEM, 1><<<grid, kThreads, 0, ctx->stream>>>(a);
     else if (a.E <= 128) k_route<ELEM, 2><<<grid, kThreads, 0, ctx->stream>>>(a);
     else if (a.E <= 256) k_route<ELEM, 4><<<grid, kThreads, 0, ctx->stream>>>(a);
@@ -270,20 +587,20 @@ __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, in
 
 }  // namespace
 
+size_t route_acc_bytes() { return (size_t)(kReplicas * kMaxExperts + kReplicas + 1) * 4; }
+
 int launch_route(vdttfs_ctx* ctx, int32_t* idx, float* wt, int32_t* count, const void* logits, int elem, int64_t ld,
-                 const float* bias, const uint8_t* row_mask, int64_t M, const vdttfs_route_opts& o) {
-    const int64_t blocks = (M + kWaves - 1) / kWaves;
-    const dim3 grid((unsigned)(blocks < 2048 ? blocks : 2048));
-    if (count && (M <= 0 || grid.x > 1)) {
-        k_zero<<<dim3(1), kThreads, 0, ctx->stream>>>(count, o.n_experts);
+                 const float* bias, const uint8_t* row_mask, int64_t M, const vdttfs_route_opts& o, int* acc) {
+    if (M <= 0) {
+        if (count) k_zero<<<dim3(1), kThreads, 0, ctx->stream>>>(count, o.n_experts);
         VD_HIP(hipGetLastError());
+        return VDTTFS_OK;
     }
-    if (M <= 0) return VDTTFS_OK;
-    const RouteArgs a{idx,           wt,      count,    logits,       ld,           bias,     row_mask, M,
-                      o.n_experts,   o.top_k, o.score,  o.groups,     o.top_groups, o.group_top, o.renorm, o.scale};
-    if (elem == VDTTFS_ELEM_F32) route_npl<VDTTFS_ELEM_F32>(ctx, a, grid);
-    else if (elem == VDTTFS_ELEM_BF16) route_npl<VDTTFS_ELEM_BF16>(ctx, a, grid);
-    else route_npl<VDTTFS_ELEM_F16>(ctx, a, grid);
+    const RouteArgs a{idx,         wt,      count,   logits,   ld,           bias,        row_mask, M,
+                      o.n_experts, o.top_k, o.score, o.groups, o.top_groups, o.group_top, o.renorm, o.scale, acc};
+    if (elem == VDTTFS_ELEM_F32) route_elem<VDTTFS_ELEM_F32>(ctx, a);
+    else if (elem == VDTTFS_ELEM_BF16) route_elem<VDTTFS_ELEM_BF16>(ctx, a);
+    else route_elem<VDTTFS_ELEM_F16>(ctx, a);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
