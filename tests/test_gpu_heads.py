@@ -490,7 +490,7 @@ def test_calls_can_be_captured_once_they_have_run(gpu_ctx_factory):
 
 def test_scratch_does_not_grow_under_capture(gpu_ctx_factory):
     c = gpu_ctx_factory(vdttfs.TaskConsts(T=64, delta=16))
-    x, w = c.to_device(np.ones((100, 500), np.float32)), c.empty((30, 500), np.int8).fill(1)
+    x, w = c.to_device(np.ones((100, 5000), np.float32)), c.empty((30, 5000), np.int8).fill(1)
     sc, out, n = c.to_device(np.ones(30, np.float32)), c.empty((100, 30), np.float32), c.empty(4, np.int32)
     logits, small = c.to_device(np.ones((3, 4), np.float32)), c.empty((3, 2), np.int32)
     wt = c.empty((3, 2), np.float32)
@@ -498,7 +498,7 @@ def test_scratch_does_not_grow_under_capture(gpu_ctx_factory):
 
     def call():
         with pytest.raises(vdttfs.VdttfsError) as e:
-            c.i8_linear(out, R.F32, 30, x, R.F32, 500, w, 500, sc, None, R.NONE, 100, 30, 500)
+            c.i8_linear(out, R.F32, 30, x, R.F32, 5000, w, 5000, sc, None, R.NONE, 100, 30, 5000)
         seen.append(e.value.code)
         c.route(small, wt, n, logits, R.F32, 4, None, None, 3, 4, 2)  # the capture goes on
 

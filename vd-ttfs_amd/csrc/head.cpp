@@ -181,8 +181,9 @@ int vdttfs_i8_matmul(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, co
     if (K > 0 && !d_q) return bad("i8_matmul", "null buffer");
     VD_TRY(check_float_ptr("i8_matmul", d_row_scale, 4));
     VD_TRY(check_product("i8_matmul", d_w, ldw, d_ch_scale, d_bias, act, K));
-    return launch_i8_dense(ctx, product(d_q, ldq, d_row_scale, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M,
-                                        N, K, act));
+    const I8Args a = product(d_q, ldq, d_row_scale, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M, N, K, act);
+    if (small_ok(M, N, K, kElemCodes) && !getenv("VD_NOSMALL")) return launch_i8_small(ctx, d_q, kElemCodes, ldq, d_row_scale, a);
+    return launch_i8_dense(ctx, a);
 }
 
 int vdttfs_i8_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const void* d_x, int x_elem,
@@ -194,6 +195,10 @@ int vdttfs_i8_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, co
     VD_TRY(check_out("i8_linear", d_out, out_elem, ldo, N));
     VD_TRY(check_in("i8_linear", d_x, x_elem, ldx, M, K));
     VD_TRY(check_product("i8_linear", d_w, ldw, d_ch_scale, d_bias, act, K));
+    if (small_ok(M, N, K, x_elem) && !getenv("VD_NOSMALL"))
+        return launch_i8_small(ctx, d_x, x_elem, ldx, nullptr,
+                               product(nullptr, 0, nullptr, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M, N,
+                                       K, act));
     const int64_t ldq = padded(K);
     Layout l;
     const size_t at_q = l.take((size_t)M * ldq), at_s = l.take((size_t)M * 4);
@@ -202,7 +207,9 @@ int vdttfs_i8_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, co
     int8_t* q = reinterpret_cast<int8_t*>(buf + at_q);
     float* s = reinterpret_cast<float*>(buf + at_s);
     VD_TRY(launch_quant_rows(ctx, d_x, x_elem, ldx, M, K, q, ldq, (int)ldq, s));
-    return launch_i8_dense(ctx, product(q, ldq, s, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M, N, K, act));
+    const I8Args a = product(q, ldq, s, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M, N, K, act);
+    if (small_ok(M, N, K, kElemCodes) && M <= 16) return launch_i8_small(ctx, q, kElemCodes, ldq, s, a);
+    return launch_i8_dense(ctx, a);
 }
 
 int vdttfs_route(vdttfs_ctx* ctx, int32_t* d_idx, float* d_weight, int32_t* d_count, const void* d_logits, int elem,

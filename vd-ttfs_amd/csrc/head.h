@@ -39,6 +39,11 @@ int launch_quant_kernel(vdttfs_ctx* ctx, const float* kernel, int c_in, int c_ou
                         float* scale);
 // bm: rows of a tile of a grouped product (i8_tile_rows of the same call)
 int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a);
+// The product of few rows (a.A and a.lda unused), quantised in the kernel from
+// elem, or codes with scales sa where elem is kElemCodes.
+constexpr int kElemCodes = 4;
+bool small_ok(int64_t M, int N, int K, int elem);
+int launch_i8_small(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const I8Args& a);
 int launch_i8_grouped(vdttfs_ctx* ctx, const I8Args& a, bool gated, int bm);
 int i8_tile_rows(int64_t pairs, int n_experts);
 

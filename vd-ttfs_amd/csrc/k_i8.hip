@@ -4,31 +4,13 @@
 // sum in 32-bit integers (v_mfma_i32_16x16x64_i8), so no order of k matters.
 #include <type_traits>
 
+#include "codes.h"
 #include "elem.h"
 #include "head.h"
 #include "wave.h"
 
 namespace vdttfs {
 namespace {
-
-typedef int v4i __attribute__((ext_vector_type(4)));
-struct __attribute__((packed, aligned(1))) Bytes16 {
-    v4i v;
-};
-
-// 16 codes at p, of which the first `valid` exist; the others are 0.  p may
-// have any alignment (gfx950 loads 16 bytes from any address).
-__device__ __forceinline__ v4i load16(const int8_t* p, int valid) {
-    if (valid >= 16) return reinterpret_cast<const Bytes16*>(p)->v;
-    uint64_t lo = 0, hi = 0;
-#pragma unroll 1
-    for (int i = 0; i < valid; ++i) {
-        const uint64_t b = (uint64_t)(uint8_t)p[i] << (8 * (i & 7));
-        if (i < 8) lo |= b;
-        else hi |= b;
-    }
-    return v4i{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
-}
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 
@@ -208,11 +190,17 @@ __global__ __launch_bounds__(WM* WN * 64) void k_i8_tile(I8Args p, int tiles_n) 
 
     v4i ra[NA], rb[NB];
     auto fetch = [&](int k0) {
-        const int valid = p.K - k0 - chunk;
+        if (k0 + kBK <= p.K) {
 #pragma unroll
-        for (int i = 0; i < NA; ++i) ra[i] = load16(pa[i] + k0 + chunk, valid);
+            for (int i = 0; i < NA; ++i) ra[i] = reinterpret_cast<const Bytes16*>(pa[i] + k0 + chunk)->v;
 #pragma unroll
-        for (int i = 0; i < NB; ++i) rb[i] = load16(pb[i] + k0 + chunk, valid);
+            for (int i = 0; i < NB; ++i) rb[i] = reinterpret_cast<const Bytes16*>(pb[i] + k0 + chunk)->v;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < NA; ++i) ra[i] = load16(pa[i], k0 + chunk, p.K);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) rb[i] = load16(pb[i], k0 + chunk, p.K);
     };
     fetch(0);
     for (int k0 = 0; k0 < p.K; k0 += kBK) {
@@ -437,14 +425,15 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
         if (S > 3 && t + 2 < tiles) multiply(std::false_type{}, s2, s2, 0);
     }
     if (tiles * BK < p.K) {
-        const int valid = p.K - tiles * BK - chunk;
+        v4i end[NL];
+#pragma unroll
+        for (int l = 0; l < NL; ++l)
+            end[l] = load16((l < NA ? a_row(l) : b_row(l - NA)) - chunk, tiles * BK + chunk, p.K);
         __syncthreads();
-#pragma unroll 1
-        for (int i = 0; i < NL; ++i) {
-            const int8_t* from = i < NA ? a_row(i) : b_row(i - NA);
-            int8_t* to = s0 + (i < NA ? wave * NA + i : BM / kRows + wave * NB + i - NA) * 1024 + lane * 16;
-            *reinterpret_cast<v4i*>(to) = load16(from + tiles * BK, valid);
-        }
+#pragma unroll
+        for (int l = 0; l < NL; ++l)
+            *reinterpret_cast<v4i*>(s0 + (l < NA ? wave * NA + l : BM / kRows + wave * NB + l - NA) * 1024 +
+                                    lane * 16) = end[l];
         __syncthreads();
         multiply(std::false_type{}, s0, s0, 0);
     }

@@ -2,32 +2,17 @@
 // the weights blob's FC kernels to the products' layout.
 #include "elem.h"
 #include "head.h"
-#include "wave.h"
+#include "quant.h"
 
 namespace vdttfs {
 namespace {
 
 constexpr int kThreads = 256;
 
-// The code of x under scale s (s finite): the IEEE quotient rounded half to
-// even.  s == 0 is a row of zeros, or one whose largest value / 127 underflows.
-__device__ __forceinline__ int code_of(float x, float s) {
-    if (s == 0.0f) return 0;
-    return (int)fminf(fmaxf(rintf(x / s), -127.0f), 127.0f);
-}
-
-// max of two values >= 0 or NaN; a NaN wins.
-__device__ __forceinline__ float nan_max(float a, float b) { return (a >= b || a != a) ? a : b; }
-
-__device__ __forceinline__ float scale_of(float amax) {
-    return amax < __builtin_inff() ? amax / 127.0f : __builtin_nanf("");
-}
-
 // The largest magnitude over WAVES waves (all of the workgroup, or one).
 template <int WAVES>
 __device__ __forceinline__ float row_max(float v, float* lds) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = nan_max(v, __shfl_xor(v, off, 64));
+    v = wave_nan_max(v);
     if constexpr (WAVES > 1) {
         if (lane_id() == 0) lds[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -39,37 +24,10 @@ __device__ __forceinline__ float row_max(float v, float* lds) {
     return v;
 }
 
-// Eight neighbouring values from column c of a row, 0 past its end.  vec: rows
-// start on 16 bytes.
-template <int ELEM>
-__device__ __forceinline__ void load8(const void* x, int64_t row, int c, int cols, bool vec, float (&f)[8]) {
-    if (vec && c + 8 <= cols) {
-        if constexpr (ELEM == VDTTFS_ELEM_F32) {
-            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + row + c);
-            const float4 a = p[0], b = p[1];
-            f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-        } else {
-            const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + row + c);
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint16_t h = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-                f[i] = ELEM == VDTTFS_ELEM_BF16 ? bf16_to_f32(h) : f16_to_f32(h);
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = c + i < cols ? load_elem<ELEM>(x, row + c + i) : 0.0f;
-}
-
 // Eight codes at column c; columns past `end` are not there.
 __device__ __forceinline__ void store8(int8_t* q, int64_t row, int c, int end, bool vec, const int (&k)[8]) {
     if (vec && c + 8 <= end) {
-        uint2 w;
-        w.x = (k[0] & 255) | (k[1] & 255) << 8 | (k[2] & 255) << 16 | k[3] << 24;
-        w.y = (k[4] & 255) | (k[5] & 255) << 8 | (k[6] & 255) << 16 | k[7] << 24;
-        *reinterpret_cast<uint2*>(q + row + c) = w;
+        *reinterpret_cast<uint2*>(q + row + c) = pack8(k);
         return;
     }
 #pragma unroll
@@ -78,33 +36,40 @@ __device__ __forceinline__ void store8(int8_t* q, int64_t row, int c, int end, b
 }
 
 // WAVES waves hold a row in registers, eight values a lane and turn (NV turns),
-// so it is read once: its largest magnitude, then its codes.  Bound by memory;
-// the IEEE quotients overlap it.
+// so it is read once: its largest magnitude, then its codes.  Bound by memory.
 template <int ELEM, int NV, int WAVES>
 __global__ __launch_bounds__(kThreads) void k_quant_rows(const void* __restrict__ x, int64_t ldx, int64_t rows,
                                                          int cols, int8_t* __restrict__ q, int64_t ldq,
-                                                         int cols_zero, float* __restrict__ scale, int vec_in,
-                                                         int vec_out) {
+                                                         int cols_zero, float* __restrict__ scale, int vec_out) {
     __shared__ float lds[kThreads / 64];
     constexpr int kRows = kThreads / 64 / WAVES, kLanes = WAVES * 64;
     const int lane = threadIdx.x % kLanes;
     for (int64_t m = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; m < rows; m += (int64_t)gridDim.x * kRows) {
-        float f[NV][8];
-        float a = 0.0f;
+        Raw8<ELEM> raw[NV];
+        float f[NV][8], a = 0.0f;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) load8<ELEM>(x, m * ldx, (v * kLanes + lane) * 8, cols, vec_in, f[v]);
+        for (int v = 0; v < NV; ++v) {
+            const int c = (v * kLanes + lane) * 8;
+            raw[v] = nothing8<ELEM>();
+            if (c + 8 <= cols) raw[v] = raw8<ELEM>(x, m * ldx + c);
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = (v * kLanes + lane) * 8;
+            unpack8<ELEM>(raw[v], f[v]);
+            if (c < cols && c + 8 > cols) tail8<ELEM>(x, m * ldx, c, cols, f[v]);
+        }
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < 8; ++i) a = nan_max(a, fabsf(f[v][i]));
         const float s = scale_of(row_max<WAVES>(a, lds));
         if (lane == 0) scale[m] = s;
-        const bool ok = s == s;
+        const Coder coder = coder_of(s);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             int k[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) k[i] = ok ? code_of(f[v][i], s) : 0;
+            codes8(f[v], coder, k);
             store8(q, m * ldq, (v * kLanes + lane) * 8, cols_zero, vec_out, k);
         }
     }
@@ -114,42 +79,45 @@ __global__ __launch_bounds__(kThreads) void k_quant_rows(const void* __restrict_
 template <int ELEM>
 __global__ __launch_bounds__(kThreads) void k_quant_long(const void* __restrict__ x, int64_t ldx, int64_t rows,
                                                          int cols, int8_t* __restrict__ q, int64_t ldq,
-                                                         int cols_zero, float* __restrict__ scale, int vec_in,
-                                                         int vec_out) {
+                                                         int cols_zero, float* __restrict__ scale, int vec_out) {
     __shared__ float lds[kThreads / 64];
     for (int64_t m = blockIdx.x; m < rows; m += gridDim.x) {
         float a = 0.0f;
         for (int c = threadIdx.x * 8; c < cols; c += kThreads * 8) {
             float f[8];
-            load8<ELEM>(x, m * ldx, c, cols, vec_in, f);
+            load8<ELEM>(x, m * ldx, c, cols, f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) a = nan_max(a, fabsf(f[i]));
         }
         const float s = scale_of(row_max<kThreads / 64>(a, lds));
         if (threadIdx.x == 0) scale[m] = s;
-        const bool ok = s == s;
+        const Coder coder = coder_of(s);
         for (int c = threadIdx.x * 8; c < cols_zero; c += kThreads * 8) {
             float f[8];
             int k[8];
-            load8<ELEM>(x, m * ldx, c, cols, vec_in, f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) k[i] = ok ? code_of(f[i], s) : 0;
+            load8<ELEM>(x, m * ldx, c, cols, f);
+            codes8(f, coder, k);
             store8(q, m * ldq, c, cols_zero, vec_out, k);
         }
     }
 }
 
-// Spike times: the scale is the same for every row.
+// Spike times: eight a thread; the scale is the same for every row.
 __global__ __launch_bounds__(kThreads) void k_quant_times(const float* __restrict__ x, int64_t ldx, int64_t rows,
                                                           int cols, int8_t* __restrict__ q, int64_t ldq,
-                                                          int cols_zero, float* __restrict__ scale, float tfs, int T) {
-    const int L = T < 127 ? T : 127;
-    for (int64_t m = blockIdx.x; m < rows; m += gridDim.x) {
-        if (threadIdx.x == 0) scale[m] = 1.0f / (float)L;
-        for (int i = threadIdx.x; i < cols_zero; i += kThreads) {
-            const int b = i < cols ? arrival_bin(x[m * ldx + i], tfs, T) : -1;
-            q[m * ldq + i] = b < 0 ? (int8_t)0 : (int8_t)(int)rintf((float)((T - b) * L) / (float)T);
-        }
+                                                          int cols_zero, float* __restrict__ scale, float tfs, int T,
+                                                          int vec_out) {
+    const int levels = T < 127 ? T : 127, per = cols_zero > 0 ? (cols_zero + 7) / 8 : 1;
+    for (int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x; at < rows * per; at += (int64_t)gridDim.x * kThreads) {
+        const int64_t m = at / per;
+        const int c = (int)(at - m * per) * 8;
+        float f[8];
+        int k[8];
+        load8<VDTTFS_ELEM_TIMES>(x, m * ldx, c, cols, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k[i] = time_code(f[i], tfs, T, levels);
+        store8(q, m * ldq, c, cols_zero, vec_out, k);
+        if (c == 0) scale[m] = 1.0f / (float)levels;
     }
 }
 
@@ -172,7 +140,7 @@ __global__ __launch_bounds__(1024) void k_quant_kernel(const float* __restrict__
     const float s = scale_of(a);
     if (part == 0) scale[n] = s;
     for (int k = part; k < c_in; k += 16)
-        q[(int64_t)n * ldq + k] = s == s ? (int8_t)code_of(w[(int64_t)k * c_out + n], s) : (int8_t)0;
+        q[(int64_t)n * ldq + k] = s > 0.0f ? (int8_t)exact_code(w[(int64_t)k * c_out + n], s) : (int8_t)0;
 }
 
 }  // namespace
@@ -181,11 +149,11 @@ namespace {
 
 template <int ELEM, int NV, int WAVES>
 void quant_nv(vdttfs_ctx* ctx, const void* x, int64_t ldx, int64_t rows, int cols, int8_t* q, int64_t ldq,
-              int cols_zero, float* scale, int vi, int vo) {
+              int cols_zero, float* scale, int vo) {
     constexpr int kRows = kThreads / 64 / WAVES;
     const int64_t blocks = (rows + kRows - 1) / kRows;
     k_quant_rows<ELEM, NV, WAVES><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), kThreads, 0, ctx->stream>>>(
-        x, ldx, rows, cols, q, ldq, cols_zero, scale, vi, vo);
+        x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
 }
 
 // A wave per row up to 2048 columns where there are rows for every SIMD, else
@@ -193,20 +161,18 @@ void quant_nv(vdttfs_ctx* ctx, const void* x, int64_t ldx, int64_t rows, int col
 template <int ELEM>
 void quant_elem(vdttfs_ctx* ctx, const void* x, int64_t ldx, int64_t rows, int cols, int8_t* q, int64_t ldq,
                 int cols_zero, float* scale) {
-    const int size = ELEM == VDTTFS_ELEM_F32 ? 4 : 2;
-    const int vi = (((uintptr_t)x | (uintptr_t)(ldx * size)) & 15) == 0;
     const int vo = (((uintptr_t)q | (uintptr_t)ldq) & 7) == 0;
-    if (cols_zero <= 512) quant_nv<ELEM, 1, 1>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vi, vo);
+    if (cols_zero <= 512) quant_nv<ELEM, 1, 1>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
     else if (cols_zero <= 1024 && rows >= 1024)
-        quant_nv<ELEM, 2, 1>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vi, vo);
+        quant_nv<ELEM, 2, 1>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
     else if (cols_zero <= 2048 && rows >= 1024)
-        quant_nv<ELEM, 4, 1>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vi, vo);
-    else if (cols_zero <= 2048) quant_nv<ELEM, 1, 4>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vi, vo);
-    else if (cols_zero <= 4096) quant_nv<ELEM, 2, 4>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vi, vo);
-    else if (cols_zero <= 8192) quant_nv<ELEM, 4, 4>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vi, vo);
+        quant_nv<ELEM, 4, 1>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
+    else if (cols_zero <= 2048) quant_nv<ELEM, 1, 4>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
+    else if (cols_zero <= 4096) quant_nv<ELEM, 2, 4>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
+    else if (cols_zero <= 8192) quant_nv<ELEM, 4, 4>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
     else
         k_quant_long<ELEM><<<dim3((unsigned)(rows < 65536 ? rows : 65536)), kThreads, 0, ctx->stream>>>(
-            x, ldx, rows, cols, q, ldq, cols_zero, scale, vi, vo);
+            x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
 }
 
 }  // namespace
@@ -217,9 +183,12 @@ int launch_quant_rows(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int
     if (elem == VDTTFS_ELEM_F32) quant_elem<VDTTFS_ELEM_F32>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale);
     else if (elem == VDTTFS_ELEM_BF16) quant_elem<VDTTFS_ELEM_BF16>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale);
     else if (elem == VDTTFS_ELEM_F16) quant_elem<VDTTFS_ELEM_F16>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale);
-    else
-        k_quant_times<<<dim3((unsigned)(rows < 65536 ? rows : 65536)), kThreads, 0, ctx->stream>>>(
-            static_cast<const float*>(x), ldx, rows, cols, q, ldq, cols_zero, scale, ctx->c.tfs, ctx->c.T);
+    else {
+        const int64_t blocks = (rows * (cols_zero > 0 ? (cols_zero + 7) / 8 : 1) + kThreads - 1) / kThreads;
+        k_quant_times<<<dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), kThreads, 0, ctx->stream>>>(
+            static_cast<const float*>(x), ldx, rows, cols, q, ldq, cols_zero, scale, ctx->c.tfs, ctx->c.T,
+            (((uintptr_t)q | (uintptr_t)ldq) & 7) == 0);
+    }
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }

@@ -292,9 +292,8 @@ __device__ __forceinline__ float row16_sum(float v) {
 // keys once and gives up its first whenever that is the row's largest, so a
 // choice costs a maximum over 16 lanes and a shift, for four rows at a time.
 // Bound by these instructions: 65536 rows of 256 experts, 8 chosen of 4 groups
-// of 8, 38 us (floor by bytes 7); a wave per row with a search for every choice took
-// 80.  At most
-// kPop choices, and groups that are whole lanes.
+// of 8, take 38 us (7 by their bytes), and 80 with a wave per row and a search
+// for every choice.  At most kPop choices, and groups that are whole lanes.
 constexpr int kPop = 8;
 template <int ELEM, int NPL>
 __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec) {

@@ -1,0 +1,322 @@
+// Products of few rows: the weights stream once from memory into the matrix
+// instructions, and the rows are quantised inside the kernel, so a call is one
+// launch (experts: two, and their sum).
+#include "codes.h"
+#include "head.h"
+#include "quant.h"
+
+namespace vdttfs {
+namespace {
+
+constexpr int kCodes = kElemCodes;  // rows that are codes already
+constexpr int kWaves = 8, kThreads = kWaves * 64;
+constexpr int kAhead = 8;  // weight loads a wave has in flight
+constexpr int kRows = 16;
+
+// Who turns which values into codes: 2^lanes_log threads share a row, each
+// with `turns` runs of eight of it, and the workgroup takes as many rows at a
+// time as it has such teams.  All of it in kUnits runs a thread, or none.
+struct Share {
+    int lanes_log, turns, passes;
+};
+constexpr int kUnits = 2;
+Share share_of(int rows, int K) {
+    const int per = (K + 63) / 64 * 8;  // runs of a row, a multiple of eight
+    int log = 3;
+    while (log < 9 && (1 << log) < per) ++log;
+    const int teams = kThreads >> log;
+    return Share{log, (per + (1 << log) - 1) >> log, (rows + teams - 1) / teams};
+}
+
+// The workgroup turns rows into codes in LDS, `stride` bytes apart (zeros from
+// K to the next 64), and their scales.  Every value is loaded once, all loads
+// at once; a row's largest magnitude is a maximum over LDS of its bits (those
+// of a NaN are above infinity's, and no order of maxima matters).  row(r):
+// where row r starts in x.  Ends with a barrier.
+template <int ELEM, typename RowAt>
+__device__ __forceinline__ void rows_to_lds(const void* x, RowAt row, int rows, int K, Share sh, float tfs, int T,
+                                            int8_t* to, int stride, float* scale, int* peak) {
+    const int end = (K + 63) & ~63;
+    if constexpr (ELEM == kCodes) {
+        const int total = rows * (end / 16);
+        for (int u = threadIdx.x; u < total; u += kThreads) {
+            const int r = u / (end / 16), c = u % (end / 16) * 16;
+            *reinterpret_cast<v4i*>(to + r * stride + c) = load16(static_cast<const int8_t*>(x) + row(r), c, K);
+        }
+        __syncthreads();
+    } else {
+        const int teams = kThreads >> sh.lanes_log, units = sh.passes * sh.turns;
+        // run i of this thread: row r[i], column c[i]
+        int r[kUnits], c[kUnits];
+        {
+            const int c0 = (threadIdx.x & ((1 << sh.lanes_log) - 1)) * 8, cstep = 8 << sh.lanes_log;
+            int row_i = threadIdx.x >> sh.lanes_log, turn = 0;
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                r[i] = row_i;
+                c[i] = c0 + turn * cstep;
+                const bool wrap = ++turn == sh.turns;
+                turn = wrap ? 0 : turn;
+                row_i += wrap ? teams : 0;
+            }
+        }
+        auto there = [&](int i) __attribute__((always_inline)) { return i < units && r[i] < rows && c[i] < end; };
+        // the same in a loop that is not unrolled
+        auto each_again = [&](unsigned which, auto what) __attribute__((always_inline)) {
+            const int c0 = (threadIdx.x & ((1 << sh.lanes_log) - 1)) * 8, cstep = 8 << sh.lanes_log;
+            int at_r = threadIdx.x >> sh.lanes_log, at_c = c0;
+#pragma unroll 1
+            for (int i = 0; i < units; ++i) {
+                if (which >> i & 1) what(at_r, at_c);
+                at_c += cstep;
+                if (at_c >= c0 + sh.turns * cstep) {
+                    at_c = c0;
+                    at_r += teams;
+                }
+            }
+        };
+        // A kernel that runs for some microseconds pays for every instruction
+        // it fetches: unrolled is only what holds values in registers, and runs
+        // that need more than that (the end of a row inside, a quotient near a
+        // half) are loaded again in loops.
+        Raw8<ELEM> raw[kUnits];
+        unsigned ends = 0;  // runs that the row's end is inside of
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            raw[i] = nothing8<ELEM>();
+            if (there(i)) {
+                if (c[i] + 8 <= K) raw[i] = raw8<ELEM>(x, row(r[i]) + c[i]);
+                else if (c[i] < K) ends |= 1u << i;
+            }
+        }
+        auto put = [&](int r, int c, const int (&k)[8]) __attribute__((always_inline)) {
+            *reinterpret_cast<uint2*>(to + r * stride + c) = pack8(k);
+        };
+        int k[8];
+        float f[8];
+        if constexpr (ELEM == VDTTFS_ELEM_TIMES) {
+            const int levels = T < 127 ? T : 127;
+            if ((int)threadIdx.x < rows) scale[threadIdx.x] = 1.0f / (float)levels;
+            auto code = [&](int r, int c) __attribute__((always_inline)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) k[e] = time_code(f[e], tfs, T, levels);
+                put(r, c, k);
+            };
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i)
+                if (there(i)) {
+                    unpack8<ELEM>(raw[i], f);
+                    code(r[i], c[i]);
+                }
+            if (K & 7)
+                each_again(ends, [&](int r, int c) __attribute__((always_inline)) {
+                    load8<ELEM>(x, row(r), c, K, f);
+                    code(r, c);
+                });
+        } else {
+            if ((int)threadIdx.x < rows) peak[threadIdx.x] = 0;
+            __syncthreads();
+            auto magnitude = [&]() __attribute__((always_inline)) {
+                int a = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) a = max(a, __float_as_int(f[e]) & 0x7fffffff);
+                return a;
+            };
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i)
+                if (i < units) {
+                    unpack8<ELEM>(raw[i], f);
+                    int a = magnitude();
+                    // eight lanes are on one row (or past the last, with zeros)
+                    a = max(a, __builtin_amdgcn_update_dpp(a, a, 0xB1, 0xf, 0xf, false));
+                    a = max(a, __builtin_amdgcn_update_dpp(a, a, 0x4E, 0xf, 0xf, false));
+                    a = max(a, __builtin_amdgcn_update_dpp(a, a, 0x141, 0xf, 0xf, false));
+                    if ((threadIdx.x & 7) == 0 && a > 0) atomicMax(&peak[r[i]], a);
+                }
+            if (K & 7)
+                each_again(ends, [&](int r, int c) __attribute__((always_inline)) {
+                    load8<ELEM>(x, row(r), c, K, f);
+                    atomicMax(&peak[r], magnitude());
+                });
+            __syncthreads();
+            if ((int)threadIdx.x < rows) scale[threadIdx.x] = scale_of(__int_as_float(peak[threadIdx.x]));
+            __syncthreads();
+            unsigned again = ends;
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i)
+                if (there(i)) {
+                    unpack8<ELEM>(raw[i], f);
+                    if (codes8_fast(f, coder_of(scale[r[i]]), k)) again |= 1u << i;
+                    put(r[i], c[i], k);
+                }
+            if (__any(again != 0))
+                each_again(again, [&](int r, int c) __attribute__((always_inline)) {
+                    load8<ELEM>(x, row(r), c, K, f);
+                    codes8_exact(f, coder_of(scale[r]), k);
+                    put(r, c, k);
+                });
+        }
+        __syncthreads();
+    }
+}
+
+// The codes of a row lie `stride` bytes apart: K rounded up to 64, and 16 more,
+// so that 16 rows read at one place come from different banks.
+__host__ __device__ __forceinline__ int lds_stride(int K) { return ((K + 63) & ~63) + 16; }
+
+// A wave's part of K for PARTS runs of 16 channels (a lane holds 16 codes of
+// channel lane & 15 at a time): its first loads are issued by begin(), before
+// anything waits for the rows.  The last K % 64 codes are the last wave's.
+template <int PARTS>
+struct Weights {
+    static constexpr int kHeld = kAhead / PARTS;
+    const int8_t* row[PARTS];
+    v4i ahead[PARTS][kHeld], tail[PARTS];
+    int first, last, K, at_tail;  // steps of 64 codes
+
+    __device__ __forceinline__ void begin(int K_, int wave) {
+        K = K_;
+        const int steps = K / 64, per = (steps + kWaves - 1) / kWaves, g = (lane_id() >> 4) * 16;
+        first = wave * per;
+        last = first + per < steps ? first + per : steps;
+        at_tail = wave == kWaves - 1 && K > steps * 64 ? steps * 64 : -1;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) row[p] += g;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                if (first + i < last)
+                    ahead[p][i] = reinterpret_cast<const Bytes16*>(row[p] + (first + i) * 64)->v;
+        if (at_tail >= 0) {
+#pragma unroll 1
+            for (int p = 0; p < PARTS; ++p) {
+                const v4i t = load16(row[p] - g, at_tail + g, K);
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q)
+                    if (q == p) tail[q] = t;
+            }
+        }
+    }
+    // acc[p] += channels x rows; rows: the lane's row of codes (lane & 15)
+    __device__ __forceinline__ void multiply(const int8_t* rows, v4i (&acc)[PARTS]) const {
+        rows += (lane_id() >> 4) * 16;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+            if (first + i < last) {
+                const v4i a = *reinterpret_cast<const v4i*>(rows + (first + i) * 64);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+                    acc[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(ahead[p][i], a, acc[p], 0, 0, 0);
+            }
+#pragma unroll 2
+        for (int s = first + kHeld; s < last; ++s) {
+            const v4i a = *reinterpret_cast<const v4i*>(rows + s * 64);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                acc[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                    reinterpret_cast<const Bytes16*>(row[p] + s * 64)->v, a, acc[p], 0, 0, 0);
+        }
+        if (at_tail >= 0) {
+            const v4i a = *reinterpret_cast<const v4i*>(rows + at_tail);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                acc[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(tail[p], a, acc[p], 0, 0, 0);
+        }
+    }
+};
+
+// Sum of the waves' parts for output (row m, channel n) of a 16 x 16 tile.
+__device__ __forceinline__ int gather(const int* part, int m, int n) {
+    int v = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v += part[w * 256 + (m + 16 * (n >> 2)) * 4 + (n & 3)];
+    return v;
+}
+
+struct SmallArgs {
+    const void* x;
+    int64_t ldx;
+    const float* sa;  // scales of rows that are codes already
+    const int8_t* w;
+    int64_t ldw;
+    const float* sb;
+    const float* bias;
+    void* out;
+    int64_t ldo;
+    int64_t M;
+    int N, K, act, out_elem;
+    float tfs;
+    int T;
+    Share sh;
+};
+
+// 16 rows x 16 channels a workgroup, its eight waves sharing K.
+template <int ELEM>
+__global__ __launch_bounds__(kThreads) void k_i8_small(SmallArgs p) {
+    extern __shared__ __align__(16) int8_t codes[];
+    __shared__ int part[kWaves * 256];
+    __shared__ float scale[kRows];
+    __shared__ int peak[kRows];
+    const int lane = lane_id(), wave = uniform(threadIdx.x >> 6), stride = lds_stride(p.K);
+    const int n0 = blockIdx.x * 16;
+    const int64_t m0 = (int64_t)blockIdx.y * kRows;
+    const int rows = p.M - m0 < kRows ? (int)(p.M - m0) : kRows;
+    Weights<1> w;
+    {
+        const int n = n0 + (lane & 15);
+        w.row[0] = p.w + (int64_t)(n < p.N ? n : p.N - 1) * p.ldw;
+    }
+    w.begin(p.K, wave);
+    if (ELEM == kCodes && (int)threadIdx.x < rows) scale[threadIdx.x] = p.sa[m0 + threadIdx.x];
+    rows_to_lds<ELEM>(p.x, [&](int r) { return (m0 + r) * p.ldx; }, rows, p.K, p.sh, p.tfs, p.T, codes, stride,
+                      scale, peak);
+    const int r = lane & 15;
+    v4i acc[1] = {v4i{0, 0, 0, 0}};
+    w.multiply(codes + (r < rows ? r : rows - 1) * stride, acc);
+    *reinterpret_cast<v4i*>(part + wave * 256 + lane * 4) = acc[0];
+    __syncthreads();
+    const int m = threadIdx.x >> 4, n = threadIdx.x & 15;
+    if (m < rows && n0 + n < p.N) {
+        float v = (float)gather(part, m, n) * scale[m] * p.sb[n0 + n];
+        if (p.bias) v += p.bias[n0 + n];
+        store_elem(p.out, (m0 + m) * p.ldo + n0 + n, apply_act(v, p.act), p.out_elem);
+    }
+}
+
+}  // namespace
+
+// Few rows, or layers so small that launches count.  Every workgroup quantises
+// its rows, some 1.1 us for each run of eight a thread has, so two at most; past
+// that a launch of its own does it (5 rows of 4096 -> 4096: TODO against TODO us).
+// Measured (us, against quantisation and tiles): 1x4096x4096 of BF16 6.7, 10.8;
+// 16x512x512 5.9, 7.3; 128x512x512 5.6, 7.2; 256x512x512 7.4, 7.0, of spike
+// times 5.7, 7.2, 512 rows of them 8.6, 6.9.  Codes, 5x4096x4096: 5.7, tiles 7.3.
+bool small_ok(int64_t M, int N, int K, int elem) {
+    const int64_t rows = M < kRows ? M : kRows;
+    const Share sh = share_of((int)rows, K);
+    if (elem != kElemCodes && sh.passes * sh.turns > kUnits) return false;
+    if (rows * lds_stride(K) > 56 * 1024) return false;
+    const int64_t blocks = (M + kRows - 1) / kRows * ((N + 15) / 16);
+    return M <= kRows || blocks <= (elem == VDTTFS_ELEM_TIMES ? 512 : 256);
+}
+
+int launch_i8_small(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const I8Args& a) {
+    const SmallArgs p{x,    ldx, sa,  a.B, a.ldb, a.sb,       a.bias,     a.out,      a.ldo,
+                      a.M,  a.N, a.K, a.act, a.out_elem, ctx->c.tfs, ctx->c.T,
+                      share_of((int)(a.M < kRows ? a.M : kRows), a.K)};
+    const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + kRows - 1) / kRows));
+    const int rows = a.M < kRows ? (int)a.M : kRows;
+    const size_t lds = (size_t)rows * lds_stride(a.K);
+    switch (elem) {
+        case VDTTFS_ELEM_F32: k_i8_small<VDTTFS_ELEM_F32><<<grid, kThreads, lds, ctx->stream>>>(p); break;
+        case VDTTFS_ELEM_BF16: k_i8_small<VDTTFS_ELEM_BF16><<<grid, kThreads, lds, ctx->stream>>>(p); break;
+        case VDTTFS_ELEM_F16: k_i8_small<VDTTFS_ELEM_F16><<<grid, kThreads, lds, ctx->stream>>>(p); break;
+        case VDTTFS_ELEM_TIMES: k_i8_small<VDTTFS_ELEM_TIMES><<<grid, kThreads, lds, ctx->stream>>>(p); break;
+        default: k_i8_small<kCodes><<<grid, kThreads, lds, ctx->stream>>>(p);
+    }
+    VD_HIP(hipGetLastError());
+    return VDTTFS_OK;
+}
+
+}  // namespace vdttfs
