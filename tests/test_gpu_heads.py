@@ -132,7 +132,8 @@ def test_quant_kernel_is_quant_rows_of_the_transpose(ctx, c_in, c_out):
 # ---- products -------------------------------------------------------------------
 SIZES = [(1, 1, 1), (1, 16, 64), (1, 100, 4096), (2, 33, 15), (4, 64, 127), (5, 129, 1000), (16, 17, 128),
          (17, 64, 129), (31, 300, 513), (64, 64, 256), (65, 127, 300), (129, 257, 385), (300, 10, 77), (256, 512, 512),
-         (7, 1024, 8192), (513, 1030, 640), (1100, 257, 300), (1500, 512, 128), (2100, 300, 1024), (1025, 70, 90)]
+         (7, 1024, 8192), (513, 1030, 640), (1100, 257, 300), (1500, 512, 128), (2100, 300, 1024), (1025, 70, 90), (1024, 1024, 400), (4100, 2600, 144), (2000, 2100, 208),
+         (1300, 5000, 272), (900, 700, 1000)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
@@ -368,7 +369,8 @@ def run_experts(ctx, bits, x_elem, ldx, idx, wt, weights, kind, gated, out_elem,
 EXPERTS = [  # M, k, E, D, F, N
     (1, 1, 1, 1, 1, 1), (1, 6, 64, 128, 64, 96), (1, 2, 4, 33, 17, 10), (2, 2, 3, 100, 70, 65), (5, 1, 2, 64, 64, 64),
     (9, 4, 8, 130, 96, 33), (40, 2, 5, 77, 50, 129), (70, 8, 8, 64, 128, 64), (257, 2, 8, 512, 512, 10),
-    (600, 3, 16, 96, 40, 72), (300, 4, 4, 256, 300, 260), (3000, 2, 12, 64, 33, 40)]
+    (600, 3, 16, 96, 40, 72), (300, 4, 4, 256, 300, 260), (3000, 2, 12, 64, 33, 40),
+    (900, 3, 3, 144, 208, 130), (1500, 1, 2, 250, 90, 300)]
 
 
 @pytest.mark.parametrize("M,k,E,D,F,N", EXPERTS)

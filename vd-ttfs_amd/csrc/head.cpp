@@ -143,6 +143,39 @@ I8Args product(const int8_t* A, int64_t lda, const float* sa, const int8_t* B, i
     return a;
 }
 
+// Scratch for copies of the operands whose rows are off 16 bytes, 0 where the
+// product is as fast from where they are.
+bool off16(const int8_t* p, int64_t ld) { return (((uintptr_t)p | (uintptr_t)ld) & 15) != 0; }
+size_t aligned_bytes(const I8Args& a) {
+    if (!i8_wants_aligned(a)) return 0;
+    Layout l;
+    if (off16(a.A, a.lda)) l.take((size_t)a.M * padded(a.K));
+    if (off16(a.B, a.ldb)) l.take((size_t)a.N * padded(a.K));
+    return l.bytes;
+}
+
+// The product, its operands copied onto 16 bytes first where that pays; scratch
+// of `bytes`, as aligned_bytes says, or none yet.
+int dense(vdttfs_ctx* ctx, I8Args a, size_t bytes, unsigned char* buf) {
+    const size_t need = aligned_bytes(a);
+    if (need > 0) {
+        if (bytes < need) VD_TRY(head_scratch(ctx, need, &buf));
+        const int64_t ld = padded(a.K);
+        if (off16(a.A, a.lda)) {
+            VD_TRY(launch_realign(ctx, a.A, a.lda, a.M, a.K, reinterpret_cast<int8_t*>(buf), ld));
+            a.A = reinterpret_cast<int8_t*>(buf);
+            a.lda = ld;
+            buf += ((size_t)a.M * ld + 255) & ~size_t(255);
+        }
+        if (off16(a.B, a.ldb)) {
+            VD_TRY(launch_realign(ctx, a.B, a.ldb, a.N, a.K, reinterpret_cast<int8_t*>(buf), ld));
+            a.B = reinterpret_cast<int8_t*>(buf);
+            a.ldb = ld;
+        }
+    }
+    return launch_i8_dense(ctx, a);
+}
+
 }  // namespace
 
 extern "C" {
@@ -182,8 +215,8 @@ int vdttfs_i8_matmul(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, co
     VD_TRY(check_float_ptr("i8_matmul", d_row_scale, 4));
     VD_TRY(check_product("i8_matmul", d_w, ldw, d_ch_scale, d_bias, act, K));
     const I8Args a = product(d_q, ldq, d_row_scale, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M, N, K, act);
-    if (small_ok(M, N, K, kElemCodes) && !getenv("VD_NOSMALL")) return launch_i8_small(ctx, d_q, kElemCodes, ldq, d_row_scale, a);
-    return launch_i8_dense(ctx, a);
+    if (small_ok(M, N, K, kElemCodes)) return launch_i8_small(ctx, d_q, kElemCodes, ldq, d_row_scale, a);
+    return dense(ctx, a, 0, nullptr);
 }
 
 int vdttfs_i8_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const void* d_x, int x_elem,
@@ -195,21 +228,27 @@ int vdttfs_i8_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, co
     VD_TRY(check_out("i8_linear", d_out, out_elem, ldo, N));
     VD_TRY(check_in("i8_linear", d_x, x_elem, ldx, M, K));
     VD_TRY(check_product("i8_linear", d_w, ldw, d_ch_scale, d_bias, act, K));
-    if (small_ok(M, N, K, x_elem) && !getenv("VD_NOSMALL"))
+    if (small_ok(M, N, K, x_elem))
         return launch_i8_small(ctx, d_x, x_elem, ldx, nullptr,
                                product(nullptr, 0, nullptr, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M, N,
                                        K, act));
+    // the codes' rows end in zeros, so a weight row may too: whole chunks
     const int64_t ldq = padded(K);
+    I8Args a = product(nullptr, ldq, nullptr, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M, N, K, act);
+    const bool small = M <= 16 && small_ok(M, N, K, kElemCodes);
     Layout l;
     const size_t at_q = l.take((size_t)M * ldq), at_s = l.take((size_t)M * 4);
+    const size_t own = l.bytes;
+    if (!small) l.take(aligned_bytes(a));
     unsigned char* buf;
     VD_TRY(head_scratch(ctx, l.bytes, &buf));
     int8_t* q = reinterpret_cast<int8_t*>(buf + at_q);
     float* s = reinterpret_cast<float*>(buf + at_s);
     VD_TRY(launch_quant_rows(ctx, d_x, x_elem, ldx, M, K, q, ldq, (int)ldq, s));
-    const I8Args a = product(q, ldq, s, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M, N, K, act);
-    if (small_ok(M, N, K, kElemCodes) && M <= 16) return launch_i8_small(ctx, q, kElemCodes, ldq, s, a);
-    return launch_i8_dense(ctx, a);
+    a.A = q;
+    a.sa = s;
+    if (small) return launch_i8_small(ctx, q, kElemCodes, ldq, s, a);
+    return dense(ctx, a, l.bytes - own, buf + own);
 }
 
 int vdttfs_route(vdttfs_ctx* ctx, int32_t* d_idx, float* d_weight, int32_t* d_count, const void* d_logits, int elem,
@@ -263,9 +302,34 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
     VD_TRY(check_product("experts", L.w2, L.d_hidden, L.s2, L.b2, L.act, L.d_hidden));
 
     const int64_t pairs = M * top_k;
+    const int64_t ldq = padded(L.d_in), ldh = padded(L.d_hidden);
+    bool fuse1, fuse2;
+    if (experts_small_ok(pairs, L, &fuse1, &fuse2)) {
+        Layout l;
+        const size_t at_q = l.take(fuse1 ? 0 : (size_t)M * ldq), at_s = l.take(fuse1 ? 0 : (size_t)M * 4);
+        const size_t at_h = l.take((size_t)pairs * L.d_hidden * 4);
+        const size_t at_hq = l.take(fuse2 ? 0 : (size_t)pairs * ldh), at_hs = l.take(fuse2 ? 0 : (size_t)pairs * 4);
+        const size_t at_z = l.take((size_t)pairs * L.d_out * 4);
+        unsigned char* buf;
+        VD_TRY(head_scratch(ctx, l.bytes, &buf));
+        int8_t* q = reinterpret_cast<int8_t*>(buf + at_q);
+        float* s = reinterpret_cast<float*>(buf + at_s);
+        float* h = reinterpret_cast<float*>(buf + at_h);
+        int8_t* hq = reinterpret_cast<int8_t*>(buf + at_hq);
+        float* hs = reinterpret_cast<float*>(buf + at_hs);
+        float* z = reinterpret_cast<float*>(buf + at_z);
+        if (!fuse1) VD_TRY(launch_quant_rows(ctx, d_x, x_elem, ldx, M, L.d_in, q, ldq, (int)ldq, s));
+        VD_TRY(fuse1 ? launch_expert_product(ctx, d_x, x_elem, ldx, nullptr, d_idx, pairs, top_k, L, false, h)
+                     : launch_expert_product(ctx, q, kElemCodes, ldq, s, d_idx, pairs, top_k, L, false, h));
+        if (!fuse2)
+            VD_TRY(launch_quant_rows(ctx, h, VDTTFS_ELEM_F32, L.d_hidden, pairs, L.d_hidden, hq, ldh, (int)ldh, hs));
+        VD_TRY(fuse2 ? launch_expert_product(ctx, h, VDTTFS_ELEM_F32, L.d_hidden, nullptr, d_idx, pairs, top_k, L,
+                                             true, z)
+                     : launch_expert_product(ctx, hq, kElemCodes, ldh, hs, d_idx, pairs, top_k, L, true, z));
+        return launch_combine(ctx, d_out, out_elem, ldo, z, d_idx, d_weight, M, L.d_out, top_k, L.n_experts);
+    }
     const int bm = i8_tile_rows(pairs, L.n_experts);
     const int64_t max_tiles = pairs / bm + (pairs < L.n_experts ? pairs : L.n_experts);
-    const int64_t ldq = padded(L.d_in), ldh = padded(L.d_hidden);
     Layout l;
     const size_t at_q = l.take((size_t)M * ldq), at_s = l.take((size_t)M * 4);
     const size_t at_h = l.take((size_t)pairs * L.d_hidden * 4);
@@ -274,6 +338,11 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
     const size_t at_pair = l.take((size_t)pairs * 4), at_row = l.take((size_t)pairs * 4);
     const size_t at_tiles = l.take((size_t)max_tiles * sizeof(int4)), at_n = l.take(4);
     const size_t at_hist = l.take((size_t)dispatch_blocks(pairs) * L.n_experts * 4);
+    // weights off 16 bytes: copied where every expert has rows enough to pay for it
+    const bool copy1 = bm > 32 && H > 0 && L.d_in > 0 && off16(L.w1, L.d_in);
+    const bool copy2 = bm > 32 && L.d_hidden > 0 && off16(L.w2, L.d_hidden);
+    const size_t at_w1 = l.take(copy1 ? (size_t)L.n_experts * H * ldq : 0);
+    const size_t at_w2 = l.take(copy2 ? (size_t)L.n_experts * L.d_out * ldh : 0);
     unsigned char* buf;
     VD_TRY(head_scratch(ctx, l.bytes, &buf));
     int8_t* q = reinterpret_cast<int8_t*>(buf + at_q);
@@ -295,6 +364,13 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
     a.max_tiles = (int)max_tiles;
     a.a_rows = d.row;
     a.b_stride = (int64_t)H * L.d_in;
+    if (copy1) {
+        int8_t* w = reinterpret_cast<int8_t*>(buf + at_w1);
+        VD_TRY(launch_realign(ctx, L.w1, L.d_in, (int64_t)L.n_experts * H, L.d_in, w, ldq));
+        a.B = w;
+        a.ldb = ldq;
+        a.b_stride = (int64_t)H * ldq;
+    }
     a.s_stride = H;
     VD_TRY(launch_i8_grouped(ctx, a, L.gated != 0, bm));
     VD_TRY(launch_quant_rows(ctx, h, VDTTFS_ELEM_F32, L.d_hidden, pairs, L.d_hidden, hq, ldh, (int)ldh, hs));
@@ -305,6 +381,13 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
     b.max_tiles = (int)max_tiles;
     b.o_rows = d.pair;
     b.b_stride = (int64_t)L.d_out * L.d_hidden;
+    if (copy2) {
+        int8_t* w = reinterpret_cast<int8_t*>(buf + at_w2);
+        VD_TRY(launch_realign(ctx, L.w2, L.d_hidden, (int64_t)L.n_experts * L.d_out, L.d_hidden, w, ldh));
+        b.B = w;
+        b.ldb = ldh;
+        b.b_stride = (int64_t)L.d_out * ldh;
+    }
     b.s_stride = L.d_out;
     VD_TRY(launch_i8_grouped(ctx, b, false, bm));
     return launch_combine(ctx, d_out, out_elem, ldo, z, d_idx, d_weight, M, L.d_out, top_k, L.n_experts);

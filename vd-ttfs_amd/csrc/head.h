@@ -39,6 +39,9 @@ int launch_quant_kernel(vdttfs_ctx* ctx, const float* kernel, int c_in, int c_ou
                         float* scale);
 // bm: rows of a tile of a grouped product (i8_tile_rows of the same call)
 int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a);
+bool i8_wants_aligned(const I8Args& a);
+// Rows of codes to rows of ld_to, a multiple of 16, zeros from K on.
+int launch_realign(vdttfs_ctx* ctx, const int8_t* from, int64_t ld, int64_t rows, int K, int8_t* to, int64_t ld_to);
 // The product of few rows (a.A and a.lda unused), quantised in the kernel from
 // elem, or codes with scales sa where elem is kElemCodes.
 constexpr int kElemCodes = 4;
@@ -46,6 +49,14 @@ bool small_ok(int64_t M, int N, int K, int elem);
 int launch_i8_small(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const I8Args& a);
 int launch_i8_grouped(vdttfs_ctx* ctx, const I8Args& a, bool gated, int bm);
 int i8_tile_rows(int64_t pairs, int n_experts);
+
+// The experts of few pairs without a sort: whether to, and whether each product
+// quantises its rows itself (d_hidden's are float [pairs][d_hidden]); one of the
+// two products, out float [pairs][its columns], x codes with scales sa where
+// elem is kElemCodes.
+bool experts_small_ok(int64_t pairs, const vdttfs_expert_layer& L, bool* fuse1, bool* fuse2);
+int launch_expert_product(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const int32_t* idx,
+                          int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool second, float* out);
 
 int launch_route(vdttfs_ctx* ctx, int32_t* idx, float* wt, int32_t* count, const void* logits, int elem, int64_t ld,
                  const float* bias, const uint8_t* row_mask, int64_t M, const vdttfs_route_opts& o, int* acc);

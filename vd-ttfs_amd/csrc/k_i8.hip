@@ -261,12 +261,14 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 // multiplied, the loads of the next S - 1 are in flight.  A wave-wide load
 // fills 1 KiB of LDS; the chunk that lies at place c of row r is chunk
 // c ^ swizzle(r), so that the 16 rows of a fragment come from all banks.
-// Needs 16-byte aligned rows; the last K % BK codes go through registers with
+// Needs 16-byte aligned rows; the last K % 16 codes go through registers with
 // zeros behind them.
 template <int BK>
 __device__ __forceinline__ int swizzle(int row) {
     return BK == 128 ? row & 7 : (row >> 2) & 3;
 }
+
+__device__ __align__(16) const int8_t kZeros[16] = {};
 
 // Waits until at most N of the wave's loads are outstanding (LDS writes: none).
 template <int N>
@@ -342,7 +344,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = v4i{0, 0, 0, 0};
 
-    const int tiles = p.K / BK;  // whole ones
+    // Tile 0 holds the whole chunks past the last whole tile, if any; the last
+    // K % 16 codes come after all.
+    const int k16 = p.K & ~15, part = k16 % BK, tiles = (k16 + BK - 1) / BK;
     auto fetch_one = [&](int8_t* s, int k0, int l) __attribute__((always_inline)) {
         if (l < NA)
             __builtin_amdgcn_global_load_lds((GlobalPtr)(pa[l] + k0), (LdsPtr)(s + (wave * NA + l) * 1024), 16, 0, 0);
@@ -350,8 +354,19 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
             __builtin_amdgcn_global_load_lds((GlobalPtr)(pb[l - NA] + k0),
                                              (LdsPtr)(s + BM * BK + (wave * NB + l - NA) * 1024), 16, 0, 0);
     };
-    auto k_of = [&](int t) __attribute__((always_inline)) {
-        return (t < tiles ? t : tiles - 1) * BK;  // past the end: loaded, not used
+    // where tile t > 0 of several starts; past the end the last, loaded and not used
+    auto k_of = [&](int t) __attribute__((always_inline)) { return ((t < tiles ? t : tiles - 1) - (part ? 1 : 0)) * BK; };
+    // Tile 0 where it is partial: chunks past its end are zeros.
+    auto fetch_part = [&](int8_t* s) __attribute__((always_inline)) {
+        const bool in = chunk < part;
+#pragma unroll
+        for (int l = 0; l < NL; ++l) {
+            const int8_t* row = l < NA ? pa[l < NA ? l : 0] : pb[l < NA ? 0 : l - NA];
+            const int8_t* from = in ? row + (k16 - part) : kZeros;
+            __builtin_amdgcn_global_load_lds(
+                (GlobalPtr)from, (LdsPtr)(s + (l < NA ? wave * NA + l : BM / kRows + wave * NB + l - NA) * 1024), 16, 0,
+                0);
+        }
     };
     auto fetch = [&](int8_t* s, int t) __attribute__((always_inline)) {
 #pragma unroll
@@ -406,8 +421,15 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
         barrier();
         multiply(std::true_type{}, s, next, k_of(t + S - 1));
     };
-    if (tiles > 0) {
-        fetch(s0, 0);
+    if (tiles == 1) {  // nothing to load ahead
+        if (part) fetch_part(s0);
+        else fetch(s0, 0);
+        wait_loads<0>();
+        barrier();
+        multiply(std::false_type{}, s0, s0, 0);
+    } else if (tiles > 1) {
+        if (part) fetch_part(s0);
+        else fetch(s0, 0);
         if (S > 2) fetch(s1, 1);
         if (S > 3) fetch(s2, 2);
         int t = 0;
@@ -424,11 +446,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
         if (S > 2 && t + 1 < tiles) multiply(std::false_type{}, s1, s1, 0);
         if (S > 3 && t + 2 < tiles) multiply(std::false_type{}, s2, s2, 0);
     }
-    if (tiles * BK < p.K) {
+    if (k16 < p.K) {
         v4i end[NL];
 #pragma unroll
         for (int l = 0; l < NL; ++l)
-            end[l] = load16((l < NA ? a_row(l) : b_row(l - NA)) - chunk, tiles * BK + chunk, p.K);
+            end[l] = load16((l < NA ? a_row(l) : b_row(l - NA)) - chunk, k16 + chunk, p.K);
         __syncthreads();
 #pragma unroll
         for (int l = 0; l < NL; ++l)
@@ -442,6 +464,17 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
                                      reinterpret_cast<float*>(s0) + wave * (Stage<FM, FN, GATED>::kBytes / 4));
 }
 
+// Rows of codes to rows on 128 bytes with zeros behind them, 16 codes a thread.
+__global__ __launch_bounds__(256) void k_realign(const int8_t* __restrict__ from, int64_t ld, int64_t rows, int K,
+                                                 int8_t* __restrict__ to, int64_t ld_to) {
+    const int64_t per = ld_to / 16, n = rows * per;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (int64_t)gridDim.x * 256) {
+        const int64_t r = at / per;
+        const int k = (int)(at - r * per) * 16;
+        *reinterpret_cast<v4i*>(to + r * ld_to + k) = load16(from + r * ld, k, K);
+    }
+}
+
 int check_grid(int64_t blocks) {
     if (blocks > 0x7fffffffll) return set_error(VDTTFS_E_UNSUPPORTED, "product of codes: too many tiles");
     return VDTTFS_OK;
@@ -451,7 +484,25 @@ bool aligned16(const I8Args& a) {
     return (((uintptr_t)a.A | (uintptr_t)a.B | (uintptr_t)a.lda | (uintptr_t)a.ldb | (uintptr_t)a.b_stride) & 15) == 0;
 }
 
+int64_t tiles_of(const I8Args& a, int bm, int bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); }
+
 }  // namespace
+
+int launch_realign(vdttfs_ctx* ctx, const int8_t* from, int64_t ld, int64_t rows, int K, int8_t* to, int64_t ld_to) {
+    const int64_t blocks = (rows * (ld_to / 16) + 255) / 256;
+    if (blocks <= 0) return VDTTFS_OK;
+    k_realign<<<dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), 256, 0, ctx->stream>>>(from, ld, rows, K, to,
+                                                                                               ld_to);
+    VD_HIP(hipGetLastError());
+    return VDTTFS_OK;
+}
+
+// Whether a product is large enough for rows off 16 bytes to be copied onto
+// them first, rather than read unaligned through registers (us, with copies and
+// without): 8192x4096x4095 153, 230; 4000x1000x1000 23, 17.
+bool i8_wants_aligned(const I8Args& a) {
+    return a.K > 0 && !aligned16(a) && (double)a.M * a.N * a.K >= 1e10 && tiles_of(a, 64, 64) >= 192;
+}
 
 template <int BM, int BN, int WM, int WN, int BK, int S>
 int run_big(vdttfs_ctx* ctx, const I8Args& a) {
@@ -483,7 +534,7 @@ int run_tile(vdttfs_ctx* ctx, const I8Args& a) {
 //   10.0, 32x32 7.6;  333x1111x1003: 64x64 8.0, 32x32 4.9
 int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
     if (a.M <= 0 || a.N <= 0) return VDTTFS_OK;
-    auto tiles = [&](int bm, int bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); };
+    auto tiles = [&](int bm, int bn) { return tiles_of(a, bm, bn); };
     if (!aligned16(a)) return tiles(64, 64) >= 192 ? run_tile<64, 64>(ctx, a) : run_tile<32, 32>(ctx, a);
     const int64_t big = tiles(256, 256), rounds = (big + 255) / 256;
     if (rounds == 1 ? big >= 160 : big * 10 >= rounds * 256 * 7) return run_big<256, 256, 2, 4, 128, 2>(ctx, a);
@@ -505,11 +556,16 @@ int run_grouped(vdttfs_ctx* ctx, const I8Args& a) {
     constexpr int kOut = GATED ? BN / 2 : BN;
     const int64_t tn = (a.N + kOut - 1) / kOut, blocks = a.max_tiles * tn;
     VD_TRY(check_grid(blocks));
-    if (aligned16(a))
+    if (aligned16(a)) {
         k_i8_big<BM, BN, WM, WN, 128, S, GATED, true>
             <<<dim3((unsigned)blocks), WM * WN * 64, 0, ctx->stream>>>(a, a.max_tiles, (int)tn);
-    else
-        k_i8_tile<BM, BN, WM, WN, GATED, true><<<dim3((unsigned)blocks), WM * WN * 64, 0, ctx->stream>>>(a, (int)tn);
+    } else {
+        if constexpr (BM > 32)
+            return set_error(VDTTFS_E_UNSUPPORTED, "product of codes: rows off 16 bytes in large tiles");
+        else
+            k_i8_tile<BM, BN, WM, WN, GATED, true>
+                <<<dim3((unsigned)blocks), WM * WN * 64, 0, ctx->stream>>>(a, (int)tn);
+    }
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }

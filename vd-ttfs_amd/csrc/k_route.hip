@@ -566,21 +566,37 @@ __global__ __launch_bounds__(kThreads) void k_sort_place(const int32_t* __restri
     }
 }
 
-// A workgroup per row: the slots' outputs summed in order.
+// The slots' outputs summed in order, VEC neighbouring columns a thread; eight
+// slots' loads are in flight at a time.
+template <int VEC>
 __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, int out_elem, int64_t ldo,
                                                       const float* __restrict__ z, const int32_t* __restrict__ idx,
                                                       const float* __restrict__ wt, int64_t M, int N, int top_k,
                                                       int E) {
-    for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
-        for (int n = threadIdx.x; n < N; n += kThreads) {
-            float sum = 0.0f;
-            for (int j = 0; j < top_k; ++j) {
-                const int64_t q = m * top_k + j;
-                const int e = idx[q];
-                if (e >= 0 && e < E) sum += wt[q] * z[q * N + n];
+    typedef float vec __attribute__((ext_vector_type(VEC)));
+    constexpr int kSlots = 8;
+    const int n = (blockIdx.x * kThreads + threadIdx.x) * VEC;
+    if (n >= N) return;
+    for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
+        vec sum = 0.0f;
+        for (int j0 = 0; j0 < top_k; j0 += kSlots) {
+            vec v[kSlots];
+            float w[kSlots];
+            bool on[kSlots];
+#pragma unroll
+            for (int j = 0; j < kSlots; ++j) {
+                const int64_t q = m * top_k + j0 + j;
+                const int e = j0 + j < top_k ? idx[q] : -1;
+                on[j] = e >= 0 && e < E;
+                w[j] = on[j] ? wt[q] : 0.0f;
+                v[j] = on[j] ? *reinterpret_cast<const vec*>(z + q * N + n) : vec(0.0f);
             }
-            store_elem(out, m * ldo + n, sum, out_elem);
+#pragma unroll
+            for (int j = 0; j < kSlots; ++j)
+                if (on[j]) sum += w[j] * v[j];
         }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) store_elem(out, m * ldo + n + i, sum[i], out_elem);
     }
 }
 
@@ -621,8 +637,10 @@ int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_
 
 int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const float* z, const int32_t* idx,
                    const float* wt, int64_t M, int N, int top_k, int n_experts) {
-    const dim3 grid((unsigned)(M < (1 << 20) ? M : 1 << 20));
-    k_combine<<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, z, idx, wt, M, N, top_k, n_experts);
+    const int vec = N % 4 == 0 ? 4 : 1;
+    const dim3 grid((unsigned)((N / vec + kThreads - 1) / kThreads), (unsigned)(M < 65535 ? M : 65535));
+    if (vec == 4) k_combine<4><<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, z, idx, wt, M, N, top_k, n_experts);
+    else k_combine<1><<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, z, idx, wt, M, N, top_k, n_experts);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }

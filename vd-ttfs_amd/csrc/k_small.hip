@@ -284,11 +284,121 @@ __global__ __launch_bounds__(kThreads) void k_i8_small(SmallArgs p) {
     }
 }
 
+// ---- experts of few pairs ---------------------------------------------------------
+// No sort and no tiles: a workgroup finds the pairs (row, slot) of its expert by
+// looking through the whole idx, at most kMaxPairs of them.  blockIdx.y names
+// the expert where there are no more experts than pairs; else it names a pair,
+// and the first pair of an expert stands for it.
+constexpr int kMaxPairs = 512;
+struct PairArgs {
+    const int32_t* idx;
+    int pairs, top_k, n_experts, by_pair;
+};
+
+// The pairs of the workgroup's expert, in order, to list; their number, 0 where
+// another workgroup has them.
+__device__ __forceinline__ int find_pairs(const PairArgs& a, int* list, int* counts, int* expert) {
+    const int lane = lane_id(), wave = threadIdx.x >> 6;
+    const int e = a.by_pair ? a.idx[blockIdx.y] : (int)blockIdx.y;
+    *expert = e;
+    if (e < 0 || e >= a.n_experts) return 0;  // the same in every thread
+    int before = 0;
+    for (int p0 = 0; p0 < a.pairs; p0 += kThreads) {
+        const int p = p0 + threadIdx.x;
+        const bool mine = p < a.pairs && a.idx[p] == e;
+        const uint64_t m = __ballot(mine);
+        if (lane == 0) counts[wave] = __popcll(m);
+        __syncthreads();
+        int at = before;
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) at += counts[w];
+            before += counts[w];
+        }
+        if (mine) list[at + __popcll(m & lanemask_lt())] = p;
+        __syncthreads();
+    }
+    if (a.by_pair && list[0] != (int)blockIdx.y) return 0;
+    return before;
+}
+
+struct ExpertArgs {
+    PairArgs pairs;
+    const void* x;
+    int64_t ldx;
+    const float* sa;  // scales of rows that are codes already
+    const int8_t* w;  // [E][channels][K]
+    const float* sb;  // [E][channels]
+    const float* bias;
+    float* out;  // [pairs][N]
+    int N, K, act, channels;
+    float tfs;
+    int T;
+    int cap;  // rows at a time
+    Share sh;  // of so many
+};
+
+// One product of the experts: out[pair] for 16 columns (of gate and up if
+// GATED) of the rows of one expert, `cap` at a time, every gridDim.z-th here.
+// The rows are x[pair / top_k], or x[pair] where BY_PAIR.
+template <int ELEM, bool GATED, bool BY_PAIR>
+__global__ __launch_bounds__(kThreads) void k_expert_small(ExpertArgs p) {
+    extern __shared__ __align__(16) int8_t codes[];
+    constexpr int kParts = GATED ? 2 : 1;
+    __shared__ int part[kParts * kWaves * 256];
+    __shared__ float scale[kRows];
+    __shared__ int peak[kRows];
+    __shared__ int list[kMaxPairs];
+    __shared__ int counts[kWaves];
+    const int lane = lane_id(), wave = uniform(threadIdx.x >> 6), stride = lds_stride(p.K);
+    int e;
+    const int n_rows = find_pairs(p.pairs, list, counts, &e);
+    const int n0 = blockIdx.x * 16;
+    if ((int)blockIdx.z * p.cap >= n_rows) return;
+    const int64_t ch0 = (int64_t)e * p.channels;
+    Weights<kParts> w;
+    {
+        const int n = n0 + (lane & 15) < p.N ? n0 + (lane & 15) : p.N - 1;
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) w.row[q] = p.w + (ch0 + n + q * p.N) * p.K;
+    }
+    w.begin(p.K, wave);
+    for (int r0 = blockIdx.z * p.cap; r0 < n_rows; r0 += gridDim.z * p.cap) {
+        const int rows = n_rows - r0 < p.cap ? n_rows - r0 : p.cap;
+        auto x_row = [&](int r) { return BY_PAIR ? list[r0 + r] : list[r0 + r] / p.pairs.top_k; };
+        if (ELEM == kCodes && (int)threadIdx.x < rows) scale[threadIdx.x] = p.sa[x_row(threadIdx.x)];
+        rows_to_lds<ELEM>(p.x, [&](int r) { return (int64_t)x_row(r) * p.ldx; }, rows, p.K, p.sh, p.tfs, p.T, codes,
+                          stride, scale, peak);
+        const int r = lane & 15;
+        v4i acc[kParts];
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) acc[q] = v4i{0, 0, 0, 0};
+        w.multiply(codes + (r < rows ? r : rows - 1) * stride, acc);
+#pragma unroll
+        for (int q = 0; q < kParts; ++q)
+            *reinterpret_cast<v4i*>(part + (q * kWaves + wave) * 256 + lane * 4) = acc[q];
+        __syncthreads();
+        const int m = threadIdx.x >> 4, n = threadIdx.x & 15;
+        if (m < rows && n0 + n < p.N) {
+            const int64_t ch = ch0 + n0 + n;
+            float v = (float)gather(part, m, n) * scale[m] * p.sb[ch];
+            if (p.bias) v += p.bias[ch];
+            v = apply_act(v, p.act);
+            if constexpr (GATED) {
+                float u = (float)gather(part + kWaves * 256, m, n) * scale[m] * p.sb[ch + p.N];
+                if (p.bias) u += p.bias[ch + p.N];
+                v *= u;
+            }
+            p.out[(int64_t)list[r0 + m] * p.N + n0 + n] = v;
+        }
+        __syncthreads();
+    }
+}
+
 }  // namespace
 
 // Few rows, or layers so small that launches count.  Every workgroup quantises
 // its rows, some 1.1 us for each run of eight a thread has, so two at most; past
-// that a launch of its own does it (5 rows of 4096 -> 4096: TODO against TODO us).
+// that a launch of its own does it (5x4096x4096 of BF16: 12.3 us, so 9.8).
 // Measured (us, against quantisation and tiles): 1x4096x4096 of BF16 6.7, 10.8;
 // 16x512x512 5.9, 7.3; 128x512x512 5.6, 7.2; 256x512x512 7.4, 7.0, of spike
 // times 5.7, 7.2, 512 rows of them 8.6, 6.9.  Codes, 5x4096x4096: 5.7, tiles 7.3.
@@ -315,6 +425,91 @@ int launch_i8_small(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const
         case VDTTFS_ELEM_TIMES: k_i8_small<VDTTFS_ELEM_TIMES><<<grid, kThreads, lds, ctx->stream>>>(p); break;
         default: k_i8_small<kCodes><<<grid, kThreads, lds, ctx->stream>>>(p);
     }
+    VD_HIP(hipGetLastError());
+    return VDTTFS_OK;
+}
+
+// Rows that a workgroup of the experts' kernels takes at a time, 0 where none.
+static int expert_rows(int64_t pairs, int K, bool codes) {
+    for (int rows = pairs < kRows ? (int)pairs : kRows; rows > 0; rows /= 2) {
+        const Share sh = share_of(rows, K);
+        if ((codes || sh.passes * sh.turns <= kUnits) && rows * lds_stride(K) <= 32 * 1024) return rows;
+    }
+    return 0;
+}
+
+// Measured (us; rows x slots of experts, d_in-d_hidden-d_out; quantising in the
+// products, before them, and sorted with tiles):
+//   1 x 6 of 64, 1024-512-1024 gated   13.5  17.3  23.8
+//   32 x 2 of 8, 512-512-512           14.2  16.8  24.2
+//   16 x 2 of 16, 2048-1024-2048 gated 42.2  37.1  41.7
+//   256 x 2 of 8, 512-512-10           28.1  21.6  30.2 (the second quantising: 19.3)
+//   256 x 2 of 8, 512-512-512 gated    34.8  25.9  28.1
+//   256 x 4 of 64, 512-512-512 gated   71.5  46.5  39.3
+bool experts_small_ok(int64_t pairs, const vdttfs_expert_layer& L, bool* fuse1, bool* fuse2) {
+    // every 16 columns quantise an expert's rows again
+    auto fuse = [&](int K, int N) {
+        return expert_rows(pairs, K, false) > 0 && (pairs * K <= 32768 || N <= 32);
+    };
+    *fuse1 = fuse(L.d_in, L.d_hidden);
+    *fuse2 = fuse(L.d_hidden, L.d_out);
+    return pairs <= kMaxPairs && expert_rows(pairs, L.d_in, !*fuse1) && expert_rows(pairs, L.d_hidden, !*fuse2);
+}
+
+template <bool GATED, bool BY_PAIR>
+static void expert_elem(vdttfs_ctx* ctx, const ExpertArgs& p, int elem, dim3 grid, size_t lds) {
+    switch (elem) {
+        case VDTTFS_ELEM_F32:
+            k_expert_small<VDTTFS_ELEM_F32, GATED, BY_PAIR><<<grid, kThreads, lds, ctx->stream>>>(p);
+            break;
+        case VDTTFS_ELEM_BF16:
+            k_expert_small<VDTTFS_ELEM_BF16, GATED, BY_PAIR><<<grid, kThreads, lds, ctx->stream>>>(p);
+            break;
+        case VDTTFS_ELEM_F16:
+            k_expert_small<VDTTFS_ELEM_F16, GATED, BY_PAIR><<<grid, kThreads, lds, ctx->stream>>>(p);
+            break;
+        case VDTTFS_ELEM_TIMES:
+            k_expert_small<VDTTFS_ELEM_TIMES, GATED, BY_PAIR><<<grid, kThreads, lds, ctx->stream>>>(p);
+            break;
+        default: k_expert_small<kCodes, GATED, BY_PAIR><<<grid, kThreads, lds, ctx->stream>>>(p);
+    }
+}
+
+int launch_expert_product(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const int32_t* idx,
+                          int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool second, float* out) {
+    const bool by_pair = pairs < L.n_experts;
+    const PairArgs pa{idx, (int)pairs, top_k, L.n_experts, by_pair};
+    const unsigned y = (unsigned)(by_pair ? pairs : L.n_experts);
+    const int K = second ? L.d_hidden : L.d_in, N = second ? L.d_out : L.d_hidden;
+    if (N <= 0) return VDTTFS_OK;
+    const bool gated = !second && L.gated;
+    const int cap = expert_rows(pairs, K, elem == kCodes);
+    const ExpertArgs p{pa,
+                       x,
+                       ldx,
+                       sa,
+                       second ? L.w2 : L.w1,
+                       second ? L.s2 : L.s1,
+                       second ? L.b2 : L.b1,
+                       out,
+                       N,
+                       K,
+                       second ? VDTTFS_ACT_NONE : L.act,
+                       gated ? 2 * N : N,
+                       ctx->c.tfs,
+                       ctx->c.T,
+                       cap,
+                       share_of(cap, K)};
+    // parts of an expert's rows: as many as its mean needs, while the chip holds
+    // all workgroups at once
+    const unsigned cols = (unsigned)((N + 15) / 16), want = (unsigned)((pairs / y + cap - 1) / cap);
+    const unsigned room = 512 / (cols * y);
+    const dim3 grid(cols, y, want < room ? want : room > 0 ? room : 1);
+    const size_t lds = (size_t)cap * lds_stride(K);
+    if (gated) expert_elem<true, false>(ctx, p, elem, grid, lds);
+    else if (!second) expert_elem<false, false>(ctx, p, elem, grid, lds);
+    else if (elem == kCodes) k_expert_small<kCodes, false, true><<<grid, kThreads, lds, ctx->stream>>>(p);
+    else k_expert_small<VDTTFS_ELEM_F32, false, true><<<grid, kThreads, lds, ctx->stream>>>(p);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
