@@ -77,8 +77,8 @@ struct Dispatch {
 int dispatch_blocks(int64_t pairs);
 int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_k, int n_experts, int bm,
                     const Dispatch& d);
-// out[m] = sum over slots of weight * z[m * top_k + slot]
-int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const float* z, const int32_t* idx,
-                   const float* wt, int64_t M, int N, int top_k, int n_experts);
+// out[m] = sum over slots of weight * z[m * top_k + slot], z F32 or BF16
+int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem,
+                   const int32_t* idx, const float* wt, int64_t M, int N, int top_k, int n_experts);
 
 }  // namespace vdttfs

@@ -243,14 +243,16 @@ __global__ __launch_bounds__(WM* WN * 64) void k_i8_tile(I8Args p, int tiles_n) 
 // row tiles, column by column, so that the tiles in flight on an XCD share
 // their rows and channels in its L2.
 constexpr int kXcds = 8, kBand = 8;
-__device__ __forceinline__ void tile_of(int b, int blocks, int tiles_m, int tiles_n, int* tm, int* tn) {
+__device__ __forceinline__ bool tile_of(int b, int blocks, int tiles_m, int tiles_n, int* tm, int* tn) {
     const int per = blocks / kXcds, rest = blocks % kXcds, x = b % kXcds;
+    if (b / kXcds >= per + (x < rest ? 1 : 0)) return false;  // past the last tile
     b = x * per + (x < rest ? x : rest) + b / kXcds;
     const int band = b / (kBand * tiles_n), in = b % (kBand * tiles_n);
     const int left = tiles_m - band * kBand;
     const int h = left < kBand ? left : kBand;
     *tm = band * kBand + in % h;
     *tn = in / h;
+    return true;
 }
 
 typedef const __attribute__((address_space(1))) void* GlobalPtr;
@@ -301,13 +303,13 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
     __shared__ __align__(16) int8_t s3[S > 3 ? kTile : 16];
 
     int tile_m, tile_n;
-    tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, &tile_m, &tile_n);
+    if (GROUPED) tiles_m = *p.n_tiles;  // the grid has room for max_tiles
+    if (!tile_of(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, &tile_m, &tile_n)) return;
     int64_t m0 = (int64_t)tile_m * BM, m_end = p.M;
     const int8_t* B = p.B;
     const float* sb = p.sb;
     const float* bias = p.bias;
     if constexpr (GROUPED) {
-        if (tile_m >= *p.n_tiles) return;
         const int4 t = p.tiles[tile_m];
         m0 = t.y;
         m_end = t.z;

@@ -489,19 +489,17 @@ void route_elem(vdttfs_ctx* ctx, const RouteArgs& a) {
 }
 
 // Experts of each workgroup's pairs: hist[block][expert].
-__global__ __launch_bounds__(kThreads) void k_sort_count(const int32_t* __restrict__ idx, int64_t pairs, int E,
-                                                         int* __restrict__ hist) {
+__global__ __launch_bounds__(1024) void k_sort_count(const int32_t* __restrict__ idx, int64_t pairs, int E,
+                                                     int* __restrict__ hist) {
     __shared__ int h[kMaxExperts];
-    for (int e = threadIdx.x; e < E; e += kThreads) h[e] = 0;
+    const int64_t q0 = (int64_t)blockIdx.x * kSortPairs + threadIdx.x, q1 = q0 + 1024;
+    const int e0 = q0 < pairs ? idx[q0] : -1, e1 = q1 < pairs ? idx[q1] : -1;
+    if ((int)threadIdx.x < E) h[threadIdx.x] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < kSortPairs; i += kThreads) {
-        const int64_t q = (int64_t)blockIdx.x * kSortPairs + i;
-        if (q >= pairs) break;
-        const int e = idx[q];
-        if (e >= 0 && e < E) atomicAdd(&h[e], 1);
-    }
+    if (e0 >= 0 && e0 < E) atomicAdd(&h[e0], 1);
+    if (e1 >= 0 && e1 < E) atomicAdd(&h[e1], 1);
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += kThreads) hist[(int64_t)blockIdx.x * E + e] = h[e];
+    if ((int)threadIdx.x < E) hist[(int64_t)blockIdx.x * E + threadIdx.x] = h[threadIdx.x];
 }
 
 // Sum of v over the threads before this one (1024 threads); total: over all.
@@ -523,64 +521,79 @@ __device__ __forceinline__ int block_excl_scan(int v, int* lds, int* total) {
 
 // One workgroup: hist[block][expert] becomes the sorted position of the
 // block's first pair of the expert; the row tiles of every expert follow.
-__global__ __launch_bounds__(1024) void k_sort_plan(int* __restrict__ hist, int blocks, int E, int bm,
+// 2^log threads go over the experts, and share the blocks in 1024 >> log runs.
+__global__ __launch_bounds__(1024) void k_sort_plan(int* __restrict__ hist, int blocks, int E, int log, int bm,
                                                     int4* __restrict__ tiles, int* __restrict__ n_tiles) {
     __shared__ int lds[16];
-    const int e = threadIdx.x;
+    __shared__ int sums[1024];
+    __shared__ int starts[kMaxExperts];
+    const int e = threadIdx.x & ((1 << log) - 1), run = threadIdx.x >> log, runs = 1024 >> log;
+    const int per = (blocks + runs - 1) / runs;
+    const int b0 = run * per, b1 = b0 + per < blocks ? b0 + per : blocks;
     int n = 0;
     if (e < E)
-        for (int b = 0; b < blocks; ++b) n += hist[(int64_t)b * E + e];
-    int all;
-    const int start = block_excl_scan(n, lds, &all);
-    if (e < E) {
-        int at = start;
-        for (int b = 0; b < blocks; ++b) {
-            const int h = hist[(int64_t)b * E + e];
-            hist[(int64_t)b * E + e] = at;
-            at += h;
-        }
-    }
-    const int t = (n + bm - 1) / bm;
-    int t_all;
+#pragma unroll 4
+        for (int b = b0; b < b1; ++b) n += hist[(int64_t)b * E + e];
+    sums[threadIdx.x] = n;
+    __syncthreads();
+    // the first run's threads have an expert's total
+    int total = 0;
+    if (run == 0)
+        for (int r = 0; r < runs; ++r) total += sums[(r << log) + e];
+    int all, t_all;
+    const int start = block_excl_scan(total, lds, &all);
+    const int t = (total + bm - 1) / bm;
     const int t0 = block_excl_scan(t, lds, &t_all);
-    for (int i = 0; i < t; ++i) tiles[t0 + i] = make_int4(e, start + i * bm, start + n, 0);
+    for (int i = 0; i < t; ++i) tiles[t0 + i] = make_int4(e, start + i * bm, start + total, 0);
     if (threadIdx.x == 0) *n_tiles = t_all;
+    if (run == 0) starts[e] = start;
+    __syncthreads();
+    if (e >= E) return;
+    int at = starts[e];
+    for (int r = 0; r < run; ++r) at += sums[(r << log) + e];
+#pragma unroll 4
+    for (int b = b0; b < b1; ++b) {
+        const int h = hist[(int64_t)b * E + e];
+        hist[(int64_t)b * E + e] = at;
+        at += h;
+    }
 }
 
 // Each pair to its place.  The order of an expert's pairs within a workgroup
 // is that of its LDS atomics; nothing that is computed depends on it.
-__global__ __launch_bounds__(kThreads) void k_sort_place(const int32_t* __restrict__ idx, int64_t pairs, int E,
-                                                         int top_k, const int* __restrict__ hist,
-                                                         int* __restrict__ pair, int* __restrict__ row) {
+__global__ __launch_bounds__(1024) void k_sort_place(const int32_t* __restrict__ idx, int64_t pairs, int E, int top_k,
+                                                     const int* __restrict__ hist, int* __restrict__ pair,
+                                                     int* __restrict__ row) {
     __shared__ int at[kMaxExperts];
-    for (int e = threadIdx.x; e < E; e += kThreads) at[e] = hist[(int64_t)blockIdx.x * E + e];
+    const int64_t q[2] = {(int64_t)blockIdx.x * kSortPairs + threadIdx.x,
+                          (int64_t)blockIdx.x * kSortPairs + threadIdx.x + 1024};
+    const int e[2] = {q[0] < pairs ? idx[q[0]] : -1, q[1] < pairs ? idx[q[1]] : -1};
+    if ((int)threadIdx.x < E) at[threadIdx.x] = hist[(int64_t)blockIdx.x * E + threadIdx.x];
     __syncthreads();
-    for (int i = threadIdx.x; i < kSortPairs; i += kThreads) {
-        const int64_t q = (int64_t)blockIdx.x * kSortPairs + i;
-        if (q >= pairs) break;
-        const int e = idx[q];
-        if (e < 0 || e >= E) continue;
-        const int to = atomicAdd(&at[e], 1);
-        pair[to] = (int)q;
-        row[to] = (int)(q / top_k);
-    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (e[i] >= 0 && e[i] < E) {
+            const int to = atomicAdd(&at[e[i]], 1);
+            pair[to] = (int)q[i];
+            row[to] = (int)(q[i] / top_k);
+        }
 }
 
 // The slots' outputs summed in order, VEC neighbouring columns a thread; eight
-// slots' loads are in flight at a time.
-template <int VEC>
+// slots' loads are in flight at a time.  Z: float, or uint16_t for BF16.
+template <int VEC, typename Z>
 __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, int out_elem, int64_t ldo,
-                                                      const float* __restrict__ z, const int32_t* __restrict__ idx,
+                                                      const Z* __restrict__ z, const int32_t* __restrict__ idx,
                                                       const float* __restrict__ wt, int64_t M, int N, int top_k,
                                                       int E) {
-    typedef float vec __attribute__((ext_vector_type(VEC)));
+    typedef Z zvec __attribute__((ext_vector_type(VEC)));
     constexpr int kSlots = 8;
     const int n = (blockIdx.x * kThreads + threadIdx.x) * VEC;
     if (n >= N) return;
     for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
-        vec sum = 0.0f;
+        float sum[VEC] = {};
         for (int j0 = 0; j0 < top_k; j0 += kSlots) {
-            vec v[kSlots];
+            zvec v[kSlots];
             float w[kSlots];
             bool on[kSlots];
 #pragma unroll
@@ -588,15 +601,35 @@ __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, in
                 const int64_t q = m * top_k + j0 + j;
                 const int e = j0 + j < top_k ? idx[q] : -1;
                 on[j] = e >= 0 && e < E;
-                w[j] = on[j] ? wt[q] : 0.0f;
-                v[j] = on[j] ? *reinterpret_cast<const vec*>(z + q * N + n) : vec(0.0f);
+                w[j] = 0.0f;
+                v[j] = zvec(Z(0));
+                if (on[j]) {
+                    w[j] = wt[q];
+                    v[j] = *reinterpret_cast<const zvec*>(z + q * N + n);
+                }
             }
 #pragma unroll
             for (int j = 0; j < kSlots; ++j)
-                if (on[j]) sum += w[j] * v[j];
-        }
+                if (on[j])
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) store_elem(out, m * ldo + n + i, sum[i], out_elem);
+                    for (int i = 0; i < VEC; ++i) {
+                        if constexpr (sizeof(Z) == 4) sum[i] += w[j] * v[j][i];
+                        else sum[i] += w[j] * bf16_to_f32(v[j][i]);
+                    }
+        }
+        const int64_t o = m * ldo + n;
+        const bool bf16 = out_elem == VDTTFS_ELEM_BF16;
+        if (VEC > 1 && out_elem != VDTTFS_ELEM_F32 && (((uintptr_t)out | (uintptr_t)(ldo * 2)) & (VEC * 2 - 1)) == 0) {
+            uint32_t p[VEC / 2 + 1];
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) p[i] = pack2(sum[2 * i], sum[2 * i + 1], bf16);
+            uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(out) + o);
+            if constexpr (VEC == 8) *reinterpret_cast<uint4*>(to) = make_uint4(p[0], p[1], p[2], p[3]);
+            if constexpr (VEC == 4) *reinterpret_cast<uint2*>(to) = make_uint2(p[0], p[1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) store_elem(out, o + i, sum[i], out_elem);
+        }
     }
 }
 
@@ -625,22 +658,29 @@ int dispatch_blocks(int64_t pairs) { return (int)((pairs + kSortPairs - 1) / kSo
 int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_k, int n_experts, int bm,
                     const Dispatch& d) {
     const int blocks = dispatch_blocks(pairs);
-    k_sort_count<<<dim3((unsigned)blocks), kThreads, 0, ctx->stream>>>(idx, pairs, n_experts, d.hist);
+    int log = 0;
+    while ((1 << log) < n_experts) ++log;
+    k_sort_count<<<dim3((unsigned)blocks), 1024, 0, ctx->stream>>>(idx, pairs, n_experts, d.hist);
     VD_HIP(hipGetLastError());
-    k_sort_plan<<<dim3(1), 1024, 0, ctx->stream>>>(d.hist, blocks, n_experts, bm, d.tiles, d.n_tiles);
+    k_sort_plan<<<dim3(1), 1024, 0, ctx->stream>>>(d.hist, blocks, n_experts, log, bm, d.tiles, d.n_tiles);
     VD_HIP(hipGetLastError());
-    k_sort_place<<<dim3((unsigned)blocks), kThreads, 0, ctx->stream>>>(idx, pairs, n_experts, top_k, d.hist, d.pair,
-                                                                       d.row);
+    k_sort_place<<<dim3((unsigned)blocks), 1024, 0, ctx->stream>>>(idx, pairs, n_experts, top_k, d.hist, d.pair,
+                                                                   d.row);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
 
-int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const float* z, const int32_t* idx,
-                   const float* wt, int64_t M, int N, int top_k, int n_experts) {
-    const int vec = N % 4 == 0 ? 4 : 1;
+int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem,
+                   const int32_t* idx, const float* wt, int64_t M, int N, int top_k, int n_experts) {
+    const bool bf16 = z_elem == VDTTFS_ELEM_BF16;
+    const int vec = bf16 && N % 8 == 0 ? 8 : !bf16 && N % 4 == 0 ? 4 : 1;
     const dim3 grid((unsigned)((N / vec + kThreads - 1) / kThreads), (unsigned)(M < 65535 ? M : 65535));
-    if (vec == 4) k_combine<4><<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, z, idx, wt, M, N, top_k, n_experts);
-    else k_combine<1><<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, z, idx, wt, M, N, top_k, n_experts);
+    const float* zf = static_cast<const float*>(z);
+    const uint16_t* zh = static_cast<const uint16_t*>(z);
+    if (vec == 8) k_combine<8><<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, zh, idx, wt, M, N, top_k, n_experts);
+    else if (bf16) k_combine<1><<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, zh, idx, wt, M, N, top_k, n_experts);
+    else if (vec == 4) k_combine<4><<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, zf, idx, wt, M, N, top_k, n_experts);
+    else k_combine<1><<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, zf, idx, wt, M, N, top_k, n_experts);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
