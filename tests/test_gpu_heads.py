@@ -133,7 +133,7 @@ def test_quant_kernel_is_quant_rows_of_the_transpose(ctx, c_in, c_out):
 SIZES = [(1, 1, 1), (1, 16, 64), (1, 100, 4096), (2, 33, 15), (4, 64, 127), (5, 129, 1000), (16, 17, 128),
          (17, 64, 129), (31, 300, 513), (64, 64, 256), (65, 127, 300), (129, 257, 385), (300, 10, 77), (256, 512, 512),
          (7, 1024, 8192), (513, 1030, 640), (1100, 257, 300), (1500, 512, 128), (2100, 300, 1024), (1025, 70, 90), (1024, 1024, 400), (4100, 2600, 144), (2000, 2100, 208),
-         (1300, 5000, 272), (900, 700, 1000)]
+         (1300, 5000, 272), (900, 700, 1000), (2600, 2600, 1500), (2561, 2500, 1601), (1100, 4100, 384)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)

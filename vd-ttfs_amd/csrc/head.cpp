@@ -143,35 +143,41 @@ I8Args product(const int8_t* A, int64_t lda, const float* sa, const int8_t* B, i
     return a;
 }
 
-// Scratch for copies of the operands whose rows are off 16 bytes, 0 where the
-// product is as fast from where they are.
+// Copies of the operands with rows on 128 bytes and zeros behind them, where
+// the product asks for it: which, and their scratch.
 bool off16(const int8_t* p, int64_t ld) { return (((uintptr_t)p | (uintptr_t)ld) & 15) != 0; }
-size_t aligned_bytes(const I8Args& a) {
-    if (!i8_wants_aligned(a)) return 0;
+struct Copies {
+    bool a, b;
+    size_t bytes;
+};
+Copies copies_of(const I8Args& a) {
+    if (!i8_wants_aligned(a)) return Copies{false, false, 0};
+    const bool part = a.K % 16 != 0;
+    Copies c{off16(a.A, a.lda) || (part && !a.a_padded), off16(a.B, a.ldb) || part, 0};
     Layout l;
-    if (off16(a.A, a.lda)) l.take((size_t)a.M * padded(a.K));
-    if (off16(a.B, a.ldb)) l.take((size_t)a.N * padded(a.K));
-    return l.bytes;
+    if (c.a) l.take((size_t)a.M * padded(a.K));
+    if (c.b) l.take((size_t)a.N * padded(a.K));
+    c.bytes = l.bytes;
+    return c;
 }
 
-// The product, its operands copied onto 16 bytes first where that pays; scratch
-// of `bytes`, as aligned_bytes says, or none yet.
+// The product, its operands copied first where copies_of says so; scratch of
+// so many bytes, or none yet.
 int dense(vdttfs_ctx* ctx, I8Args a, size_t bytes, unsigned char* buf) {
-    const size_t need = aligned_bytes(a);
-    if (need > 0) {
-        if (bytes < need) VD_TRY(head_scratch(ctx, need, &buf));
-        const int64_t ld = padded(a.K);
-        if (off16(a.A, a.lda)) {
-            VD_TRY(launch_realign(ctx, a.A, a.lda, a.M, a.K, reinterpret_cast<int8_t*>(buf), ld));
-            a.A = reinterpret_cast<int8_t*>(buf);
-            a.lda = ld;
-            buf += ((size_t)a.M * ld + 255) & ~size_t(255);
-        }
-        if (off16(a.B, a.ldb)) {
-            VD_TRY(launch_realign(ctx, a.B, a.ldb, a.N, a.K, reinterpret_cast<int8_t*>(buf), ld));
-            a.B = reinterpret_cast<int8_t*>(buf);
-            a.ldb = ld;
-        }
+    const Copies c = copies_of(a);
+    const int64_t ld = padded(a.K);
+    if (c.bytes > bytes) VD_TRY(head_scratch(ctx, c.bytes, &buf));
+    if (c.a) {
+        VD_TRY(launch_realign(ctx, a.A, a.lda, a.M, a.K, reinterpret_cast<int8_t*>(buf), ld));
+        a.A = reinterpret_cast<int8_t*>(buf);
+        a.lda = ld;
+        buf += ((size_t)a.M * ld + 255) & ~size_t(255);
+    }
+    if (c.b) {
+        VD_TRY(launch_realign(ctx, a.B, a.ldb, a.N, a.K, reinterpret_cast<int8_t*>(buf), ld));
+        a.B = reinterpret_cast<int8_t*>(buf);
+        a.ldb = ld;
+        if (c.a || a.a_padded) a.K = (int)ld;  // zeros on both sides
     }
     return launch_i8_dense(ctx, a);
 }
@@ -235,11 +241,12 @@ int vdttfs_i8_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, co
     // the codes' rows end in zeros, so a weight row may too: whole chunks
     const int64_t ldq = padded(K);
     I8Args a = product(nullptr, ldq, nullptr, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M, N, K, act);
+    a.a_padded = true;
     const bool small = M <= 16 && small_ok(M, N, K, kElemCodes);
     Layout l;
     const size_t at_q = l.take((size_t)M * ldq), at_s = l.take((size_t)M * 4);
     const size_t own = l.bytes;
-    if (!small) l.take(aligned_bytes(a));
+    if (!small) l.take(copies_of(a).bytes);
     unsigned char* buf;
     VD_TRY(head_scratch(ctx, l.bytes, &buf));
     int8_t* q = reinterpret_cast<int8_t*>(buf + at_q);
@@ -329,7 +336,7 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
         return launch_combine(ctx, d_out, out_elem, ldo, z, VDTTFS_ELEM_F32, d_idx, d_weight, M, L.d_out, top_k,
                               L.n_experts);
     }
-    const int bm = i8_tile_rows(pairs, L.n_experts);
+    const int bm = i8_tile_rows(pairs, L.n_experts, L.d_in < L.d_hidden ? L.d_in : L.d_hidden);
     const int64_t max_tiles = pairs / bm + (pairs < L.n_experts ? pairs : L.n_experts);
     Layout l;
     const size_t at_q = l.take((size_t)M * ldq), at_s = l.take((size_t)M * 4);
@@ -376,6 +383,7 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
         a.B = w;
         a.ldb = ldq;
         a.b_stride = (int64_t)H * ldq;
+        a.K = (int)ldq;  // zeros on both sides
     }
     a.s_stride = H;
     VD_TRY(launch_i8_grouped(ctx, a, L.gated != 0, bm));
@@ -393,6 +401,7 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
         b.B = w;
         b.ldb = ldh;
         b.b_stride = (int64_t)L.d_out * ldh;
+        b.K = (int)ldh;
     }
     b.s_stride = L.d_out;
     VD_TRY(launch_i8_grouped(ctx, b, false, bm));

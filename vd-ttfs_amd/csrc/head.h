@@ -30,6 +30,7 @@ struct I8Args {
     int64_t b_stride;  // codes of one expert's B
     int s_stride;      // channels of one expert
     int max_tiles;     // bound on *n_tiles
+    bool a_padded;     // A's rows end in zeros up to a multiple of 128
 };
 
 // Rows to codes; columns [cols, ldq_zero) of each row get 0.
@@ -48,7 +49,7 @@ constexpr int kElemCodes = 4;
 bool small_ok(int64_t M, int N, int K, int elem);
 int launch_i8_small(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const I8Args& a);
 int launch_i8_grouped(vdttfs_ctx* ctx, const I8Args& a, bool gated, int bm);
-int i8_tile_rows(int64_t pairs, int n_experts);
+int i8_tile_rows(int64_t pairs, int n_experts, int k_min);
 
 // The experts of few pairs without a sort: whether to, and whether each product
 // quantises its rows itself (d_hidden's are float [pairs][d_hidden]); one of the

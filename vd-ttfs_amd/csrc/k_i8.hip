@@ -423,7 +423,65 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
         barrier();
         multiply(std::true_type{}, s, next, k_of(t + S - 1));
     };
-    if (tiles == 1) {  // nothing to load ahead
+    if constexpr (S == 2) {
+        // Two stages, the barrier before a tile's last two groups: by then all
+        // its fragments are in registers, so the next tile's first ones are
+        // read, and the loads of the one after that are issued into its LDS,
+        // while the matrix instructions go on.
+        static_assert(G % 4 == 0 && G >= 4, "the ring of fragments comes round with the tile");
+        const int r = lane & 15;
+        v4i fa[4], fb[2][FN];
+        auto read_a = [&](const int8_t* s, int g) __attribute__((always_inline)) {
+            const int c = ((g / FM * 4 + (lane >> 4)) ^ swizzle<BK>(r)) * 16;
+            fa[g % 4] = *reinterpret_cast<const v4i*>(s + (wm + g % FM * 16 + r) * BK + c);
+        };
+        auto read_b = [&](const int8_t* s, int kk, int j) __attribute__((always_inline)) {
+            const int c = ((kk * 4 + (lane >> 4)) ^ swizzle<BK>(r)) * 16;
+            fb[kk & 1][j] = *reinterpret_cast<const v4i*>(s + (BM + wn + j * 16 + r) * BK + c);
+        };
+        auto first = [&](const int8_t* s) __attribute__((always_inline)) {
+            read_a(s, 0);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) read_b(s, 0, j);
+            read_a(s, 1);
+        };
+        auto run = [&](int8_t* s, int8_t* next, int t) __attribute__((always_inline)) {
+            const int k0 = k_of(t + 2);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int kk = g / FM, i = g % FM;
+                if (g + 2 < G) read_a(s, g + 2);
+                if (kk + 1 < KK) {
+#pragma unroll
+                    for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j) read_b(s, kk + 1, j);
+                }
+                if (g == G - 2) {
+                    wait_loads<0>();
+                    barrier();
+                    first(next);
+                }
+                if (g >= G - 2) {
+#pragma unroll
+                    for (int l = (g - (G - 2)) * NL / 2; l < (g - (G - 2) + 1) * NL / 2; ++l) fetch_one(s, k0, l);
+                }
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[kk & 1][j], fa[g % 4], acc[i][j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // at least two tiles (deep_ok)
+        if (part) fetch_part(s0);
+        else fetch(s0, 0);
+        fetch(s1, 1);
+        wait_loads<0>();
+        barrier();
+        first(s0);
+        for (int t = 0; t < tiles; t += 2) {
+            run(s0, s1, t);
+            if (t + 1 < tiles) run(s1, s0, t + 1);
+        }
+    } else if (tiles == 1) {  // nothing to load ahead
         if (part) fetch_part(s0);
         else fetch(s0, 0);
         wait_loads<0>();
@@ -448,7 +506,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
         if (S > 2 && t + 1 < tiles) multiply(std::false_type{}, s1, s1, 0);
         if (S > 3 && t + 2 < tiles) multiply(std::false_type{}, s2, s2, 0);
     }
-    if (k16 < p.K) {
+    if (S > 2 && k16 < p.K) {
         v4i end[NL];
 #pragma unroll
         for (int l = 0; l < NL; ++l)
@@ -461,7 +519,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
         __syncthreads();
         multiply(std::false_type{}, s0, s0, 0);
     }
-    __syncthreads();
+    wait_loads<0>();  // also those past the end: the stage takes their place
+    barrier();
     epilogue<FM, FN, GATED, GROUPED>(p, acc, m0 + wm, m_end, n0, wn, sb, bias,
                                      reinterpret_cast<float*>(s0) + wave * (Stage<FM, FN, GATED>::kBytes / 4));
 }
@@ -482,9 +541,14 @@ int check_grid(int64_t blocks) {
     return VDTTFS_OK;
 }
 
+// Rows that 16-byte loads to LDS can take.
 bool aligned16(const I8Args& a) {
     return (((uintptr_t)a.A | (uintptr_t)a.B | (uintptr_t)a.lda | (uintptr_t)a.ldb | (uintptr_t)a.b_stride) & 15) == 0;
 }
+
+// What the two-stage tiles ask of K: whole chunks, and two tiles at least.
+constexpr int kDeepK = 256;
+bool deep_ok(const I8Args& a) { return aligned16(a) && a.K % 16 == 0 && a.K >= kDeepK; }
 
 int64_t tiles_of(const I8Args& a, int bm, int bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); }
 
@@ -499,11 +563,11 @@ int launch_realign(vdttfs_ctx* ctx, const int8_t* from, int64_t ld, int64_t rows
     return VDTTFS_OK;
 }
 
-// Whether a product is large enough for rows off 16 bytes to be copied onto
-// them first, rather than read unaligned through registers (us, with copies and
-// without): 8192x4096x4095 153, 230; 4000x1000x1000 23, 17.
+// Whether a product is large enough for rows that the two-stage tiles do not
+// take to be copied first, rather than read unaligned through registers (us,
+// with copies and without): 8192x4096x4095 153, 230; 4000x1000x1000 23, 17.
 bool i8_wants_aligned(const I8Args& a) {
-    return a.K > 0 && !aligned16(a) && (double)a.M * a.N * a.K >= 1e10 && tiles_of(a, 64, 64) >= 192;
+    return a.K >= kDeepK && !deep_ok(a) && (double)a.M * a.N * a.K >= 1e10 && tiles_of(a, 64, 64) >= 192;
 }
 
 template <int BM, int BN, int WM, int WN, int BK, int S>
@@ -539,8 +603,10 @@ int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
     auto tiles = [&](int bm, int bn) { return tiles_of(a, bm, bn); };
     if (!aligned16(a)) return tiles(64, 64) >= 192 ? run_tile<64, 64>(ctx, a) : run_tile<32, 32>(ctx, a);
     const int64_t big = tiles(256, 256), rounds = (big + 255) / 256;
-    if (rounds == 1 ? big >= 160 : big * 10 >= rounds * 256 * 7) return run_big<256, 256, 2, 4, 128, 2>(ctx, a);
-    if (tiles(128, 128) >= 384) return run_big<128, 128, 2, 2, 128, 2>(ctx, a);
+    const bool deep = deep_ok(a);
+    if (deep && (rounds == 1 ? big >= 160 : big * 10 >= rounds * 256 * 7))
+        return run_big<256, 256, 2, 4, 128, 2>(ctx, a);
+    if (deep && tiles(128, 128) >= 384) return run_big<128, 128, 2, 2, 128, 2>(ctx, a);
     if (tiles(64, 128) >= 384) return run_big<64, 128, 2, 2, 128, 3>(ctx, a);
     if (tiles(64, 64) >= 192) return run_big<64, 64, 2, 2, 128, 4>(ctx, a);
     return run_big<32, 32, 2, 2, 128, 4>(ctx, a);
@@ -548,8 +614,9 @@ int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
 
 // Rows of a grouped product's tiles: the largest that an expert's rows fill on
 // average.
-int i8_tile_rows(int64_t pairs, int n_experts) {
+int i8_tile_rows(int64_t pairs, int n_experts, int k_min) {
     const int64_t mean = pairs / n_experts;
+    if (k_min < kDeepK) return mean >= 40 ? 64 : 32;
     return mean >= 256 ? 256 : mean >= 96 ? 128 : mean >= 40 ? 64 : 32;
 }
 
@@ -558,7 +625,7 @@ int run_grouped(vdttfs_ctx* ctx, const I8Args& a) {
     constexpr int kOut = GATED ? BN / 2 : BN;
     const int64_t tn = (a.N + kOut - 1) / kOut, blocks = a.max_tiles * tn;
     VD_TRY(check_grid(blocks));
-    if (aligned16(a)) {
+    if (S == 2 ? deep_ok(a) : aligned16(a)) {
         k_i8_big<BM, BN, WM, WN, 128, S, GATED, true>
             <<<dim3((unsigned)blocks), WM * WN * 64, 0, ctx->stream>>>(a, a.max_tiles, (int)tn);
     } else {
