@@ -14,11 +14,16 @@ namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 
-// v[0..3] of p, zero past the first n_ok
-__device__ __forceinline__ v4f take4(const float* p, int n_ok) {
+struct __attribute__((packed, aligned(4))) Floats4 {
+    v4f v;
+};
+// p[0..3], the last of the first n_ok again past them (n_ok <= 0: p[0] .. is
+// not there, and p[n_ok - 1] is).
+__device__ __forceinline__ v4f take4(const float* p, int n_ok, bool whole) {
+    if (whole) return reinterpret_cast<const Floats4*>(p)->v;
     v4f r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = e < n_ok ? p[e] : 0.0f;
+    for (int e = 0; e < 4; ++e) r[e] = p[e < n_ok ? e : n_ok - 1];
     return r;
 }
 
@@ -43,26 +48,44 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
     const int nw = n0 + (GATED ? wn / 2 : wn);  // the wave's first output column
     const int size = p.out_elem == VDTTFS_ELEM_F32 ? 4 : 2;
     const bool bf16 = p.out_elem == VDTTFS_ELEM_BF16;
-    const bool vec = nw + S::kCols <= p.N && ((p.ldo * size) & 15) == 0 &&
-                     (((uintptr_t)p.out + (size_t)nw * size) & 15) == 0;
+    const bool whole = nw + S::kCols <= p.N;
+    const bool vec = whole && ((p.ldo * size) & 15) == 0 && (((uintptr_t)p.out + (size_t)nw * size) & 15) == 0;
+    // everything that comes from memory first: the stores below may alias it,
+    // so a load between them would wait in line
+    constexpr int kFrags = GATED ? FN / 2 : FN, kStep = GATED ? 2 : 1;
+    v4f s[kFrags], b[kFrags], s2[kFrags], b2[kFrags];
+#pragma unroll
+    for (int j = 0; j < kFrags; ++j) {
+        const int n = nw + j * 16 + (lane >> 4) * 4;
+        s[j] = take4(sb + n, p.N - n, whole);
+        if (bias) b[j] = take4(bias + n, p.N - n, whole);
+        if constexpr (GATED) {
+            s2[j] = take4(sb + p.N + n, p.N - n, whole);
+            if (bias) b2[j] = take4(bias + p.N + n, p.N - n, whole);
+        }
+    }
+    float sa[FM];
+    int o_row[FM];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        int64_t m = m0 + i * 16 + (lane & 15);
+        if (m >= m_end) m = m_end - 1;
+        sa[i] = p.sa[GROUPED && p.a_rows ? p.a_rows[m] : m];
+        o_row[i] = GROUPED && p.o_rows ? p.o_rows[m] : (int)m;
+    }
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
         const int64_t mi = m0 + i * 16;
         if (mi >= m_end) break;
-        const int64_t m = mi + (lane & 15) < m_end ? mi + (lane & 15) : m_end - 1;
-        const float sa = p.sa[GROUPED && p.a_rows ? p.a_rows[m] : m];
 #pragma unroll
-        for (int j = 0; j < FN; j += GATED ? 2 : 1) {
-            const int c = (GATED ? j * 8 : j * 16) + (lane >> 4) * 4;  // column of the wave's outputs
-            const int n = nw + c, n_ok = p.N - n;
-            const v4f s = take4(sb + n, n_ok);
+        for (int j = 0; j < kFrags; ++j) {
+            const int c = j * 16 + (lane >> 4) * 4;  // column of the wave's outputs
             v4f v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * sa * s[e];
+            for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j * kStep][e] * sa[i] * s[j][e];
             if (bias) {
-                const v4f b = take4(bias + n, n_ok);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] += b[e];
+                for (int e = 0; e < 4; ++e) v[e] += b[j][e];
             }
             if (p.act == VDTTFS_ACT_RELU) {
 #pragma unroll
@@ -72,14 +95,12 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
                 for (int e = 0; e < 4; ++e) v[e] = apply_act(v[e], VDTTFS_ACT_SILU);
             }
             if constexpr (GATED) {
-                const v4f s2 = take4(sb + p.N + n, n_ok);
                 v4f u;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) u[e] = (float)acc[i][j + 1][e] * sa * s2[e];
+                for (int e = 0; e < 4; ++e) u[e] = (float)acc[i][j * 2 + 1][e] * sa[i] * s2[j][e];
                 if (bias) {
-                    const v4f b = take4(bias + p.N + n, n_ok);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) u[e] += b[e];
+                    for (int e = 0; e < 4; ++e) u[e] += b2[j][e];
                 }
                 v *= u;
             }
@@ -91,10 +112,10 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
 #pragma unroll
             for (int r = 0; r < 16; r += 64 / kLanes) {
                 const int row = r + lane / kLanes, c = lane % kLanes * 8;
+                const int64_t o = __shfl(o_row[i], row & 15, 64) * p.ldo + nw + c;
                 if (row >= 16 || mi + row >= m_end) continue;
                 const float* f = stage + row * S::kRow + c;
                 const v4f x = *reinterpret_cast<const v4f*>(f), y = *reinterpret_cast<const v4f*>(f + 4);
-                const int64_t o = (GROUPED && p.o_rows ? p.o_rows[mi + row] : mi + row) * p.ldo + nw + c;
                 *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + o) = make_uint4(
                     pack2(x[0], x[1], bf16), pack2(x[2], x[3], bf16), pack2(y[0], y[1], bf16), pack2(y[2], y[3], bf16));
             }
@@ -103,8 +124,8 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
 #pragma unroll
             for (int r = 0; r < 16; r += 64 / kLanes) {
                 const int row = r + lane / kLanes, c = lane % kLanes * 4;
+                const int64_t o = __shfl(o_row[i], row & 15, 64) * p.ldo + nw + c;
                 if (row >= 16 || mi + row >= m_end) continue;
-                const int64_t o = (GROUPED && p.o_rows ? p.o_rows[mi + row] : mi + row) * p.ldo + nw + c;
                 *reinterpret_cast<v4f*>(static_cast<float*>(p.out) + o) =
                     *reinterpret_cast<const v4f*>(stage + row * S::kRow + c);
             }
@@ -112,8 +133,8 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
 #pragma unroll 1
             for (int at = lane; at < 16 * S::kCols; at += 64) {
                 const int row = at / S::kCols, c = at % S::kCols;
+                const int64_t o = __shfl(o_row[i], row, 64) * p.ldo + nw + c;
                 if (mi + row >= m_end || nw + c >= p.N) continue;
-                const int64_t o = (GROUPED && p.o_rows ? p.o_rows[mi + row] : mi + row) * p.ldo + nw + c;
                 store_elem(p.out, o, stage[row * S::kRow + c], p.out_elem);
             }
         }
@@ -445,8 +466,13 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
             for (int j = 0; j < FN; ++j) read_b(s, 0, j);
             read_a(s, 1);
         };
+        // A tile's first kEarly loads go out behind the barrier that frees its
+        // LDS, the others between the first groups of the next tile: all at
+        // once they hold up the fragment reads.
+        constexpr int kEarly = 2, kPer = (NL - kEarly + G / 2 - 3) / (G / 2 - 2 > 0 ? G / 2 - 2 : 1);
+        static_assert(kEarly + kPer * (G - 2) >= NL, "all loads go out");
         auto run = [&](int8_t* s, int8_t* next, int t) __attribute__((always_inline)) {
-            const int k0 = k_of(t + 2);
+            const int k0 = k_of(t + 2), k1 = k_of(t + 1);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const int kk = g / FM, i = g % FM;
@@ -460,10 +486,10 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
                     barrier();
                     first(next);
                 }
-                if (g >= G - 2) {
+                if (g >= G - 2) fetch_one(s, k0, g - (G - 2));
+                else
 #pragma unroll
-                    for (int l = (g - (G - 2)) * NL / 2; l < (g - (G - 2) + 1) * NL / 2; ++l) fetch_one(s, k0, l);
-                }
+                    for (int l = kEarly + g * kPer; l < kEarly + (g + 1) * kPer && l < NL; ++l) fetch_one(next, k1, l);
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[kk & 1][j], fa[g % 4], acc[i][j], 0, 0, 0);
@@ -473,8 +499,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
         // at least two tiles (deep_ok)
         if (part) fetch_part(s0);
         else fetch(s0, 0);
-        fetch(s1, 1);
         wait_loads<0>();
+#pragma unroll
+        for (int l = 0; l < kEarly; ++l) fetch_one(s1, k_of(1), l);
         barrier();
         first(s0);
         for (int t = 0; t < tiles; t += 2) {
