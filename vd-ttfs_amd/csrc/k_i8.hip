@@ -40,9 +40,29 @@ struct Stage {
     static constexpr int kRow = kCols + 4;                  // floats from row to row
     static constexpr int kBytes = 16 * kRow * 4;
 };
-template <int FM, int FN, bool GATED, bool GROUPED>
-__device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][FN], int64_t m0, int64_t m_end, int n0,
-                                         int wn, const float* sb, const float* bias, float* stage) {
+// A lane's rows (m0 + 16 i + lane % 16): their scales and output rows.  Loaded
+// before the products, whose end would wait for them.
+template <int FM>
+struct Rows {
+    float sa[FM];
+    int o_row[FM];
+};
+template <int FM, bool GROUPED>
+__device__ __forceinline__ Rows<FM> rows_of(const I8Args& p, int64_t m0, int64_t m_end) {
+    Rows<FM> r;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        int64_t m = m0 + i * 16 + (lane_id() & 15);
+        if (m >= m_end) m = m_end - 1;
+        r.sa[i] = p.sa[GROUPED && p.a_rows ? p.a_rows[m] : m];
+        r.o_row[i] = GROUPED && p.o_rows ? p.o_rows[m] : (int)m;
+    }
+    return r;
+}
+template <int FM, int FN, bool GATED>
+__device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][FN], const Rows<FM>& rows, int64_t m0,
+                                         int64_t m_end, int n0, int wn, const float* sb, const float* bias,
+                                         float* stage) {
     typedef Stage<FM, FN, GATED> S;
     const int lane = lane_id();
     const int nw = n0 + (GATED ? wn / 2 : wn);  // the wave's first output column
@@ -64,15 +84,6 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
             if (bias) b2[j] = take4(bias + p.N + n, p.N - n, whole);
         }
     }
-    float sa[FM];
-    int o_row[FM];
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        int64_t m = m0 + i * 16 + (lane & 15);
-        if (m >= m_end) m = m_end - 1;
-        sa[i] = p.sa[GROUPED && p.a_rows ? p.a_rows[m] : m];
-        o_row[i] = GROUPED && p.o_rows ? p.o_rows[m] : (int)m;
-    }
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
         const int64_t mi = m0 + i * 16;
@@ -82,7 +93,7 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
             const int c = j * 16 + (lane >> 4) * 4;  // column of the wave's outputs
             v4f v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j * kStep][e] * sa[i] * s[j][e];
+            for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j * kStep][e] * rows.sa[i] * s[j][e];
             if (bias) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] += b[j][e];
@@ -97,7 +108,7 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
             if constexpr (GATED) {
                 v4f u;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) u[e] = (float)acc[i][j * 2 + 1][e] * sa[i] * s2[j][e];
+                for (int e = 0; e < 4; ++e) u[e] = (float)acc[i][j * 2 + 1][e] * rows.sa[i] * s2[j][e];
                 if (bias) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) u[e] += b2[j][e];
@@ -112,28 +123,29 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
 #pragma unroll
             for (int r = 0; r < 16; r += 64 / kLanes) {
                 const int row = r + lane / kLanes, c = lane % kLanes * 8;
-                const int64_t o = __shfl(o_row[i], row & 15, 64) * p.ldo + nw + c;
+                const int64_t o = __shfl(rows.o_row[i], row & 15, 64) * p.ldo + nw + c;
                 if (row >= 16 || mi + row >= m_end) continue;
                 const float* f = stage + row * S::kRow + c;
                 const v4f x = *reinterpret_cast<const v4f*>(f), y = *reinterpret_cast<const v4f*>(f + 4);
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + o) = make_uint4(
-                    pack2(x[0], x[1], bf16), pack2(x[2], x[3], bf16), pack2(y[0], y[1], bf16), pack2(y[2], y[3], bf16));
+                const v4i w = {(int)pack2(x[0], x[1], bf16), (int)pack2(x[2], x[3], bf16),
+                               (int)pack2(y[0], y[1], bf16), (int)pack2(y[2], y[3], bf16)};
+                __builtin_nontemporal_store(w, reinterpret_cast<v4i*>(static_cast<uint16_t*>(p.out) + o));
             }
         } else if (vec) {
             constexpr int kLanes = S::kCols / 4;
 #pragma unroll
             for (int r = 0; r < 16; r += 64 / kLanes) {
                 const int row = r + lane / kLanes, c = lane % kLanes * 4;
-                const int64_t o = __shfl(o_row[i], row & 15, 64) * p.ldo + nw + c;
+                const int64_t o = __shfl(rows.o_row[i], row & 15, 64) * p.ldo + nw + c;
                 if (row >= 16 || mi + row >= m_end) continue;
-                *reinterpret_cast<v4f*>(static_cast<float*>(p.out) + o) =
-                    *reinterpret_cast<const v4f*>(stage + row * S::kRow + c);
+                __builtin_nontemporal_store(*reinterpret_cast<const v4f*>(stage + row * S::kRow + c),
+                                            reinterpret_cast<v4f*>(static_cast<float*>(p.out) + o));
             }
         } else {
 #pragma unroll 1
             for (int at = lane; at < 16 * S::kCols; at += 64) {
                 const int row = at / S::kCols, c = at % S::kCols;
-                const int64_t o = __shfl(o_row[i], row, 64) * p.ldo + nw + c;
+                const int64_t o = __shfl(rows.o_row[i], row, 64) * p.ldo + nw + c;
                 if (mi + row >= m_end || nw + c >= p.N) continue;
                 store_elem(p.out, o, stage[row * S::kRow + c], p.out_elem);
             }
@@ -203,6 +215,7 @@ __global__ __launch_bounds__(WM* WN * 64) void k_i8_tile(I8Args p, int tiles_n) 
 
     const int wave = uniform(tid >> 6);
     const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+    const Rows<FM> rows = rows_of<FM, GROUPED>(p, m0 + wm, m_end);
     v4i acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -255,8 +268,8 @@ __global__ __launch_bounds__(WM* WN * 64) void k_i8_tile(I8Args p, int tiles_n) 
     }
 
     __syncthreads();
-    epilogue<FM, FN, GATED, GROUPED>(p, acc, m0 + wm, m_end, n0, wn, sb, bias,
-                                     reinterpret_cast<float*>(lds) + wave * (Stage<FM, FN, GATED>::kBytes / 4));
+    epilogue<FM, FN, GATED>(p, acc, rows, m0 + wm, m_end, n0, wn, sb, bias,
+                            reinterpret_cast<float*>(lds) + wave * (Stage<FM, FN, GATED>::kBytes / 4));
 }
 
 // XCD-aware tile order: workgroups are handed to the eight XCDs in turn, so
@@ -361,6 +374,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
 #pragma unroll
     for (int i = 0; i < NB; ++i) pb[i] = b_row(i);
     const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+    const Rows<FM> rows = rows_of<FM, GROUPED>(p, m0 + wm, m_end);
     v4i acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -548,8 +562,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
     }
     wait_loads<0>();  // also those past the end: the stage takes their place
     barrier();
-    epilogue<FM, FN, GATED, GROUPED>(p, acc, m0 + wm, m_end, n0, wn, sb, bias,
-                                     reinterpret_cast<float*>(s0) + wave * (Stage<FM, FN, GATED>::kBytes / 4));
+    epilogue<FM, FN, GATED>(p, acc, rows, m0 + wm, m_end, n0, wn, sb, bias,
+                            reinterpret_cast<float*>(s0) + wave * (Stage<FM, FN, GATED>::kBytes / 4));
 }
 
 // Rows of codes to rows on 128 bytes with zeros behind them, 16 codes a thread.
