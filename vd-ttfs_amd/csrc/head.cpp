@@ -333,21 +333,23 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
         VD_TRY(fuse2 ? launch_expert_product(ctx, h, VDTTFS_ELEM_F32, L.d_hidden, nullptr, d_idx, pairs, top_k, L,
                                              true, z)
                      : launch_expert_product(ctx, hq, kElemCodes, ldh, hs, d_idx, pairs, top_k, L, true, z));
-        return launch_combine(ctx, d_out, out_elem, ldo, z, VDTTFS_ELEM_F32, d_idx, d_weight, M, L.d_out, top_k,
-                              L.n_experts);
+        return launch_combine(ctx, d_out, out_elem, ldo, z, VDTTFS_ELEM_F32, L.d_out, d_idx, d_weight, M, L.d_out,
+                              top_k, L.n_experts);
     }
-    const int bm = i8_tile_rows(pairs, L.n_experts, L.d_in < L.d_hidden ? L.d_in : L.d_hidden);
+    const int bm = i8_tile_rows(pairs, L);
     const int64_t max_tiles = pairs / bm + (pairs < L.n_experts ? pairs : L.n_experts);
     Layout l;
     const size_t at_q = l.take((size_t)M * ldq), at_s = l.take((size_t)M * 4);
-    const size_t at_h = l.take((size_t)pairs * L.d_hidden * 4);
+    // rows of whole vectors, so that they are stored and read as such
+    const int64_t ldf = ((int64_t)L.d_hidden + 3) / 4 * 4, ldz = ((int64_t)L.d_out + 7) / 8 * 8;
+    const size_t at_h = l.take((size_t)pairs * ldf * 4);
     const size_t at_hq = l.take((size_t)pairs * ldh), at_hs = l.take((size_t)pairs * 4);
     // A BF16 output takes the slots' products in BF16: they are written and read
     // again, 2 x 537 MB in 32 bits for 8192 rows of 8 slots of 2048, and their
     // rounding is of the size of the output's own.  F16 would not hold a product
     // that its weight brings back into range, so it keeps 32 bits.
     const int z_elem = out_elem == VDTTFS_ELEM_BF16 ? VDTTFS_ELEM_BF16 : VDTTFS_ELEM_F32;
-    const size_t at_z = l.take((size_t)pairs * L.d_out * elem_size(z_elem));
+    const size_t at_z = l.take((size_t)pairs * ldz * elem_size(z_elem));
     const size_t at_pair = l.take((size_t)pairs * 4), at_row = l.take((size_t)pairs * 4);
     const size_t at_tiles = l.take((size_t)max_tiles * sizeof(int4)), at_n = l.take(4);
     const size_t at_hist = l.take((size_t)dispatch_blocks(pairs) * L.n_experts * 4);
@@ -370,7 +372,7 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
 
     VD_TRY(launch_quant_rows(ctx, d_x, x_elem, ldx, M, L.d_in, q, ldq, (int)ldq, s));
     VD_TRY(launch_dispatch(ctx, d_idx, pairs, top_k, L.n_experts, bm, d));
-    I8Args a = product(q, ldq, s, L.w1, L.d_in, L.s1, L.b1, h, VDTTFS_ELEM_F32, L.d_hidden, 0, L.d_hidden, L.d_in,
+    I8Args a = product(q, ldq, s, L.w1, L.d_in, L.s1, L.b1, h, VDTTFS_ELEM_F32, ldf, 0, L.d_hidden, L.d_in,
                        L.act);
     a.tiles = d.tiles;
     a.n_tiles = d.n_tiles;
@@ -387,8 +389,8 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
     }
     a.s_stride = H;
     VD_TRY(launch_i8_grouped(ctx, a, L.gated != 0, bm));
-    VD_TRY(launch_quant_rows(ctx, h, VDTTFS_ELEM_F32, L.d_hidden, pairs, L.d_hidden, hq, ldh, (int)ldh, hs));
-    I8Args b = product(hq, ldh, hs, L.w2, L.d_hidden, L.s2, L.b2, z, z_elem, L.d_out, 0, L.d_out,
+    VD_TRY(launch_quant_rows(ctx, h, VDTTFS_ELEM_F32, ldf, pairs, L.d_hidden, hq, ldh, (int)ldh, hs));
+    I8Args b = product(hq, ldh, hs, L.w2, L.d_hidden, L.s2, L.b2, z, z_elem, ldz, 0, L.d_out,
                        L.d_hidden, VDTTFS_ACT_NONE);
     b.tiles = d.tiles;
     b.n_tiles = d.n_tiles;
@@ -405,7 +407,7 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
     }
     b.s_stride = L.d_out;
     VD_TRY(launch_i8_grouped(ctx, b, false, bm));
-    return launch_combine(ctx, d_out, out_elem, ldo, z, z_elem, d_idx, d_weight, M, L.d_out, top_k, L.n_experts);
+    return launch_combine(ctx, d_out, out_elem, ldo, z, z_elem, ldz, d_idx, d_weight, M, L.d_out, top_k, L.n_experts);
 }
 
 }  // extern "C"

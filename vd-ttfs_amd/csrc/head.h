@@ -49,7 +49,7 @@ constexpr int kElemCodes = 4;
 bool small_ok(int64_t M, int N, int K, int elem);
 int launch_i8_small(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const I8Args& a);
 int launch_i8_grouped(vdttfs_ctx* ctx, const I8Args& a, bool gated, int bm);
-int i8_tile_rows(int64_t pairs, int n_experts, int k_min);
+int i8_tile_rows(int64_t pairs, const vdttfs_expert_layer& L);
 
 // The experts of few pairs without a sort: whether to, and whether each product
 // quantises its rows itself (d_hidden's are float [pairs][d_hidden]); one of the
@@ -78,8 +78,9 @@ struct Dispatch {
 int dispatch_blocks(int64_t pairs);
 int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_k, int n_experts, int bm,
                     const Dispatch& d);
-// out[m] = sum over slots of weight * z[m * top_k + slot], z F32 or BF16
-int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem,
+// out[m] = sum over slots of weight * z[m * top_k + slot], z F32 or BF16 in rows
+// of ldz, aligned for whole vectors (4 floats, 8 of BF16) if ldz is a multiple of one
+int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem, int64_t ldz,
                    const int32_t* idx, const float* wt, int64_t M, int N, int top_k, int n_experts);
 
 }  // namespace vdttfs

@@ -69,7 +69,7 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
     const int size = p.out_elem == VDTTFS_ELEM_F32 ? 4 : 2;
     const bool bf16 = p.out_elem == VDTTFS_ELEM_BF16;
     const bool whole = nw + S::kCols <= p.N;
-    const bool vec = whole && ((p.ldo * size) & 15) == 0 && (((uintptr_t)p.out + (size_t)nw * size) & 15) == 0;
+    const bool vec = ((p.ldo * size) & 15) == 0 && (((uintptr_t)p.out + (size_t)nw * size) & 15) == 0;
     // everything that comes from memory first: the stores below may alias it,
     // so a load between them would wait in line
     constexpr int kFrags = GATED ? FN / 2 : FN, kStep = GATED ? 2 : 1;
@@ -126,6 +126,11 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
                 const int64_t o = __shfl(rows.o_row[i], row & 15, 64) * p.ldo + nw + c;
                 if (row >= 16 || mi + row >= m_end) continue;
                 const float* f = stage + row * S::kRow + c;
+                if (nw + c + 8 > p.N) {
+#pragma unroll 1
+                    for (int e = 0; e < p.N - nw - c; ++e) store_elem(p.out, o + e, f[e], p.out_elem);
+                    continue;
+                }
                 const v4f x = *reinterpret_cast<const v4f*>(f), y = *reinterpret_cast<const v4f*>(f + 4);
                 const v4i w = {(int)pack2(x[0], x[1], bf16), (int)pack2(x[2], x[3], bf16),
                                (int)pack2(y[0], y[1], bf16), (int)pack2(y[2], y[3], bf16)};
@@ -138,6 +143,11 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
                 const int row = r + lane / kLanes, c = lane % kLanes * 4;
                 const int64_t o = __shfl(rows.o_row[i], row & 15, 64) * p.ldo + nw + c;
                 if (row >= 16 || mi + row >= m_end) continue;
+                if (nw + c + 4 > p.N) {
+#pragma unroll 1
+                    for (int e = 0; e < p.N - nw - c; ++e) store_elem(p.out, o + e, stage[row * S::kRow + c + e], p.out_elem);
+                    continue;
+                }
                 __builtin_nontemporal_store(*reinterpret_cast<const v4f*>(stage + row * S::kRow + c),
                                             reinterpret_cast<v4f*>(static_cast<float*>(p.out) + o));
             }
@@ -653,12 +663,19 @@ int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
     return run_big<32, 32, 2, 2, 128, 4>(ctx, a);
 }
 
-// Rows of a grouped product's tiles: the largest that an expert's rows fill on
-// average.
-int i8_tile_rows(int64_t pairs, int n_experts, int k_min) {
-    const int64_t mean = pairs / n_experts;
-    if (k_min < kDeepK) return mean >= 40 ? 64 : 32;
-    return mean >= 256 ? 256 : mean >= 96 ? 128 : mean >= 40 ? 64 : 32;
+// Rows of the tiles of a layer's two products: the largest that an expert's
+// rows fill on average, of which there are enough for the chip.
+int i8_tile_rows(int64_t pairs, const vdttfs_expert_layer& L) {
+    const int64_t mean = pairs / L.n_experts;
+    const int k_min = L.d_in < L.d_hidden ? L.d_in : L.d_hidden;
+    const int64_t hidden = L.gated ? 2 * (int64_t)L.d_hidden : L.d_hidden;
+    auto enough = [&](int bm, int bn) {
+        const int64_t rows = pairs / bm + L.n_experts / 2;
+        return rows * ((hidden + bn - 1) / bn) >= 192 && rows * ((L.d_out + bn - 1) / bn) >= 192;
+    };
+    if (k_min >= kDeepK && mean >= 256 && enough(256, 256)) return 256;
+    if (k_min >= kDeepK && mean >= 96 && enough(128, 128)) return 128;
+    return mean >= 40 && enough(64, 64) ? 64 : 32;
 }
 
 template <int BM, int BN, int WM, int WN, int S, bool GATED>

@@ -620,9 +620,9 @@ __global__ __launch_bounds__(1024) void k_sort_one(const int32_t* __restrict__ i
 // slots' loads are in flight at a time.  Z: float, or uint16_t for BF16.
 template <int VEC, typename Z>
 __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, int out_elem, int64_t ldo,
-                                                      const Z* __restrict__ z, const int32_t* __restrict__ idx,
-                                                      const float* __restrict__ wt, int64_t M, int N, int top_k,
-                                                      int E) {
+                                                      const Z* __restrict__ z, int64_t ldz,
+                                                      const int32_t* __restrict__ idx, const float* __restrict__ wt,
+                                                      int64_t M, int N, int top_k, int E) {
     typedef Z zvec __attribute__((ext_vector_type(VEC)));
     constexpr int kSlots = 8;
     const int n = (blockIdx.x * kThreads + threadIdx.x) * VEC;
@@ -642,7 +642,7 @@ __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, in
                 v[j] = zvec(Z(0));
                 if (on[j]) {
                     w[j] = wt[q];
-                    v[j] = *reinterpret_cast<const zvec*>(z + q * N + n);
+                    v[j] = *reinterpret_cast<const zvec*>(z + q * ldz + n);
                 }
             }
 #pragma unroll
@@ -656,7 +656,8 @@ __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, in
         }
         const int64_t o = m * ldo + n;
         const bool bf16 = out_elem == VDTTFS_ELEM_BF16;
-        if (VEC > 1 && out_elem != VDTTFS_ELEM_F32 && (((uintptr_t)out | (uintptr_t)(ldo * 2)) & (VEC * 2 - 1)) == 0) {
+        if (VEC > 1 && out_elem != VDTTFS_ELEM_F32 && n + VEC <= N &&
+            (((uintptr_t)out | (uintptr_t)(ldo * 2)) & (VEC * 2 - 1)) == 0) {
             uint32_t p[VEC / 2 + 1];
 #pragma unroll
             for (int i = 0; i < VEC / 2; ++i) p[i] = pack2(sum[2 * i], sum[2 * i + 1], bf16);
@@ -665,7 +666,8 @@ __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, in
             if constexpr (VEC == 4) *reinterpret_cast<uint2*>(to) = make_uint2(p[0], p[1]);
         } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) store_elem(out, o + i, sum[i], out_elem);
+            for (int i = 0; i < VEC; ++i)
+                if (n + i < N) store_elem(out, o + i, sum[i], out_elem);
         }
     }
 }
@@ -713,17 +715,18 @@ int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_
     return VDTTFS_OK;
 }
 
-int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem,
+int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem, int64_t ldz,
                    const int32_t* idx, const float* wt, int64_t M, int N, int top_k, int n_experts) {
     const bool bf16 = z_elem == VDTTFS_ELEM_BF16;
-    const int vec = bf16 && N % 8 == 0 ? 8 : !bf16 && N % 4 == 0 ? 4 : 1;
-    const dim3 grid((unsigned)((N / vec + kThreads - 1) / kThreads), (unsigned)(M < 65535 ? M : 65535));
-    const float* zf = static_cast<const float*>(z);
-    const uint16_t* zh = static_cast<const uint16_t*>(z);
-    if (vec == 8) k_combine<8><<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, zh, idx, wt, M, N, top_k, n_experts);
-    else if (bf16) k_combine<1><<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, zh, idx, wt, M, N, top_k, n_experts);
-    else if (vec == 4) k_combine<4><<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, zf, idx, wt, M, N, top_k, n_experts);
-    else k_combine<1><<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, zf, idx, wt, M, N, top_k, n_experts);
+    const int vec = bf16 && ldz % 8 == 0 ? 8 : !bf16 && ldz % 4 == 0 ? 4 : 1;
+    const dim3 grid((unsigned)(((N + vec - 1) / vec + kThreads - 1) / kThreads), (unsigned)(M < 65535 ? M : 65535));
+    const float* f = static_cast<const float*>(z);
+    const uint16_t* h = static_cast<const uint16_t*>(z);
+    const hipStream_t st = ctx->stream;
+    if (vec == 8) k_combine<8><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, h, ldz, idx, wt, M, N, top_k, n_experts);
+    else if (bf16) k_combine<1><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, h, ldz, idx, wt, M, N, top_k, n_experts);
+    else if (vec == 4) k_combine<4><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, f, ldz, idx, wt, M, N, top_k, n_experts);
+    else k_combine<1><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, f, ldz, idx, wt, M, N, top_k, n_experts);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
