@@ -395,6 +395,26 @@ def test_experts(ctx, M, k, E, D, F, N, x_elem, out_elem, kind, gated, bias, pad
     check(got, out_elem, y, d)
 
 
+@pytest.mark.parametrize("M,k,E,D,F,N", [
+    (16, 16, 64, 32, 200, 40),  # sixteen experts a workgroup, eight waves
+    (3, 9, 20, 24, 1000, 17), (7, 5, 9, 40, 130, 31), (30, 16, 16, 16, 65, 5), (2, 17, 20, 32, 70, 20),
+    (1, 3, 3, 48, 4000, 16), (11, 1, 2, 30, 64, 100)])
+@pytest.mark.parametrize("x_elem,out_elem,pad", [(R.F32, R.F32, 1), (R.BF16, R.BF16, 0)])
+def test_experts_of_few_rows(ctx, M, k, E, D, F, N, x_elem, out_elem, pad):
+    """Slots that do and do not divide a fragment's rows, and more of them; few and many experts a workgroup."""
+    rng = np.random.default_rng(M * 7 + k)
+    weights = expert_case(rng, E, D, F, N, False, True)
+    idx, wt = choose(rng, M, k, E)
+    bits = R.to_bits(rng.standard_normal((M, D)).astype(np.float32), x_elem)
+    got = run_experts(ctx, bits, x_elem, D, idx, wt, weights, R.RELU, False, out_elem, pad)
+    skip = (idx < 0) | (idx >= E)
+    y, d, mag = R.experts(*R.quant_rows(R.from_bits(bits, x_elem)), np.where(skip, -1, idx), np.where(skip, 0, wt),
+                          *weights, R.RELU, False)
+    if out_elem == R.BF16:
+        d = d + R.OUT_U[R.BF16] * mag
+    check(got, out_elem, y, d)
+
+
 def test_experts_uneven_and_unused(ctx):
     """All rows on one expert of many, then every slot of a row on the same one."""
     rng = np.random.default_rng(3)

@@ -316,7 +316,8 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
         const size_t at_q = l.take(fuse1 ? 0 : (size_t)M * ldq), at_s = l.take(fuse1 ? 0 : (size_t)M * 4);
         const size_t at_h = l.take((size_t)pairs * L.d_hidden * 4);
         const size_t at_hq = l.take(fuse2 ? 0 : (size_t)pairs * ldh), at_hs = l.take(fuse2 ? 0 : (size_t)pairs * 4);
-        const size_t at_z = l.take((size_t)pairs * L.d_out * 4);
+        const bool join = expert_out_ok(pairs, top_k, L, fuse2);
+        const size_t at_z = l.take(join ? 0 : (size_t)pairs * L.d_out * 4);
         unsigned char* buf;
         VD_TRY(head_scratch(ctx, l.bytes, &buf));
         int8_t* q = reinterpret_cast<int8_t*>(buf + at_q);
@@ -330,6 +331,10 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
                      : launch_expert_product(ctx, q, kElemCodes, ldq, s, d_idx, pairs, top_k, L, false, h));
         if (!fuse2)
             VD_TRY(launch_quant_rows(ctx, h, VDTTFS_ELEM_F32, L.d_hidden, pairs, L.d_hidden, hq, ldh, (int)ldh, hs));
+        if (join)
+            return fuse2 ? launch_expert_out(ctx, h, false, L.d_hidden, nullptr, d_idx, d_weight, M, top_k, L, d_out,
+                                             out_elem, ldo)
+                         : launch_expert_out(ctx, hq, true, ldh, hs, d_idx, d_weight, M, top_k, L, d_out, out_elem, ldo);
         VD_TRY(fuse2 ? launch_expert_product(ctx, h, VDTTFS_ELEM_F32, L.d_hidden, nullptr, d_idx, pairs, top_k, L,
                                              true, z)
                      : launch_expert_product(ctx, hq, kElemCodes, ldh, hs, d_idx, pairs, top_k, L, true, z));

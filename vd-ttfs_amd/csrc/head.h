@@ -78,6 +78,12 @@ struct Dispatch {
 int dispatch_blocks(int64_t pairs);
 int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_k, int n_experts, int bm,
                     const Dispatch& d);
+// The second product of few pairs and the sum over slots in one launch: out
+// from h [pairs][d_hidden], F32 (`fuse`, quantised in the kernel) or codes.
+bool expert_out_ok(int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool fuse);
+int launch_expert_out(vdttfs_ctx* ctx, const void* h, bool is_codes, int64_t ldh, const float* sa, const int32_t* idx,
+                      const float* wt, int64_t M, int top_k, const vdttfs_expert_layer& L, void* out, int out_elem,
+                      int64_t ldo);
 // out[m] = sum over slots of weight * z[m * top_k + slot], z F32 or BF16 in rows
 // of ldz, aligned for whole vectors (4 floats, 8 of BF16) if ldz is a multiple of one
 int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem, int64_t ldz,

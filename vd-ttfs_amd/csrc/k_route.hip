@@ -14,11 +14,16 @@ constexpr int kSortPairs = 2048;  // pairs a workgroup of the sort takes
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
-// Another lane's value by a data-parallel-primitive move (no LDS trip).
+// Another lane's value by a data-parallel-primitive move (no LDS trip); of all
+// lanes, or only of the rows in a mask, the others keeping theirs.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ int dpp_bits(int v) {
+    if constexpr (ROWS == 0xf) return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true);
+    else return __builtin_amdgcn_update_dpp(v, v, CTRL, ROWS, 0xf, false);
+}
 template <int CTRL, int ROWS = 0xf>
 __device__ __forceinline__ float dpp(float v) {
-    const int i = __float_as_int(v);
-    return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, ROWS, 0xf, false));
+    return __int_as_float(dpp_bits<CTRL, ROWS>(__float_as_int(v)));
 }
 constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140, kBcast15 = 0x142, kBcast31 = 0x143;
 
@@ -249,31 +254,49 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
 // 32-bit value leaves free, with the expert's index in them so that equal
 // values differ, the lower index above.  A maximum is then one instruction with
 // no second value to carry.
-constexpr double kNoKey = -1e300;  // not choosable
+// An infinite value goes as the largest finite one, and minus infinity, which
+// is not choosable, as one below kNoKey.
+constexpr double kNoKey = -1e299;
 __device__ __forceinline__ double make_key(float c, int e) {
-    // an infinite value goes as the largest finite one
-    const double d = (double)__builtin_amdgcn_fmed3f(c, -3.402823466e38f, 3.402823466e38f);
-    int hi = __double2hiint(d), lo = __double2loint(d);
-    lo |= (255 - e) ^ (hi >> 31 & 255);
-    const bool ok = c > neg_inf();
-    hi = ok ? hi : __double2hiint(kNoKey);
-    lo = ok ? lo : __double2loint(kNoKey);
-    return __hiloint2double(hi, lo);
+    const double d = __builtin_fmax((double)fminf(c, 3.402823466e38f), -1e300);
+    const int hi = __double2hiint(d), lo = __double2loint(d);
+    return __hiloint2double(hi, lo | (((255 - e) ^ hi >> 31) & 255));
 }
-__device__ __forceinline__ int key_expert(double key) {
-    return 255 - ((__double2loint(key) ^ __double2hiint(key) >> 31) & 255);
+// The choice value of a key as an integer of the same order, and the expert
+// from it and the key's low word.  kNone: the value of a key below kNoKey.
+__device__ __forceinline__ int key_value(double key) {
+    const int f = __float_as_int((float)key);
+    return f ^ ((f >> 31) & 0x7fffffff);
 }
-template <int CTRL>
-__device__ __forceinline__ double dpp64(double v) {
-    const int lo = __double2loint(v), hi = __double2hiint(v);
-    return __hiloint2double(__builtin_amdgcn_update_dpp(hi, hi, CTRL, 0xf, 0xf, false),
-                            __builtin_amdgcn_update_dpp(lo, lo, CTRL, 0xf, 0xf, false));
+__device__ __forceinline__ int key_expert(int value, int low) { return 255 - ((low ^ value >> 31) & 255); }
+constexpr int kNone = (int)(0xff800000u ^ 0x7fffffffu);
+// key[p0 .. p0 + N) in descending order, by Batcher's odd-even merges (K. E.
+// Batcher, "Sorting networks and their applications", 1968).
+template <int N>
+__device__ __forceinline__ void exchange(double (&key)[N], int i, int j) {
+    const double x = key[i], y = key[j];
+    key[i] = __builtin_fmax(x, y);
+    key[j] = __builtin_fmin(x, y);
 }
-__device__ __forceinline__ double row16_max(double v) {
-    v = __builtin_fmax(v, dpp64<kXor1>(v));
-    v = __builtin_fmax(v, dpp64<kXor2>(v));
-    v = __builtin_fmax(v, dpp64<kHalfMirror>(v));
-    return __builtin_fmax(v, dpp64<kMirror>(v));
+template <int COUNT, int N>
+__device__ __forceinline__ void sort_keys(double (&key)[N], int p0) {
+#pragma unroll
+    for (int p = 1; p < COUNT; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < COUNT; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < COUNT && (i + j) / (2 * p) == (i + j + q) / (2 * p))
+                        exchange(key, p0 + i + j, p0 + i + j + q);
+}
+// The largest over 16 lanes.
+__device__ __forceinline__ int row16_max(int v) {
+    v = max(v, dpp_bits<kXor1>(v));
+    v = max(v, dpp_bits<kXor2>(v));
+    v = max(v, dpp_bits<kHalfMirror>(v));
+    return max(v, dpp_bits<kMirror>(v));
 }
 __device__ __forceinline__ float row16_maxf(float v) {
     v = fmaxf(v, dpp<kXor1>(v));
@@ -292,14 +315,17 @@ __device__ __forceinline__ float row16_sum(float v) {
 // keys once and gives up its first whenever that is the row's largest, so a
 // choice costs a maximum over 16 lanes and a shift, for four rows at a time.
 // Bound by these instructions: 65536 rows of 256 experts, 8 chosen of 4 groups
-// of 8, take 38 us (7 by their bytes), and 80 with a wave per row and a search
+// of 8, take 36 us (7 by their bytes; some 850 vector instructions for four
+// rows, 200 of them the lanes' sorts), and 80 with a wave per row and a search
 // for every choice.  At most kPop choices, and groups that are whole lanes.
 constexpr int kPop = 8;
 template <int ELEM, int NPL>
 __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec) {
     __shared__ int hist[256];
     __shared__ int last;
+    __shared__ int chosen[64][kPop];  // of each row, from the lanes that held them
     const int lane = lane_id() & 15;
+    const uint64_t before = ((1ull << lane) - 1) << (lane_id() & 48);  // lanes of the row
     const int rows = blockDim.x / 16;
     if (a.count) {
         for (int e = threadIdx.x; e < a.E; e += blockDim.x) hist[e] = 0;
@@ -348,7 +374,7 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
             l[i] = l[i] > neg_inf() ? l[i] : neg_inf();  // NaN: not choosable
-            mx = fmaxf(mx, l[i]);
+            mx = __builtin_amdgcn_fmed3f(mx, l[i], -neg_inf());
         }
         float c[NPL];
         if (a.score == VDTTFS_SCORE_SOFTMAX) {
@@ -358,10 +384,9 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
             for (int i = 0; i < NPL; ++i) {
                 const float x = fast_exp(l[i] - mx);
                 c[i] = l[i] == mx ? 1.0f : x;  // an infinity less itself is none
-                c[i] = l[i] > neg_inf() ? c[i] : 0.0f;
                 sum += c[i];
             }
-            inv = 1.0f / row16_sum(sum);  // of a row without experts: not used
+            inv = 1.0f / row16_sum(sum);  // a row without experts has some too, not used
 #pragma unroll
             for (int i = 0; i < NPL; ++i) c[i] *= inv;
         } else {
@@ -371,13 +396,13 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
             const float v = c[i] + bias[i];
-            c[i] = l[i] > neg_inf() && v > neg_inf() ? v : neg_inf();
+            c[i] = fmaxf(l[i] > neg_inf() ? v : neg_inf(), neg_inf());
         }
         if (a.groups > 1) {
             float t0 = neg_inf(), t1 = neg_inf();
 #pragma unroll
             for (int i = 0; i < NPL; ++i) {
-                t1 = fmaxf(t1, fminf(t0, c[i]));
+                t1 = __builtin_amdgcn_fmed3f(t0, t1, c[i]);  // t1 <= t0
                 t0 = fmaxf(t0, c[i]);
             }
             auto merge = [&](float o0, float o1) {
@@ -403,43 +428,55 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
         double key[NPL];
 #pragma unroll
         for (int i = 0; i < NPL; ++i) key[i] = make_key(c[i], lane * NPL + i);
-        // descending, by Batcher's odd-even merges (K. E. Batcher, "Sorting
-        // networks and their applications", 1968)
+        if constexpr (NPL == 2 * kPop) {
+            // Of two sorted halves the larger of each first and the other's last:
+            // the first kPop of all, rising and then falling, so that exchanges
+            // over 4, 2 and 1 sort them.
+            sort_keys<kPop>(key, 0);
+            sort_keys<kPop>(key, kPop);
 #pragma unroll
-        for (int p = 1; p < NPL; p *= 2)
+            for (int i = 0; i < kPop; ++i) key[i] = __builtin_fmax(key[i], key[2 * kPop - 1 - i]);
 #pragma unroll
-            for (int q = p; q >= 1; q /= 2)
+            for (int q = kPop / 2; q >= 1; q /= 2)
 #pragma unroll
-                for (int j = q % p; j + q < NPL; j += 2 * q)
+                for (int i = 0; i < kPop; ++i)
+                    if ((i & q) == 0) exchange(key, i, i + q);
+        } else {
+            static_assert(NPL <= kPop, "a lane's keys");
+            sort_keys<NPL>(key, 0);
+        }
+        // Heads are compared by value; of lanes with the same the first, which has
+        // the lower experts, wins.
+        constexpr int kHeld = NPL < kPop ? NPL : kPop;
+        int value[kHeld], low[kHeld];
 #pragma unroll
-                    for (int i = 0; i < q; ++i)
-                        if (i + j + q < NPL && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
-                            const double x = key[i + j], y = key[i + j + q];
-                            key[i + j] = __builtin_fmax(x, y);
-                            key[i + j + q] = __builtin_fmin(x, y);
-                        }
-        double mine = kNoKey;
+        for (int i = 0; i < kHeld; ++i) {
+            value[i] = key_value(key[i]);
+            low[i] = __double2loint(key[i]);
+        }
+        int mine = kNone;
 #pragma unroll
         for (int j = 0; j < kPop; ++j) {
             if (j < a.k) {
-                const double best = row16_max(key[0]);
-                const bool win = key[0] == best;  // one lane, but where nothing is left
+                const int best = row16_max(value[0]);
+                const uint64_t heads = __ballot(value[0] == best);
+                const bool win = value[0] == best && (heads & before) == 0;
+                if (win) chosen[threadIdx.x / 16][j] = low[0];
 #pragma unroll
-                for (int i = 0; i + 1 < NPL && i + 1 < kPop - j; ++i) {
-                    const double up = key[i + 1], stay = key[i];
-                    key[i] = win ? up : stay;
+                for (int i = 0; i + 1 < kHeld && i + 1 < kPop - j; ++i) {
+                    const int v = value[i + 1], w = low[i + 1];
+                    value[i] = win ? v : value[i];
+                    low[i] = win ? w : low[i];
                 }
-                if (NPL < kPop - j) {
-                    const double stay = key[NPL - 1];
-                    key[NPL - 1] = win ? kNoKey : stay;
-                }
+                if (kHeld < kPop - j) value[kHeld - 1] = win ? kNone : value[kHeld - 1];
                 mine = lane == j ? best : mine;
             }
         }
+        wave_sync();
         int e = -1;
         float w = 0.0f;
-        if (mine > kNoKey) {
-            e = key_expert(mine);
+        if (mine > kNone) {
+            e = key_expert(mine, chosen[threadIdx.x / 16][lane]);
             const float v = load_elem<ELEM>(a.logits, m * a.ld + e);
             w = a.score != VDTTFS_SCORE_SOFTMAX ? fast_rcp(1.0f + fast_exp(-v))
                                                 : (v == mx ? 1.0f : fast_exp(v - mx)) * inv;
@@ -453,6 +490,7 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
             a.wt[m * a.k + lane] = w * a.scale;
             if (a.count && e >= 0) atomicAdd(&hist[e], 1);
         }
+        wave_sync();
     }
     if (a.count) finish_counts(a, hist, &last);
 }
@@ -718,13 +756,12 @@ int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_
 int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem, int64_t ldz,
                    const int32_t* idx, const float* wt, int64_t M, int N, int top_k, int n_experts) {
     const bool bf16 = z_elem == VDTTFS_ELEM_BF16;
-    const int vec = bf16 && ldz % 8 == 0 ? 8 : !bf16 && ldz % 4 == 0 ? 4 : 1;
+    const int vec = bf16 ? 8 : ldz % 4 == 0 ? 4 : 1;
     const dim3 grid((unsigned)(((N + vec - 1) / vec + kThreads - 1) / kThreads), (unsigned)(M < 65535 ? M : 65535));
     const float* f = static_cast<const float*>(z);
     const uint16_t* h = static_cast<const uint16_t*>(z);
     const hipStream_t st = ctx->stream;
-    if (vec == 8) k_combine<8><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, h, ldz, idx, wt, M, N, top_k, n_experts);
-    else if (bf16) k_combine<1><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, h, ldz, idx, wt, M, N, top_k, n_experts);
+    if (bf16) k_combine<8><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, h, ldz, idx, wt, M, N, top_k, n_experts);
     else if (vec == 4) k_combine<4><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, f, ldz, idx, wt, M, N, top_k, n_experts);
     else k_combine<1><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, f, ldz, idx, wt, M, N, top_k, n_experts);
     VD_HIP(hipGetLastError());

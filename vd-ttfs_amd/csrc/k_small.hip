@@ -164,9 +164,9 @@ __device__ __forceinline__ void rows_to_lds(const void* x, RowAt row, int rows, 
 // so that 16 rows read at one place come from different banks.
 __host__ __device__ __forceinline__ int lds_stride(int K) { return ((K + 63) & ~63) + 16; }
 
-// A wave's part of K for PARTS runs of 16 channels (a lane holds 16 codes of
+// One of `of` parts of K for PARTS runs of 16 channels (a lane holds 16 codes of
 // channel lane & 15 at a time): its first loads are issued by begin(), before
-// anything waits for the rows.  The last K % 64 codes are the last wave's.
+// anything waits for the rows.  The last K % 64 codes are the last part's.
 template <int PARTS>
 struct Weights {
     static constexpr int kHeld = kAhead / PARTS;
@@ -174,12 +174,12 @@ struct Weights {
     v4i ahead[PARTS][kHeld], tail[PARTS];
     int first, last, K, at_tail;  // steps of 64 codes
 
-    __device__ __forceinline__ void begin(int K_, int wave) {
+    __device__ __forceinline__ void begin(int K_, int part, int of) {
         K = K_;
-        const int steps = K / 64, per = (steps + kWaves - 1) / kWaves, g = (lane_id() >> 4) * 16;
-        first = wave * per;
+        const int steps = K / 64, per = (steps + of - 1) / of, g = (lane_id() >> 4) * 16;
+        first = part * per;
         last = first + per < steps ? first + per : steps;
-        at_tail = wave == kWaves - 1 && K > steps * 64 ? steps * 64 : -1;
+        at_tail = part == of - 1 && K > steps * 64 ? steps * 64 : -1;
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) row[p] += g;
 #pragma unroll
@@ -198,27 +198,32 @@ struct Weights {
             }
         }
     }
-    // acc[p] += channels x rows; rows: the lane's row of codes (lane & 15)
-    __device__ __forceinline__ void multiply(const int8_t* rows, v4i (&acc)[PARTS]) const {
+    // acc[p] += channels x rows; rows: the lane's row of codes (lane & 15), zeros
+    // in its place unless `keep`
+    __device__ __forceinline__ void multiply(const int8_t* rows, v4i (&acc)[PARTS], bool keep = true) const {
         rows += (lane_id() >> 4) * 16;
+        auto codes = [&](int k) __attribute__((always_inline)) {
+            const v4i a = *reinterpret_cast<const v4i*>(rows + k);
+            return keep ? a : v4i{0, 0, 0, 0};
+        };
 #pragma unroll
         for (int i = 0; i < kHeld; ++i)
             if (first + i < last) {
-                const v4i a = *reinterpret_cast<const v4i*>(rows + (first + i) * 64);
+                const v4i a = codes((first + i) * 64);
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p)
                     acc[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(ahead[p][i], a, acc[p], 0, 0, 0);
             }
 #pragma unroll 2
         for (int s = first + kHeld; s < last; ++s) {
-            const v4i a = *reinterpret_cast<const v4i*>(rows + s * 64);
+            const v4i a = codes(s * 64);
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
                 acc[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
                     reinterpret_cast<const Bytes16*>(row[p] + s * 64)->v, a, acc[p], 0, 0, 0);
         }
         if (at_tail >= 0) {
-            const v4i a = *reinterpret_cast<const v4i*>(rows + at_tail);
+            const v4i a = codes(at_tail);
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
                 acc[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(tail[p], a, acc[p], 0, 0, 0);
@@ -267,7 +272,7 @@ __global__ __launch_bounds__(kThreads) void k_i8_small(SmallArgs p) {
         const int n = n0 + (lane & 15);
         w.row[0] = p.w + (int64_t)(n < p.N ? n : p.N - 1) * p.ldw;
     }
-    w.begin(p.K, wave);
+    w.begin(p.K, wave, kWaves);
     if (ELEM == kCodes && (int)threadIdx.x < rows) scale[threadIdx.x] = p.sa[m0 + threadIdx.x];
     rows_to_lds<ELEM>(p.x, [&](int r) { return (m0 + r) * p.ldx; }, rows, p.K, p.sh, p.tfs, p.T, codes, stride,
                       scale, peak);
@@ -361,7 +366,7 @@ __global__ __launch_bounds__(kThreads) void k_expert_small(ExpertArgs p) {
 #pragma unroll
         for (int q = 0; q < kParts; ++q) w.row[q] = p.w + (ch0 + n + q * p.N) * p.K;
     }
-    w.begin(p.K, wave);
+    w.begin(p.K, wave, kWaves);
     for (int r0 = blockIdx.z * p.cap; r0 < n_rows; r0 += gridDim.z * p.cap) {
         const int rows = n_rows - r0 < p.cap ? n_rows - r0 : p.cap;
         auto x_row = [&](int r) { return BY_PAIR ? list[r0 + r] : list[r0 + r] / p.pairs.top_k; };
@@ -391,6 +396,117 @@ __global__ __launch_bounds__(kThreads) void k_expert_small(ExpertArgs p) {
             p.out[(int64_t)list[r0 + m] * p.N + n0 + n] = v;
         }
         __syncthreads();
+    }
+}
+
+// The experts' second product and its sum over the slots: out for 16 columns of
+// a few rows, whose pairs (16 at most) are the rows of one fragment.  Their
+// experts, each once, are shared out over the waves, and K too where there are
+// fewer; a pair's codes count in the products of its own expert alone, so one
+// accumulator serves them all.
+struct OutArgs {
+    const void* h;  // [pairs][K]
+    int64_t ldh;
+    const float* sa;  // scales of rows that are codes already
+    const int8_t* w;  // [E][N][K]
+    const float* sb;  // [E][N]
+    const float* bias;
+    const int32_t* idx;
+    const float* wt;
+    void* out;
+    int64_t ldo;
+    int64_t M;
+    int out_elem, N, K, top_k, n_experts;
+    int m_rows;  // rows of a workgroup
+    Share sh;
+};
+
+template <int ELEM>
+__global__ __launch_bounds__(kThreads) void k_expert_out(OutArgs p) {
+    extern __shared__ __align__(16) int8_t codes[];
+    __shared__ int part[kWaves * 256];
+    __shared__ float scale[kRows];
+    __shared__ int peak[kRows];
+    __shared__ float z[kRows][17];
+    const int lane = lane_id(), wave = uniform(threadIdx.x >> 6), stride = lds_stride(p.K);
+    const int n0 = blockIdx.x * 16;
+    const int64_t m0 = (int64_t)blockIdx.y * p.m_rows, q0 = m0 * p.top_k;
+    const int m_here = p.M - m0 < p.m_rows ? (int)(p.M - m0) : p.m_rows, pairs = m_here * p.top_k;
+    // the expert of pair lane & 15, -1 where it has none
+    int e = (lane & 15) < pairs ? p.idx[q0 + (lane & 15)] : -1;
+    if (e < 0 || e >= p.n_experts) e = -1;
+    int distinct = 0;
+    uint32_t firsts = 0;  // the first pair of each expert
+    for (int j = 0; j < pairs; ++j) {
+        const int ej = __builtin_amdgcn_readlane(e, j);
+        const uint32_t same = (uint32_t)__ballot(e == ej) & 0xffff;
+        if (ej >= 0 && __builtin_ctz(same) == j) {
+            firsts |= 1u << j;
+            ++distinct;
+        }
+    }
+    // expert number d (by its first pair); -1: the wave has none
+    auto expert_of = [&](int d) __attribute__((always_inline)) {
+        uint32_t left = firsts;
+        for (; d > 0; --d) left &= left - 1;
+        return __builtin_amdgcn_readlane(e, __builtin_ctz(left));
+    };
+    const int parts = distinct > 0 && distinct < kWaves ? kWaves / distinct : 1;
+    const int share = distinct < kWaves ? distinct : kWaves;  // waves of one part
+    const int my_part = share > 0 ? wave / share : parts;
+    int d = share > 0 ? wave % share : 0;
+    const int n_lane = n0 + (lane & 15) < p.N ? n0 + (lane & 15) : p.N - 1;
+    Weights<1> w;
+    int my_e = -1;
+    auto begin = [&]() __attribute__((always_inline)) {
+        my_e = expert_of(d);
+        w.row[0] = p.w + ((int64_t)my_e * p.N + n_lane) * p.K;
+        w.begin(p.K, my_part, parts);
+    };
+    if (my_part < parts) begin();
+    // what thread (pair, column) needs at the end
+    const int pair = threadIdx.x >> 4, n = n0 + (threadIdx.x & 15);
+    float sb = 0.0f, bias = 0.0f, wt = 0.0f;
+    int pe = -1;
+    if (pair < pairs && n < p.N) {
+        pe = p.idx[q0 + pair];
+        if (pe >= 0 && pe < p.n_experts) {
+            sb = p.sb[(int64_t)pe * p.N + n];
+            if (p.bias) bias = p.bias[(int64_t)pe * p.N + n];
+            wt = p.wt[q0 + pair];
+        } else {
+            pe = -1;
+        }
+    }
+    if (ELEM == kCodes && (int)threadIdx.x < pairs) scale[threadIdx.x] = p.sa[q0 + threadIdx.x];
+    rows_to_lds<ELEM>(p.h, [&](int r) { return (q0 + r) * p.ldh; }, pairs, p.K, p.sh, 0.0f, 1, codes, stride, scale,
+                      peak);
+    v4i acc[1] = {v4i{0, 0, 0, 0}};
+    if (my_part < parts) {
+        const int r = lane & 15;
+        const int8_t* row = codes + (r < pairs ? r : 0) * stride;
+        w.multiply(row, acc, e == my_e);
+        for (d += kWaves; d < distinct; d += kWaves) {
+            begin();
+            w.multiply(row, acc, e == my_e);
+        }
+    }
+    *reinterpret_cast<v4i*>(part + wave * 256 + lane * 4) = acc[0];
+    __syncthreads();
+    if (pair < kRows) {
+        float v = 0.0f;
+        if (pe >= 0) {
+            v = (float)gather(part, pair, threadIdx.x & 15) * scale[pair] * sb;
+            if (p.bias) v += bias;
+            v *= wt;
+        }
+        z[pair][threadIdx.x & 15] = v;
+    }
+    __syncthreads();
+    if (pair < m_here && n < p.N) {  // a row here
+        float sum = 0.0f;
+        for (int j = 0; j < p.top_k; ++j) sum += z[pair * p.top_k + j][threadIdx.x & 15];
+        store_elem(p.out, (m0 + pair) * p.ldo + n, sum, p.out_elem);
     }
 }
 
@@ -510,6 +626,40 @@ int launch_expert_product(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx,
     else if (!second) expert_elem<false, false>(ctx, p, elem, grid, lds);
     else if (elem == kCodes) k_expert_small<kCodes, false, true><<<grid, kThreads, lds, ctx->stream>>>(p);
     else k_expert_small<VDTTFS_ELEM_F32, false, true><<<grid, kThreads, lds, ctx->stream>>>(p);
+    VD_HIP(hipGetLastError());
+    return VDTTFS_OK;
+}
+
+// Every workgroup reads all experts of its rows' pairs, and quantises the pairs
+// if `fuse`, so it pays while there are few.  Measured (us, joined and with
+// launches of their own for product and sum; workgroups, MB of weights read):
+//   1 x 6 of 64, 1024-512-1024 gated (64, 3)      11.6  13.2
+//   256 x 2 of 8, 512-512-10 (32, 2)              17.2  19.3
+//   16 x 16 of 64, 512-512-512 (512, 64)          29.5  31.9
+//   40 x 4 of 32, 512-2048-512 (320, 160)         56.1  40.6
+//   256 x 2 of 8, 512-512-512 gated (1024, 64)    28.9  23.3
+bool expert_out_ok(int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool fuse) {
+    if (top_k > kRows) return false;
+    const int rows = (pairs < kRows ? (int)pairs : kRows) / top_k * top_k;
+    const int64_t blocks = (pairs + rows - 1) / rows * ((L.d_out + 15) / 16);
+    if (blocks > 512 || blocks * (rows < L.n_experts ? rows : L.n_experts) * 16 * L.d_hidden > 64 << 20) return false;
+    const Share sh = share_of(rows, L.d_hidden);
+    if (fuse && sh.passes * sh.turns > kUnits) return false;
+    return rows * lds_stride(L.d_hidden) <= 48 * 1024;
+}
+
+int launch_expert_out(vdttfs_ctx* ctx, const void* h, bool is_codes, int64_t ldh, const float* sa, const int32_t* idx,
+                      const float* wt, int64_t M, int top_k, const vdttfs_expert_layer& L, void* out, int out_elem,
+                      int64_t ldo) {
+    int m_rows = kRows / top_k;
+    if (M < m_rows) m_rows = (int)M;
+    const OutArgs p{h,   ldh, sa, L.w2,     L.s2,    L.b2,       idx,   wt,          out,
+                    ldo, M,   out_elem, L.d_out, L.d_hidden, top_k, L.n_experts, m_rows,
+                    share_of(m_rows * top_k, L.d_hidden)};
+    const dim3 grid((unsigned)((L.d_out + 15) / 16), (unsigned)((M + m_rows - 1) / m_rows));
+    const size_t lds = (size_t)m_rows * top_k * lds_stride(L.d_hidden);
+    if (is_codes) k_expert_out<kCodes><<<grid, kThreads, lds, ctx->stream>>>(p);
+    else k_expert_out<VDTTFS_ELEM_F32><<<grid, kThreads, lds, ctx->stream>>>(p);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
