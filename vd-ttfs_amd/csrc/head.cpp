@@ -311,7 +311,7 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
     const int64_t pairs = M * top_k;
     const int64_t ldq = padded(L.d_in), ldh = padded(L.d_hidden);
     bool fuse1, fuse2;
-    if (experts_small_ok(pairs, L, &fuse1, &fuse2)) {
+    if (experts_small_ok(pairs, top_k, L, &fuse1, &fuse2)) {
         Layout l;
         const size_t at_q = l.take(fuse1 ? 0 : (size_t)M * ldq), at_s = l.take(fuse1 ? 0 : (size_t)M * 4);
         const size_t at_h = l.take((size_t)pairs * L.d_hidden * 4);

@@ -55,7 +55,7 @@ int i8_tile_rows(int64_t pairs, const vdttfs_expert_layer& L);
 // quantises its rows itself (d_hidden's are float [pairs][d_hidden]); one of the
 // two products, out float [pairs][its columns], x codes with scales sa where
 // elem is kElemCodes.
-bool experts_small_ok(int64_t pairs, const vdttfs_expert_layer& L, bool* fuse1, bool* fuse2);
+bool experts_small_ok(int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool* fuse1, bool* fuse2);
 int launch_expert_product(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const int32_t* idx,
                           int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool second, float* out);
 

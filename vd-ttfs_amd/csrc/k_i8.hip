@@ -308,7 +308,12 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 // fills 1 KiB of LDS; the chunk that lies at place c of row r is chunk
 // c ^ swizzle(r), so that the 16 rows of a fragment come from all banks.
 // Needs 16-byte aligned rows; the last K % 16 codes go through registers with
-// zeros behind them.
+// zeros behind them (S > 2; the two-stage tiles take whole chunks only).
+// 8192x4096x4096 with the 256x256 tile takes 115 to 131 us, 2.1 to 2.4 POP/s of
+// the 5 there are, as the codes' own bits let the clock be.  A step of 128 codes
+// in K is 0.85 us of matrix instructions at their peak, 1.05 with the reads of
+// their fragments from LDS and 1.4 to 1.5 with the loads into it, so the loads
+// (64 KiB a step, from the XCD's L2) bound it; 10 us are the outputs.
 template <int BK>
 __device__ __forceinline__ int swizzle(int row) {
     return BK == 128 ? row & 7 : (row >> 2) & 3;
@@ -424,7 +429,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
     // address unit, and its matrix instructions with it.  Each group is one row
     // fragment against all channel fragments; fragments are read two groups
     // (channels: one k step) ahead.
-    constexpr int KK = BK / 64, G = KK * FM, kSpread = S == 2 ? (G + 1) / 2 : G;
+    constexpr int KK = BK / 64, G = KK * FM;
     auto multiply = [&](auto with_loads, const int8_t* s, int8_t* next, int k0) __attribute__((always_inline)) {
         const int r = lane & 15;
         v4i fa[3], fb[2][FN];
@@ -451,7 +456,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
             if constexpr (with_loads.value) {
 #pragma unroll
                 for (int l = 0; l < NL; ++l)
-                    if (l * kSpread / NL == g) fetch_one(next, k0, l);
+                    if (l * G / NL == g) fetch_one(next, k0, l);
             }
 #pragma unroll
             for (int j = 0; j < FN; ++j)
@@ -541,20 +546,20 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m
     } else if (tiles > 1) {
         if (part) fetch_part(s0);
         else fetch(s0, 0);
-        if (S > 2) fetch(s1, 1);
+        fetch(s1, 1);
         if (S > 3) fetch(s2, 2);
         int t = 0;
         for (; t + S <= tiles; t += S) {
-            step(s0, S == 2 ? s1 : S == 3 ? s2 : s3, t);
+            step(s0, S == 3 ? s2 : s3, t);
             step(s1, s0, t + 1);
-            if (S > 2) step(s2, s1, t + 2);
+            step(s2, s1, t + 2);
             if (S > 3) step(s3, s2, t + 3);
         }
         // the last tiles % S are in flight
         wait_loads<0>();
         barrier();
         if (t < tiles) multiply(std::false_type{}, s0, s0, 0);
-        if (S > 2 && t + 1 < tiles) multiply(std::false_type{}, s1, s1, 0);
+        if (t + 1 < tiles) multiply(std::false_type{}, s1, s1, 0);
         if (S > 3 && t + 2 < tiles) multiply(std::false_type{}, s2, s2, 0);
     }
     if (S > 2 && k16 < p.K) {
@@ -616,7 +621,7 @@ int launch_realign(vdttfs_ctx* ctx, const int8_t* from, int64_t ld, int64_t rows
 
 // Whether a product is large enough for rows that the two-stage tiles do not
 // take to be copied first, rather than read unaligned through registers (us,
-// with copies and without): 8192x4096x4095 153, 230; 4000x1000x1000 23, 17.
+// with copies and without): 8192x4096x4095 147, 394; 4000x1000x1000 23, 17.
 bool i8_wants_aligned(const I8Args& a) {
     return a.K >= kDeepK && !deep_ok(a) && (double)a.M * a.N * a.K >= 1e10 && tiles_of(a, 64, 64) >= 192;
 }
@@ -643,12 +648,13 @@ int run_tile(vdttfs_ctx* ctx, const I8Args& a) {
 // Rows on 16 bytes take the tiles that go to LDS directly: the largest tile of
 // which there are enough to fill the chip, as below that a CU's time goes by
 // the number of steps in K, whatever the tile.  Measured (us, K last):
-//   8192x4096x4096: 256x256 128, 128x128 158, 64x128 187
-//   1536x8192x2048 (192 tiles of 256): 34, 39, 41;  2560x8192x2048 (320, so
-//   two rounds, the second a quarter full): 65, 60, 67
-//   1024x4096x4096 (256 of 128): 128x128 29, 64x128 27, 64x64 34
-//   256x4096x4096: 64x128 14.7, 64x64 10.4, 32x32 15.1;  64x4096x4096: 64x64
-//   10.0, 32x32 7.6;  333x1111x1003: 64x64 8.0, 32x32 4.9
+//   8192x4096x4096: 256x256 131, 128x128 155, 64x128 183, 64x64 219
+//   1536x8192x2048 (192 tiles of 256): 32, 36, 37, 45;  2560x8192x2048 (320, so
+//   two rounds, the second a quarter full): 62, 53, 58, 72
+//   1024x4096x4096 (256 of 128): 128x128 28, 64x128 23, 64x64 27
+//   256x4096x4096: 64x128 14.7, 64x64 10.2, 32x32 14.2;  64x4096x4096: 64x64
+//   9.6, 32x32 7.6;  333x1111x1024: 64x64 7.3, 32x32 4.6
+// Rows off 16 bytes and not worth a copy go through registers.
 int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
     if (a.M <= 0 || a.N <= 0) return VDTTFS_OK;
     auto tiles = [&](int bm, int bn) { return tiles_of(a, bm, bn); };

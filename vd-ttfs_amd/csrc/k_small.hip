@@ -1,6 +1,6 @@
 // Products of few rows: the weights stream once from memory into the matrix
 // instructions, and the rows are quantised inside the kernel, so a call is one
-// launch (experts: two, and their sum).
+// launch (experts: two or three).
 #include "codes.h"
 #include "head.h"
 #include "quant.h"
@@ -515,9 +515,10 @@ __global__ __launch_bounds__(kThreads) void k_expert_out(OutArgs p) {
 // Few rows, or layers so small that launches count.  Every workgroup quantises
 // its rows, some 1.1 us for each run of eight a thread has, so two at most; past
 // that a launch of its own does it (5x4096x4096 of BF16: 12.3 us, so 9.8).
-// Measured (us, against quantisation and tiles): 1x4096x4096 of BF16 6.7, 10.8;
-// 16x512x512 5.9, 7.3; 128x512x512 5.6, 7.2; 256x512x512 7.4, 7.0, of spike
-// times 5.7, 7.2, 512 rows of them 8.6, 6.9.  Codes, 5x4096x4096: 5.7, tiles 7.3.
+// Measured (us, against quantisation and tiles): 1x4096x4096 of BF16 6.7, 11.2;
+// 16x512x512 5.5, 7.3; 128x512x512 5.6, 7.4; 256x512x512 7.7, 6.8, of spike
+// times 5.7, 7.2, 512 rows of them 8.6, 6.9.  Codes, 1x4096x4096: 5.2 (3.2 TB/s
+// of weights, and a launch), tiles 7.5; 5 rows 5.8, 7.6.
 bool small_ok(int64_t M, int N, int K, int elem) {
     const int64_t rows = M < kRows ? M : kRows;
     const Share sh = share_of((int)rows, K);
@@ -556,20 +557,29 @@ static int expert_rows(int64_t pairs, int K, bool codes) {
 
 // Measured (us; rows x slots of experts, d_in-d_hidden-d_out; quantising in the
 // products, before them, and sorted with tiles):
-//   1 x 6 of 64, 1024-512-1024 gated   13.5  17.3  23.8
-//   32 x 2 of 8, 512-512-512           14.2  16.8  24.2
-//   16 x 2 of 16, 2048-1024-2048 gated 42.2  37.1  41.7
-//   256 x 2 of 8, 512-512-10           28.1  21.6  30.2 (the second quantising: 19.3)
-//   256 x 2 of 8, 512-512-512 gated    34.8  25.9  28.1
-//   256 x 4 of 64, 512-512-512 gated   71.5  46.5  39.3
-bool experts_small_ok(int64_t pairs, const vdttfs_expert_layer& L, bool* fuse1, bool* fuse2) {
+//   1 x 6 of 64, 1024-512-1024 gated   11.4  15.7  21.8
+//   32 x 2 of 8, 512-512-512           14.7  16.6  21.9 (the second before: 14.1)
+//   256 x 2 of 8, 512-512-10           22.9  18.9  23.5 (the first before: 17.2)
+//   256 x 2 of 8, 512-512-512 gated    30.9  23.3  23.4
+// Past two workgroups a CU in the first product, sorted tiles are as good or
+// better, but for one row, which shares no weights (these kernels, and tiles):
+//   2 x 4 of 16, 2048-1024-2048 gated (512 workgroups)    19.0  27.1
+//   4 x 2 of 8, 4096-1024-4096 gated (512)                27.2  34.8
+//   16 x 2 of 16, 2048-1024-2048 gated (1024)             41.4  35.3
+//   32 x 4 of 32, 512-512-512 (1024)                      22.8  23.8
+//   128 x 4 of 64, 512-512-512 gated (2048)               37.2  30.5
+//   1 x 4 of 8, 4096-4096-4096 gated (1024)               55.9  65.9
+//   1 x 8 of 128, 4096-2048-4096 gated (1024)             59.7  57.1
+bool experts_small_ok(int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool* fuse1, bool* fuse2) {
     // every 16 columns quantise an expert's rows again
     auto fuse = [&](int K, int N) {
         return expert_rows(pairs, K, false) > 0 && (pairs * K <= 32768 || N <= 32);
     };
     *fuse1 = fuse(L.d_in, L.d_hidden);
     *fuse2 = fuse(L.d_hidden, L.d_out);
-    return pairs <= kMaxPairs && expert_rows(pairs, L.d_in, !*fuse1) && expert_rows(pairs, L.d_hidden, !*fuse2);
+    const int64_t blocks = (pairs < L.n_experts ? pairs : L.n_experts) * ((L.d_hidden + 15) / 16);
+    if (pairs > kMaxPairs || (blocks > 512 && pairs > top_k)) return false;
+    return expert_rows(pairs, L.d_in, !*fuse1) && expert_rows(pairs, L.d_hidden, !*fuse2);
 }
 
 template <bool GATED, bool BY_PAIR>
