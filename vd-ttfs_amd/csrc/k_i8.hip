@@ -88,6 +88,18 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
     for (int i = 0; i < FM; ++i) {
         const int64_t mi = m0 + i * 16;
         if (mi >= m_end) break;
+        // the vectors that a lane stores where all 16 rows and all columns are
+        // there: their places are known before the sums are
+        constexpr int kPut2 = S::kCols < 32 ? 1 : S::kCols / 32, kPut4 = S::kCols / 16;  // of 2 bytes, of 4
+        int64_t to[kPut4];
+        const bool full = whole && vec && mi + 16 <= m_end && (S::kCols >= 32 || size == 4);
+        if (full) {
+            const int per = size == 2 ? S::kCols / 8 : S::kCols / 4;  // lanes of a row
+#pragma unroll
+            for (int r = 0; r < kPut4; ++r)
+                if (r < kPut2 || size == 4)
+                    to[r] = __shfl(rows.o_row[i], (r * (64 / per) + lane / per) & 15, 64) * p.ldo + nw + lane % per * (16 / size);
+        }
 #pragma unroll
         for (int j = 0; j < kFrags; ++j) {
             const int c = j * 16 + (lane >> 4) * 4;  // column of the wave's outputs
@@ -118,7 +130,35 @@ __device__ __forceinline__ void epilogue(const I8Args& p, const v4i (&acc)[FM][F
             *reinterpret_cast<v4f*>(stage + (lane & 15) * S::kRow + c) = v;
         }
         wave_sync();
-        if (vec && size == 2) {
+        if (full && size == 2) {
+            constexpr int kLanes = S::kCols / 8;
+            v4f x[kPut2], y[kPut2];
+#pragma unroll
+            for (int r = 0; r < kPut2; ++r) {
+                const float* f = stage + (r * (64 / kLanes) + lane / kLanes) * S::kRow + lane % kLanes * 8;
+                x[r] = *reinterpret_cast<const v4f*>(f);
+                y[r] = *reinterpret_cast<const v4f*>(f + 4);
+            }
+#pragma unroll
+            for (int r = 0; r < kPut2; ++r) {
+                v4i w;
+                if (bf16) w = v4i{(int)pack2(x[r][0], x[r][1], true), (int)pack2(x[r][2], x[r][3], true),
+                                  (int)pack2(y[r][0], y[r][1], true), (int)pack2(y[r][2], y[r][3], true)};
+                else w = v4i{(int)pack2(x[r][0], x[r][1], false), (int)pack2(x[r][2], x[r][3], false),
+                             (int)pack2(y[r][0], y[r][1], false), (int)pack2(y[r][2], y[r][3], false)};
+                __builtin_nontemporal_store(w, reinterpret_cast<v4i*>(static_cast<uint16_t*>(p.out) + to[r]));
+            }
+        } else if (full) {
+            constexpr int kLanes = S::kCols / 4;
+            v4f x[kPut4];
+#pragma unroll
+            for (int r = 0; r < kPut4; ++r)
+                x[r] = *reinterpret_cast<const v4f*>(stage + (r * (64 / kLanes) + lane / kLanes) * S::kRow +
+                                                     lane % kLanes * 4);
+#pragma unroll
+            for (int r = 0; r < kPut4; ++r)
+                __builtin_nontemporal_store(x[r], reinterpret_cast<v4f*>(static_cast<float*>(p.out) + to[r]));
+        } else if (vec && size == 2) {
             constexpr int kLanes = S::kCols / 8;  // lanes of a row
 #pragma unroll
             for (int r = 0; r < 16; r += 64 / kLanes) {
