@@ -349,7 +349,7 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 // c ^ swizzle(r), so that the 16 rows of a fragment come from all banks.
 // Needs 16-byte aligned rows; the last K % 16 codes go through registers with
 // zeros behind them (S > 2; the two-stage tiles take whole chunks only).
-// 8192x4096x4096 with the 256x256 tile takes 115 to 131 us, 2.1 to 2.4 POP/s of
+// 8192x4096x4096 with the 256x256 tile takes 114 to 125 us, 2.2 to 2.4 POP/s of
 // the 5 there are, as the codes' own bits let the clock be.  A step of 128 codes
 // in K is 0.85 us of matrix instructions at their peak, 1.05 with the reads of
 // their fragments from LDS and 1.4 to 1.5 with the loads into it, so the loads
@@ -688,7 +688,7 @@ int run_tile(vdttfs_ctx* ctx, const I8Args& a) {
 // Rows on 16 bytes take the tiles that go to LDS directly: the largest tile of
 // which there are enough to fill the chip, as below that a CU's time goes by
 // the number of steps in K, whatever the tile.  Measured (us, K last):
-//   8192x4096x4096: 256x256 131, 128x128 155, 64x128 183, 64x64 219
+//   8192x4096x4096: 256x256 125, 128x128 155, 64x128 183, 64x64 219
 //   1536x8192x2048 (192 tiles of 256): 32, 36, 37, 45;  2560x8192x2048 (320, so
 //   two rounds, the second a quarter full): 62, 53, 58, 72
 //   1024x4096x4096 (256 of 128): 128x128 28, 64x128 23, 64x64 27

@@ -257,10 +257,12 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
 // An infinite value goes as the largest finite one, and minus infinity, which
 // is not choosable, as one below kNoKey.
 constexpr double kNoKey = -1e299;
-__device__ __forceinline__ double make_key(float c, int e) {
-    const double d = __builtin_fmax((double)fminf(c, 3.402823466e38f), -1e300);
+__device__ __forceinline__ double with_index(double d, int e) {
     const int hi = __double2hiint(d), lo = __double2loint(d);
     return __hiloint2double(hi, lo | (((255 - e) ^ hi >> 31) & 255));
+}
+__device__ __forceinline__ double make_key(float c, int e) {
+    return with_index(__builtin_fmax((double)fminf(c, 3.402823466e38f), -1e300), e);
 }
 // The choice value of a key as an integer of the same order, and the expert
 // from it and the key's low word.  kNone: the value of a key below kNoKey.
@@ -315,7 +317,7 @@ __device__ __forceinline__ float row16_sum(float v) {
 // keys once and gives up its first whenever that is the row's largest, so a
 // choice costs a maximum over 16 lanes and a shift, for four rows at a time.
 // Bound by these instructions: 65536 rows of 256 experts, 8 chosen of 4 groups
-// of 8, take 36 us (7 by their bytes; some 850 vector instructions for four
+// of 8, take 35 us (7 by their bytes; some 800 vector instructions for four
 // rows, 200 of them the lanes' sorts), and 80 with a wave per row and a search
 // for every choice.  At most kPop choices, and groups that are whole lanes.
 constexpr int kPop = 8;
@@ -324,6 +326,7 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
     __shared__ int hist[256];
     __shared__ int last;
     __shared__ int chosen[64][kPop];  // of each row, from the lanes that held them
+    __shared__ __align__(16) double group_keys[64][16];
     const int lane = lane_id() & 15;
     const uint64_t before = ((1ull << lane) - 1) << (lane_id() & 48);  // lanes of the row
     const int rows = blockDim.x / 16;
@@ -414,12 +417,21 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
             if (span > 4) merge(dpp<kHalfMirror>(t0), dpp<kHalfMirror>(t1));
             if (span > 8) merge(dpp<kMirror>(t0), dpp<kMirror>(t1));
             const float g = a.group_top == 2 && t1 > neg_inf() ? t0 + t1 : t0;
-            const int mine = lane / span;
-            int rank = 0;  // a group stays if fewer than top_groups come before it
-            for (int o = 0; o < a.groups; ++o) {
-                const float v = __shfl(g, o * span, 16);
-                rank += v > g || (v == g && o < mine) ? 1 : 0;
+            // a group stays if fewer than top_groups come before it: keys again,
+            // the row's through LDS
+            const double k = with_index(__builtin_fmin(__builtin_fmax((double)g, -1e300), 1e300), lane / span);
+            double* keys = group_keys[threadIdx.x / 16];
+            if (lane % span == 0) keys[lane / span] = k;
+            if (lane >= a.groups) keys[lane] = 2 * -1e300;
+            wave_sync();
+            int rank = 0;
+#pragma unroll
+            for (int o = 0; o < 8; ++o) rank += keys[o] > k ? 1 : 0;
+            if (a.groups > 8) {
+#pragma unroll
+                for (int o = 8; o < 16; ++o) rank += keys[o] > k ? 1 : 0;
             }
+            wave_sync();
             if (rank >= a.top_groups) {
 #pragma unroll
                 for (int i = 0; i < NPL; ++i) c[i] = neg_inf();
