@@ -228,7 +228,7 @@ int vdttfs_destroy(vdttfs_ctx* ctx) {
     (void)hipSetDevice(ctx->device);
     (void)hipStreamSynchronize(ctx->stream);
     void* bufs[] = {ctx->ref_cin,  ctx->ref_tin,     ctx->ref_off,  ctx->bin_ev,
-                    ctx->mrg_list, ctx->d_counters, ctx->split_buf, ctx->head_buf, ctx->route_acc};
+                    ctx->mrg_list, ctx->d_counters, ctx->split_buf};
     for (void* b : bufs)
         if (b) (void)hipFree(b);
     for (void* b : ctx->split_kept) (void)hipFree(b);

@@ -17,6 +17,21 @@ struct __align__(8) vd_event {
     float alpha;
 };
 
+// Scratch of the 8-bit heads: grown as split_buf is, and freed with its context.
+struct HeadScratch {
+    void* buf = nullptr;
+    size_t bytes = 0;
+    bool captured = false;     // a captured graph holds buf's address
+    int* route_acc = nullptr;  // routing's counters, 0 between calls
+    HeadScratch() = default;
+    HeadScratch(const HeadScratch&) = delete;
+    HeadScratch& operator=(const HeadScratch&) = delete;
+    ~HeadScratch() {
+        if (buf) (void)hipFree(buf);
+        if (route_acc) (void)hipFree(route_acc);
+    }
+};
+
 struct vdttfs_ctx {
     vdttfs_consts c;
     int NC;  // ceil(T/delta)
@@ -42,11 +57,7 @@ struct vdttfs_ctx {
     size_t split_bytes;
     bool split_captured;
     std::vector<void*> split_kept;
-    // scratch of the 8-bit heads, kept as split_buf is
-    void* head_buf;
-    size_t head_bytes;
-    bool head_captured;
-    int* route_acc;  // routing's counters, 0 between calls
+    HeadScratch head;
     bool named_skip;  // a split call could not size its named plan's scratch too
     unsigned long long* d_counters;  // kCounterStripes x 4 u64 (summed on the host)
     hipEvent_t timer[2];             // vdttfs_timer_begin/end (created on first use)

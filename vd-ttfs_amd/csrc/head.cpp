@@ -62,28 +62,28 @@ int head_scratch(vdttfs_ctx* ctx, size_t bytes, unsigned char** out) {
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     VD_HIP(hipStreamIsCapturing(ctx->stream, &cs));
     const bool capturing = cs != hipStreamCaptureStatusNone;
-    if (!ctx->head_buf || ctx->head_bytes < bytes) {
+    if (!ctx->head.buf || ctx->head.bytes < bytes) {
         if (capturing)
             return set_error(VDTTFS_E_UNSUPPORTED,
                              "the context's scratch is too small and cannot grow under stream capture: run the call "
                              "once before capturing it");
         VD_HIP(hipStreamSynchronize(ctx->stream));
-        if (ctx->head_captured)
-            ctx->split_kept.push_back(ctx->head_buf);
-        else if (ctx->head_buf)
-            VD_HIP(hipFree(ctx->head_buf));
-        ctx->head_buf = nullptr;
-        ctx->head_bytes = 0;
-        ctx->head_captured = false;
-        if (hipMalloc(&ctx->head_buf, bytes) != hipSuccess) {
-            ctx->head_buf = nullptr;
+        if (ctx->head.captured)
+            ctx->split_kept.push_back(ctx->head.buf);
+        else if (ctx->head.buf)
+            VD_HIP(hipFree(ctx->head.buf));
+        ctx->head.buf = nullptr;
+        ctx->head.bytes = 0;
+        ctx->head.captured = false;
+        if (hipMalloc(&ctx->head.buf, bytes) != hipSuccess) {
+            ctx->head.buf = nullptr;
             (void)hipGetLastError();
             return set_error(VDTTFS_E_NOMEM, "device allocation of %zu bytes failed", bytes);
         }
-        ctx->head_bytes = bytes;
+        ctx->head.bytes = bytes;
     }
-    ctx->head_captured |= capturing;
-    *out = static_cast<unsigned char*>(ctx->head_buf);
+    ctx->head.captured |= capturing;
+    *out = static_cast<unsigned char*>(ctx->head.buf);
     return VDTTFS_OK;
 }
 
@@ -107,7 +107,7 @@ int route_counters(vdttfs_ctx* ctx) {
         (void)hipFree(p);
         return hip_error(e, "route counters", __LINE__);
     }
-    ctx->route_acc = static_cast<int*>(p);
+    ctx->head.route_acc = static_cast<int*>(p);
     return VDTTFS_OK;
 }
 
@@ -283,8 +283,8 @@ int vdttfs_route(vdttfs_ctx* ctx, int32_t* d_idx, float* d_weight, int32_t* d_co
         VD_TRY(check_float_ptr("route", d_logits, elem_size(elem)));
         if (d_bias) VD_TRY(check_float_ptr("route", d_bias, 4));
     }
-    if (d_count && M > kRouteAlone && !ctx->route_acc) VD_TRY(route_counters(ctx));
-    return launch_route(ctx, d_idx, d_weight, d_count, d_logits, elem, ld, d_bias, d_row_mask, M, o, ctx->route_acc);
+    if (d_count && M > kRouteAlone && !ctx->head.route_acc) VD_TRY(route_counters(ctx));
+    return launch_route(ctx, d_idx, d_weight, d_count, d_logits, elem, ld, d_bias, d_row_mask, M, o, ctx->head.route_acc);
 }
 
 int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const void* d_x, int x_elem, int64_t ldx,

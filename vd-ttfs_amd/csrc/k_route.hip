@@ -255,8 +255,7 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
 // values differ, the lower index above.  A maximum is then one instruction with
 // no second value to carry.
 // An infinite value goes as the largest finite one, and minus infinity, which
-// is not choosable, as one below kNoKey.
-constexpr double kNoKey = -1e299;
+// is not choosable, as one below all floats.
 __device__ __forceinline__ double with_index(double d, int e) {
     const int hi = __double2hiint(d), lo = __double2loint(d);
     return __hiloint2double(hi, lo | (((255 - e) ^ hi >> 31) & 255));
@@ -265,7 +264,8 @@ __device__ __forceinline__ double make_key(float c, int e) {
     return with_index(__builtin_fmax((double)fminf(c, 3.402823466e38f), -1e300), e);
 }
 // The choice value of a key as an integer of the same order, and the expert
-// from it and the key's low word.  kNone: the value of a key below kNoKey.
+// from it and the key's low word.  kNone: the value of a key that is below all
+// floats, minus infinity.
 __device__ __forceinline__ int key_value(double key) {
     const int f = __float_as_int((float)key);
     return f ^ ((f >> 31) & 0x7fffffff);

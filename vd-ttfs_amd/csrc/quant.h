@@ -71,8 +71,9 @@ struct Raw8 {
     static constexpr bool kWide = ELEM == VDTTFS_ELEM_F32 || ELEM == VDTTFS_ELEM_TIMES;
     uint4 v[kWide ? 2 : 1];
 };
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 struct __attribute__((packed, aligned(1))) AnyUint4 {
-    uint4 v;
+    v4u v;
 };
 // What is not there: 0, or no spike.
 template <int ELEM>
@@ -90,8 +91,12 @@ __device__ __forceinline__ Raw8<ELEM> raw8(const void* x, int64_t at) {
     Raw8<ELEM> r;
     const AnyUint4* p =
         reinterpret_cast<const AnyUint4*>(static_cast<const char*>(x) + at * (Raw8<ELEM>::kWide ? 4 : 2));
-    r.v[0] = p[0].v;
-    if constexpr (Raw8<ELEM>::kWide) r.v[1] = p[1].v;
+    const v4u a = p[0].v;
+    r.v[0] = make_uint4(a[0], a[1], a[2], a[3]);
+    if constexpr (Raw8<ELEM>::kWide) {
+        const v4u b = p[1].v;
+        r.v[1] = make_uint4(b[0], b[1], b[2], b[3]);
+    }
     return r;
 }
 template <int ELEM>
