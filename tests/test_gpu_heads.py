@@ -283,6 +283,16 @@ def test_route(ctx, case, elem, M, pad):
         assert len(set(gi[m][there])) == there.sum() == (ri[m] >= 0).sum()
 
 
+@pytest.mark.parametrize("case", [  # groups that end inside a lane's experts, or leave lanes without any
+    (12, 4, 0, 2, 1, 1, False, True), (48, 5, 1, 8, 3, 2, True, True), (24, 8, 1, 4, 3, 2, True, False),
+    (60, 3, 0, 3, 2, 1, False, True), (35, 8, 1, 5, 2, 2, True, True), (51, 4, 0, 1, 1, 1, True, False),
+    (198, 6, 1, 6, 3, 2, True, True), (250, 8, 0, 2, 1, 2, False, True), (16, 2, 1, 16, 5, 1, True, True)],
+    ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("elem,M,pad", [(R.F32, 700, 0), (R.BF16, 133, 4), (R.F16, 5001, 1)])
+def test_route_groups_of_any_size(ctx, case, elem, M, pad):
+    test_route(ctx, case, elem, M, pad)
+
+
 @pytest.mark.parametrize("E,groups", [(16, 1), (64, 4), (200, 1), (256, 8), (1024, 1)])
 @pytest.mark.parametrize("score", [0, 1])
 def test_route_ties_go_to_the_lowest_index(ctx, E, groups, score):

@@ -349,11 +349,12 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
     const int64_t ldf = ((int64_t)L.d_hidden + 3) / 4 * 4, ldz = ((int64_t)L.d_out + 7) / 8 * 8;
     const size_t at_h = l.take((size_t)pairs * ldf * 4);
     const size_t at_hq = l.take((size_t)pairs * ldh), at_hs = l.take((size_t)pairs * 4);
-    // A BF16 output takes the slots' products in BF16: they are written and read
-    // again, 2 x 537 MB in 32 bits for 8192 rows of 8 slots of 2048, and their
-    // rounding is of the size of the output's own.  F16 would not hold a product
-    // that its weight brings back into range, so it keeps 32 bits.
-    const int z_elem = out_elem == VDTTFS_ELEM_BF16 ? VDTTFS_ELEM_BF16 : VDTTFS_ELEM_F32;
+    // Many slots of a BF16 output are kept in BF16: past what the L2s hold they are
+    // written and read again, 2 x 537 MB in 32 bits for 8192 rows of 8 slots of
+    // 2048 (60 us of 750), and their rounding is of the size of the output's own.
+    // F16 would not hold a product that its weight brings back into range.
+    const bool narrow = out_elem == VDTTFS_ELEM_BF16 && pairs * ldz * 4 > 32 << 20;
+    const int z_elem = narrow ? VDTTFS_ELEM_BF16 : VDTTFS_ELEM_F32;
     const size_t at_z = l.take((size_t)pairs * ldz * elem_size(z_elem));
     const size_t at_pair = l.take((size_t)pairs * 4), at_row = l.take((size_t)pairs * 4);
     const size_t at_tiles = l.take((size_t)max_tiles * sizeof(int4)), at_n = l.take(4);

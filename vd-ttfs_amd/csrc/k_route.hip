@@ -319,7 +319,8 @@ __device__ __forceinline__ float row16_sum(float v) {
 // Bound by these instructions: 65536 rows of 256 experts, 8 chosen of 4 groups
 // of 8, take 35 us (7 by their bytes; some 800 vector instructions for four
 // rows, 200 of them the lanes' sorts), and 80 with a wave per row and a search
-// for every choice.  At most kPop choices, and groups that are whole lanes.
+// for every choice.  At most kPop choices; a group has `span` lanes, a power of
+// two, the last of which may have fewer experts or none.
 constexpr int kPop = 8;
 template <int ELEM, int NPL>
 __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec) {
@@ -334,29 +335,30 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
         for (int e = threadIdx.x; e < a.E; e += blockDim.x) hist[e] = 0;
         __syncthreads();
     }
+    // the lane's experts: e0 .. e0 + here - 1
+    const int per = a.E / a.groups, group = lane / span;
+    const int e0 = group * per + lane % span * NPL, left = group < a.groups ? per - lane % span * NPL : 0;
+    const int here = left < NPL ? left : NPL;
     float bias[NPL];
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-        const int e = lane * NPL + i;
-        bias[i] = a.bias && e < a.E ? a.bias[e] : 0.0f;
-    }
+    for (int i = 0; i < NPL; ++i) bias[i] = a.bias && i < here ? a.bias[e0 + i] : 0.0f;
     const int64_t groups_of_rows = (a.M + rows - 1) / rows;
     for (int64_t b = blockIdx.x; b < groups_of_rows; b += gridDim.x) {
         const int64_t m = b * rows + threadIdx.x / 16;
         const bool row = m < a.M && (!a.row_mask || a.row_mask[m] != 0);
         float l[NPL];
-        if (row && vec && (lane + 1) * NPL <= a.E) {
+        if (row && vec && here == NPL) {
             if constexpr (ELEM == VDTTFS_ELEM_F32) {
-                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.logits) + m * a.ld) +
-                                  lane * (NPL / 4);
+                const float4* p =
+                    reinterpret_cast<const float4*>(static_cast<const float*>(a.logits) + m * a.ld + e0);
 #pragma unroll
                 for (int i = 0; i < NPL / 4; ++i) {
                     const float4 v = p[i];
                     l[4 * i] = v.x, l[4 * i + 1] = v.y, l[4 * i + 2] = v.z, l[4 * i + 3] = v.w;
                 }
             } else {
-                const uint2* p = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.logits) + m * a.ld) +
-                                 lane * (NPL / 4);
+                const uint2* p =
+                    reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.logits) + m * a.ld + e0);
 #pragma unroll
                 for (int i = 0; i < NPL / 4; ++i) {
                     const uint2 v = p[i];
@@ -368,10 +370,8 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < NPL; ++i) {
-                const int e = lane * NPL + i;
-                l[i] = row && e < a.E ? load_elem<ELEM>(a.logits, m * a.ld + e) : neg_inf();
-            }
+            for (int i = 0; i < NPL; ++i)
+                l[i] = row && i < here ? load_elem<ELEM>(a.logits, m * a.ld + e0 + i) : neg_inf();
         }
         float mx = neg_inf(), inv = 1.0f;
 #pragma unroll
@@ -419,9 +419,9 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
             const float g = a.group_top == 2 && t1 > neg_inf() ? t0 + t1 : t0;
             // a group stays if fewer than top_groups come before it: keys again,
             // the row's through LDS
-            const double k = with_index(__builtin_fmin(__builtin_fmax((double)g, -1e300), 1e300), lane / span);
+            const double k = with_index(__builtin_fmin(__builtin_fmax((double)g, -1e300), 1e300), group);
             double* keys = group_keys[threadIdx.x / 16];
-            if (lane % span == 0) keys[lane / span] = k;
+            if (lane % span == 0 && group < a.groups) keys[group] = k;
             if (lane >= a.groups) keys[lane] = 2 * -1e300;
             wave_sync();
             int rank = 0;
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
         }
         double key[NPL];
 #pragma unroll
-        for (int i = 0; i < NPL; ++i) key[i] = make_key(c[i], lane * NPL + i);
+        for (int i = 0; i < NPL; ++i) key[i] = make_key(c[i], e0 + i);
         if constexpr (NPL == 2 * kPop) {
             // Of two sorted halves the larger of each first and the other's last:
             // the first kPop of all, rising and then falling, so that exchanges
@@ -512,18 +512,24 @@ __global__ void k_zero(int* p, int n) {
 }
 
 // Four rows a wave where it can: up to 256 experts, 8 slots, and groups that
-// are a power of two of its lanes; else a wave per row.
+// fit its lanes; else a wave per row (29887 rows of 12 experts in groups of 6: 27
+// us, four rows a wave 9).
 template <int ELEM>
 void route_elem(vdttfs_ctx* ctx, const RouteArgs& a) {
-    const int size = ELEM == VDTTFS_ELEM_F32 ? 4 : 2;
-    const int npl = a.E <= 64 ? 4 : a.E <= 128 ? 8 : 16, per = a.E / a.groups;
-    const int span = a.groups == 1 ? 16 : per % npl ? 0 : per / npl;
-    if (a.E <= 256 && a.k <= kPop && (span == 1 || span == 2 || span == 4 || span == 8 || span == 16)) {
+    const int size = ELEM == VDTTFS_ELEM_F32 ? 4 : 2, per = a.E / a.groups;
+    // the fewest experts a lane with which the groups' lanes fit
+    int npl = 4, span = 16;
+    for (; npl <= 16; npl *= 2) {
+        for (span = 1; span * npl < per; span *= 2) {
+        }
+        if (span * a.groups <= 16) break;
+    }
+    if (a.E <= 256 && a.k <= kPop && npl <= 16) {
         // one workgroup a CU at most, of 16 waves where there are rows for them
         const int threads = a.M > 4096 ? 1024 : kThreads;
         const int64_t blocks = (a.M + threads / 16 - 1) / (threads / 16);
         const dim3 grid((unsigned)(blocks < 256 ? blocks : 256));
-        const int vec = (((uintptr_t)a.logits | (uintptr_t)(a.ld * size)) & (4 * size - 1)) == 0;
+        const int vec = per % 4 == 0 && (((uintptr_t)a.logits | (uintptr_t)(a.ld * size)) & (4 * size - 1)) == 0;
         if (npl == 4) k_route16<ELEM, 4><<<grid, threads, 0, ctx->stream>>>(a, span, vec);
         else if (npl == 8) k_route16<ELEM, 8><<<grid, threads, 0, ctx->stream>>>(a, span, vec);
         else k_route16<ELEM, 16><<<grid, threads, 0, ctx->stream>>>(a, span, vec);
