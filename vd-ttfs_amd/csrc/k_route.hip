@@ -74,14 +74,14 @@ struct RouteArgs {
 // workgroup, told by tickets (one for each copy, and one for the copies), moves
 // them out and leaves zeros behind: no launch of its own to clear or to sum.
 // Whole numbers, so no order matters.
-constexpr int kReplicas = 8;
+constexpr int kReplicas = 8, kOneCopy = 64;  // up to so many workgroups add to one copy
 __device__ __forceinline__ void finish_counts(const RouteArgs& a, const int* hist, int* last) {
     __syncthreads();
     if (gridDim.x == 1) {
         for (int e = threadIdx.x; e < a.E; e += blockDim.x) a.count[e] = hist[e];
         return;
     }
-    const int copy = blockIdx.x % kReplicas;
+    const int replicas = gridDim.x > kOneCopy ? kReplicas : 1, copy = blockIdx.x % replicas;
     int* mine = a.acc + copy * kMaxExperts;
     int* tickets = a.acc + kReplicas * kMaxExperts;  // of each copy, then of the copies
     for (int e = threadIdx.x; e < a.E; e += blockDim.x)
@@ -91,17 +91,18 @@ __device__ __forceinline__ void finish_counts(const RouteArgs& a, const int* his
         }
     __syncthreads();
     if (threadIdx.x == 0) {
-        const int copies = gridDim.x < kReplicas ? gridDim.x : kReplicas;
-        const int blocks = (gridDim.x - copy + kReplicas - 1) / kReplicas;  // that add to this copy
+        const int blocks = (gridDim.x - copy + replicas - 1) / replicas;  // that add to this copy
         bool all = atomicAdd(&tickets[copy], 1) == blocks - 1;
-        if (all) all = atomicAdd(&tickets[kReplicas], 1) == copies - 1;
+        if (all && replicas > 1) all = atomicAdd(&tickets[kReplicas], 1) == replicas - 1;
         *last = all;
     }
     __syncthreads();
     if (!*last) return;
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
         int n = 0;
-        for (int r = 0; r < kReplicas; ++r) n += atomicExch(&a.acc[r * kMaxExperts + e], 0);
+        if (replicas == 1) n = atomicExch(&a.acc[e], 0);
+        else
+            for (int r = 0; r < kReplicas; ++r) n += atomicExch(&a.acc[r * kMaxExperts + e], 0);
         a.count[e] = n;
     }
     if (threadIdx.x <= kReplicas) atomicExch(&tickets[threadIdx.x], 0);
@@ -513,7 +514,7 @@ __global__ void k_zero(int* p, int n) {
 
 // Four rows a wave where it can: up to 256 experts, 8 slots, and groups that
 // fit its lanes; else a wave per row (29887 rows of 12 experts in groups of 6: 27
-// us, four rows a wave 9).
+// us, four rows a wave 13).
 template <int ELEM>
 void route_elem(vdttfs_ctx* ctx, const RouteArgs& a) {
     const int size = ELEM == VDTTFS_ELEM_F32 ? 4 : 2, per = a.E / a.groups;
@@ -526,7 +527,7 @@ void route_elem(vdttfs_ctx* ctx, const RouteArgs& a) {
     }
     if (a.E <= 256 && a.k <= kPop && npl <= 16) {
         // one workgroup a CU at most, of 16 waves where there are rows for them
-        const int threads = a.M > 4096 ? 1024 : kThreads;
+        const int threads = a.M > 1024 ? 1024 : kThreads;
         const int64_t blocks = (a.M + threads / 16 - 1) / (threads / 16);
         const dim3 grid((unsigned)(blocks < 256 ? blocks : 256));
         const int vec = per % 4 == 0 && (((uintptr_t)a.logits | (uintptr_t)(a.ld * size)) & (4 * size - 1)) == 0;
