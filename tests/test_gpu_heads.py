@@ -192,6 +192,21 @@ def test_matmul_past_32_bit_offsets(ctx):
     q.free()
 
 
+@pytest.mark.parametrize("M,K", [(16, 7277), (100, 7277), (33, 9001), (50, 9301), (3, 20011)])
+def test_products_of_long_odd_rows(ctx, M, K):
+    N = 41
+    rng = np.random.default_rng(K + M)
+    x, w = rng.standard_normal((M, K)).astype(np.float32), codes(rng, N, K)
+    c = (rng.random(N) / 50).astype(np.float32)
+    q, s = R.quant_rows(x)
+    dw, dc = ctx.to_device(w), ctx.to_device(c)
+    lin, mul = Out(ctx, M, N, N, np.float32), Out(ctx, M, N, N, np.float32)
+    ctx.i8_linear(lin, R.F32, N, ctx.to_device(x), R.F32, K, dw, K, dc, None, R.NONE, M, N, K)
+    ctx.i8_matmul(mul, R.F32, N, ctx.to_device(q), K, ctx.to_device(s), dw, K, dc, None, R.NONE, M, N, K)
+    for out in (lin, mul):
+        check(out.get(), R.F32, *R.product(q, s, w, c, None, R.NONE))
+
+
 @pytest.mark.parametrize("M", [1, 3, 16, 20, 150])
 @pytest.mark.parametrize("x_elem", [R.F32, R.BF16, R.F16, R.TIMES])
 def test_linear_is_quant_rows_then_matmul(ctx, M, x_elem):

@@ -221,7 +221,8 @@ int vdttfs_i8_matmul(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, co
     VD_TRY(check_float_ptr("i8_matmul", d_row_scale, 4));
     VD_TRY(check_product("i8_matmul", d_w, ldw, d_ch_scale, d_bias, act, K));
     const I8Args a = product(d_q, ldq, d_row_scale, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M, N, K, act);
-    if (small_ok(M, N, K, kElemCodes)) return launch_i8_small(ctx, d_q, kElemCodes, ldq, d_row_scale, a);
+    const bool off = off16(d_q, ldq) || off16(d_w, ldw);
+    if (small_ok(M, N, K, kElemCodes, off)) return launch_i8_small(ctx, d_q, kElemCodes, ldq, d_row_scale, a);
     return dense(ctx, a, 0, nullptr);
 }
 
@@ -234,7 +235,8 @@ int vdttfs_i8_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, co
     VD_TRY(check_out("i8_linear", d_out, out_elem, ldo, N));
     VD_TRY(check_in("i8_linear", d_x, x_elem, ldx, M, K));
     VD_TRY(check_product("i8_linear", d_w, ldw, d_ch_scale, d_bias, act, K));
-    if (small_ok(M, N, K, x_elem))
+    const bool off = off16(d_w, ldw);
+    if (small_ok(M, N, K, x_elem, off))
         return launch_i8_small(ctx, d_x, x_elem, ldx, nullptr,
                                product(nullptr, 0, nullptr, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M, N,
                                        K, act));
@@ -242,7 +244,7 @@ int vdttfs_i8_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, co
     const int64_t ldq = padded(K);
     I8Args a = product(nullptr, ldq, nullptr, d_w, ldw, d_ch_scale, d_bias, d_out, out_elem, ldo, M, N, K, act);
     a.a_padded = true;
-    const bool small = M <= 16 && small_ok(M, N, K, kElemCodes);
+    const bool small = small_ok(M, N, K, kElemCodes, off);
     Layout l;
     const size_t at_q = l.take((size_t)M * ldq), at_s = l.take((size_t)M * 4);
     const size_t own = l.bytes;

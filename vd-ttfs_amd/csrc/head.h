@@ -46,7 +46,7 @@ int launch_realign(vdttfs_ctx* ctx, const int8_t* from, int64_t ld, int64_t rows
 // The product of few rows (a.A and a.lda unused), quantised in the kernel from
 // elem, or codes with scales sa where elem is kElemCodes.
 constexpr int kElemCodes = 4;
-bool small_ok(int64_t M, int N, int K, int elem);
+bool small_ok(int64_t M, int N, int K, int elem, bool off16);
 int launch_i8_small(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const I8Args& a);
 int launch_i8_grouped(vdttfs_ctx* ctx, const I8Args& a, bool gated, int bm);
 int i8_tile_rows(int64_t pairs, const vdttfs_expert_layer& L);

@@ -518,12 +518,14 @@ __global__ __launch_bounds__(kThreads) void k_expert_out(OutArgs p) {
 // Measured (us, against quantisation and tiles): 1x4096x4096 of BF16 6.7, 11.2;
 // 16x512x512 5.5, 7.3; 128x512x512 5.6, 7.4; 256x512x512 7.7, 6.8, of spike
 // times 5.7, 7.2, 512 rows of them 8.6, 6.9.  Codes, 1x4096x4096: 5.2 (3.2 TB/s
-// of weights, and a launch), tiles 7.5; 5 rows 5.8, 7.6.
-bool small_ok(int64_t M, int N, int K, int elem) {
+// of weights, and a launch), tiles 7.5; 5 rows 5.8, 7.6.  Long rows of codes
+// leave a CU one workgroup, which the tiles beat (64x64x8192: 17.8, 16.0) unless
+// rows off 16 bytes take them through registers (215x57x7276: 15.4, 28.6).
+bool small_ok(int64_t M, int N, int K, int elem, bool off16) {
     const int64_t rows = M < kRows ? M : kRows;
     const Share sh = share_of((int)rows, K);
     if (elem != kElemCodes && sh.passes * sh.turns > kUnits) return false;
-    if (rows * lds_stride(K) > 56 * 1024) return false;
+    if (rows * lds_stride(K) > (elem == kElemCodes && off16 ? 144 : 56) * 1024) return false;
     const int64_t blocks = (M + kRows - 1) / kRows * ((N + 15) / 16);
     return M <= kRows || blocks <= (elem == VDTTFS_ELEM_TIMES ? 512 : 256);
 }
