@@ -35,16 +35,26 @@ __device__ __forceinline__ void store8(int8_t* q, int64_t row, int c, int end, b
         if (c + i < end) q[row + c + i] = (int8_t)k[i];
 }
 
-// WAVES waves hold a row in registers, eight values a lane and turn (NV turns),
+// The largest magnitude over LANES lanes that share a row: a part of a wave, a
+// wave, or the workgroup.
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v, float* lds) {
+    if constexpr (LANES >= 64) return row_max<LANES / 64>(v, lds);
+#pragma unroll
+    for (int o = 1; o < LANES && o < 64; o *= 2) v = nan_max(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+// LANES lanes hold a row in registers, eight values a lane and turn (NV turns),
 // so it is read once: its largest magnitude, then its codes.  Bound by memory:
 // 8192 x 4096 of BF16 in 27 us, 3.7 TB/s; 61000 x 1024 of F32 that a product has
 // just left in 57, 5.4.
-template <int ELEM, int NV, int WAVES>
+template <int ELEM, int NV, int LANES>
 __global__ __launch_bounds__(kThreads) void k_quant_rows(const void* __restrict__ x, int64_t ldx, int64_t rows,
                                                          int cols, int8_t* __restrict__ q, int64_t ldq,
                                                          int cols_zero, float* __restrict__ scale, int vec_out) {
     __shared__ float lds[kThreads / 64];
-    constexpr int kRows = kThreads / 64 / WAVES, kLanes = WAVES * 64;
+    constexpr int kRows = kThreads / LANES, kLanes = LANES;
     const int lane = threadIdx.x % kLanes;
     for (int64_t m = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; m < rows; m += (int64_t)gridDim.x * kRows) {
         Raw8<ELEM> raw[NV];
@@ -65,7 +75,7 @@ __global__ __launch_bounds__(kThreads) void k_quant_rows(const void* __restrict_
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < 8; ++i) a = nan_max(a, fabsf(f[v][i]));
-        const float s = scale_of(row_max<WAVES>(a, lds));
+        const float s = scale_of(lanes_max<LANES>(a, lds));
         if (lane == 0) scale[m] = s;
         const Coder coder = coder_of(s);
 #pragma unroll
@@ -150,29 +160,32 @@ __global__ __launch_bounds__(1024) void k_quant_kernel(const float* __restrict__
 
 namespace {
 
-template <int ELEM, int NV, int WAVES>
+template <int ELEM, int NV, int LANES>
 void quant_nv(vdttfs_ctx* ctx, const void* x, int64_t ldx, int64_t rows, int cols, int8_t* q, int64_t ldq,
               int cols_zero, float* scale, int vo) {
-    constexpr int kRows = kThreads / 64 / WAVES;
+    constexpr int kRows = kThreads / LANES;
     const int64_t blocks = (rows + kRows - 1) / kRows;
-    k_quant_rows<ELEM, NV, WAVES><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), kThreads, 0, ctx->stream>>>(
+    k_quant_rows<ELEM, NV, LANES><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), kThreads, 0, ctx->stream>>>(
         x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
 }
 
-// A wave per row up to 2048 columns where there are rows for every SIMD, else
-// four.
+// As many rows a wave as fit up to 256 columns (36477 x 60: 14.8 us with a wave
+// per row, 6 so); a wave per row up to 2048 where there are rows for every SIMD;
+// else four.
 template <int ELEM>
 void quant_elem(vdttfs_ctx* ctx, const void* x, int64_t ldx, int64_t rows, int cols, int8_t* q, int64_t ldq,
                 int cols_zero, float* scale) {
     const int vo = (((uintptr_t)q | (uintptr_t)ldq) & 7) == 0;
-    if (cols_zero <= 512) quant_nv<ELEM, 1, 1>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
+    if (cols_zero <= 128) quant_nv<ELEM, 1, 16>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
+    else if (cols_zero <= 256) quant_nv<ELEM, 1, 32>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
+    else if (cols_zero <= 512) quant_nv<ELEM, 1, 64>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
     else if (cols_zero <= 1024 && rows >= 1024)
-        quant_nv<ELEM, 2, 1>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
+        quant_nv<ELEM, 2, 64>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
     else if (cols_zero <= 2048 && rows >= 1024)
-        quant_nv<ELEM, 4, 1>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
-    else if (cols_zero <= 2048) quant_nv<ELEM, 1, 4>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
-    else if (cols_zero <= 4096) quant_nv<ELEM, 2, 4>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
-    else if (cols_zero <= 8192) quant_nv<ELEM, 4, 4>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
+        quant_nv<ELEM, 4, 64>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
+    else if (cols_zero <= 2048) quant_nv<ELEM, 1, 256>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
+    else if (cols_zero <= 4096) quant_nv<ELEM, 2, 256>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
+    else if (cols_zero <= 8192) quant_nv<ELEM, 4, 256>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
     else
         k_quant_long<ELEM><<<dim3((unsigned)(rows < 65536 ? rows : 65536)), kThreads, 0, ctx->stream>>>(
             x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
