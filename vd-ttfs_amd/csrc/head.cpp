@@ -378,8 +378,8 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
                      reinterpret_cast<int4*>(buf + at_tiles), reinterpret_cast<int*>(buf + at_n),
                      reinterpret_cast<int*>(buf + at_hist)};
 
-    VD_TRY(launch_quant_rows(ctx, d_x, x_elem, ldx, M, L.d_in, q, ldq, (int)ldq, s));
-    VD_TRY(launch_dispatch(ctx, d_idx, pairs, top_k, L.n_experts, bm, d));
+    VD_TRY(launch_quant_dispatch(ctx, d_x, x_elem, ldx, M, L.d_in, q, ldq, (int)ldq, s, d_idx, pairs, top_k,
+                                 L.n_experts, bm, d));
     I8Args a = product(q, ldq, s, L.w1, L.d_in, L.s1, L.b1, h, VDTTFS_ELEM_F32, ldf, 0, L.d_hidden, L.d_in,
                        L.act);
     a.tiles = d.tiles;

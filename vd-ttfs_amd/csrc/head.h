@@ -78,6 +78,10 @@ struct Dispatch {
 int dispatch_blocks(int64_t pairs);
 int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_k, int n_experts, int bm,
                     const Dispatch& d);
+// launch_quant_rows and launch_dispatch, in one launch where they are small.
+int launch_quant_dispatch(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int64_t rows, int cols, int8_t* q,
+                          int64_t ldq, int cols_zero, float* scale, const int32_t* idx, int64_t pairs, int top_k,
+                          int n_experts, int bm, const Dispatch& d);
 // The second product of few pairs and the sum over slots in one launch: out
 // from h [pairs][d_hidden], F32 (`fuse`, quantised in the kernel) or codes.
 bool expert_out_ok(int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool fuse);

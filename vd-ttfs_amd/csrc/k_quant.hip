@@ -3,6 +3,7 @@
 #include "elem.h"
 #include "head.h"
 #include "quant.h"
+#include "sort.h"
 
 namespace vdttfs {
 namespace {
@@ -49,14 +50,16 @@ __device__ __forceinline__ float lanes_max(float v, float* lds) {
 // so it is read once: its largest magnitude, then its codes.  Bound by memory:
 // 8192 x 4096 of BF16 in 27 us, 3.7 TB/s; 61000 x 1024 of F32 that a product has
 // just left in 57, 5.4.
-template <int ELEM, int NV, int LANES>
-__global__ __launch_bounds__(kThreads) void k_quant_rows(const void* __restrict__ x, int64_t ldx, int64_t rows,
-                                                         int cols, int8_t* __restrict__ q, int64_t ldq,
-                                                         int cols_zero, float* __restrict__ scale, int vec_out) {
-    __shared__ float lds[kThreads / 64];
-    constexpr int kRows = kThreads / LANES, kLanes = LANES;
+// THREADS a workgroup, this one `block` of `blocks`.
+template <int ELEM, int NV, int LANES, int THREADS>
+__device__ __forceinline__ void quant_rows(const void* __restrict__ x, int64_t ldx, int64_t rows, int cols,
+                                           int8_t* __restrict__ q, int64_t ldq, int cols_zero,
+                                           float* __restrict__ scale, int vec_out, unsigned block, unsigned blocks) {
+    static_assert(LANES <= 64 || LANES == THREADS, "a row has a part of a wave, a wave or the workgroup");
+    __shared__ float lds[THREADS / 64];
+    constexpr int kRows = THREADS / LANES, kLanes = LANES;
     const int lane = threadIdx.x % kLanes;
-    for (int64_t m = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; m < rows; m += (int64_t)gridDim.x * kRows) {
+    for (int64_t m = (int64_t)block * kRows + threadIdx.x / kLanes; m < rows; m += (int64_t)blocks * kRows) {
         Raw8<ELEM> raw[NV];
         float f[NV][8], a = 0.0f;
 #pragma unroll
@@ -85,6 +88,12 @@ __global__ __launch_bounds__(kThreads) void k_quant_rows(const void* __restrict_
             store8(q, m * ldq, (v * kLanes + lane) * 8, cols_zero, vec_out, k);
         }
     }
+}
+template <int ELEM, int NV, int LANES>
+__global__ __launch_bounds__(kThreads) void k_quant_rows(const void* __restrict__ x, int64_t ldx, int64_t rows,
+                                                         int cols, int8_t* __restrict__ q, int64_t ldq,
+                                                         int cols_zero, float* __restrict__ scale, int vec_out) {
+    quant_rows<ELEM, NV, LANES, kThreads>(x, ldx, rows, cols, q, ldq, cols_zero, scale, vec_out, blockIdx.x, gridDim.x);
 }
 
 // Longer rows: a workgroup each, read twice (the second time from the caches).
@@ -115,12 +124,12 @@ __global__ __launch_bounds__(kThreads) void k_quant_long(const void* __restrict_
 }
 
 // Spike times: eight a thread; the scale is the same for every row.
-__global__ __launch_bounds__(kThreads) void k_quant_times(const float* __restrict__ x, int64_t ldx, int64_t rows,
-                                                          int cols, int8_t* __restrict__ q, int64_t ldq,
-                                                          int cols_zero, float* __restrict__ scale, float tfs, int T,
-                                                          int vec_out) {
+__device__ __forceinline__ void quant_times(const float* __restrict__ x, int64_t ldx, int64_t rows, int cols,
+                                            int8_t* __restrict__ q, int64_t ldq, int cols_zero,
+                                            float* __restrict__ scale, float tfs, int T, int vec_out, unsigned block,
+                                            unsigned blocks) {
     const int levels = T < 127 ? T : 127, per = cols_zero > 0 ? (cols_zero + 7) / 8 : 1;
-    for (int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x; at < rows * per; at += (int64_t)gridDim.x * kThreads) {
+    for (int64_t at = (int64_t)block * blockDim.x + threadIdx.x; at < rows * per; at += (int64_t)blocks * blockDim.x) {
         const int64_t m = at / per;
         const int c = (int)(at - m * per) * 8;
         float f[8];
@@ -130,6 +139,31 @@ __global__ __launch_bounds__(kThreads) void k_quant_times(const float* __restric
         for (int i = 0; i < 8; ++i) k[i] = time_code(f[i], tfs, T, levels);
         store8(q, m * ldq, c, cols_zero, vec_out, k);
         if (c == 0) scale[m] = 1.0f / (float)levels;
+    }
+}
+__global__ __launch_bounds__(kThreads) void k_quant_times(const float* __restrict__ x, int64_t ldx, int64_t rows,
+                                                          int cols, int8_t* __restrict__ q, int64_t ldq,
+                                                          int cols_zero, float* __restrict__ scale, float tfs, int T,
+                                                          int vec_out) {
+    quant_times(x, ldx, rows, cols, q, ldq, cols_zero, scale, tfs, T, vec_out, blockIdx.x, gridDim.x);
+}
+
+// Rows quantised and, by the first workgroup, the pairs of the experts that will
+// take them sorted: neither needs the other, so one launch does both.
+constexpr int kSortThreads = 1024;
+template <int ELEM, int NV, int LANES>
+__global__ __launch_bounds__(kSortThreads) void k_quant_sort(SortOne sort, const void* __restrict__ x, int64_t ldx,
+                                                             int64_t rows, int cols, int8_t* __restrict__ q,
+                                                             int64_t ldq, int cols_zero, float* __restrict__ scale,
+                                                             float tfs, int T, int vec_out) {
+    if (blockIdx.x == 0) {
+        sort_one(sort);
+    } else if constexpr (ELEM == VDTTFS_ELEM_TIMES) {
+        quant_times(static_cast<const float*>(x), ldx, rows, cols, q, ldq, cols_zero, scale, tfs, T, vec_out,
+                    blockIdx.x - 1, gridDim.x - 1);
+    } else {
+        quant_rows<ELEM, NV, LANES, kSortThreads>(x, ldx, rows, cols, q, ldq, cols_zero, scale, vec_out,
+                                                  blockIdx.x - 1, gridDim.x - 1);
     }
 }
 
@@ -191,6 +225,29 @@ void quant_elem(vdttfs_ctx* ctx, const void* x, int64_t ldx, int64_t rows, int c
             x, ldx, rows, cols, q, ldq, cols_zero, scale, vo);
 }
 
+template <int ELEM, int NV, int LANES>
+void quant_sort(vdttfs_ctx* ctx, const SortOne& sort, const void* x, int64_t ldx, int64_t rows, int cols, int8_t* q,
+                int64_t ldq, int cols_zero, float* scale) {
+    // rows of a workgroup; of spike times, eight values a thread
+    const int64_t blocks = ELEM == VDTTFS_ELEM_TIMES
+                               ? (rows * (cols_zero > 0 ? (cols_zero + 7) / 8 : 1) + kSortThreads - 1) / kSortThreads
+                               : (rows + kSortThreads / LANES - 1) / (kSortThreads / LANES);
+    const int vo = (((uintptr_t)q | (uintptr_t)ldq) & 7) == 0;
+    k_quant_sort<ELEM, NV, LANES><<<dim3(1 + (unsigned)(blocks < 65536 ? blocks : 65536)), kSortThreads, 0, ctx->stream>>>(
+        sort, x, ldx, rows, cols, q, ldq, cols_zero, scale, ctx->c.tfs, ctx->c.T, vo);
+}
+
+constexpr int kMaxSortCols = 2048;  // a wave holds a row
+template <int ELEM>
+void quant_sort_elem(vdttfs_ctx* ctx, const SortOne& sort, const void* x, int64_t ldx, int64_t rows, int cols, int8_t* q,
+                     int64_t ldq, int cols_zero, float* scale) {
+    if (cols_zero <= 128) quant_sort<ELEM, 1, 16>(ctx, sort, x, ldx, rows, cols, q, ldq, cols_zero, scale);
+    else if (cols_zero <= 256) quant_sort<ELEM, 1, 32>(ctx, sort, x, ldx, rows, cols, q, ldq, cols_zero, scale);
+    else if (cols_zero <= 512) quant_sort<ELEM, 1, 64>(ctx, sort, x, ldx, rows, cols, q, ldq, cols_zero, scale);
+    else if (cols_zero <= 1024) quant_sort<ELEM, 2, 64>(ctx, sort, x, ldx, rows, cols, q, ldq, cols_zero, scale);
+    else quant_sort<ELEM, 4, 64>(ctx, sort, x, ldx, rows, cols, q, ldq, cols_zero, scale);
+}
+
 }  // namespace
 
 int launch_quant_rows(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int64_t rows, int cols, int8_t* q,
@@ -205,6 +262,25 @@ int launch_quant_rows(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int
             static_cast<const float*>(x), ldx, rows, cols, q, ldq, cols_zero, scale, ctx->c.tfs, ctx->c.T,
             (((uintptr_t)q | (uintptr_t)ldq) & 7) == 0);
     }
+    VD_HIP(hipGetLastError());
+    return VDTTFS_OK;
+}
+
+int launch_quant_dispatch(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int64_t rows, int cols, int8_t* q,
+                          int64_t ldq, int cols_zero, float* scale, const int32_t* idx, int64_t pairs, int top_k,
+                          int n_experts, int bm, const Dispatch& d) {
+    if (pairs > kSortOne || cols_zero > kMaxSortCols) {
+        VD_TRY(launch_quant_rows(ctx, x, elem, ldx, rows, cols, q, ldq, cols_zero, scale));
+        return launch_dispatch(ctx, idx, pairs, top_k, n_experts, bm, d);
+    }
+    const SortOne s{idx, (int)pairs, n_experts, top_k, bm, d.tiles, d.n_tiles, d.pair, d.row};
+    if (elem == VDTTFS_ELEM_F32)
+        quant_sort_elem<VDTTFS_ELEM_F32>(ctx, s, x, ldx, rows, cols, q, ldq, cols_zero, scale);
+    else if (elem == VDTTFS_ELEM_BF16)
+        quant_sort_elem<VDTTFS_ELEM_BF16>(ctx, s, x, ldx, rows, cols, q, ldq, cols_zero, scale);
+    else if (elem == VDTTFS_ELEM_F16)
+        quant_sort_elem<VDTTFS_ELEM_F16>(ctx, s, x, ldx, rows, cols, q, ldq, cols_zero, scale);
+    else quant_sort<VDTTFS_ELEM_TIMES, 1, 64>(ctx, s, x, ldx, rows, cols, q, ldq, cols_zero, scale);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }

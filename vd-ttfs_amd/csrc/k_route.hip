@@ -2,6 +2,7 @@
 // weighted sum of the experts' outputs.
 #include "elem.h"
 #include "head.h"
+#include "sort.h"
 #include "wave.h"
 
 namespace vdttfs {
@@ -9,7 +10,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kMaxExperts = 1024;
 constexpr int kSortPairs = 2048;  // pairs a workgroup of the sort takes
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
@@ -559,23 +559,6 @@ __global__ __launch_bounds__(1024) void k_sort_count(const int32_t* __restrict__
     if ((int)threadIdx.x < E) hist[(int64_t)blockIdx.x * E + threadIdx.x] = h[threadIdx.x];
 }
 
-// Sum of v over the threads before this one (1024 threads); total: over all.
-__device__ __forceinline__ int block_excl_scan(int v, int* lds, int* total) {
-    const int incl = wave_incl_scan(v);
-    const int wave = threadIdx.x >> 6;
-    if (lane_id() == 63) lds[wave] = incl;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int i = 0; i < 16; ++i) {
-        const int s = lds[i];
-        if (i < wave) before += s;
-        all += s;
-    }
-    __syncthreads();
-    *total = all;
-    return before + incl - v;
-}
-
 // One workgroup: hist[block][expert] becomes the sorted position of the
 // block's first pair of the expert; the row tiles of every expert follow.
 // 2^log threads go over the experts, and share the blocks in 1024 >> log runs.
@@ -636,42 +619,7 @@ __global__ __launch_bounds__(1024) void k_sort_place(const int32_t* __restrict__
         }
 }
 
-// All of the sort in one workgroup, for up to kSortOne pairs: one launch of some
-// 5 us in place of three of 10.
-constexpr int kSortOne = 8192;
-__global__ __launch_bounds__(1024) void k_sort_one(const int32_t* __restrict__ idx, int pairs, int E, int top_k, int bm,
-                                                   int4* __restrict__ tiles, int* __restrict__ n_tiles,
-                                                   int* __restrict__ pair, int* __restrict__ row) {
-    __shared__ int lds[16];
-    __shared__ int at[kMaxExperts];
-    int e[kSortOne / 1024];
-#pragma unroll
-    for (int i = 0; i < kSortOne / 1024; ++i) {
-        const int q = i * 1024 + threadIdx.x;
-        e[i] = q < pairs ? idx[q] : -1;
-    }
-    at[threadIdx.x] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kSortOne / 1024; ++i)
-        if (e[i] >= 0 && e[i] < E) atomicAdd(&at[e[i]], 1);
-    __syncthreads();
-    const int n = at[threadIdx.x], t = (n + bm - 1) / bm;
-    int all, t_all;
-    const int start = block_excl_scan(n, lds, &all);
-    const int t0 = block_excl_scan(t, lds, &t_all);
-    for (int i = 0; i < t; ++i) tiles[t0 + i] = make_int4(threadIdx.x, start + i * bm, start + n, 0);
-    if (threadIdx.x == 0) *n_tiles = t_all;
-    at[threadIdx.x] = start;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kSortOne / 1024; ++i)
-        if (e[i] >= 0 && e[i] < E) {
-            const int q = i * 1024 + threadIdx.x, to = atomicAdd(&at[e[i]], 1);
-            pair[to] = q;
-            row[to] = q / top_k;
-        }
-}
+__global__ __launch_bounds__(1024) void k_sort_one(SortOne a) { sort_one(a); }
 
 // The slots' outputs summed in order, VEC neighbouring columns a thread; eight
 // slots' loads are in flight at a time.  Z: float, or uint16_t for BF16.
@@ -755,8 +703,8 @@ int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_
                     const Dispatch& d) {
     const int blocks = dispatch_blocks(pairs);
     if (pairs <= kSortOne) {
-        k_sort_one<<<dim3(1), 1024, 0, ctx->stream>>>(idx, (int)pairs, n_experts, top_k, bm, d.tiles, d.n_tiles, d.pair,
-                                                      d.row);
+        k_sort_one<<<dim3(1), 1024, 0, ctx->stream>>>(
+            SortOne{idx, (int)pairs, n_experts, top_k, bm, d.tiles, d.n_tiles, d.pair, d.row});
         VD_HIP(hipGetLastError());
         return VDTTFS_OK;
     }
