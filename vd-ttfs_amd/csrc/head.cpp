@@ -318,8 +318,6 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
         const size_t at_q = l.take(fuse1 ? 0 : (size_t)M * ldq), at_s = l.take(fuse1 ? 0 : (size_t)M * 4);
         const size_t at_h = l.take((size_t)pairs * L.d_hidden * 4);
         const size_t at_hq = l.take(fuse2 ? 0 : (size_t)pairs * ldh), at_hs = l.take(fuse2 ? 0 : (size_t)pairs * 4);
-        const bool join = expert_out_ok(pairs, top_k, L, fuse2);
-        const size_t at_z = l.take(join ? 0 : (size_t)pairs * L.d_out * 4);
         unsigned char* buf;
         VD_TRY(head_scratch(ctx, l.bytes, &buf));
         int8_t* q = reinterpret_cast<int8_t*>(buf + at_q);
@@ -327,21 +325,14 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
         float* h = reinterpret_cast<float*>(buf + at_h);
         int8_t* hq = reinterpret_cast<int8_t*>(buf + at_hq);
         float* hs = reinterpret_cast<float*>(buf + at_hs);
-        float* z = reinterpret_cast<float*>(buf + at_z);
         if (!fuse1) VD_TRY(launch_quant_rows(ctx, d_x, x_elem, ldx, M, L.d_in, q, ldq, (int)ldq, s));
-        VD_TRY(fuse1 ? launch_expert_product(ctx, d_x, x_elem, ldx, nullptr, d_idx, pairs, top_k, L, false, h)
-                     : launch_expert_product(ctx, q, kElemCodes, ldq, s, d_idx, pairs, top_k, L, false, h));
+        VD_TRY(fuse1 ? launch_expert_product(ctx, d_x, x_elem, ldx, nullptr, d_idx, pairs, top_k, L, h)
+                     : launch_expert_product(ctx, q, kElemCodes, ldq, s, d_idx, pairs, top_k, L, h));
         if (!fuse2)
             VD_TRY(launch_quant_rows(ctx, h, VDTTFS_ELEM_F32, L.d_hidden, pairs, L.d_hidden, hq, ldh, (int)ldh, hs));
-        if (join)
-            return fuse2 ? launch_expert_out(ctx, h, false, L.d_hidden, nullptr, d_idx, d_weight, M, top_k, L, d_out,
-                                             out_elem, ldo)
-                         : launch_expert_out(ctx, hq, true, ldh, hs, d_idx, d_weight, M, top_k, L, d_out, out_elem, ldo);
-        VD_TRY(fuse2 ? launch_expert_product(ctx, h, VDTTFS_ELEM_F32, L.d_hidden, nullptr, d_idx, pairs, top_k, L,
-                                             true, z)
-                     : launch_expert_product(ctx, hq, kElemCodes, ldh, hs, d_idx, pairs, top_k, L, true, z));
-        return launch_combine(ctx, d_out, out_elem, ldo, z, VDTTFS_ELEM_F32, L.d_out, d_idx, d_weight, M, L.d_out,
-                              top_k, L.n_experts);
+        return fuse2 ? launch_expert_out(ctx, h, false, L.d_hidden, nullptr, d_idx, d_weight, M, top_k, L, d_out,
+                                         out_elem, ldo)
+                     : launch_expert_out(ctx, hq, true, ldh, hs, d_idx, d_weight, M, top_k, L, d_out, out_elem, ldo);
     }
     const int bm = i8_tile_rows(pairs, L);
     const int64_t max_tiles = pairs / bm + (pairs < L.n_experts ? pairs : L.n_experts);

@@ -52,12 +52,15 @@ int launch_i8_grouped(vdttfs_ctx* ctx, const I8Args& a, bool gated, int bm);
 int i8_tile_rows(int64_t pairs, const vdttfs_expert_layer& L);
 
 // The experts of few pairs without a sort: whether to, and whether each product
-// quantises its rows itself (d_hidden's are float [pairs][d_hidden]); one of the
-// two products, out float [pairs][its columns], x codes with scales sa where
-// elem is kElemCodes.
+// quantises its rows itself.  The first product, out float [pairs][d_hidden], x
+// codes with scales sa where elem is kElemCodes; the second with the sum over
+// slots, from h [pairs][d_hidden], floats quantised in the kernel, or codes.
 bool experts_small_ok(int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool* fuse1, bool* fuse2);
 int launch_expert_product(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const int32_t* idx,
-                          int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool second, float* out);
+                          int64_t pairs, int top_k, const vdttfs_expert_layer& L, float* out);
+int launch_expert_out(vdttfs_ctx* ctx, const void* h, bool is_codes, int64_t ldh, const float* sa, const int32_t* idx,
+                      const float* wt, int64_t M, int top_k, const vdttfs_expert_layer& L, void* out, int out_elem,
+                      int64_t ldo);
 
 int launch_route(vdttfs_ctx* ctx, int32_t* idx, float* wt, int32_t* count, const void* logits, int elem, int64_t ld,
                  const float* bias, const uint8_t* row_mask, int64_t M, const vdttfs_route_opts& o, int* acc);
@@ -82,14 +85,8 @@ int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_
 int launch_quant_dispatch(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int64_t rows, int cols, int8_t* q,
                           int64_t ldq, int cols_zero, float* scale, const int32_t* idx, int64_t pairs, int top_k,
                           int n_experts, int bm, const Dispatch& d);
-// The second product of few pairs and the sum over slots in one launch: out
-// from h [pairs][d_hidden], F32 (`fuse`, quantised in the kernel) or codes.
-bool expert_out_ok(int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool fuse);
-int launch_expert_out(vdttfs_ctx* ctx, const void* h, bool is_codes, int64_t ldh, const float* sa, const int32_t* idx,
-                      const float* wt, int64_t M, int top_k, const vdttfs_expert_layer& L, void* out, int out_elem,
-                      int64_t ldo);
 // out[m] = sum over slots of weight * z[m * top_k + slot], z F32 or BF16 in rows
-// of ldz, aligned for whole vectors (4 floats, 8 of BF16) if ldz is a multiple of one
+// of ldz, aligned whole vectors (4 floats, 8 of BF16)
 int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem, int64_t ldz,
                    const int32_t* idx, const float* wt, int64_t M, int N, int top_k, int n_experts);
 

@@ -661,9 +661,9 @@ __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, in
         }
         const int64_t o = m * ldo + n;
         const bool bf16 = out_elem == VDTTFS_ELEM_BF16;
-        if (VEC > 1 && out_elem != VDTTFS_ELEM_F32 && n + VEC <= N &&
+        if (out_elem != VDTTFS_ELEM_F32 && n + VEC <= N &&
             (((uintptr_t)out | (uintptr_t)(ldo * 2)) & (VEC * 2 - 1)) == 0) {
-            uint32_t p[VEC / 2 + 1];
+            uint32_t p[VEC / 2];
 #pragma unroll
             for (int i = 0; i < VEC / 2; ++i) p[i] = pack2(sum[2 * i], sum[2 * i + 1], bf16);
             uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(out) + o);
@@ -723,14 +723,13 @@ int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_
 int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem, int64_t ldz,
                    const int32_t* idx, const float* wt, int64_t M, int N, int top_k, int n_experts) {
     const bool bf16 = z_elem == VDTTFS_ELEM_BF16;
-    const int vec = bf16 ? 8 : ldz % 4 == 0 ? 4 : 1;
+    const int vec = bf16 ? 8 : 4;
     const dim3 grid((unsigned)(((N + vec - 1) / vec + kThreads - 1) / kThreads), (unsigned)(M < 65535 ? M : 65535));
     const float* f = static_cast<const float*>(z);
     const uint16_t* h = static_cast<const uint16_t*>(z);
     const hipStream_t st = ctx->stream;
     if (bf16) k_combine<8><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, h, ldz, idx, wt, M, N, top_k, n_experts);
-    else if (vec == 4) k_combine<4><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, f, ldz, idx, wt, M, N, top_k, n_experts);
-    else k_combine<1><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, f, ldz, idx, wt, M, N, top_k, n_experts);
+    else k_combine<4><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, f, ldz, idx, wt, M, N, top_k, n_experts);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }

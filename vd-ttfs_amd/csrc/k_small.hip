@@ -342,10 +342,9 @@ struct ExpertArgs {
     Share sh;  // of so many
 };
 
-// One product of the experts: out[pair] for 16 columns (of gate and up if
+// The experts' first product: out[pair] for 16 columns (of gate and up if
 // GATED) of the rows of one expert, `cap` at a time, every gridDim.z-th here.
-// The rows are x[pair / top_k], or x[pair] where BY_PAIR.
-template <int ELEM, bool GATED, bool BY_PAIR>
+template <int ELEM, bool GATED>
 __global__ __launch_bounds__(kThreads) void k_expert_small(ExpertArgs p) {
     extern __shared__ __align__(16) int8_t codes[];
     constexpr int kParts = GATED ? 2 : 1;
@@ -369,7 +368,7 @@ __global__ __launch_bounds__(kThreads) void k_expert_small(ExpertArgs p) {
     w.begin(p.K, wave, kWaves);
     for (int r0 = blockIdx.z * p.cap; r0 < n_rows; r0 += gridDim.z * p.cap) {
         const int rows = n_rows - r0 < p.cap ? n_rows - r0 : p.cap;
-        auto x_row = [&](int r) { return BY_PAIR ? list[r0 + r] : list[r0 + r] / p.pairs.top_k; };
+        auto x_row = [&](int r) { return list[r0 + r] / p.pairs.top_k; };
         if (ELEM == kCodes && (int)threadIdx.x < rows) scale[threadIdx.x] = p.sa[x_row(threadIdx.x)];
         rows_to_lds<ELEM>(p.x, [&](int r) { return (int64_t)x_row(r) * p.ldx; }, rows, p.K, p.sh, p.tfs, p.T, codes,
                           stride, scale, peak);
@@ -557,14 +556,33 @@ static int expert_rows(int64_t pairs, int K, bool codes) {
     return 0;
 }
 
+// Every workgroup reads all experts of its rows' pairs, and quantises the pairs
+// if `fuse`, so it pays while there are few; else the pairs are sorted.  Measured
+// (us, joined and, before the sort was as fast, with launches of their own for
+// product and sum; workgroups, MB of weights read):
+//   1 x 6 of 64, 1024-512-1024 gated (64, 3)      11.6  13.2
+//   256 x 2 of 8, 512-512-10 (32, 2)              17.2  19.3
+//   16 x 16 of 64, 512-512-512 (512, 64)          29.5  31.9
+//   40 x 4 of 32, 512-2048-512 (320, 160)         56.1  40.6
+//   256 x 2 of 8, 512-512-512 gated (1024, 64)    28.9  23.3
+static bool expert_out_ok(int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool fuse) {
+    if (top_k > kRows) return false;
+    const int rows = (pairs < kRows ? (int)pairs : kRows) / top_k * top_k;
+    const int64_t blocks = (pairs + rows - 1) / rows * ((L.d_out + 15) / 16);
+    if (blocks > 512 || blocks * (rows < L.n_experts ? rows : L.n_experts) * 16 * L.d_hidden > 64 << 20) return false;
+    const Share sh = share_of(rows, L.d_hidden);
+    if (fuse && sh.passes * sh.turns > kUnits) return false;
+    return rows * lds_stride(L.d_hidden) <= 48 * 1024;
+}
+
 // Measured (us; rows x slots of experts, d_in-d_hidden-d_out; quantising in the
 // products, before them, and sorted with tiles):
 //   1 x 6 of 64, 1024-512-1024 gated   11.4  15.7  21.8
 //   32 x 2 of 8, 512-512-512           14.7  16.6  21.9 (the second before: 14.1)
 //   256 x 2 of 8, 512-512-10           22.9  18.9  23.5 (the first before: 17.2)
-//   256 x 2 of 8, 512-512-512 gated    30.9  23.3  23.4
 // Past two workgroups a CU in the first product, sorted tiles are as good or
-// better, but for one row, which shares no weights (these kernels, and tiles):
+// better, but for one row, which shares no weights (these kernels, and tiles;
+// the tiles have since lost another 3 us):
 //   2 x 4 of 16, 2048-1024-2048 gated (512 workgroups)    19.0  27.1
 //   4 x 2 of 8, 4096-1024-4096 gated (512)                27.2  34.8
 //   16 x 2 of 16, 2048-1024-2048 gated (1024)             41.4  35.3
@@ -574,90 +592,45 @@ static int expert_rows(int64_t pairs, int K, bool codes) {
 //   1 x 8 of 128, 4096-2048-4096 gated (1024)             59.7  57.1
 bool experts_small_ok(int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool* fuse1, bool* fuse2) {
     // every 16 columns quantise an expert's rows again
-    auto fuse = [&](int K, int N) {
-        return expert_rows(pairs, K, false) > 0 && (pairs * K <= 32768 || N <= 32);
-    };
-    *fuse1 = fuse(L.d_in, L.d_hidden);
-    *fuse2 = fuse(L.d_hidden, L.d_out);
+    auto fuse = [&](int K, int N) { return pairs * K <= 32768 || N <= 32; };
+    *fuse1 = fuse(L.d_in, L.d_hidden) && expert_rows(pairs, L.d_in, false) > 0;
+    *fuse2 = fuse(L.d_hidden, L.d_out) && expert_out_ok(pairs, top_k, L, true);
     const int64_t blocks = (pairs < L.n_experts ? pairs : L.n_experts) * ((L.d_hidden + 15) / 16);
     if (pairs > kMaxPairs || (blocks > 512 && pairs > top_k)) return false;
-    return expert_rows(pairs, L.d_in, !*fuse1) && expert_rows(pairs, L.d_hidden, !*fuse2);
+    return expert_rows(pairs, L.d_in, !*fuse1) > 0 && expert_out_ok(pairs, top_k, L, *fuse2);
 }
 
-template <bool GATED, bool BY_PAIR>
+template <bool GATED>
 static void expert_elem(vdttfs_ctx* ctx, const ExpertArgs& p, int elem, dim3 grid, size_t lds) {
     switch (elem) {
-        case VDTTFS_ELEM_F32:
-            k_expert_small<VDTTFS_ELEM_F32, GATED, BY_PAIR><<<grid, kThreads, lds, ctx->stream>>>(p);
-            break;
-        case VDTTFS_ELEM_BF16:
-            k_expert_small<VDTTFS_ELEM_BF16, GATED, BY_PAIR><<<grid, kThreads, lds, ctx->stream>>>(p);
-            break;
-        case VDTTFS_ELEM_F16:
-            k_expert_small<VDTTFS_ELEM_F16, GATED, BY_PAIR><<<grid, kThreads, lds, ctx->stream>>>(p);
-            break;
-        case VDTTFS_ELEM_TIMES:
-            k_expert_small<VDTTFS_ELEM_TIMES, GATED, BY_PAIR><<<grid, kThreads, lds, ctx->stream>>>(p);
-            break;
-        default: k_expert_small<kCodes, GATED, BY_PAIR><<<grid, kThreads, lds, ctx->stream>>>(p);
+        case VDTTFS_ELEM_F32: k_expert_small<VDTTFS_ELEM_F32, GATED><<<grid, kThreads, lds, ctx->stream>>>(p); break;
+        case VDTTFS_ELEM_BF16: k_expert_small<VDTTFS_ELEM_BF16, GATED><<<grid, kThreads, lds, ctx->stream>>>(p); break;
+        case VDTTFS_ELEM_F16: k_expert_small<VDTTFS_ELEM_F16, GATED><<<grid, kThreads, lds, ctx->stream>>>(p); break;
+        case VDTTFS_ELEM_TIMES: k_expert_small<VDTTFS_ELEM_TIMES, GATED><<<grid, kThreads, lds, ctx->stream>>>(p); break;
+        default: k_expert_small<kCodes, GATED><<<grid, kThreads, lds, ctx->stream>>>(p);
     }
 }
 
 int launch_expert_product(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const int32_t* idx,
-                          int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool second, float* out) {
+                          int64_t pairs, int top_k, const vdttfs_expert_layer& L, float* out) {
     const bool by_pair = pairs < L.n_experts;
     const PairArgs pa{idx, (int)pairs, top_k, L.n_experts, by_pair};
     const unsigned y = (unsigned)(by_pair ? pairs : L.n_experts);
-    const int K = second ? L.d_hidden : L.d_in, N = second ? L.d_out : L.d_hidden;
+    const int K = L.d_in, N = L.d_hidden;
     if (N <= 0) return VDTTFS_OK;
-    const bool gated = !second && L.gated;
     const int cap = expert_rows(pairs, K, elem == kCodes);
-    const ExpertArgs p{pa,
-                       x,
-                       ldx,
-                       sa,
-                       second ? L.w2 : L.w1,
-                       second ? L.s2 : L.s1,
-                       second ? L.b2 : L.b1,
-                       out,
-                       N,
-                       K,
-                       second ? VDTTFS_ACT_NONE : L.act,
-                       gated ? 2 * N : N,
-                       ctx->c.tfs,
-                       ctx->c.T,
-                       cap,
-                       share_of(cap, K)};
+    const ExpertArgs p{pa,  x, ldx, sa,    L.w1,  L.s1, L.b1, out, N, K, L.act, L.gated ? 2 * N : N, ctx->c.tfs,
+                       ctx->c.T, cap, share_of(cap, K)};
     // parts of an expert's rows: as many as its mean needs, while the chip holds
     // all workgroups at once
     const unsigned cols = (unsigned)((N + 15) / 16), want = (unsigned)((pairs / y + cap - 1) / cap);
     const unsigned room = 512 / (cols * y);
     const dim3 grid(cols, y, want < room ? want : room > 0 ? room : 1);
     const size_t lds = (size_t)cap * lds_stride(K);
-    if (gated) expert_elem<true, false>(ctx, p, elem, grid, lds);
-    else if (!second) expert_elem<false, false>(ctx, p, elem, grid, lds);
-    else if (elem == kCodes) k_expert_small<kCodes, false, true><<<grid, kThreads, lds, ctx->stream>>>(p);
-    else k_expert_small<VDTTFS_ELEM_F32, false, true><<<grid, kThreads, lds, ctx->stream>>>(p);
+    if (L.gated) expert_elem<true>(ctx, p, elem, grid, lds);
+    else expert_elem<false>(ctx, p, elem, grid, lds);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
-}
-
-// Every workgroup reads all experts of its rows' pairs, and quantises the pairs
-// if `fuse`, so it pays while there are few.  Measured (us, joined and with
-// launches of their own for product and sum; workgroups, MB of weights read):
-//   1 x 6 of 64, 1024-512-1024 gated (64, 3)      11.6  13.2
-//   256 x 2 of 8, 512-512-10 (32, 2)              17.2  19.3
-//   16 x 16 of 64, 512-512-512 (512, 64)          29.5  31.9
-//   40 x 4 of 32, 512-2048-512 (320, 160)         56.1  40.6
-//   256 x 2 of 8, 512-512-512 gated (1024, 64)    28.9  23.3
-bool expert_out_ok(int64_t pairs, int top_k, const vdttfs_expert_layer& L, bool fuse) {
-    if (top_k > kRows) return false;
-    const int rows = (pairs < kRows ? (int)pairs : kRows) / top_k * top_k;
-    const int64_t blocks = (pairs + rows - 1) / rows * ((L.d_out + 15) / 16);
-    if (blocks > 512 || blocks * (rows < L.n_experts ? rows : L.n_experts) * 16 * L.d_hidden > 64 << 20) return false;
-    const Share sh = share_of(rows, L.d_hidden);
-    if (fuse && sh.passes * sh.turns > kUnits) return false;
-    return rows * lds_stride(L.d_hidden) <= 48 * 1024;
 }
 
 int launch_expert_out(vdttfs_ctx* ctx, const void* h, bool is_codes, int64_t ldh, const float* sa, const int32_t* idx,
