@@ -519,14 +519,15 @@ __global__ __launch_bounds__(kThreads) void k_expert_out(OutArgs p) {
 // times 5.7, 7.2, 512 rows of them 8.6, 6.9.  Codes, 1x4096x4096: 5.2 (3.2 TB/s
 // of weights, and a launch), tiles 7.5; 5 rows 5.8, 7.6.  Long rows of codes
 // leave a CU one workgroup, which the tiles beat (64x64x8192: 17.8, 16.0) unless
-// rows off 16 bytes take them through registers (215x57x7276: 15.4, 28.6).
+// rows off 16 bytes take them through registers (215x57x7276: 15.4, 28.6;
+// 26x3942x7254: 33, 38; 100x1000x1003: 5.5, 6.8).
 bool small_ok(int64_t M, int N, int K, int elem, bool off16) {
     const int64_t rows = M < kRows ? M : kRows;
     const Share sh = share_of((int)rows, K);
     if (elem != kElemCodes && sh.passes * sh.turns > kUnits) return false;
     if (rows * lds_stride(K) > (elem == kElemCodes && off16 ? 144 : 56) * 1024) return false;
     const int64_t blocks = (M + kRows - 1) / kRows * ((N + 15) / 16);
-    return M <= kRows || blocks <= (elem == VDTTFS_ELEM_TIMES ? 512 : 256);
+    return M <= kRows || blocks <= (elem == VDTTFS_ELEM_TIMES || (elem == kElemCodes && off16) ? 512 : 256);
 }
 
 int launch_i8_small(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const I8Args& a) {
