@@ -661,9 +661,13 @@ int launch_realign(vdttfs_ctx* ctx, const int8_t* from, int64_t ld, int64_t rows
 
 // Whether a product is large enough for rows that the two-stage tiles do not
 // take to be copied first, rather than read unaligned through registers (us,
-// with copies and without): 8192x4096x4095 147, 394; 4000x1000x1000 23, 17.
+// with copies and without): 8192x4096x4095 147, 394; 4000x1000x1000 23, 17.  Of
+// rows quantised in scratch only the weights are copied (from BF16, with and
+// without): 4000x1000x1001 22.5, 27.1; 1000x1000x1001 13.6, 16.2; 8000x200x301
+// 15.6, 16.5; 6165x337x571 25.3, 24.6.
 bool i8_wants_aligned(const I8Args& a) {
-    return a.K >= kDeepK && !deep_ok(a) && (double)a.M * a.N * a.K >= 1e10 && tiles_of(a, 64, 64) >= 192;
+    return a.K >= kDeepK && !deep_ok(a) && (double)a.M * a.N * a.K >= (a.a_padded ? 2e8 : 1e10) &&
+           tiles_of(a, 64, 64) >= 192;
 }
 
 template <int BM, int BN, int WM, int WN, int BK, int S>
