@@ -599,8 +599,7 @@ int vdttfs_route(vdttfs_ctx* ctx, int32_t* d_idx, float* d_weight, int32_t* d_co
  * 32-bit floats; a row whose slots are all skipped is 0.  Device pointers, all
  * dense: w1 [E][H][d_in], s1 and b1 [E][H] with H = d_hidden or 2 * d_hidden,
  * w2 [E][d_out][d_hidden], s2 and b2 [E][d_out]; b1 and b2 may be NULL.
- * With a BF16 out the weighted products of the slots may pass through BF16
- * before their sum.  n_experts <= 1024, top_k <= 64, M * top_k < 2^31. */
+ * n_experts <= 1024, top_k <= 64, M * top_k < 2^31. */
 typedef struct vdttfs_expert_layer {
     int32_t n_experts, d_in, d_hidden, d_out;
     int32_t act, gated;

@@ -1,0 +1,53 @@
+"""The 8-bit heads where they went, or could go, wrong: rounding that depends on
+the batch, choices between infinite values, scores and activations far from zero,
+sizes at the ends of their types, empty widths, graphs on other streams."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import headref as R
+import vdttfs
+from vdttfs import _lib
+from test_gpu_heads import (Out, View, check, codes, ctx, expert_case, refused, run_experts,  # noqa: F401
+                            run_route)
+from test_gpu_scratch import Captured
+
+pytestmark = pytest.mark.gpu
+FLT_MAX = np.finfo(np.float32).max
+
+
+# ---- slots of a 16-bit output are summed in 32 bits ----------------------------------
+@pytest.mark.parametrize("out_elem", [R.BF16, R.F16])
+def test_slots_of_a_large_batch_cancel(ctx, out_elem):
+    """Both slots of a row name one expert, and their weights differ by 2^-8: the
+    sum is exact to the roundings of 32 bits, whatever the batch."""
+    M, E, D, F, N = 8300, 8, 64, 64, 520
+    assert M * 2 * N * 4 > 32 << 20
+    rng = np.random.default_rng(11)
+    weights = expert_case(rng, E, D, F, N, False, True)
+    idx = np.repeat(rng.integers(0, E, (M, 1)), 2, axis=1).astype(np.int32)
+    wt = np.repeat((0.5 + rng.random((M, 1))).astype(np.float32), 2, axis=1)
+    wt[:, 1] *= -np.float32(1 - 2.0 ** -8)
+    bits = R.to_bits(rng.standard_normal((M, D)).astype(np.float32), out_elem)
+    got = run_experts(ctx, bits, out_elem, D, idx, wt, weights, R.RELU, False, out_elem)
+    at = np.unique(np.concatenate([[0, 1, M - 1], rng.integers(0, M, 200)]))
+    q, s = R.quant_rows(R.from_bits(bits[at], out_elem))
+    y, d, _ = R.experts(q, s, idx[at], wt[at], *weights, R.RELU, False)
+    check(got[at], out_elem, y, d)
+
+
+@pytest.mark.parametrize("elem", [R.BF16, R.F16])
+def test_expert_rows_do_not_depend_on_the_batch(ctx, elem):
+    """16-bit rows alone, in a small batch and in one of more than 32 MB of slots: the same bits."""
+    M, k, E, D, F, N = 2100, 8, 12, 96, 64, 520
+    assert M * k * N * 4 > 32 << 20
+    rng = np.random.default_rng(12)
+    weights = expert_case(rng, E, D, F, N, True, True)
+    bits = R.to_bits(rng.standard_normal((M, D)).astype(np.float32), elem)
+    idx = np.argsort(rng.random((M, E)), axis=1)[:, :k].astype(np.int32)
+    wt = rng.random((M, k)).astype(np.float32)
+    large = run_experts(ctx, bits, elem, D, idx, wt, weights, R.SILU, True, elem)
+    for n in (1, 5, 60, 400):
+        some = run_experts(ctx, bits[:n], elem, D, idx[:n], wt[:n], weights, R.SILU, True, elem)
+        np.testing.assert_array_equal(some, large[:n])

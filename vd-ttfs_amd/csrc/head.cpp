@@ -339,16 +339,12 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
     Layout l;
     const size_t at_q = l.take((size_t)M * ldq), at_s = l.take((size_t)M * 4);
     // rows of whole vectors, so that they are stored and read as such
-    const int64_t ldf = ((int64_t)L.d_hidden + 3) / 4 * 4, ldz = ((int64_t)L.d_out + 7) / 8 * 8;
+    const int64_t ldf = ((int64_t)L.d_hidden + 3) / 4 * 4, ldz = ((int64_t)L.d_out + 3) / 4 * 4;
     const size_t at_h = l.take((size_t)pairs * ldf * 4);
     const size_t at_hq = l.take((size_t)pairs * ldh), at_hs = l.take((size_t)pairs * 4);
-    // Many slots of a BF16 output are kept in BF16: past what the L2s hold they are
-    // written and read again, 2 x 537 MB in 32 bits for 8192 rows of 8 slots of
-    // 2048 (60 us of 750), and their rounding is of the size of the output's own.
-    // F16 would not hold a product that its weight brings back into range.
-    const bool narrow = out_elem == VDTTFS_ELEM_BF16 && pairs * ldz * 4 > 32 << 20;
-    const int z_elem = narrow ? VDTTFS_ELEM_BF16 : VDTTFS_ELEM_F32;
-    const size_t at_z = l.take((size_t)pairs * ldz * elem_size(z_elem));
+    // The slots' products stay in 32 bits whatever the output's type: rounded to it
+    // before their sum they would add an error of their own size, not of the sum's.
+    const size_t at_z = l.take((size_t)pairs * ldz * 4);
     const size_t at_pair = l.take((size_t)pairs * 4), at_row = l.take((size_t)pairs * 4);
     const size_t at_tiles = l.take((size_t)max_tiles * sizeof(int4)), at_n = l.take(4);
     const size_t at_hist = l.take((size_t)dispatch_blocks(pairs) * L.n_experts * 4);
@@ -364,7 +360,7 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
     float* h = reinterpret_cast<float*>(buf + at_h);
     int8_t* hq = reinterpret_cast<int8_t*>(buf + at_hq);
     float* hs = reinterpret_cast<float*>(buf + at_hs);
-    void* z = buf + at_z;
+    float* z = reinterpret_cast<float*>(buf + at_z);
     const Dispatch d{reinterpret_cast<int*>(buf + at_pair), reinterpret_cast<int*>(buf + at_row),
                      reinterpret_cast<int4*>(buf + at_tiles), reinterpret_cast<int*>(buf + at_n),
                      reinterpret_cast<int*>(buf + at_hist)};
@@ -389,7 +385,7 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
     a.s_stride = H;
     VD_TRY(launch_i8_grouped(ctx, a, L.gated != 0, bm));
     VD_TRY(launch_quant_rows(ctx, h, VDTTFS_ELEM_F32, ldf, pairs, L.d_hidden, hq, ldh, (int)ldh, hs));
-    I8Args b = product(hq, ldh, hs, L.w2, L.d_hidden, L.s2, L.b2, z, z_elem, ldz, 0, L.d_out,
+    I8Args b = product(hq, ldh, hs, L.w2, L.d_hidden, L.s2, L.b2, z, VDTTFS_ELEM_F32, ldz, 0, L.d_out,
                        L.d_hidden, VDTTFS_ACT_NONE);
     b.tiles = d.tiles;
     b.n_tiles = d.n_tiles;
@@ -406,7 +402,7 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
     }
     b.s_stride = L.d_out;
     VD_TRY(launch_i8_grouped(ctx, b, false, bm));
-    return launch_combine(ctx, d_out, out_elem, ldo, z, z_elem, ldz, d_idx, d_weight, M, L.d_out, top_k, L.n_experts);
+    return launch_combine(ctx, d_out, out_elem, ldo, z, ldz, d_idx, d_weight, M, L.d_out, top_k, L.n_experts);
 }
 
 }  // extern "C"

@@ -85,9 +85,9 @@ int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_
 int launch_quant_dispatch(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int64_t rows, int cols, int8_t* q,
                           int64_t ldq, int cols_zero, float* scale, const int32_t* idx, int64_t pairs, int top_k,
                           int n_experts, int bm, const Dispatch& d);
-// out[m] = sum over slots of weight * z[m * top_k + slot], z F32 or BF16 in rows
-// of ldz, aligned whole vectors (4 floats, 8 of BF16)
-int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem, int64_t ldz,
+// out[m] = sum over slots of weight * z[m * top_k + slot], z in rows of ldz, whole
+// vectors of 4 floats
+int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const float* z, int64_t ldz,
                    const int32_t* idx, const float* wt, int64_t M, int N, int top_k, int n_experts);
 
 }  // namespace vdttfs

@@ -621,15 +621,14 @@ __global__ __launch_bounds__(1024) void k_sort_place(const int32_t* __restrict__
 
 __global__ __launch_bounds__(1024) void k_sort_one(SortOne a) { sort_one(a); }
 
-// The slots' outputs summed in order, VEC neighbouring columns a thread; eight
-// slots' loads are in flight at a time.  Z: float, or uint16_t for BF16.
-template <int VEC, typename Z>
+// The slots' outputs summed in order, four neighbouring columns a thread; eight
+// slots' loads are in flight at a time.
 __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, int out_elem, int64_t ldo,
-                                                      const Z* __restrict__ z, int64_t ldz,
+                                                      const float* __restrict__ z, int64_t ldz,
                                                       const int32_t* __restrict__ idx, const float* __restrict__ wt,
                                                       int64_t M, int N, int top_k, int E) {
-    typedef Z zvec __attribute__((ext_vector_type(VEC)));
-    constexpr int kSlots = 8;
+    constexpr int VEC = 4, kSlots = 8;
+    typedef float zvec __attribute__((ext_vector_type(VEC)));
     const int n = (blockIdx.x * kThreads + threadIdx.x) * VEC;
     if (n >= N) return;
     for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
@@ -644,7 +643,7 @@ __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, in
                 const int e = j0 + j < top_k ? idx[q] : -1;
                 on[j] = e >= 0 && e < E;
                 w[j] = 0.0f;
-                v[j] = zvec(Z(0));
+                v[j] = zvec(0.0f);
                 if (on[j]) {
                     w[j] = wt[q];
                     v[j] = *reinterpret_cast<const zvec*>(z + q * ldz + n);
@@ -654,21 +653,14 @@ __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, in
             for (int j = 0; j < kSlots; ++j)
                 if (on[j])
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        if constexpr (sizeof(Z) == 4) sum[i] += w[j] * v[j][i];
-                        else sum[i] += w[j] * bf16_to_f32(v[j][i]);
-                    }
+                    for (int i = 0; i < VEC; ++i) sum[i] += w[j] * v[j][i];
         }
         const int64_t o = m * ldo + n;
         const bool bf16 = out_elem == VDTTFS_ELEM_BF16;
         if (out_elem != VDTTFS_ELEM_F32 && n + VEC <= N &&
             (((uintptr_t)out | (uintptr_t)(ldo * 2)) & (VEC * 2 - 1)) == 0) {
-            uint32_t p[VEC / 2];
-#pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) p[i] = pack2(sum[2 * i], sum[2 * i + 1], bf16);
-            uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(out) + o);
-            if constexpr (VEC == 8) *reinterpret_cast<uint4*>(to) = make_uint4(p[0], p[1], p[2], p[3]);
-            if constexpr (VEC == 4) *reinterpret_cast<uint2*>(to) = make_uint2(p[0], p[1]);
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + o) =
+                make_uint2(pack2(sum[0], sum[1], bf16), pack2(sum[2], sum[3], bf16));
         } else {
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
@@ -720,16 +712,10 @@ int launch_dispatch(vdttfs_ctx* ctx, const int32_t* idx, int64_t pairs, int top_
     return VDTTFS_OK;
 }
 
-int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem, int64_t ldz,
+int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const float* z, int64_t ldz,
                    const int32_t* idx, const float* wt, int64_t M, int N, int top_k, int n_experts) {
-    const bool bf16 = z_elem == VDTTFS_ELEM_BF16;
-    const int vec = bf16 ? 8 : 4;
-    const dim3 grid((unsigned)(((N + vec - 1) / vec + kThreads - 1) / kThreads), (unsigned)(M < 65535 ? M : 65535));
-    const float* f = static_cast<const float*>(z);
-    const uint16_t* h = static_cast<const uint16_t*>(z);
-    const hipStream_t st = ctx->stream;
-    if (bf16) k_combine<8><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, h, ldz, idx, wt, M, N, top_k, n_experts);
-    else k_combine<4><<<grid, kThreads, 0, st>>>(out, out_elem, ldo, f, ldz, idx, wt, M, N, top_k, n_experts);
+    const dim3 grid((unsigned)(((N + 3) / 4 + kThreads - 1) / kThreads), (unsigned)(M < 65535 ? M : 65535));
+    k_combine<<<grid, kThreads, 0, ctx->stream>>>(out, out_elem, ldo, z, ldz, idx, wt, M, N, top_k, n_experts);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
