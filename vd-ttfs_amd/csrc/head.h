@@ -38,7 +38,11 @@ int launch_quant_rows(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int
                       int64_t ldq, int cols_zero, float* scale);
 int launch_quant_kernel(vdttfs_ctx* ctx, const float* kernel, int c_in, int c_out, int8_t* w, int64_t ldw,
                         float* scale);
-// bm: rows of a tile of a grouped product (i8_tile_rows of the same call)
+// Rows and channels of the tile that a dense product takes.
+struct I8Tile {
+    int bm, bn;
+};
+I8Tile i8_dense_tile(int64_t M, int N, int K, bool aligned);
 int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a);
 bool i8_wants_aligned(const I8Args& a);
 // Rows of codes to rows of ld_to, a multiple of 16, zeros from K on.
@@ -48,6 +52,7 @@ int launch_realign(vdttfs_ctx* ctx, const int8_t* from, int64_t ld, int64_t rows
 constexpr int kElemCodes = 4;
 bool small_ok(int64_t M, int N, int K, int elem, bool off16);
 int launch_i8_small(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, const float* sa, const I8Args& a);
+// bm: rows of a tile of a grouped product (i8_tile_rows of the same call)
 int launch_i8_grouped(vdttfs_ctx* ctx, const I8Args& a, bool gated, int bm);
 int i8_tile_rows(int64_t pairs, const vdttfs_expert_layer& L);
 

@@ -644,9 +644,10 @@ bool aligned16(const I8Args& a) {
 
 // What the two-stage tiles ask of K: whole chunks, and two tiles at least.
 constexpr int kDeepK = 256;
-bool deep_ok(const I8Args& a) { return aligned16(a) && a.K % 16 == 0 && a.K >= kDeepK; }
+bool deep_k(int K) { return K % 16 == 0 && K >= kDeepK; }
+bool deep_ok(const I8Args& a) { return aligned16(a) && deep_k(a.K); }
 
-int64_t tiles_of(const I8Args& a, int bm, int bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); }
+int64_t tiles_of(int64_t M, int N, int bm, int bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); }
 
 }  // namespace
 
@@ -667,7 +668,7 @@ int launch_realign(vdttfs_ctx* ctx, const int8_t* from, int64_t ld, int64_t rows
 // 15.6, 16.5; 6165x337x571 25.3, 24.6.
 bool i8_wants_aligned(const I8Args& a) {
     return a.K >= kDeepK && !deep_ok(a) && (double)a.M * a.N * a.K >= (a.a_padded ? 2e8 : 1e10) &&
-           tiles_of(a, 64, 64) >= 192;
+           tiles_of(a.M, a.N, 64, 64) >= 192;
 }
 
 template <int BM, int BN, int WM, int WN, int BK, int S>
@@ -699,18 +700,26 @@ int run_tile(vdttfs_ctx* ctx, const I8Args& a) {
 //   256x4096x4096: 64x128 14.7, 64x64 10.2, 32x32 14.2;  64x4096x4096: 64x64
 //   9.6, 32x32 7.6;  333x1111x1024: 64x64 7.3, 32x32 4.6
 // Rows off 16 bytes and not worth a copy go through registers.
+I8Tile i8_dense_tile(int64_t M, int N, int K, bool aligned) {
+    auto tiles = [&](int bm, int bn) { return tiles_of(M, N, bm, bn); };
+    if (!aligned) return tiles(64, 64) >= 192 ? I8Tile{64, 64} : I8Tile{32, 32};
+    const int64_t big = tiles(256, 256), rounds = (big + 255) / 256;
+    const bool deep = deep_k(K);
+    if (deep && (rounds == 1 ? big >= 160 : big * 10 >= rounds * 256 * 7)) return I8Tile{256, 256};
+    if (deep && tiles(128, 128) >= 384) return I8Tile{128, 128};
+    if (tiles(64, 128) >= 384) return I8Tile{64, 128};
+    return tiles(64, 64) >= 192 ? I8Tile{64, 64} : I8Tile{32, 32};
+}
+
 int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
     if (a.M <= 0 || a.N <= 0) return VDTTFS_OK;
-    auto tiles = [&](int bm, int bn) { return tiles_of(a, bm, bn); };
-    if (!aligned16(a)) return tiles(64, 64) >= 192 ? run_tile<64, 64>(ctx, a) : run_tile<32, 32>(ctx, a);
-    const int64_t big = tiles(256, 256), rounds = (big + 255) / 256;
-    const bool deep = deep_ok(a);
-    if (deep && (rounds == 1 ? big >= 160 : big * 10 >= rounds * 256 * 7))
-        return run_big<256, 256, 2, 4, 128, 2>(ctx, a);
-    if (deep && tiles(128, 128) >= 384) return run_big<128, 128, 2, 2, 128, 2>(ctx, a);
-    if (tiles(64, 128) >= 384) return run_big<64, 128, 2, 2, 128, 3>(ctx, a);
-    if (tiles(64, 64) >= 192) return run_big<64, 64, 2, 2, 128, 4>(ctx, a);
-    return run_big<32, 32, 2, 2, 128, 4>(ctx, a);
+    const bool aligned = aligned16(a);
+    const I8Tile t = i8_dense_tile(a.M, a.N, a.K, aligned);
+    if (!aligned) return t.bm == 64 ? run_tile<64, 64>(ctx, a) : run_tile<32, 32>(ctx, a);
+    if (t.bm == 256) return run_big<256, 256, 2, 4, 128, 2>(ctx, a);
+    if (t.bm == 128) return run_big<128, 128, 2, 2, 128, 2>(ctx, a);
+    if (t.bn == 128) return run_big<64, 128, 2, 2, 128, 3>(ctx, a);
+    return t.bm == 64 ? run_big<64, 64, 2, 2, 128, 4>(ctx, a) : run_big<32, 32, 2, 2, 128, 4>(ctx, a);
 }
 
 // Rows of the tiles of a layer's two products: the largest that an expert's
