@@ -51,3 +51,35 @@ def test_expert_rows_do_not_depend_on_the_batch(ctx, elem):
     for n in (1, 5, 60, 400):
         some = run_experts(ctx, bits[:n], elem, D, idx[:n], wt[:n], weights, R.SILU, True, elem)
         np.testing.assert_array_equal(some, large[:n])
+
+
+# ---- choices between infinite values -------------------------------------------------
+def routed(ctx, l, bias, k, score, groups, top_groups, group_top):
+    """The choice, checked against the definition; every row of it is told apart or equal."""
+    args = (k, score, groups, top_groups, group_top, False, 1.0)
+    gi, gw = run_route(ctx, l, R.F32, bias, None, *args)
+    ri, rw, decided = R.route(l, bias, None, *args)
+    assert decided.all()
+    np.testing.assert_array_equal(gi, ri)
+    assert (np.abs(gw - rw) <= R.route_bound(l.shape[1]) * rw + 1e-37).all()
+    return gi
+
+
+# experts, slots: the second takes another kernel (more than 256 experts or 8 slots)
+KERNELS = [(64, 4), (320, 4), (64, 10)]
+
+
+@pytest.mark.parametrize("E,k", KERNELS)
+@pytest.mark.parametrize("groups", [8, 16])
+@pytest.mark.parametrize("top_groups,group_top", [(1, 1), (1, 2), (2, 2), (3, 1)])
+def test_groups_of_infinite_value(ctx, E, k, groups, top_groups, group_top):
+    """A bias of +inf in one to four groups: the first of them are kept, and no others."""
+    per = E // groups
+    l = np.tile(np.linspace(-1, 1, E, dtype=np.float32)[::-1], (3, 1))
+    for infinite in ([4], [0, 4], [2, 4], [1, 5], [3, 7], [0, 1, 4], [1, 3, 5, 7], [6, 2, 4]):
+        bias = np.zeros(E, np.float32)
+        for g in infinite:
+            bias[g * per + per // 2] = np.inf
+        gi = routed(ctx, l, bias, k, 1, groups, top_groups, group_top)
+        kept = set(gi[0][gi[0] >= 0] // per)
+        assert len(kept) <= top_groups and sorted(infinite)[0] in kept

@@ -256,13 +256,15 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
 // values differ, the lower index above.  A maximum is then one instruction with
 // no second value to carry.
 // An infinite value goes as the largest finite one, and minus infinity, which
-// is not choosable, as one below all floats.
+// is not choosable, as one below all floats.  kFar, past all floats and their
+// sums, stands for an infinity where it has to leave those bits free.
+constexpr double kFar = 0x1p300;
 __device__ __forceinline__ double with_index(double d, int e) {
     const int hi = __double2hiint(d), lo = __double2loint(d);
     return __hiloint2double(hi, lo | (((255 - e) ^ hi >> 31) & 255));
 }
 __device__ __forceinline__ double make_key(float c, int e) {
-    return with_index(__builtin_fmax((double)fminf(c, 3.402823466e38f), -1e300), e);
+    return with_index(__builtin_fmax((double)fminf(c, 3.402823466e38f), -kFar), e);
 }
 // The choice value of a key as an integer of the same order, and the expert
 // from it and the key's low word.  kNone: the value of a key that is below all
@@ -420,10 +422,10 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
             const float g = a.group_top == 2 && t1 > neg_inf() ? t0 + t1 : t0;
             // a group stays if fewer than top_groups come before it: keys again,
             // the row's through LDS
-            const double k = with_index(__builtin_fmin(__builtin_fmax((double)g, -1e300), 1e300), group);
+            const double k = with_index(__builtin_fmin(__builtin_fmax((double)g, -kFar), kFar), group);
             double* keys = group_keys[threadIdx.x / 16];
             if (lane % span == 0 && group < a.groups) keys[group] = k;
-            if (lane >= a.groups) keys[lane] = 2 * -1e300;
+            if (lane >= a.groups) keys[lane] = -2 * kFar;
             wave_sync();
             int rank = 0;
 #pragma unroll
