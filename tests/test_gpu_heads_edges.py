@@ -83,3 +83,26 @@ def test_groups_of_infinite_value(ctx, E, k, groups, top_groups, group_top):
         gi = routed(ctx, l, bias, k, 1, groups, top_groups, group_top)
         kept = set(gi[0][gi[0] >= 0] // per)
         assert len(kept) <= top_groups and sorted(infinite)[0] in kept
+
+
+@pytest.mark.parametrize("E,k", KERNELS)
+def test_sums_of_a_group_past_the_largest_float(ctx, E, k):
+    """Groups whose best two sum past the largest float, above and below, are still ordered by their sums."""
+    per = E // 8
+    l = np.zeros((2, E), np.float32)
+    big = lambda v: np.float32(v) * FLT_MAX  # noqa: E731
+    bias = np.zeros(E, np.float32)
+    for g, v in enumerate((0.6, 0.9, 0.7, 1.0, 0.8, 0.3, 0.55, 1.0)):
+        bias[g * per:(g + 1) * per] = big(v)
+    for top in (1, 2, 3):
+        gi = routed(ctx, l, bias, k, 1, 8, top, 2)
+        assert set(gi[0][gi[0] >= 0] // per) <= set([3, 7, 1][:top])
+    # masked by the lowest value, not by -inf: these experts can be chosen, those of a group of -inf cannot
+    bias[:] = -np.inf
+    bias[5 * per:6 * per] = -FLT_MAX
+    bias[6 * per:7 * per] = -0.75 * FLT_MAX
+    for top in (1, 2):
+        gi = routed(ctx, l, bias, k, 1, 8, top, 2)
+        assert gi[0, 0] == 6 * per
+    bias[6 * per:7 * per] = -np.inf
+    assert routed(ctx, l, bias, k, 1, 8, 1, 2)[0, 0] == 5 * per

@@ -54,6 +54,16 @@ __device__ __forceinline__ float wave_sum(float v) {
 __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 __device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 
+// What a group is worth from its two largest values t0 >= t1.  Their sum is
+// rounded to 24 bits as any float; past the largest float it is formed of halves,
+// so groups are told apart there too, and one of lowest values is above one that
+// has none.
+__device__ __forceinline__ double group_worth(float t0, float t1, int group_top) {
+    if (group_top != 2 || !(t1 > neg_inf())) return t0;
+    const float s = t0 + t1;
+    return fabsf(s) < -neg_inf() ? (double)s : 2.0 * (double)(0.5f * t0 + 0.5f * t1);
+}
+
 struct RouteArgs {
     int32_t* idx;
     float* wt;
@@ -187,12 +197,13 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
                     for (int i = 0; i < per; ++i) take(group_c[wave][lane * per + i]);
                 wave_sync();
             }
-            const float g = a.group_top == 2 && t1 > neg_inf() ? t0 + t1 : t0;
+            const double g = group_worth(t0, t1, a.group_top);
             // a group stays if fewer than top_groups come before it
             const int mine = in_lanes ? lane / span : lane;
             int rank = 0;
             for (int o = 0; o < a.groups; ++o) {
-                const float v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), o * span));
+                const double v = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(g), o * span),
+                                                  __builtin_amdgcn_readlane(__double2loint(g), o * span));
                 rank += v > g || (v == g && o < mine) ? 1 : 0;
             }
             const bool stays = rank < a.top_groups;
@@ -419,10 +430,10 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
             if (span > 2) merge(dpp<kXor2>(t0), dpp<kXor2>(t1));
             if (span > 4) merge(dpp<kHalfMirror>(t0), dpp<kHalfMirror>(t1));
             if (span > 8) merge(dpp<kMirror>(t0), dpp<kMirror>(t1));
-            const float g = a.group_top == 2 && t1 > neg_inf() ? t0 + t1 : t0;
+            const double g = group_worth(t0, t1, a.group_top);
             // a group stays if fewer than top_groups come before it: keys again,
             // the row's through LDS
-            const double k = with_index(__builtin_fmin(__builtin_fmax((double)g, -kFar), kFar), group);
+            const double k = with_index(__builtin_fmin(__builtin_fmax(g, -kFar), kFar), group);
             double* keys = group_keys[threadIdx.x / 16];
             if (lane % span == 0 && group < a.groups) keys[group] = k;
             if (lane >= a.groups) keys[lane] = -2 * kFar;
