@@ -106,3 +106,12 @@ def test_sums_of_a_group_past_the_largest_float(ctx, E, k):
         assert gi[0, 0] == 6 * per
     bias[6 * per:7 * per] = -np.inf
     assert routed(ctx, l, bias, k, 1, 8, 1, 2)[0, 0] == 5 * per
+
+
+@pytest.mark.parametrize("E,k", KERNELS)
+def test_infinity_is_above_the_largest_float(ctx, E, k):
+    l = np.zeros((2, E), np.float32)
+    bias = np.zeros(E, np.float32)
+    bias[[1, 3]], bias[[7, 50]], bias[60] = FLT_MAX, np.inf, FLT_MAX / 2
+    gi = routed(ctx, l, bias, k, 1, 1, 1, 1)
+    np.testing.assert_array_equal(gi[0, :4], [7, 50, 1, 3])

@@ -266,20 +266,19 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
 // 32-bit value leaves free, with the expert's index in them so that equal
 // values differ, the lower index above.  A maximum is then one instruction with
 // no second value to carry.
-// An infinite value goes as the largest finite one, and minus infinity, which
-// is not choosable, as one below all floats.  kFar, past all floats and their
-// sums, stands for an infinity where it has to leave those bits free.
+// kFar, past all floats and the sums of two, stands for an infinity, which has
+// no such bits; minus infinity is not choosable.
 constexpr double kFar = 0x1p300;
 __device__ __forceinline__ double with_index(double d, int e) {
     const int hi = __double2hiint(d), lo = __double2loint(d);
     return __hiloint2double(hi, lo | (((255 - e) ^ hi >> 31) & 255));
 }
 __device__ __forceinline__ double make_key(float c, int e) {
-    return with_index(__builtin_fmax((double)fminf(c, 3.402823466e38f), -kFar), e);
+    return with_index(__builtin_fmin(__builtin_fmax((double)c, -kFar), kFar), e);
 }
 // The choice value of a key as an integer of the same order, and the expert
-// from it and the key's low word.  kNone: the value of a key that is below all
-// floats, minus infinity.
+// from it and the key's low word.  kFar is infinity again; kNone: the value of a
+// key that is below all floats, minus infinity.
 __device__ __forceinline__ int key_value(double key) {
     const int f = __float_as_int((float)key);
     return f ^ ((f >> 31) & 0x7fffffff);
