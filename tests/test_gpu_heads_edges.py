@@ -115,3 +115,45 @@ def test_infinity_is_above_the_largest_float(ctx, E, k):
     bias[[1, 3]], bias[[7, 50]], bias[60] = FLT_MAX, np.inf, FLT_MAX / 2
     gi = routed(ctx, l, bias, k, 1, 1, 1, 1)
     np.testing.assert_array_equal(gi[0, :4], [7, 50, 1, 3])
+
+
+# ---- routing keeps nothing between calls ------------------------------------------------
+def test_route_with_counts_needs_no_earlier_call(gpu_ctx_factory):
+    """The first call of a context may be a captured one, and graphs of it may run beside it on other streams."""
+    c = gpu_ctx_factory(vdttfs.TaskConsts(T=64, delta=16))
+    E, k, M = 64, 4, 30000
+    rng = np.random.default_rng(3)
+    sets = []
+    for _ in range(3):
+        l = c.to_device(rng.standard_normal((M, E)).astype(np.float32))
+        sets.append((l, c.empty((M, k), np.int32), c.empty((M, k)), c.empty(E, np.int32)))
+
+    def call(i):
+        l, idx, wt, n = sets[i]
+        c.route(idx, wt, n, l, R.F32, E, None, None, M, E, k)
+
+    graphs = [Captured(c, lambda i=i: call(i)) for i in range(2)]
+    streams = []
+    for g in graphs:
+        s = ctypes.c_void_p()
+        assert g.h.hipStreamCreateWithFlags(ctypes.byref(s), 1) == 0
+        g.s = s
+        streams.append(s)
+    for turn in range(4):
+        for _, idx, _, n in sets:
+            idx.fill(0xFF)
+            n.fill(0x7F)
+        c.synchronize()
+        for g in graphs:
+            g.replay()
+        call(2)
+        c.synchronize()
+        for s in streams:
+            assert graphs[0].h.hipStreamSynchronize(s) == 0
+        for _, idx, _, n in sets:
+            got = idx.download()
+            assert (got >= 0).all()
+            np.testing.assert_array_equal(n.download(), np.bincount(got.ravel(), minlength=E))
+    for g, s in zip(graphs, streams):
+        g.close()
+        assert g.h.hipStreamDestroy(s) == 0

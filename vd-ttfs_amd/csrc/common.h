@@ -21,14 +21,12 @@ struct __align__(8) vd_event {
 struct HeadScratch {
     void* buf = nullptr;
     size_t bytes = 0;
-    bool captured = false;     // a captured graph holds buf's address
-    int* route_acc = nullptr;  // routing's counters, 0 between calls
+    bool captured = false;  // a captured graph holds buf's address
     HeadScratch() = default;
     HeadScratch(const HeadScratch&) = delete;
     HeadScratch& operator=(const HeadScratch&) = delete;
     ~HeadScratch() {
         if (buf) (void)hipFree(buf);
-        if (route_acc) (void)hipFree(route_acc);
     }
 };
 

@@ -87,30 +87,6 @@ int head_scratch(vdttfs_ctx* ctx, size_t bytes, unsigned char** out) {
     return VDTTFS_OK;
 }
 
-// The counters that routing sums its counts in: made once, cleared, and left
-// clear by every call.
-int route_counters(vdttfs_ctx* ctx) {
-    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    VD_HIP(hipStreamIsCapturing(ctx->stream, &cs));
-    if (cs != hipStreamCaptureStatusNone)
-        return set_error(VDTTFS_E_UNSUPPORTED,
-                         "the context's route counters cannot be made under stream capture: run the call once before "
-                         "capturing it");
-    void* p = nullptr;
-    if (hipMalloc(&p, route_acc_bytes()) != hipSuccess) {
-        (void)hipGetLastError();
-        return set_error(VDTTFS_E_NOMEM, "device allocation of %zu bytes failed", route_acc_bytes());
-    }
-    hipError_t e = hipMemsetAsync(p, 0, route_acc_bytes(), ctx->stream);
-    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
-    if (e != hipSuccess) {
-        (void)hipFree(p);
-        return hip_error(e, "route counters", __LINE__);
-    }
-    ctx->head.route_acc = static_cast<int*>(p);
-    return VDTTFS_OK;
-}
-
 // Parts of one scratch buffer, each on a 256-byte boundary.
 struct Layout {
     size_t bytes = 0;
@@ -285,8 +261,7 @@ int vdttfs_route(vdttfs_ctx* ctx, int32_t* d_idx, float* d_weight, int32_t* d_co
         VD_TRY(check_float_ptr("route", d_logits, elem_size(elem)));
         if (d_bias) VD_TRY(check_float_ptr("route", d_bias, 4));
     }
-    if (d_count && M > kRouteAlone && !ctx->head.route_acc) VD_TRY(route_counters(ctx));
-    return launch_route(ctx, d_idx, d_weight, d_count, d_logits, elem, ld, d_bias, d_row_mask, M, o, ctx->head.route_acc);
+    return launch_route(ctx, d_idx, d_weight, d_count, d_logits, elem, ld, d_bias, d_row_mask, M, o);
 }
 
 int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const void* d_x, int x_elem, int64_t ldx,

@@ -68,11 +68,7 @@ int launch_expert_out(vdttfs_ctx* ctx, const void* h, bool is_codes, int64_t ldh
                       int64_t ldo);
 
 int launch_route(vdttfs_ctx* ctx, int32_t* idx, float* wt, int32_t* count, const void* logits, int elem, int64_t ld,
-                 const float* bias, const uint8_t* row_mask, int64_t M, const vdttfs_route_opts& o, int* acc);
-// Device memory that launch_route's counts pass through, 0 between calls;
-// calls of at most kRouteAlone rows do without.
-constexpr int kRouteAlone = 4;
-size_t route_acc_bytes();
+                 const float* bias, const uint8_t* row_mask, int64_t M, const vdttfs_route_opts& o);
 
 // The pairs (row, slot) sorted by expert.  pair[i]: row * top_k + slot of
 // sorted row i, row[i]: its row; tiles as in I8Args with bm rows each.

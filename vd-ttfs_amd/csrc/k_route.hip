@@ -75,47 +75,18 @@ struct RouteArgs {
     int64_t M;
     int E, k, score, groups, top_groups, group_top, renorm;
     float scale;
-    int* acc;  // [kReplicas][kMaxExperts] sums and the tickets, all 0 between calls; one workgroup: unused
 };
 
-// The workgroup's counts into the call's.  Adds to a few busy lines cost (65536
-// rows over 64 experts: 4096 workgroups add 40 us to the call, 1024 8 us), so
-// there are few workgroups, and sums go to one of kReplicas copies; the last
-// workgroup, told by tickets (one for each copy, and one for the copies), moves
-// them out and leaves zeros behind: no launch of its own to clear or to sum.
-// Whole numbers, so no order matters.
-constexpr int kReplicas = 8, kOneCopy = 64;  // up to so many workgroups add to one copy
-__device__ __forceinline__ void finish_counts(const RouteArgs& a, const int* hist, int* last) {
+// The workgroup's counts into the call's, which a launch before has cleared where
+// there are several workgroups (2 us more than a call without counts; 65536 rows
+// of 256 experts 5): nothing is kept between calls, whose graphs may run side by
+// side.  Whole numbers, so no order matters.
+__device__ __forceinline__ void finish_counts(const RouteArgs& a, const int* hist) {
     __syncthreads();
-    if (gridDim.x == 1) {
-        for (int e = threadIdx.x; e < a.E; e += blockDim.x) a.count[e] = hist[e];
-        return;
-    }
-    const int replicas = gridDim.x > kOneCopy ? kReplicas : 1, copy = blockIdx.x % replicas;
-    int* mine = a.acc + copy * kMaxExperts;
-    int* tickets = a.acc + kReplicas * kMaxExperts;  // of each copy, then of the copies
-    for (int e = threadIdx.x; e < a.E; e += blockDim.x)
-        if (hist[e]) {
-            const int done = atomicAdd(&mine[e], hist[e]);
-            asm volatile("" ::"v"(done));  // wait for it: the ticket comes after every sum
-        }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const int blocks = (gridDim.x - copy + replicas - 1) / replicas;  // that add to this copy
-        bool all = atomicAdd(&tickets[copy], 1) == blocks - 1;
-        if (all && replicas > 1) all = atomicAdd(&tickets[kReplicas], 1) == replicas - 1;
-        *last = all;
-    }
-    __syncthreads();
-    if (!*last) return;
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
-        int n = 0;
-        if (replicas == 1) n = atomicExch(&a.acc[e], 0);
-        else
-            for (int r = 0; r < kReplicas; ++r) n += atomicExch(&a.acc[r * kMaxExperts + e], 0);
-        a.count[e] = n;
+        if (gridDim.x == 1) a.count[e] = hist[e];
+        else if (hist[e]) atomicAdd(&a.count[e], hist[e]);
     }
-    if (threadIdx.x <= kReplicas) atomicExch(&tickets[threadIdx.x], 0);
 }
 
 // A wave per row, NPL neighbouring experts a lane: the largest value of the
@@ -123,7 +94,6 @@ __device__ __forceinline__ void finish_counts(const RouteArgs& a, const int* his
 template <int ELEM, int NPL>
 __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
     __shared__ int hist[kMaxExperts];
-    __shared__ int last;
     __shared__ float group_c[kWaves][64 * NPL];
     const int lane = lane_id(), wave = threadIdx.x >> 6;
     if (a.count) {
@@ -258,7 +228,7 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
             if (a.count && my_idx >= 0) atomicAdd(&hist[my_idx], 1);
         }
     }
-    if (a.count) finish_counts(a, hist, &last);
+    if (a.count) finish_counts(a, hist);
 }
 
 // ---- four rows a wave -----------------------------------------------------------
@@ -338,7 +308,6 @@ constexpr int kPop = 8;
 template <int ELEM, int NPL>
 __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec) {
     __shared__ int hist[256];
-    __shared__ int last;
     __shared__ int chosen[64][kPop];  // of each row, from the lanes that held them
     __shared__ __align__(16) double group_keys[64][16];
     const int lane = lane_id() & 15;
@@ -517,11 +486,14 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
         }
         wave_sync();
     }
-    if (a.count) finish_counts(a, hist, &last);
+    if (a.count) finish_counts(a, hist);
 }
 
 __global__ void k_zero(int* p, int n) {
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) p[i] = 0;
+}
+void clear_counts(vdttfs_ctx* ctx, int* count, int E) {
+    if (count) k_zero<<<dim3(1), kThreads, 0, ctx->stream>>>(count, E);
 }
 
 // Four rows a wave where it can: up to 256 experts, 8 slots, and groups that
@@ -542,6 +514,7 @@ void route_elem(vdttfs_ctx* ctx, const RouteArgs& a) {
         const int threads = a.M > 1024 ? 1024 : kThreads;
         const int64_t blocks = (a.M + threads / 16 - 1) / (threads / 16);
         const dim3 grid((unsigned)(blocks < 256 ? blocks : 256));
+        if (blocks > 1) clear_counts(ctx, a.count, a.E);
         const int vec = per % 4 == 0 && (((uintptr_t)a.logits | (uintptr_t)(a.ld * size)) & (4 * size - 1)) == 0;
         if (npl == 4) k_route16<ELEM, 4><<<grid, threads, 0, ctx->stream>>>(a, span, vec);
         else if (npl == 8) k_route16<ELEM, 8><<<grid, threads, 0, ctx->stream>>>(a, span, vec);
@@ -550,6 +523,7 @@ void route_elem(vdttfs_ctx* ctx, const RouteArgs& a) {
     }
     const int64_t blocks = (a.M + kWaves - 1) / kWaves;
     const dim3 grid((unsigned)(blocks < 1024 ? blocks : 1024));
+    if (blocks > 1) clear_counts(ctx, a.count, a.E);
     if (a.E <= 64) k_route<ELEM, 1><<<grid, kThreads, 0, ctx->stream>>>(a);
     else if (a.E <= 128) k_route<ELEM, 2><<<grid, kThreads, 0, ctx->stream>>>(a);
     else if (a.E <= 256) k_route<ELEM, 4><<<grid, kThreads, 0, ctx->stream>>>(a);
@@ -683,17 +657,15 @@ __global__ __launch_bounds__(kThreads) void k_combine(void* __restrict__ out, in
 
 }  // namespace
 
-size_t route_acc_bytes() { return (size_t)(kReplicas * kMaxExperts + kReplicas + 1) * 4; }
-
 int launch_route(vdttfs_ctx* ctx, int32_t* idx, float* wt, int32_t* count, const void* logits, int elem, int64_t ld,
-                 const float* bias, const uint8_t* row_mask, int64_t M, const vdttfs_route_opts& o, int* acc) {
+                 const float* bias, const uint8_t* row_mask, int64_t M, const vdttfs_route_opts& o) {
     if (M <= 0) {
-        if (count) k_zero<<<dim3(1), kThreads, 0, ctx->stream>>>(count, o.n_experts);
+        clear_counts(ctx, count, o.n_experts);
         VD_HIP(hipGetLastError());
         return VDTTFS_OK;
     }
     const RouteArgs a{idx,         wt,      count,   logits,   ld,           bias,        row_mask, M,
-                      o.n_experts, o.top_k, o.score, o.groups, o.top_groups, o.group_top, o.renorm, o.scale, acc};
+                      o.n_experts, o.top_k, o.score, o.groups, o.top_groups, o.group_top, o.renorm, o.scale};
     if (elem == VDTTFS_ELEM_F32) route_elem<VDTTFS_ELEM_F32>(ctx, a);
     else if (elem == VDTTFS_ELEM_BF16) route_elem<VDTTFS_ELEM_BF16>(ctx, a);
     else route_elem<VDTTFS_ELEM_F16>(ctx, a);
