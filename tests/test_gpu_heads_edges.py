@@ -157,3 +157,31 @@ def test_route_with_counts_needs_no_earlier_call(gpu_ctx_factory):
     for g, s in zip(graphs, streams):
         g.close()
         assert g.h.hipStreamDestroy(s) == 0
+
+
+# ---- activations and scores far from zero ---------------------------------------------
+@pytest.mark.parametrize("M", [1, 40, 700])
+def test_silu_of_any_size(ctx, M):
+    """v / (1 + exp(-v)) of products without terms, whose values are their biases.  Bound: the
+    hardware's exp2 and reciprocal are within 1 ulp (2 U each), the correction of the
+    exponent, the sum and the product round once each (3 U), and U more covers second
+    order; a subnormal result is within 2^-149."""
+    v = np.concatenate([
+        [-80, -87, -87.25, -87.33, -87.34, -87.4, -88, -88.1, -89, -90, -95, -100, -103, -103.9, -104.5, -110, -126,
+         -127, -150, -1000, -1e10, -3e38, -FLT_MAX, 0.0, -0.0, 1e-45, -1e-45, 1e-30, -1e-30, 60, 80, 87.4, 88.7, 89, 104,
+         200, 1e10, 3e38, FLT_MAX, np.inf, -np.inf, np.nan],
+        -np.linspace(55, 112, 400), np.linspace(-30, 30, 301), np.linspace(80, 100, 41)]).astype(np.float32)
+    N = len(v)
+    out, one = Out(ctx, M, N, N, np.float32), ctx.to_device(np.ones(max(M, N), np.float32))
+    null = View(one, 0)
+    ctx.i8_matmul(out, R.F32, N, null, 0, one, null, 0, one, ctx.to_device(v), R.SILU, M, N, 0)
+    with np.errstate(all="ignore"):
+        w = v.astype(np.float64)
+        y = w / (1.0 + np.exp(-w))
+    assert np.isnan(y[41]) and np.isnan(y[40]) and y[39] == np.inf
+    got = out.get().astype(np.float64)
+    finite = np.isfinite(y)
+    np.testing.assert_array_equal(got[:, ~finite], np.broadcast_to(y[~finite], (M, (~finite).sum())))
+    tol = 8 * R.U * np.abs(y[finite]) + 2.0 ** -149
+    off = np.abs(got[:, finite] - y[finite]) - tol
+    assert (off <= 0).all(), w[finite][off.max(axis=0) > 0]
