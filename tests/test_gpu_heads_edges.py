@@ -185,3 +185,25 @@ def test_silu_of_any_size(ctx, M):
     tol = 8 * R.U * np.abs(y[finite]) + 2.0 ** -149
     off = np.abs(got[:, finite] - y[finite]) - tol
     assert (off <= 0).all(), w[finite][off.max(axis=0) > 0]
+
+
+@pytest.mark.parametrize("E,k", KERNELS)
+@pytest.mark.parametrize("score", [0, 1])
+def test_neighbouring_logits_have_scores_of_their_own(ctx, E, k, score):
+    """Of two logits one last bit apart the larger is chosen, where a last bit of the logit is
+    eight of the score's or more: below -8 a score is within 3.5 of its last bits (the
+    hardware's exp2 and reciprocal one each, the exponent's correction, the sum and the
+    softmax's quotient half a one each)."""
+    rng = np.random.default_rng(E)
+    M = 3000
+    low = -rng.uniform(16, 80, M).astype(np.float32)
+    l = np.full((M, E), -100, np.float32)
+    if score == 0:
+        l[:, 3] = 0.0  # the sum is 1: the others are far below it
+    first, second = rng.integers(4, E // 2, M), rng.integers(E // 2, E, M)
+    l[np.arange(M), first] = low
+    l[np.arange(M), second] = np.nextafter(low, np.float32(0))
+    gi, _ = run_route(ctx, l, R.F32, None, None, k, score, 1, 1, 1, False, 1.0)
+    at = 1 if score == 0 else 0
+    np.testing.assert_array_equal(gi[:, at], second)
+    np.testing.assert_array_equal(gi[:, at + 1], first)

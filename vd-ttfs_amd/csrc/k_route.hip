@@ -49,9 +49,21 @@ __device__ __forceinline__ float wave_sum(float v) {
     return s;
 }
 
-// exp and 1 / x of the scores, by the hardware's exp2 and reciprocal: relative
-// errors below (2 + |x|) 2^-23, equal inputs give equal scores.
-__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+// exp and 1 / x of the scores, by the hardware's exp2 and reciprocal; equal inputs
+// give equal scores.  Of 32-bit logits the exponent's rounding, which grows with
+// |x|, is taken out again: neighbours past 11 would share a score without it.  The
+// bounds keep what it multiplies finite, and give 0 and a sigmoid of 0 as the exp
+// itself does.  16-bit logits lie 2^13 times as far apart as that rounding: the
+// relative error is below (2 + |x|) 2^-23.
+template <int ELEM>
+__device__ __forceinline__ float fast_exp(float x) {
+    constexpr float kHi = 1.44269504088896341f, kLo = 1.925963033500e-8f, kLn2 = 0.693147180559945f;
+    if constexpr (ELEM != VDTTFS_ELEM_F32) return __builtin_amdgcn_exp2f(x * kHi);
+    const float c = __builtin_amdgcn_fmed3f(x, -120.0f, 88.0f), t = c * kHi;
+    const float r = __builtin_fmaf(c, kLo, __builtin_fmaf(c, kHi, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e, r * kLn2, e);
+}
 __device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 
 // What a group is worth from its two largest values t0 >= t1.  Their sum is
@@ -123,7 +135,7 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < NPL; ++i) {
-                p[i] = c[i] > neg_inf() ? (c[i] == mx ? 1.0f : fast_exp(c[i] - mx)) : 0.0f;
+                p[i] = c[i] > neg_inf() ? (c[i] == mx ? 1.0f : fast_exp<ELEM>(c[i] - mx)) : 0.0f;
                 sum += p[i];
             }
             sum = 1.0f / wave_sum(sum);  // of a row without experts: not read
@@ -131,7 +143,7 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a) {
             for (int i = 0; i < NPL; ++i) p[i] *= sum;
         } else {
 #pragma unroll
-            for (int i = 0; i < NPL; ++i) p[i] = fast_rcp(1.0f + fast_exp(-c[i]));
+            for (int i = 0; i < NPL; ++i) p[i] = fast_rcp(1.0f + fast_exp<ELEM>(-c[i]));
         }
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
@@ -367,7 +379,7 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < NPL; ++i) {
-                const float x = fast_exp(l[i] - mx);
+                const float x = fast_exp<ELEM>(l[i] - mx);
                 c[i] = l[i] == mx ? 1.0f : x;  // an infinity less itself is none
                 sum += c[i];
             }
@@ -376,7 +388,7 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
             for (int i = 0; i < NPL; ++i) c[i] *= inv;
         } else {
 #pragma unroll
-            for (int i = 0; i < NPL; ++i) c[i] = fast_rcp(1.0f + fast_exp(-l[i]));
+            for (int i = 0; i < NPL; ++i) c[i] = fast_rcp(1.0f + fast_exp<ELEM>(-l[i]));
         }
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
@@ -472,8 +484,8 @@ __global__ __launch_bounds__(1024) void k_route16(RouteArgs a, int span, int vec
         if (mine > kNone) {
             e = key_expert(mine, chosen[threadIdx.x / 16][lane]);
             const float v = load_elem<ELEM>(a.logits, m * a.ld + e);
-            w = a.score != VDTTFS_SCORE_SOFTMAX ? fast_rcp(1.0f + fast_exp(-v))
-                                                : (v == mx ? 1.0f : fast_exp(v - mx)) * inv;
+            w = a.score != VDTTFS_SCORE_SOFTMAX ? fast_rcp(1.0f + fast_exp<ELEM>(-v))
+                                                : (v == mx ? 1.0f : fast_exp<ELEM>(v - mx)) * inv;
         }
         if (a.renorm) {
             const float sum = row16_sum(w);
