@@ -11,6 +11,7 @@ import vdttfs
 from vdttfs import _lib
 from test_gpu_heads import (Out, View, check, codes, ctx, expert_case, refused, run_experts,  # noqa: F401
                             run_route)
+from test_gpu_heads_paths import tile_rows
 from test_gpu_scratch import Captured
 
 pytestmark = pytest.mark.gpu
@@ -207,3 +208,33 @@ def test_neighbouring_logits_have_scores_of_their_own(ctx, E, k, score):
     at = 1 if score == 0 else 0
     np.testing.assert_array_equal(gi[:, at], second)
     np.testing.assert_array_equal(gi[:, at + 1], first)
+
+
+# ---- empty widths ----------------------------------------------------------------------
+@pytest.mark.parametrize("M,D,F,N,tile", [(2000, 0, 400, 390, 64), (2000, 20, 0, 390, 32), (30, 0, 16, 20, 1),
+                                          (2000, 0, 0, 40, 32)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_experts_of_empty_widths_and_unaligned_weights(ctx, M, D, F, N, tile, gated):
+    """Nothing is read of weights that have no terms, so their address does not matter."""
+    E, k = 4, 1
+    assert tile_rows(M, k, E, D, F, N, gated) == tile
+    rng = np.random.default_rng(M + D + F)
+    weights = expert_case(rng, E, D, F, N, gated, True)
+    w1, s1, b1, w2, s2, b2 = weights
+    idx = rng.integers(0, E, (M, k)).astype(np.int32)
+    wt = rng.random((M, k)).astype(np.float32)
+    x = rng.standard_normal((M, max(D, 1))).astype(np.float32)
+
+    def off(a):  # one byte past its alignment
+        return View(ctx.to_device(np.concatenate([np.zeros(1, np.int8), a.ravel(), np.zeros(16, np.int8)])), 1)
+
+    def some(a):
+        return ctx.to_device(a if a.size else np.zeros(4, np.float32))
+
+    dev = off(w1), some(s1), some(b1), off(w2), some(s2), some(b2)
+    out = Out(ctx, M, N, N, np.float32)
+    ctx.experts(out, R.F32, N, ctx.to_device(x), R.F32, max(D, 1), ctx.to_device(idx), ctx.to_device(wt), M, k,
+                vdttfs.ExpertWeights(E, D, F, N, R.RELU, gated, *dev))
+    q, s = R.quant_rows(x[:, :D])
+    y, d, _ = R.experts(q, s, idx, wt, *weights, R.RELU, gated)
+    check(out.get(), R.F32, y, d)

@@ -742,7 +742,7 @@ int run_grouped(vdttfs_ctx* ctx, const I8Args& a) {
     constexpr int kOut = GATED ? BN / 2 : BN;
     const int64_t tn = (a.N + kOut - 1) / kOut, blocks = a.max_tiles * tn;
     VD_TRY(check_grid(blocks));
-    if (S == 2 ? deep_ok(a) : aligned16(a)) {
+    if (S == 2 ? deep_ok(a) : aligned16(a) || a.K == 0) {  // of no terms nothing is read
         k_i8_big<BM, BN, WM, WN, 128, S, GATED, true>
             <<<dim3((unsigned)blocks), WM * WN * 64, 0, ctx->stream>>>(a, a.max_tiles, (int)tn);
     } else {
