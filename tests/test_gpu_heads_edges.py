@@ -238,3 +238,22 @@ def test_experts_of_empty_widths_and_unaligned_weights(ctx, M, D, F, N, tile, ga
     q, s = R.quant_rows(x[:, :D])
     y, d, _ = R.experts(q, s, idx, wt, *weights, R.RELU, gated)
     check(out.get(), R.F32, y, d)
+
+
+def test_a_call_without_scratch_can_be_captured_at_once(gpu_ctx_factory):
+    """Few pairs of experts without hidden channels: the biases alone, and no scratch."""
+    c = gpu_ctx_factory(vdttfs.TaskConsts(T=64, delta=16))
+    rng = np.random.default_rng(1)
+    E, D, N, M, k = 4, 20, 12, 5, 2
+    s2, b2 = np.ones((E, N), np.float32), rng.standard_normal((E, N)).astype(np.float32)
+    idx, wt = rng.integers(0, E, (M, k)).astype(np.int32), np.ones((M, k), np.float32)
+    one = c.empty(64)
+    ew = vdttfs.ExpertWeights(E, D, 0, N, R.NONE, False, one, one, None, one, c.to_device(s2), c.to_device(b2))
+    x, di, dw, out = c.to_device(np.ones((M, D), np.float32)), c.to_device(idx), c.to_device(wt), c.empty((M, N))
+    g = Captured(c, lambda: c.experts(out, R.F32, N, x, R.F32, D, di, dw, M, k, ew))
+    for _ in range(3):
+        out.fill(0xFF)
+        g.replay()
+        c.synchronize()
+        np.testing.assert_array_equal(out.download(), b2[idx[:, 0]] + b2[idx[:, 1]])
+    g.close()

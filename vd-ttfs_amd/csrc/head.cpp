@@ -62,7 +62,7 @@ int head_scratch(vdttfs_ctx* ctx, size_t bytes, unsigned char** out) {
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     VD_HIP(hipStreamIsCapturing(ctx->stream, &cs));
     const bool capturing = cs != hipStreamCaptureStatusNone;
-    if (!ctx->head.buf || ctx->head.bytes < bytes) {
+    if (ctx->head.bytes < bytes) {
         if (capturing)
             return set_error(VDTTFS_E_UNSUPPORTED,
                              "the context's scratch is too small and cannot grow under stream capture: run the call "
