@@ -257,3 +257,56 @@ def test_a_call_without_scratch_can_be_captured_at_once(gpu_ctx_factory):
         c.synchronize()
         np.testing.assert_array_equal(out.download(), b2[idx[:, 0]] + b2[idx[:, 1]])
     g.close()
+
+
+# ---- sizes at the ends of their types ---------------------------------------------------
+class Piece:
+    """Part of a device array of `n` elements, from element `at` on."""
+
+    def __init__(self, arr, at, n):
+        self.ctx, self.ptr = arr.ctx, ctypes.c_void_p(arr.ptr.value + at * arr.dtype.itemsize)
+        self.n, self.dtype = n, arr.dtype
+
+    def put(self, values):
+        h = np.ascontiguousarray(values, self.dtype)
+        assert h.size == self.n
+        _lib.check(vdttfs.lib().vdttfs_h2d(self.ctx.handle, self.ptr, ctypes.c_void_p(h.ctypes.data), h.nbytes))
+
+    def get(self):
+        h = np.empty(self.n, self.dtype)
+        _lib.check(vdttfs.lib().vdttfs_d2h(self.ctx.handle, ctypes.c_void_p(h.ctypes.data), self.ptr, h.nbytes))
+        return h
+
+
+@pytest.mark.parametrize("elem", [R.BF16, R.TIMES])
+def test_a_row_of_nearly_2_31_columns(ctx, elem):
+    """The last of a thread's columns is past 2^31; 127 columns fewer end inside a thread's eight."""
+    cols = (1 << 31) - 1
+    x, q, s = ctx.empty(cols, R.np_type(elem)), ctx.empty(cols + 8, np.int8), ctx.empty(1)
+    ends = np.arange(3000)
+    if elem == R.BF16:
+        x.fill(0x3F)  # 0x3F3F: 0.746
+        h = R.to_bits(((ends % 255 - 127) / 127).astype(np.float32), elem)
+    else:
+        x.fill(0x7F)  # past every window
+        h = (ends % 70).astype(np.float32)
+    for n in (cols, cols - 127):
+        Piece(x, 0, 3000).put(h)
+        Piece(x, n - 3000, 3000).put(h)
+        q.fill(0x5A)
+        ctx.quant_rows(x, elem, cols, 1, n, q, cols, s)
+        if elem == R.BF16:
+            v = R.from_bits(h, elem)
+            rq, rs = R.quant_rows(np.concatenate([v, [R.from_bits(np.full(1, 0x3F3F, np.uint16), elem)[0]]])[None])
+            rq, filler = rq[0, :3000], rq[0, 3000]
+        else:
+            rq, rs = R.quant_times(h[None], 64, 0.0)
+            rq, filler = rq[0], 0
+        np.testing.assert_array_equal(Piece(q, 0, 3000).get(), rq)
+        np.testing.assert_array_equal(Piece(q, n - 3000, 3000).get(), rq)
+        assert (Piece(q, n, 8).get() == 0x5A).all()
+        for at in (3000, n // 2, n - 4000):
+            assert (Piece(q, at, 1000).get() == filler).all()
+        assert s.download()[0] == rs[0]
+    for a in (x, q):
+        a.free()

@@ -27,13 +27,13 @@ __device__ __forceinline__ float row_max(float v, float* lds) {
 
 // Eight codes at column c; columns past `end` are not there.
 __device__ __forceinline__ void store8(int8_t* q, int64_t row, int c, int end, bool vec, const int (&k)[8]) {
-    if (vec && c + 8 <= end) {
+    if (vec && end - c >= 8) {
         *reinterpret_cast<uint2*>(q + row + c) = pack8(k);
         return;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (c + i < end) q[row + c + i] = (int8_t)k[i];
+        if (i < end - c) q[row + c + i] = (int8_t)k[i];
 }
 
 // The largest magnitude over LANES lanes that share a row: a part of a wave, a
@@ -104,31 +104,35 @@ __global__ __launch_bounds__(kThreads) void k_quant_long(const void* __restrict_
     __shared__ float lds[kThreads / 64];
     for (int64_t m = blockIdx.x; m < rows; m += gridDim.x) {
         float a = 0.0f;
-        for (int c = threadIdx.x * 8; c < cols; c += kThreads * 8) {
+        // unsigned: a thread's column goes past the row's end, and past 2^31
+        for (unsigned c = threadIdx.x * 8; c < (unsigned)cols; c += kThreads * 8) {
             float f[8];
-            load8<ELEM>(x, m * ldx, c, cols, f);
+            load8<ELEM>(x, m * ldx, (int)c, cols, f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) a = nan_max(a, fabsf(f[i]));
         }
         const float s = scale_of(row_max<kThreads / 64>(a, lds));
         if (threadIdx.x == 0) scale[m] = s;
         const Coder coder = coder_of(s);
-        for (int c = threadIdx.x * 8; c < cols_zero; c += kThreads * 8) {
+        for (unsigned c = threadIdx.x * 8; c < (unsigned)cols_zero; c += kThreads * 8) {
             float f[8];
             int k[8];
-            load8<ELEM>(x, m * ldx, c, cols, f);
+            load8<ELEM>(x, m * ldx, (int)c, cols, f);
             codes8(f, coder, k);
-            store8(q, m * ldq, c, cols_zero, vec_out, k);
+            store8(q, m * ldq, (int)c, cols_zero, vec_out, k);
         }
     }
 }
+
+// Runs of eight in a row, at least one.
+__host__ __device__ __forceinline__ int runs_of(int cols) { return cols > 0 ? (cols - 1) / 8 + 1 : 1; }
 
 // Spike times: eight a thread; the scale is the same for every row.
 __device__ __forceinline__ void quant_times(const float* __restrict__ x, int64_t ldx, int64_t rows, int cols,
                                             int8_t* __restrict__ q, int64_t ldq, int cols_zero,
                                             float* __restrict__ scale, float tfs, int T, int vec_out, unsigned block,
                                             unsigned blocks) {
-    const int levels = T < 127 ? T : 127, per = cols_zero > 0 ? (cols_zero + 7) / 8 : 1;
+    const int levels = T < 127 ? T : 127, per = runs_of(cols_zero);
     for (int64_t at = (int64_t)block * blockDim.x + threadIdx.x; at < rows * per; at += (int64_t)blocks * blockDim.x) {
         const int64_t m = at / per;
         const int c = (int)(at - m * per) * 8;
@@ -179,14 +183,14 @@ __global__ __launch_bounds__(1024) void k_quant_kernel(const float* __restrict__
     const int n = blockIdx.x * 64 + lane;
     float a = 0.0f;
     if (n < c_out)
-        for (int k = part; k < c_in; k += 16) a = nan_max(a, fabsf(w[(int64_t)k * c_out + n]));
+        for (unsigned k = part; k < (unsigned)c_in; k += 16) a = nan_max(a, fabsf(w[(int64_t)k * c_out + n]));
     lds[part][lane] = a;
     __syncthreads();
     for (int i = 0; i < 16; ++i) a = nan_max(a, lds[i][lane]);
     if (n >= c_out) return;
     const float s = scale_of(a);
     if (part == 0) scale[n] = s;
-    for (int k = part; k < c_in; k += 16)
+    for (unsigned k = part; k < (unsigned)c_in; k += 16)
         q[(int64_t)n * ldq + k] = s > 0.0f ? (int8_t)exact_code(w[(int64_t)k * c_out + n], s) : (int8_t)0;
 }
 
@@ -230,7 +234,7 @@ void quant_sort(vdttfs_ctx* ctx, const SortOne& sort, const void* x, int64_t ldx
                 int64_t ldq, int cols_zero, float* scale) {
     // rows of a workgroup; of spike times, eight values a thread
     const int64_t blocks = ELEM == VDTTFS_ELEM_TIMES
-                               ? (rows * (cols_zero > 0 ? (cols_zero + 7) / 8 : 1) + kSortThreads - 1) / kSortThreads
+                               ? (rows * runs_of(cols_zero) + kSortThreads - 1) / kSortThreads
                                : (rows + kSortThreads / LANES - 1) / (kSortThreads / LANES);
     const int vo = (((uintptr_t)q | (uintptr_t)ldq) & 7) == 0;
     k_quant_sort<ELEM, NV, LANES><<<dim3(1 + (unsigned)(blocks < 65536 ? blocks : 65536)), kSortThreads, 0, ctx->stream>>>(
@@ -257,7 +261,7 @@ int launch_quant_rows(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int
     else if (elem == VDTTFS_ELEM_BF16) quant_elem<VDTTFS_ELEM_BF16>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale);
     else if (elem == VDTTFS_ELEM_F16) quant_elem<VDTTFS_ELEM_F16>(ctx, x, ldx, rows, cols, q, ldq, cols_zero, scale);
     else {
-        const int64_t blocks = (rows * (cols_zero > 0 ? (cols_zero + 7) / 8 : 1) + kThreads - 1) / kThreads;
+        const int64_t blocks = (rows * runs_of(cols_zero) + kThreads - 1) / kThreads;
         k_quant_times<<<dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), kThreads, 0, ctx->stream>>>(
             static_cast<const float*>(x), ldx, rows, cols, q, ldq, cols_zero, scale, ctx->c.tfs, ctx->c.T,
             (((uintptr_t)q | (uintptr_t)ldq) & 7) == 0);

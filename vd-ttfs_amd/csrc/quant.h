@@ -116,17 +116,18 @@ __device__ __forceinline__ void unpack8(const Raw8<ELEM>& r, float (&f)[8]) {
         }
     }
 }
-// The run from column c of a row of `cols`, which ends inside it.
+// The run from column c of a row of `cols`, which ends inside it.  (Columns are
+// compared by differences: c + 8 can pass 2^31.)
 template <int ELEM>
 __device__ __forceinline__ void tail8(const void* x, int64_t row, int c, int cols, float (&f)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (c + i < cols) f[i] = load_elem<ELEM>(x, row + c + i);
+        if (i < cols - c) f[i] = load_elem<ELEM>(x, row + c + i);
 }
 template <int ELEM>
 __device__ __forceinline__ void load8(const void* x, int64_t row, int c, int cols, float (&f)[8]) {
-    unpack8<ELEM>(c + 8 <= cols ? raw8<ELEM>(x, row + c) : nothing8<ELEM>(), f);
-    if (c < cols && c + 8 > cols) tail8<ELEM>(x, row, c, cols, f);
+    unpack8<ELEM>(cols - c >= 8 ? raw8<ELEM>(x, row + c) : nothing8<ELEM>(), f);
+    if (c < cols && cols - c < 8) tail8<ELEM>(x, row, c, cols, f);
 }
 
 __device__ __forceinline__ uint2 pack8(const int (&k)[8]) {
