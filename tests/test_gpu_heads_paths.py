@@ -12,7 +12,8 @@ import pytest
 import headref as R
 import vdttfs
 from vdttfs import _lib
-from test_gpu_heads import View, Out, check, codes, ctx, expert_case, run_experts, strided, test_route  # noqa: F401
+from test_gpu_heads import View, Out, check, codes, ctx, expert_case, run_experts  # noqa: F401
+from test_gpu_heads import test_route as check_route
 
 pytestmark = pytest.mark.gpu
 
@@ -183,4 +184,4 @@ def test_experts_sorted_in_three_launches(ctx, M, k, E):
 def test_route_of_more_rows_than_the_grid(ctx, case, elem, M, pad):
     """256 workgroups of 64 rows (past 256 experts 1024 of 4): each goes on to further rows."""
     assert M > 256 * 64
-    test_route(ctx, case, elem, M, pad)
+    check_route(ctx, case, elem, M, pad)
