@@ -535,6 +535,7 @@ int vdttfs_stepnet_create_culif(vdttfs_ctx* ctx, const vdttfs_culif_layer* layer
 #define VDTTFS_ACT_RELU 1
 #define VDTTFS_ACT_SILU 2
 #define VDTTFS_I8_MAX_K 131071  /* 128 * 128 * K stays below 2^31 */
+#define VDTTFS_I8_MAX_N 134217600  /* output channels: a launch stays below 2^32 threads */
 
 /* Rows to codes.  Floats: s = max|x| / 127, q = x / s rounded to the nearest
  * whole number (half to even, within [-127, 127]); both divisions in 32-bit
@@ -548,13 +549,15 @@ int vdttfs_quant_rows(vdttfs_ctx* ctx, const void* d_x, int elem, int64_t ldx, i
                       int8_t* d_q, int64_t ldq, float* d_scale);
 /* An FC kernel in the reference layout, float [C_in][C_out] as the weights
  * blob holds it, to the products' layout: codes [C_out][ldw] and a scale for
- * each output channel, each channel quantised as quant_rows does a row. */
+ * each output channel, each channel quantised as quant_rows does a row.
+ * C_out <= VDTTFS_I8_MAX_N. */
 int vdttfs_quant_kernel(vdttfs_ctx* ctx, const float* d_kernel, int C_in, int C_out, int8_t* d_w, int64_t ldw,
                         float* d_ch_scale);
 /* out[m][n] = act(sum_k q[m][k] * w[n][k] * row_scale[m] * ch_scale[n] + bias[n]),
  * the sum exact in 32-bit integers, the scales applied in this order in 32-bit
  * floats and rounded once to out_elem (F32, BF16 or F16).  d_bias may be NULL.
- * Any int8 values, -128 too; K <= VDTTFS_I8_MAX_K. */
+ * Any int8 values, -128 too; M < 2^31, N <= VDTTFS_I8_MAX_N,
+ * K <= VDTTFS_I8_MAX_K. */
 int vdttfs_i8_matmul(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const int8_t* d_q, int64_t ldq,
                      const float* d_row_scale, const int8_t* d_w, int64_t ldw, const float* d_ch_scale,
                      const float* d_bias, int act, int64_t M, int N, int K);
@@ -599,7 +602,9 @@ int vdttfs_route(vdttfs_ctx* ctx, int32_t* d_idx, float* d_weight, int32_t* d_co
  * 32-bit floats; a row whose slots are all skipped is 0.  Device pointers, all
  * dense: w1 [E][H][d_in], s1 and b1 [E][H] with H = d_hidden or 2 * d_hidden,
  * w2 [E][d_out][d_hidden], s2 and b2 [E][d_out]; b1 and b2 may be NULL.
- * n_experts <= 1024, top_k <= 64, M * top_k < 2^31. */
+ * n_experts <= 1024, top_k <= 64, M * top_k < 2^31, d_in and d_hidden <=
+ * VDTTFS_I8_MAX_K, d_out <= VDTTFS_I8_MAX_N, and fewer than 2^32 threads for
+ * either product's tiles. */
 typedef struct vdttfs_expert_layer {
     int32_t n_experts, d_in, d_hidden, d_out;
     int32_t act, gated;

@@ -310,3 +310,38 @@ def test_a_row_of_nearly_2_31_columns(ctx, elem):
         assert s.download()[0] == rs[0]
     for a in (x, q):
         a.free()
+
+
+def test_refusals_of_sizes_that_no_launch_serves(ctx):
+    f, q, i = ctx.empty(64), ctx.empty(64, np.int8), ctx.empty(64, np.int32)
+    for N in (_lib.I8_MAX_N + 1, (1 << 31) - 1):
+        refused(_lib.E_UNSUPPORTED, ctx.quant_kernel, f, 1, N, q, 1, f)
+        refused(_lib.E_UNSUPPORTED, ctx.i8_matmul, f, R.BF16, N, q, 1, f, q, 1, f, None, 0, 1, N, 1)
+        refused(_lib.E_UNSUPPORTED, ctx.i8_linear, f, R.BF16, N, f, 0, 1, q, 1, f, None, 0, 1, N, 1)
+        refused(_lib.E_UNSUPPORTED, ctx.experts, f, R.BF16, N, f, 0, 1, i, f, 1, 1,
+                vdttfs.ExpertWeights(1, 1, 1, N, 0, False, q, f, None, q, f, None))
+    for K in (_lib.I8_MAX_K + 1, (1 << 31) - 1):
+        refused(_lib.E_UNSUPPORTED, ctx.experts, f, R.F32, 1, f, 0, K, i, f, 1, 1,
+                vdttfs.ExpertWeights(1, K, 0, 1, 0, False, q, f, None, q, f, None))
+
+
+@pytest.mark.parametrize("K", [1, 16])
+def test_matmul_of_more_tiles_than_a_launch(ctx, K):
+    """2^30 rows and some, one output each: 2^24 tiles of 64 rows, where a launch has fewer than 2^23."""
+    M, a_launch = (1 << 30) + 77, ((1 << 23) - 1) * 64
+    q, s, out = ctx.empty((M, K), np.int8), ctx.empty(M), ctx.empty(M, np.uint16)
+    q.fill(1), s.fill(0x3F), out.fill(0xFF)
+    scale = np.full(1, 0x3F3F3F3F, np.uint32).view(np.float32)[0]
+    ends = [0, a_launch - 3, 2 * a_launch - 3, M - 6]
+    for n, at in enumerate(ends):
+        Piece(q, at * K, 6 * K).put(np.repeat(np.arange(6, dtype=np.int8) - 20 * (n + 1), K))
+        Piece(s, at, 6).put(scale * np.arange(1, 7, dtype=np.float32))
+    c = ctx.to_device(np.full(1, 1.0, np.float32))
+    ctx.i8_matmul(out, R.BF16, 1, q, K, s, ctx.to_device(np.ones((1, K), np.int8)), K, c, None, R.NONE, M, 1, K)
+    want = np.full(M, R.to_bits(np.full(1, K * scale, np.float32), R.BF16)[0], np.uint16)
+    for n, at in enumerate(ends):
+        v = K * (np.arange(6) - 20.0 * (n + 1)) * (scale * np.arange(1, 7, dtype=np.float32))
+        want[at:at + 6] = R.to_bits(v.astype(np.float32), R.BF16)
+    np.testing.assert_array_equal(out.download(), want)
+    for a in (q, s, out):
+        a.free()

@@ -37,6 +37,12 @@ int check_out(const char* what, const void* out, int elem, int64_t ldo, int N) {
     return check_float_ptr(what, out, elem_size(elem));
 }
 
+int check_channels(const char* what, int N) {
+    if (N > VDTTFS_I8_MAX_N)
+        return set_error(VDTTFS_E_UNSUPPORTED, "%s: %d output channels, at most %d", what, N, VDTTFS_I8_MAX_N);
+    return VDTTFS_OK;
+}
+
 // Shape and weights of one product; the outputs are not empty.
 int check_product(const char* what, const int8_t* w, int64_t ldw, const float* ch, const float* bias, int act,
                   int K) {
@@ -53,7 +59,7 @@ int check_product(const char* what, const int8_t* w, int64_t ldw, const float* c
 int check_mnk(const char* what, int64_t M, int N, int K) {
     if (M < 0 || N < 0 || K < 0) return bad(what, "negative size");
     if (M > kMaxRows) return set_error(VDTTFS_E_UNSUPPORTED, "%s: 2^31 rows or more", what);
-    return VDTTFS_OK;
+    return check_channels(what, N);
 }
 
 // The context's scratch of these calls, at least `bytes`; a buffer whose
@@ -179,6 +185,7 @@ int vdttfs_quant_kernel(vdttfs_ctx* ctx, const float* d_kernel, int C_in, int C_
     if (C_in < 0 || C_out < 0) return bad("quant_kernel", "negative size");
     if (ldw < C_in) return bad("quant_kernel", "leading dimension below the columns");
     if (C_out == 0) return VDTTFS_OK;
+    VD_TRY(check_channels("quant_kernel", C_out));
     if (C_in > 0 && !d_w) return bad("quant_kernel", "null buffer");
     if (C_in > 0) VD_TRY(check_float_ptr("quant_kernel", d_kernel, 4));
     VD_TRY(check_float_ptr("quant_kernel", d_ch_scale, 4));
@@ -277,11 +284,14 @@ int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, cons
                          kMaxTopK);
     if (L.gated && L.d_hidden > kMaxRows / 2) return bad("experts", "hidden width too large");
     if (M == 0 || L.d_out == 0) return VDTTFS_OK;
+    VD_TRY(check_channels("experts", L.d_out));
     VD_TRY(check_out("experts", d_out, out_elem, ldo, L.d_out));
     VD_TRY(check_in("experts", d_x, x_elem, ldx, M, L.d_in));
     VD_TRY(check_float_ptr("experts", d_idx, 4));
     VD_TRY(check_float_ptr("experts", d_weight, 4));
     const int H = L.gated ? 2 * L.d_hidden : L.d_hidden;
+    if (L.d_in > VDTTFS_I8_MAX_K)  // where there is no first product too: its rows are quantised
+        return set_error(VDTTFS_E_UNSUPPORTED, "experts: %d inputs, at most %d", L.d_in, VDTTFS_I8_MAX_K);
     if (H > 0) VD_TRY(check_product("experts", L.w1, L.d_in, L.s1, L.b1, L.act, L.d_in));
     VD_TRY(check_product("experts", L.w2, L.d_hidden, L.s2, L.b2, L.act, L.d_hidden));
 

@@ -632,10 +632,8 @@ __global__ __launch_bounds__(256) void k_realign(const int8_t* __restrict__ from
     }
 }
 
-int check_grid(int64_t blocks) {
-    if (blocks > 0x7fffffffll) return set_error(VDTTFS_E_UNSUPPORTED, "product of codes: too many tiles");
-    return VDTTFS_OK;
-}
+// Workgroups of a launch: fewer than 2^32 threads.
+constexpr int64_t max_blocks(int threads) { return ((int64_t)1 << 32) / threads - 1; }
 
 // Rows that 16-byte loads to LDS can take.
 bool aligned16(const I8Args& a) {
@@ -674,7 +672,6 @@ bool i8_wants_aligned(const I8Args& a) {
 template <int BM, int BN, int WM, int WN, int BK, int S>
 int run_big(vdttfs_ctx* ctx, const I8Args& a) {
     const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
-    VD_TRY(check_grid(tm * tn));
     k_i8_big<BM, BN, WM, WN, BK, S, false, false>
         <<<dim3((unsigned)(tm * tn)), WM * WN * 64, 0, ctx->stream>>>(a, (int)tm, (int)tn);
     VD_HIP(hipGetLastError());
@@ -684,7 +681,6 @@ int run_big(vdttfs_ctx* ctx, const I8Args& a) {
 template <int BM, int BN>
 int run_tile(vdttfs_ctx* ctx, const I8Args& a) {
     const int64_t tn = (a.N + BN - 1) / BN, blocks = (a.M + BM - 1) / BM * tn;
-    VD_TRY(check_grid(blocks));
     k_i8_tile<BM, BN, 2, 2, false, false><<<dim3((unsigned)blocks), 256, 0, ctx->stream>>>(a, (int)tn);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
@@ -711,15 +707,30 @@ I8Tile i8_dense_tile(int64_t M, int N, int K, bool aligned) {
     return tiles(64, 64) >= 192 ? I8Tile{64, 64} : I8Tile{32, 32};
 }
 
-int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
-    if (a.M <= 0 || a.N <= 0) return VDTTFS_OK;
-    const bool aligned = aligned16(a);
-    const I8Tile t = i8_dense_tile(a.M, a.N, a.K, aligned);
+static int run_dense(vdttfs_ctx* ctx, const I8Args& a, I8Tile t, bool aligned) {
     if (!aligned) return t.bm == 64 ? run_tile<64, 64>(ctx, a) : run_tile<32, 32>(ctx, a);
     if (t.bm == 256) return run_big<256, 256, 2, 4, 128, 2>(ctx, a);
     if (t.bm == 128) return run_big<128, 128, 2, 2, 128, 2>(ctx, a);
     if (t.bn == 128) return run_big<64, 128, 2, 2, 128, 3>(ctx, a);
     return t.bm == 64 ? run_big<64, 64, 2, 2, 128, 4>(ctx, a) : run_big<32, 32, 2, 2, 128, 4>(ctx, a);
+}
+
+int launch_i8_dense(vdttfs_ctx* ctx, const I8Args& a) {
+    if (a.M <= 0 || a.N <= 0) return VDTTFS_OK;
+    const bool aligned = aligned16(a);
+    const I8Tile t = i8_dense_tile(a.M, a.N, a.K, aligned);
+    // as many rows a launch as its tiles allow: one tile of rows at least, with
+    // VDTTFS_I8_MAX_N channels
+    const int64_t rows = max_blocks(512) / ((a.N + t.bn - 1) / t.bn) * t.bm;
+    for (int64_t m = 0; m < a.M; m += rows) {
+        I8Args part = a;
+        part.A += m * a.lda;
+        part.sa += m;
+        part.out = static_cast<char*>(a.out) + m * a.ldo * (a.out_elem == VDTTFS_ELEM_F32 ? 4 : 2);
+        part.M = a.M - m < rows ? a.M - m : rows;
+        VD_TRY(run_dense(ctx, part, t, aligned));
+    }
+    return VDTTFS_OK;
 }
 
 // Rows of the tiles of a layer's two products: the largest that an expert's
@@ -741,7 +752,9 @@ template <int BM, int BN, int WM, int WN, int S, bool GATED>
 int run_grouped(vdttfs_ctx* ctx, const I8Args& a) {
     constexpr int kOut = GATED ? BN / 2 : BN;
     const int64_t tn = (a.N + kOut - 1) / kOut, blocks = a.max_tiles * tn;
-    VD_TRY(check_grid(blocks));
+    if (blocks > max_blocks(WM * WN * 64))
+        return set_error(VDTTFS_E_UNSUPPORTED, "experts: %lld tiles, at most %lld", (long long)blocks,
+                         (long long)max_blocks(WM * WN * 64));
     if (S == 2 ? deep_ok(a) : aligned16(a) || a.K == 0) {  // of no terms nothing is read
         k_i8_big<BM, BN, WM, WN, 128, S, GATED, true>
             <<<dim3((unsigned)blocks), WM * WN * 64, 0, ctx->stream>>>(a, a.max_tiles, (int)tn);

@@ -10,7 +10,7 @@ from ._lib import (INF_TIME, LIB_PATH, VdttfsError, lib, last_error,  # noqa: F4
                    PATH_FUSED, PATH_REG, PATH_WINDOW, ROUTE_PLAN, ROUTE_SPLIT, ROUTE_LISTS,
                    ROUTE_PIXEL, POOL_FUSE_OFF, POOL_FUSE_ALL, POOL_FUSE_AUTO,
                    ELEM_F32, ELEM_BF16, ELEM_F16, ELEM_TIMES, ACT_NONE, ACT_RELU, ACT_SILU, SCORE_SOFTMAX,
-                   SCORE_SIGMOID, I8_MAX_K)
+                   SCORE_SIGMOID, I8_MAX_K, I8_MAX_N)
 from .core import (Context, CulifLayerSpec, ExpertWeights, CulifNet, CulifStepNet, DeviceArray, Layer, Net, StepNet,  # noqa: F401
                    TaskConsts, build_luts_host, device_count, task1_consts, task2_consts,
                    task3_consts)

@@ -34,7 +34,7 @@ POOL_FUSE_OFF, POOL_FUSE_ALL, POOL_FUSE_AUTO = 0, 1, 2
 ELEM_F32, ELEM_BF16, ELEM_F16, ELEM_TIMES = 0, 1, 2, 3
 ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
-I8_MAX_K = 131071
+I8_MAX_K, I8_MAX_N = 131071, 134217600
 
 
 class VdttfsError(RuntimeError):
