@@ -49,15 +49,27 @@ class ExpertHead:
     (T + 1 floats); w1 [experts][width][hidden], w2 [experts][hidden][classes]
     and their biases: host floats in the FC layout of the weights blob.
     `balance` is added to a sample's scores where experts are chosen, and not to
-    their weights."""
+    their weights.  Shapes that do not go together raise ValueError."""
 
     def __init__(self, ctx: Context, B: int, project, project_bias, router, router_bias, alpha, w1, b1, w2, b2,
                  top_k: int = 2, balance=None):
         self.ctx, self.B, self.top_k = ctx, B, top_k
+        # the kernels read these sizes, whatever the arrays hold
+        if any(len(np.shape(a)) != n for a, n in ((project, 2), (w1, 3), (w2, 3))):
+            raise ValueError("project has two dimensions, w1 and w2 have three")
+        self.features, self.width = np.shape(project)
+        self.n_experts, _, self.hidden = np.shape(w1)
+        self.classes = np.shape(w2)[2]
+        F, W, E, H, N = self.features, self.width, self.n_experts, self.hidden, self.classes
+        for name, a, shape in (("project_bias", project_bias, (W,)), ("router", router, (F, E)),
+                               ("router_bias", router_bias, (E,)), ("alpha", alpha, (ctx.consts.T + 1,)),
+                               ("w1", w1, (E, W, H)), ("b1", b1, (E, H)), ("w2", w2, (E, H, N)), ("b2", b2, (E, N)),
+                               ("balance", balance, (E,))):
+            if (a is not None or name != "balance") and np.shape(a) != shape:
+                raise ValueError(f"{name} has shape {np.shape(a)}, not {shape}")
+        if B < 1 or not 1 <= top_k <= E:
+            raise ValueError(f"a batch of {B} and {top_k} of {E} experts")
         self.project = QuantizedKernel(ctx, project)
-        self.features, self.width = project.shape
-        self.n_experts, _, self.hidden = w1.shape
-        self.classes = w2.shape[2]
         f32 = lambda a: ctx.to_device(np.ascontiguousarray(a, np.float32))  # noqa: E731
         self.project_bias, self.router, self.router_bias, self.alpha = map(
             f32, (project_bias, router, router_bias, alpha))
