@@ -520,10 +520,14 @@ int vdttfs_stepnet_create_culif(vdttfs_ctx* ctx, const vdttfs_culif_layer* layer
  * Matrices are row-major with a leading dimension in elements, >= the columns;
  * a row's elements are contiguous.  Codes need no alignment (rows that start
  * on 16 bytes are read fastest), floats that of their type.  Outputs must not
- * overlap inputs.  Calls are stream-ordered on the context's stream; scratch
- * is the context's and grows on demand: under stream capture a call that needs
- * more than an earlier one made fails with VDTTFS_E_UNSUPPORTED, so run it
- * once before capturing it. */
+ * overlap inputs.  Calls are stream-ordered on the context's stream, which waits
+ * for no other: what other streams write is finished before a call that reads
+ * it, and they wait for the context before they read its outputs or give up its
+ * inputs.  Scratch is the context's and grows on demand: under stream capture a
+ * call that needs more than an earlier one made fails with
+ * VDTTFS_E_UNSUPPORTED, so run it once before capturing it.  A graph of such a
+ * call holds the scratch, so it runs in turn with the context's other calls;
+ * routing has none, and its graphs may run beside them. */
 /* Element types.  TIMES, an input only: float spike times as the engine's maps
  * hold them, under the context's T and tfs. */
 #define VDTTFS_ELEM_F32   0
@@ -570,10 +574,12 @@ int vdttfs_i8_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, co
  * An expert can be chosen where its logit is above -inf (NaN is not) and, with
  * d_row_mask (uint8 [M], NULL: every row), the row's byte is not 0.  Scores p
  * over those experts: softmax, exp(l - max) / sum, or sigmoid,
- * 1 / (1 + exp(-l)).  The choice goes by c = p + d_bias (float [E], NULL: p
- * itself; a bias of -inf or NaN takes the expert out).  With groups > 1 the E
- * experts are `groups` runs of neighbours; a run is worth the sum of its
- * group_top (1 or 2) largest c, and only the top_groups best runs stay.
+ * 1 / (1 + exp(-l)), in 32-bit floats, where those below the normal range may
+ * be 0.  The choice goes by c = p + d_bias (float [E], NULL: p itself; a bias of
+ * -inf or NaN takes the expert out, one of +inf puts it before all finite ones).
+ * With groups > 1 the E experts are `groups` runs of neighbours; a run is worth
+ * the sum of its group_top (1 or 2) largest c, and only the top_groups best runs
+ * stay, of equal ones the first.
  * d_idx [M][top_k] receives the experts of largest c, largest first, ties to
  * the lowest index, -1 where none is left; d_weight [M][top_k] their p (0
  * where idx is -1), divided by their sum where renorm != 0 and the sum is above

@@ -349,7 +349,7 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 // c ^ swizzle(r), so that the 16 rows of a fragment come from all banks.
 // Needs 16-byte aligned rows; the last K % 16 codes go through registers with
 // zeros behind them (S > 2; the two-stage tiles take whole chunks only).
-// 8192x4096x4096 with the 256x256 tile takes 114 to 125 us, 2.2 to 2.4 POP/s of
+// 8192x4096x4096 with the 256x256 tile takes 110 to 125 us, 2.2 to 2.5 POP/s of
 // the 5 there are, as the codes' own bits let the clock be.  A step of 128 codes
 // in K is 0.85 us of matrix instructions at their peak, 1.05 with the reads of
 // their fragments from LDS and 1.4 to 1.5 with the loads into it, so the loads

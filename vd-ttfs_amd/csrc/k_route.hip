@@ -312,7 +312,7 @@ __device__ __forceinline__ float row16_sum(float v) {
 // keys once and gives up its first whenever that is the row's largest, so a
 // choice costs a maximum over 16 lanes and a shift, for four rows at a time.
 // Bound by these instructions: 65536 rows of 256 experts, 8 chosen of 4 groups
-// of 8, take 35 us (7 by their bytes; some 800 vector instructions for four
+// of 8, take 36 us with counts (7 by their bytes; some 800 vector instructions for four
 // rows, 200 of them the lanes' sorts), and 80 with a wave per row and a search
 // for every choice.  At most kPop choices; a group has `span` lanes, a power of
 // two, the last of which may have fewer experts or none.
