@@ -570,6 +570,66 @@ int vdttfs_i8_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, co
                      int64_t ldx, const int8_t* d_w, int64_t ldw, const float* d_ch_scale, const float* d_bias,
                      int act, int64_t M, int N, int K);
 
+/* Microscaled rows in 4 bits: beside the 8-bit codes above, with half of their
+ * bytes and twice the matrix units' rate.  A block is 32 neighbours of a row (the
+ * last of a row may have fewer), with a scale byte b that stands for 2^(b - 127),
+ * 255 for NaN, and elements of the type e2m1: code c in 0..7 is 0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6, and c + 8 its negative.  (The layout of the OCP microscaling formats,
+ * version 1.0, MXFP4.)  Codes lie two a byte, the first in the low half; a row has
+ * (cols + 1) / 2 bytes of codes and (cols + 31) / 32 of scales, each with a leading
+ * dimension in bytes of its own.  Neither needs an alignment (rows of codes on 16
+ * bytes with scales on 4 are read fastest). */
+#define VDTTFS_MX_BLOCK 32
+/* Rows to blocks.  With a = max|x| of a block, X = floor(log2 a) - 2 within
+ * [-127, 127] (-127 for zeros) and elements x / 2^X rounded to the nearest, half to
+ * even, what is past 6 to 6.  A block with an infinity or a NaN has scale 255 and
+ * codes 0, so that products with it are NaN.  Floats are taken as they are; spike
+ * times as a linear encoding's pixel value (T - b) / T, b the arrival bin, 0 where
+ * nothing arrives inside the window.  The upper half of an odd row's last byte is
+ * written as 0. */
+int vdttfs_mx4_quant_rows(vdttfs_ctx* ctx, const void* d_x, int elem, int64_t ldx, int64_t rows, int cols,
+                          uint8_t* d_q, int64_t ldq, uint8_t* d_s, int64_t lds);
+/* An FC kernel in the reference layout, float [C_in][C_out], to the product's:
+ * codes [C_out][ldw] and scales [C_out][ldws], each channel as mx4_quant_rows
+ * does a row. */
+int vdttfs_mx4_quant_kernel(vdttfs_ctx* ctx, const float* d_kernel, int C_in, int C_out, uint8_t* d_w, int64_t ldw,
+                            uint8_t* d_ws, int64_t ldws);
+/* out[m][n] = act(sum_k x[m][k] * w[n][k] + bias[n]) of what the codes stand for:
+ * sums of a block exact, over blocks in 32-bit floats, rounded once to out_elem
+ * (F32, BF16 or F16).  d_bias may be NULL.  Whatever the upper half of an odd
+ * row's last byte holds does not count.  M < 2^31, N <= VDTTFS_I8_MAX_N. */
+int vdttfs_mx4_matmul(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const uint8_t* d_q, int64_t ldq,
+                      const uint8_t* d_s, int64_t lds, const uint8_t* d_w, int64_t ldw, const uint8_t* d_ws,
+                      int64_t ldws, const float* d_bias, int act, int64_t M, int N, int K);
+/* mx4_quant_rows of d_x (any element type), then mx4_matmul. */
+int vdttfs_mx4_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const void* d_x, int x_elem,
+                      int64_t ldx, const uint8_t* d_w, int64_t ldw, const uint8_t* d_ws, int64_t ldws,
+                      const float* d_bias, int act, int64_t M, int N, int K);
+
+/* Rows over their root mean square, what a product reads of a residual stream:
+ *   h = x + res          in 32 bits (d_res NULL: h = x)
+ *   u = h * gain         (d_gain float [cols], NULL: 1)
+ *   y = u / sqrt(mean(h^2) + eps)
+ * d_sum (NULL: not stored) receives h rounded to the residual's type; it may be
+ * d_res itself, with the same leading dimension, which adds to the residual in
+ * place.  The mean is of h before that rounding.  x, res: F32, BF16 or F16, each of
+ * its own type.  eps >= 0; a row of zeros gives zeros, with an eps of 0 too.  Rows
+ * of any finite values: squares past the range of 32 bits are scaled.  cols >= 1.
+ *   norm_rows:  y rounded to y_elem
+ *   norm_quant: 8-bit codes of a row and their scale, for i8_matmul: the codes that
+ *     quant_rows gives of the row u (a factor of all of a row does not change its
+ *     codes) and its scale over the root, so codes do not depend on the sum's order
+ *   norm_mx4:   y as mx4_quant_rows gives it, for mx4_matmul */
+int vdttfs_norm_rows(vdttfs_ctx* ctx, void* d_y, int y_elem, int64_t ldy, const void* d_x, int x_elem, int64_t ldx,
+                     const void* d_res, int res_elem, int64_t ldr, void* d_sum, int64_t ldsum, const float* d_gain,
+                     float eps, int64_t rows, int cols);
+int vdttfs_norm_quant(vdttfs_ctx* ctx, int8_t* d_q, int64_t ldq, float* d_scale, const void* d_x, int x_elem,
+                      int64_t ldx, const void* d_res, int res_elem, int64_t ldr, void* d_sum, int64_t ldsum,
+                      const float* d_gain, float eps, int64_t rows, int cols);
+int vdttfs_norm_mx4(vdttfs_ctx* ctx, uint8_t* d_q, int64_t ldq, uint8_t* d_s, int64_t lds, const void* d_x,
+                    int x_elem, int64_t ldx, const void* d_res, int res_elem, int64_t ldr, void* d_sum, int64_t ldsum,
+                    const float* d_gain, float eps, int64_t rows, int cols);
+
 /* Routing of rows to experts from their logits (F32, BF16 or F16 [M][ld]).
  * An expert can be chosen where its logit is above -inf (NaN is not) and, with
  * d_row_mask (uint8 [M], NULL: every row), the row's byte is not 0.  Scores p
@@ -624,6 +684,36 @@ typedef struct vdttfs_expert_layer {
 int vdttfs_experts(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const void* d_x, int x_elem,
                    int64_t ldx, const int32_t* d_idx, const float* d_weight, int64_t M, int top_k,
                    const vdttfs_expert_layer* layer);
+
+/* Rows to the order of their experts and back, for a caller's own experts between
+ * route and the sum over slots.  A pair is (row m, slot j); one whose idx lies
+ * outside [0, n_experts) is skipped, as in experts.
+ *   dispatch: z[place[m][j]] = x[m] (cols values of one float type), the pairs in the
+ *     order of their experts and, of one expert, in their own (m, then j).  d_place
+ *     int32 [M][top_k] receives each pair's row of z, -1 where it is skipped; d_start
+ *     (int32 [n_experts + 1], NULL: not stored) the first row of each expert and,
+ *     last, the number of rows used.  z has room for M * top_k rows; those past the
+ *     last used one stay as they are.
+ *   combine: out[m] = sum_j weight[m][j] * z[place[m][j]], summed in the order of the
+ *     slots in 32-bit floats and rounded once (d_weight float [M][top_k], NULL: 1).
+ *     Slots whose place lies outside [0, M * top_k) are skipped, their weights not
+ *     read; a row without slots is 0.
+ * And the gradients of a loss, from those of their outputs:
+ *   dispatch_grad: dx[m] = sum_j dz[place[m][j]]
+ *   combine_grad:  dz[place[m][j]] = weight[m][j] * dout[m], of z's type, rows that no
+ *     pair has stay as they are; dw[m][j] = sum(dout[m] * z[place[m][j]]), 0 where the
+ *     slot is skipped.  d_dz or d_dw may be NULL (d_z is not read then).
+ * Places are those of dispatch: no two pairs share a row.  n_experts <= 1024,
+ * top_k <= 64, M * top_k < 2^31. */
+int vdttfs_dispatch(vdttfs_ctx* ctx, void* d_z, int64_t ldz, int32_t* d_place, int32_t* d_start, const void* d_x,
+                    int elem, int64_t ldx, const int32_t* d_idx, int64_t M, int top_k, int n_experts, int cols);
+int vdttfs_combine(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const void* d_z, int z_elem, int64_t ldz,
+                   const int32_t* d_place, const float* d_weight, int64_t M, int top_k, int cols);
+int vdttfs_dispatch_grad(vdttfs_ctx* ctx, void* d_dx, int elem, int64_t lddx, const void* d_dz, int64_t lddz,
+                         const int32_t* d_place, int64_t M, int top_k, int cols);
+int vdttfs_combine_grad(vdttfs_ctx* ctx, void* d_dz, int64_t lddz, float* d_dw, const void* d_z, int z_elem,
+                        int64_t ldz, const void* d_dout, int out_elem, int64_t lddo, const int32_t* d_place,
+                        const float* d_weight, int64_t M, int top_k, int cols);
 
 /* ---- gather-roof probe (measurement; no reference counterpart) --------- */
 /* The integrator's weight-gather pattern alone: `waves` waves each stream

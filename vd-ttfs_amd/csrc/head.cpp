@@ -2,68 +2,12 @@
 // order of launches.
 #include <cmath>
 
-#include "head.h"
+#include "head_check.h"
 
 using namespace vdttfs;
 
-namespace {
+namespace vdttfs {
 
-constexpr int kMaxExperts = 1024, kMaxTopK = 64, kMaxGroups = 64;
-constexpr int64_t kMaxRows = 0x7fffffff;
-constexpr int kRowBytes = 128;  // rows of codes in scratch start on whole cache lines
-
-int bad(const char* what, const char* why) { return set_error(VDTTFS_E_INVALID, "%s: %s", what, why); }
-
-size_t elem_size(int elem) { return elem == VDTTFS_ELEM_BF16 || elem == VDTTFS_ELEM_F16 ? 2 : 4; }
-
-int check_float_ptr(const char* what, const void* p, size_t align) {
-    if (!p) return bad(what, "null buffer");
-    if ((uintptr_t)p % align) return bad(what, "a float buffer is not aligned to its type");
-    return VDTTFS_OK;
-}
-
-int check_in(const char* what, const void* x, int elem, int64_t ldx, int64_t rows, int cols) {
-    if (elem < VDTTFS_ELEM_F32 || elem > VDTTFS_ELEM_TIMES) return bad(what, "unknown input element type");
-    if (rows < 0 || cols < 0) return bad(what, "negative size");
-    if (rows > kMaxRows) return set_error(VDTTFS_E_UNSUPPORTED, "%s: 2^31 rows or more", what);
-    if (ldx < cols) return bad(what, "leading dimension below the columns");
-    if (rows > 0 && cols > 0) VD_TRY(check_float_ptr(what, x, elem_size(elem)));
-    return VDTTFS_OK;
-}
-
-int check_out(const char* what, const void* out, int elem, int64_t ldo, int N) {
-    if (elem < VDTTFS_ELEM_F32 || elem > VDTTFS_ELEM_F16) return bad(what, "unknown output element type");
-    if (ldo < N) return bad(what, "leading dimension below the columns");
-    return check_float_ptr(what, out, elem_size(elem));
-}
-
-int check_channels(const char* what, int N) {
-    if (N > VDTTFS_I8_MAX_N)
-        return set_error(VDTTFS_E_UNSUPPORTED, "%s: %d output channels, at most %d", what, N, VDTTFS_I8_MAX_N);
-    return VDTTFS_OK;
-}
-
-// Shape and weights of one product; the outputs are not empty.
-int check_product(const char* what, const int8_t* w, int64_t ldw, const float* ch, const float* bias, int act,
-                  int K) {
-    if (act < VDTTFS_ACT_NONE || act > VDTTFS_ACT_SILU) return bad(what, "unknown activation");
-    if (K > VDTTFS_I8_MAX_K)
-        return set_error(VDTTFS_E_UNSUPPORTED, "%s: %d terms a sum, at most %d fit 32 bits", what, K, VDTTFS_I8_MAX_K);
-    if (ldw < K) return bad(what, "leading dimension below the columns");
-    if (K > 0 && !w) return bad(what, "null buffer");
-    VD_TRY(check_float_ptr(what, ch, 4));
-    if (bias) VD_TRY(check_float_ptr(what, bias, 4));
-    return VDTTFS_OK;
-}
-
-int check_mnk(const char* what, int64_t M, int N, int K) {
-    if (M < 0 || N < 0 || K < 0) return bad(what, "negative size");
-    if (M > kMaxRows) return set_error(VDTTFS_E_UNSUPPORTED, "%s: 2^31 rows or more", what);
-    return check_channels(what, N);
-}
-
-// The context's scratch of these calls, at least `bytes`; a buffer whose
-// address a captured graph holds is set aside until the context ends.
 int head_scratch(vdttfs_ctx* ctx, size_t bytes, unsigned char** out) {
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     VD_HIP(hipStreamIsCapturing(ctx->stream, &cs));
@@ -93,15 +37,25 @@ int head_scratch(vdttfs_ctx* ctx, size_t bytes, unsigned char** out) {
     return VDTTFS_OK;
 }
 
-// Parts of one scratch buffer, each on a 256-byte boundary.
-struct Layout {
-    size_t bytes = 0;
-    size_t take(size_t n) {
-        const size_t at = bytes;
-        bytes += (n + 255) & ~size_t(255);
-        return at;
-    }
-};
+}  // namespace vdttfs
+
+namespace {
+
+constexpr int kMaxExperts = 1024;
+constexpr int kRowBytes = 128;  // rows of codes in scratch start on whole cache lines
+
+// Shape and weights of one product; the outputs are not empty.
+int check_product(const char* what, const int8_t* w, int64_t ldw, const float* ch, const float* bias, int act,
+                  int K) {
+    if (act < VDTTFS_ACT_NONE || act > VDTTFS_ACT_SILU) return bad(what, "unknown activation");
+    if (K > VDTTFS_I8_MAX_K)
+        return set_error(VDTTFS_E_UNSUPPORTED, "%s: %d terms a sum, at most %d fit 32 bits", what, K, VDTTFS_I8_MAX_K);
+    if (ldw < K) return bad(what, "leading dimension below the columns");
+    if (K > 0 && !w) return bad(what, "null buffer");
+    VD_TRY(check_float_ptr(what, ch, 4));
+    if (bias) VD_TRY(check_float_ptr(what, bias, 4));
+    return VDTTFS_OK;
+}
 
 int64_t padded(int cols) { return ((int64_t)cols + kRowBytes - 1) / kRowBytes * kRowBytes; }
 

@@ -91,4 +91,75 @@ int launch_quant_dispatch(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx,
 int launch_combine(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const float* z, int64_t ldz,
                    const int32_t* idx, const float* wt, int64_t M, int N, int top_k, int n_experts);
 
+// Rows over their root mean square: floats to y, codes of 4 bits to q with
+// scales ms, or codes of 8 bits to q with scale.
+struct NormArgs {
+    const void* x;
+    int64_t ldx;
+    const void* res;  // nullable
+    int64_t ldr;
+    void* sum;  // nullable; of the residual's type, and it may be the residual
+    int64_t lds;
+    const float* gain;  // nullable
+    float eps;
+    int64_t rows;
+    int cols;
+    void* y;
+    int y_elem;
+    int64_t ldy;
+    void* q;
+    int64_t ldq;
+    float* scale;
+    uint8_t* ms;
+    int64_t ldms;
+    int kind;  // set by the launch
+};
+int launch_norm(vdttfs_ctx* ctx, NormArgs a, int x_elem, int res_elem);
+
+// Rows to microscaled codes of 4 bits; columns [cols, cols_zero) of each row get
+// codes and scales of 0 (cols_zero: cols itself, or a multiple of 32).
+int launch_mx4_quant_rows(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int64_t rows, int cols, uint8_t* q,
+                          int64_t ldq, uint8_t* s, int64_t lds, int cols_zero);
+int launch_mx4_quant_kernel(vdttfs_ctx* ctx, const float* kernel, int c_in, int c_out, uint8_t* w, int64_t ldw,
+                            uint8_t* s, int64_t lds);
+// A product of microscaled rows: activations A [M], weights B [N].
+struct Mx4Args {
+    const uint8_t* A;
+    int64_t lda;
+    const uint8_t* sa;
+    int64_t ldsa;
+    const uint8_t* B;
+    int64_t ldb;
+    const uint8_t* sb;
+    int64_t ldsb;
+    const float* bias;  // per channel, nullable
+    void* out;
+    int64_t ldo;
+    int64_t M;
+    int N, K;
+    int act, out_elem;
+};
+int launch_mx4(vdttfs_ctx* ctx, const Mx4Args& a);
+
+// Rows to the order of their experts: place[row * top_k + slot], start[0 .. E]
+// (nullable), and the rows themselves; hist: scratch of dispatch_place_bytes.
+struct PlaceArgs {
+    int32_t* place;
+    int32_t* start;
+    const int32_t* idx;
+    int64_t M;
+    int top_k, E;
+};
+size_t dispatch_place_bytes(int64_t pairs, int n_experts);
+int launch_place(vdttfs_ctx* ctx, const PlaceArgs& a, int* hist);
+int launch_dispatch_rows(vdttfs_ctx* ctx, const PlaceArgs& a, void* z, int64_t ldz, const void* x, int elem, int64_t ldx,
+                         int cols);
+// out[m] = sum over slots of wt * z[place] (wt null: of z[place])
+int launch_gather_sum(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem, int64_t ldz,
+                      const int32_t* place, const float* wt, int64_t M, int top_k, int cols);
+// dz[place] = wt * dout (of z's type), dw = dout . z[place]; either nullable
+int launch_combine_grad(vdttfs_ctx* ctx, void* dz, int64_t lddz, float* dw, const void* z, int z_elem, int64_t ldz,
+                        const void* dout, int out_elem, int64_t ldo, const int32_t* place, const float* wt, int64_t M,
+                        int top_k, int cols);
+
 }  // namespace vdttfs

@@ -35,6 +35,7 @@ ELEM_F32, ELEM_BF16, ELEM_F16, ELEM_TIMES = 0, 1, 2, 3
 ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 I8_MAX_K, I8_MAX_N = 131071, 134217600
+MX_BLOCK = 32
 
 
 class VdttfsError(RuntimeError):
@@ -248,6 +249,17 @@ SIGNATURES = {
     "vdttfs_i8_linear": [_vp, _vp, _i, _i64, _vp, _i, _i64, _vp, _i64, _vp, _vp, _i, _i64, _i, _i],
     "vdttfs_route": [_vp, _vp, _vp, _vp, _vp, _i, _i64, _vp, _vp, _i64, C.POINTER(RouteOpts)],
     "vdttfs_experts": [_vp, _vp, _i, _i64, _vp, _i, _i64, _vp, _vp, _i64, _i, C.POINTER(ExpertLayer)],
+    "vdttfs_mx4_quant_rows": [_vp, _vp, _i, _i64, _i64, _i, _vp, _i64, _vp, _i64],
+    "vdttfs_mx4_quant_kernel": [_vp, _vp, _i, _i, _vp, _i64, _vp, _i64],
+    "vdttfs_mx4_matmul": [_vp, _vp, _i, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i, _i64, _i, _i],
+    "vdttfs_mx4_linear": [_vp, _vp, _i, _i64, _vp, _i, _i64, _vp, _i64, _vp, _i64, _vp, _i, _i64, _i, _i],
+    "vdttfs_norm_rows": [_vp, _vp, _i, _i64, _vp, _i, _i64, _vp, _i, _i64, _vp, _i64, _vp, _f, _i64, _i],
+    "vdttfs_norm_quant": [_vp, _vp, _i64, _vp, _vp, _i, _i64, _vp, _i, _i64, _vp, _i64, _vp, _f, _i64, _i],
+    "vdttfs_norm_mx4": [_vp, _vp, _i64, _vp, _i64, _vp, _i, _i64, _vp, _i, _i64, _vp, _i64, _vp, _f, _i64, _i],
+    "vdttfs_dispatch": [_vp, _vp, _i64, _vp, _vp, _vp, _i, _i64, _vp, _i64, _i, _i, _i],
+    "vdttfs_combine": [_vp, _vp, _i, _i64, _vp, _i, _i64, _vp, _vp, _i64, _i, _i],
+    "vdttfs_dispatch_grad": [_vp, _vp, _i, _i64, _vp, _i64, _vp, _i64, _i, _i],
+    "vdttfs_combine_grad": [_vp, _vp, _i64, _vp, _vp, _i, _i64, _vp, _i, _i64, _vp, _vp, _i64, _i, _i],
     "vdttfs_timer_begin": [_vp],
     "vdttfs_timer_end": [_vp, C.POINTER(C.c_double)],
     "vdttfs_probe_gather": [_vp, _i, _i64, _i, _i64, _i, C.POINTER(C.c_double)],

@@ -28,6 +28,11 @@ def _ptr(a: np.ndarray) -> C.c_void_p:
     return C.c_void_p(a.ctypes.data)
 
 
+def _opt(d):
+    """The address of a buffer that may be left out."""
+    return d.ptr if d is not None else None
+
+
 def device_count() -> int:
     n = C.c_int(0)
     check(lib().vdttfs_device_count(C.byref(n)))
@@ -292,6 +297,63 @@ class Context:
         """Each row's experts applied and summed by weight (vdttfs_experts)."""
         check(lib().vdttfs_experts(self.handle, d_out.ptr, out_elem, ldo, d_x.ptr, x_elem, ldx, d_idx.ptr,
                                    d_weight.ptr, M, top_k, C.byref(weights.c)))
+
+    def mx4_quant_rows(self, d_x, elem, ldx, rows, cols, d_q, ldq, d_s, lds):
+        """Rows of floats or spike times to microscaled 4-bit codes and block scales (vdttfs_mx4_quant_rows)."""
+        check(lib().vdttfs_mx4_quant_rows(self.handle, d_x.ptr, elem, ldx, rows, cols, d_q.ptr, ldq, d_s.ptr, lds))
+
+    def mx4_quant_kernel(self, d_kernel, C_in, C_out, d_w, ldw, d_ws, ldws):
+        """A float [C_in][C_out] FC kernel to codes [C_out][ldw] and scales [C_out][ldws] (vdttfs_mx4_quant_kernel)."""
+        check(lib().vdttfs_mx4_quant_kernel(self.handle, d_kernel.ptr, C_in, C_out, d_w.ptr, ldw, d_ws.ptr, ldws))
+
+    def mx4_matmul(self, d_out, out_elem, ldo, d_q, ldq, d_s, lds, d_w, ldw, d_ws, ldws, d_bias, act, M, N, K):
+        """act(rows x channels + bias) of microscaled 4-bit operands (vdttfs_mx4_matmul)."""
+        check(lib().vdttfs_mx4_matmul(self.handle, d_out.ptr, out_elem, ldo, d_q.ptr, ldq, d_s.ptr, lds, d_w.ptr, ldw,
+                                      d_ws.ptr, ldws, _opt(d_bias), act, M, N, K))
+
+    def mx4_linear(self, d_out, out_elem, ldo, d_x, x_elem, ldx, d_w, ldw, d_ws, ldws, d_bias, act, M, N, K):
+        """mx4_quant_rows of d_x, then mx4_matmul, in one call (vdttfs_mx4_linear)."""
+        check(lib().vdttfs_mx4_linear(self.handle, d_out.ptr, out_elem, ldo, d_x.ptr, x_elem, ldx, d_w.ptr, ldw,
+                                      d_ws.ptr, ldws, _opt(d_bias), act, M, N, K))
+
+    def norm_rows(self, d_y, y_elem, ldy, d_x, x_elem, ldx, d_res, res_elem, ldr, d_sum, ldsum, d_gain, eps, rows,
+                  cols):
+        """(x + res) * gain over its root mean square, and x + res (vdttfs_norm_rows)."""
+        check(lib().vdttfs_norm_rows(self.handle, d_y.ptr, y_elem, ldy, d_x.ptr, x_elem, ldx, _opt(d_res), res_elem,
+                                     ldr, _opt(d_sum), ldsum, _opt(d_gain), eps, rows, cols))
+
+    def norm_quant(self, d_q, ldq, d_scale, d_x, x_elem, ldx, d_res, res_elem, ldr, d_sum, ldsum, d_gain, eps, rows,
+                   cols):
+        """norm_rows as 8-bit codes with a scale a row, for i8_matmul (vdttfs_norm_quant)."""
+        check(lib().vdttfs_norm_quant(self.handle, d_q.ptr, ldq, d_scale.ptr, d_x.ptr, x_elem, ldx, _opt(d_res),
+                                      res_elem, ldr, _opt(d_sum), ldsum, _opt(d_gain), eps, rows, cols))
+
+    def norm_mx4(self, d_q, ldq, d_s, lds, d_x, x_elem, ldx, d_res, res_elem, ldr, d_sum, ldsum, d_gain, eps, rows,
+                 cols):
+        """norm_rows as microscaled 4-bit codes, for mx4_matmul (vdttfs_norm_mx4)."""
+        check(lib().vdttfs_norm_mx4(self.handle, d_q.ptr, ldq, d_s.ptr, lds, d_x.ptr, x_elem, ldx, _opt(d_res),
+                                    res_elem, ldr, _opt(d_sum), ldsum, _opt(d_gain), eps, rows, cols))
+
+    def dispatch(self, d_z, ldz, d_place, d_start, d_x, elem, ldx, d_idx, M, top_k, n_experts, cols):
+        """Rows to the order of their experts: rows, places and starts (vdttfs_dispatch)."""
+        check(lib().vdttfs_dispatch(self.handle, d_z.ptr, ldz, d_place.ptr, _opt(d_start), d_x.ptr, elem, ldx,
+                                    d_idx.ptr, M, top_k, n_experts, cols))
+
+    def combine(self, d_out, out_elem, ldo, d_z, z_elem, ldz, d_place, d_weight, M, top_k, cols):
+        """The sum over a row's slots of weight * z[place] (vdttfs_combine)."""
+        check(lib().vdttfs_combine(self.handle, d_out.ptr, out_elem, ldo, d_z.ptr, z_elem, ldz, d_place.ptr,
+                                   _opt(d_weight), M, top_k, cols))
+
+    def dispatch_grad(self, d_dx, elem, lddx, d_dz, lddz, d_place, M, top_k, cols):
+        """The gradient of dispatch's rows (vdttfs_dispatch_grad)."""
+        check(lib().vdttfs_dispatch_grad(self.handle, d_dx.ptr, elem, lddx, d_dz.ptr, lddz, d_place.ptr, M, top_k,
+                                         cols))
+
+    def combine_grad(self, d_dz, lddz, d_dw, d_z, z_elem, ldz, d_dout, out_elem, lddo, d_place, d_weight, M, top_k,
+                     cols):
+        """The gradients of combine's rows and weights (vdttfs_combine_grad)."""
+        check(lib().vdttfs_combine_grad(self.handle, _opt(d_dz), lddz, _opt(d_dw), _opt(d_z), z_elem, ldz, d_dout.ptr,
+                                        out_elem, lddo, d_place.ptr, _opt(d_weight), M, top_k, cols))
 
     def launch_pool(self, d_in, d_out, H_in, W_in, Cc, B):
         check(lib().vdttfs_launch_pool_sync(self.handle, d_in.ptr, d_out.ptr, H_in, W_in, Cc, B))
