@@ -7,6 +7,7 @@
 #include "codes.h"
 #include "elem.h"
 #include "head.h"
+#include "tiles.h"
 #include "wave.h"
 
 namespace vdttfs {
@@ -322,26 +323,6 @@ __global__ __launch_bounds__(WM* WN * 64) void k_i8_tile(I8Args p, int tiles_n) 
                             reinterpret_cast<float*>(lds) + wave * (Stage<FM, FN, GATED>::kBytes / 4));
 }
 
-// XCD-aware tile order: workgroups are handed to the eight XCDs in turn, so
-// every XCD gets a contiguous run of tiles; a run goes through bands of kBand
-// row tiles, column by column, so that the tiles in flight on an XCD share
-// their rows and channels in its L2.
-constexpr int kXcds = 8, kBand = 8;
-__device__ __forceinline__ bool tile_of(int b, int blocks, int tiles_m, int tiles_n, int* tm, int* tn) {
-    const int per = blocks / kXcds, rest = blocks % kXcds, x = b % kXcds;
-    if (b / kXcds >= per + (x < rest ? 1 : 0)) return false;  // past the last tile
-    b = x * per + (x < rest ? x : rest) + b / kXcds;
-    const int band = b / (kBand * tiles_n), in = b % (kBand * tiles_n);
-    const int left = tiles_m - band * kBand;
-    const int h = left < kBand ? left : kBand;
-    *tm = band * kBand + in % h;
-    *tn = in / h;
-    return true;
-}
-
-typedef const __attribute__((address_space(1))) void* GlobalPtr;
-typedef __attribute__((address_space(3))) void* LdsPtr;
-
 // The large product: tiles of BK codes a row go from memory to LDS directly
 // (16 bytes a lane, no registers between), S tiles deep: while one is
 // multiplied, the loads of the next S - 1 are in flight.  A wave-wide load
@@ -360,19 +341,6 @@ __device__ __forceinline__ int swizzle(int row) {
 }
 
 __device__ __align__(16) const int8_t kZeros[16] = {};
-
-// Waits until at most N of the wave's loads are outstanding (LDS writes: none).
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4 | 0 << 8);
-    asm volatile("" ::: "memory");
-}
-__device__ __forceinline__ void barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
 
 template <int BM, int BN, int WM, int WN, int BK, int S, bool GATED, bool GROUPED>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_i8_big(I8Args p, int tiles_m, int tiles_n) {
@@ -631,9 +599,6 @@ __global__ __launch_bounds__(256) void k_realign(const int8_t* __restrict__ from
         *reinterpret_cast<v4i*>(to + r * ld_to + k) = load16(from + r * ld, k, K);
     }
 }
-
-// Workgroups of a launch: fewer than 2^32 threads.
-constexpr int64_t max_blocks(int threads) { return ((int64_t)1 << 32) / threads - 1; }
 
 // Rows that 16-byte loads to LDS can take.
 bool aligned16(const I8Args& a) {

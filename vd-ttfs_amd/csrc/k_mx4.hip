@@ -6,12 +6,19 @@
 // lane, so the scales cost no instruction of their own.  Products of two elements
 // are multiples of a quarter up to 36, so a block's sum is exact; the sum over
 // blocks is in 32-bit floats.
+#include <type_traits>
+
 #include "codes.h"
 #include "elem.h"
 #include "head.h"
 #include "mx4.h"
+#include "tiles.h"
 #include "wave.h"
 
+#ifndef MX4_EARLY
+#define MX4_EARLY 0
+#define MX4_PER 2
+#endif
 namespace vdttfs {
 namespace {
 
@@ -111,11 +118,16 @@ __device__ __forceinline__ v4i codes16(const uint8_t* row, int k, int K) {
 constexpr int kBK = 128;        // bytes of a row in one LDS tile: 256 elements, 8 blocks
 constexpr int kBlocks = kBK / 16;
 
+// Chunk c (a block's 16 bytes) of row r lies at chunk c ^ swizzle(r) of the row.  A
+// lane takes chunks 2 (l / 16) and the next one, so its two scales are neighbours.
+// 16-byte reads are served in groups of 16 lanes, {0-3, 12-15, 20-23, 24-27} and so
+// on, over 256 bytes of banks: with these two bits of the row all 16 come from
+// different banks (with r & 7 in their place every other one collided: 26 M cycles
+// of conflicts in 8192 x 8192 x 8192, and 300 us).
+__device__ __forceinline__ int swizzle(int r) { return (r >> 1 & 1) | (r & 4); }
+
 // A workgroup of WM x WN waves computes BM rows x BN channels.  Operands at any
-// alignment pass through registers to LDS; chunk c (a block's 16 bytes) of row r
-// lies at chunk c ^ (r & 7), so that the 16 rows of a fragment read at one chunk
-// come from different banks.  A lane takes chunks 2 (l / 16) and the next one: its
-// two scales are then neighbours too.
+// alignment pass through registers to LDS.
 template <int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN * 64) void k_mx4_tile(Mx4Args p, int tiles_n) {
     constexpr int kT = WM * WN * 64;
@@ -170,7 +182,7 @@ __global__ __launch_bounds__(WM* WN * 64) void k_mx4_tile(Mx4Args p, int tiles_n
 #pragma unroll
         for (int i = 0; i < N16; ++i) {
             const int at = tid + i * kT, r = at / 8;
-            *reinterpret_cast<v4i*>(lds + r * kBK + (at % 8 ^ (r & 7)) * 16) = raw[i];
+            *reinterpret_cast<v4i*>(lds + r * kBK + (at % 8 ^ swizzle(r)) * 16) = raw[i];
         }
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
@@ -188,7 +200,7 @@ __global__ __launch_bounds__(WM* WN * 64) void k_mx4_tile(Mx4Args p, int tiles_n
             sb[j] = *reinterpret_cast<const uint16_t*>(scales + (BM + wn + j * 16 + r16) * kBlocks + g * 2);
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
-            const int c = ((g * 2 + kk) ^ (r16 & 7)) * 16;
+            const int c = ((g * 2 + kk) ^ swizzle(r16)) * 16;
             v4i fa[FM], fb[FN];
 #pragma unroll
             for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const v4i*>(lds + (wm + i * 16 + r16) * kBK + c);
@@ -220,7 +232,381 @@ __global__ __launch_bounds__(WM* WN * 64) void k_mx4_tile(Mx4Args p, int tiles_n
     }
 }
 
-constexpr int64_t max_blocks(int threads) { return ((int64_t)1 << 32) / threads - 1; }
+// p[0..3], the last of the first n_ok again past them (n_ok <= 0: p[0] .. is
+// not there, and p[n_ok - 1] is).
+struct __attribute__((packed, aligned(4))) Floats4 {
+    v4f v;
+};
+__device__ __forceinline__ v4f take4(const float* p, int n_ok, bool whole) {
+    if (whole) return reinterpret_cast<const Floats4*>(p)->v;
+    v4f r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = p[e < n_ok ? e : n_ok - 1];
+    return r;
+}
+
+// A wave's sums to its outputs.  A lane has four neighbouring channels of a row;
+// stored from there, a wave would write 32 bytes of each of 16 rows at a time.  So
+// 16 rows at a time pass through the wave's own part of LDS (stage) and leave as 16
+// bytes a lane, a row's outputs together.  nw: the wave's first channel.
+template <int FN>
+struct Stage {
+    static constexpr int kCols = FN * 16, kRow = kCols + 4;  // floats from row to row
+    static constexpr int kBytes = 16 * kRow * 4;
+};
+template <int FM, int FN>
+__device__ __forceinline__ void epilogue(const Mx4Args& p, const v4f (&acc)[FM][FN], int64_t m0, int nw, float* stage) {
+    typedef Stage<FN> S;
+    const int lane = lane_id();
+    const int size = p.out_elem == VDTTFS_ELEM_F32 ? 4 : 2;
+    const bool bf16 = p.out_elem == VDTTFS_ELEM_BF16;
+    const bool whole = nw + S::kCols <= p.N;
+    const bool vec = ((p.ldo * size) & 15) == 0 && (((uintptr_t)p.out + (size_t)nw * size) & 15) == 0;
+    v4f b[FN];  // before the stores: a load between them would wait in line
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int n = nw + j * 16 + (lane >> 4) * 4;
+        b[j] = p.bias ? take4(p.bias + n, p.N - n, whole) : v4f{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int64_t mi = m0 + i * 16;
+        if (mi >= p.M) break;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            v4f v = acc[i][j];
+            if (p.bias) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += b[j][e];
+            }
+            if (p.act == VDTTFS_ACT_RELU) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = apply_act(v[e], VDTTFS_ACT_RELU);
+            } else if (p.act == VDTTFS_ACT_SILU) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = apply_act(v[e], VDTTFS_ACT_SILU);
+            }
+            *reinterpret_cast<v4f*>(stage + (lane & 15) * S::kRow + j * 16 + (lane >> 4) * 4) = v;
+        }
+        wave_sync();
+        if (vec) {
+            // lanes of a row: eight columns each of two bytes, four of four
+            const int cols = size == 2 ? 8 : 4, lanes = S::kCols / cols, per = 64 / lanes;
+#pragma unroll
+            for (int r0 = 0; r0 < 16; r0 += 64 / (S::kCols / 4)) {
+                // (16-bit rows take every second turn's rows too)
+                const int r = size == 2 ? 2 * r0 + lane / lanes : r0 + lane / lanes;
+                if (size == 2 && 2 * r0 >= 16) break;
+                const int c = lane % lanes * cols;
+                if (r >= 16 || r - (size == 2 ? 2 * r0 : r0) >= per || mi + r >= p.M) continue;
+                const float* f = stage + r * S::kRow + c;
+                const int64_t o = (mi + r) * p.ldo + nw + c;
+                if (nw + c + cols > p.N) {
+#pragma unroll 1
+                    for (int e = 0; e < p.N - nw - c; ++e) store_elem(p.out, o + e, f[e], p.out_elem);
+                    continue;
+                }
+                const v4f x = *reinterpret_cast<const v4f*>(f);
+                if (size == 4) {
+                    __builtin_nontemporal_store(x, reinterpret_cast<v4f*>(static_cast<float*>(p.out) + o));
+                } else {
+                    const v4f y = *reinterpret_cast<const v4f*>(f + 4);
+                    const v4i w = {(int)pack2(x[0], x[1], bf16), (int)pack2(x[2], x[3], bf16),
+                                   (int)pack2(y[0], y[1], bf16), (int)pack2(y[2], y[3], bf16)};
+                    __builtin_nontemporal_store(w, reinterpret_cast<v4i*>(static_cast<uint16_t*>(p.out) + o));
+                }
+            }
+        } else {
+#pragma unroll 1
+            for (int at = lane; at < 16 * S::kCols; at += 64) {
+                const int row = at / S::kCols, c = at % S::kCols;
+                if (mi + row >= p.M || nw + c >= p.N) continue;
+                store_elem(p.out, (mi + row) * p.ldo + nw + c, stage[row * S::kRow + c], p.out_elem);
+            }
+        }
+        wave_sync();
+    }
+}
+
+// The large product: tiles of 128 bytes a row and the 8 scales of their blocks go
+// from memory to LDS directly (16 and 4 bytes a lane, no registers between).  Rows
+// of codes on 16 bytes, of scales on 4.  The last K % 256 elements come through
+// registers with zeros behind them.
+template <int BM, int BN, int WM, int WN, int S>
+__global__ __launch_bounds__(WM* WN * 64, WM* WN == 4 && BM == 256 ? 1 : 2) void k_mx4_big(Mx4Args p, int tiles_m,
+                                                                                          int tiles_n) {
+    constexpr int kW = WM * WN;
+    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+    constexpr int NA = BM / 8 / kW, NB = BN / 8 / kW;  // loads of codes of a wave and tile, 8 rows each
+    constexpr int kScaleLoads = (BM + BN) / 32, NS = (kScaleLoads + kW - 1) / kW;
+    constexpr int NL = NA + NB + (S > 2 ? NS : 0);
+    constexpr int kCodes = (BM + BN) * kBK, kTile = kCodes + (S > 2 ? (BM + BN) * kBlocks : 0);
+    // two stages: the scales of four tiles at a time, 32 bytes a row, two deep
+    constexpr int kSpan = 4, kRowScales = S > 2 ? kBlocks : kSpan * kBlocks, kScales = (BM + BN) * kRowScales;
+    static_assert(NA * kW * 8 == BM && NB * kW * 8 == BN && BM % 32 == 0 && BN % 32 == 0, "loads divide");
+    static_assert(S >= 2 && S <= 4 && (S - 2) * NL < 64, "stages");
+    constexpr int kStage = kW * Stage<FN>::kBytes;
+    // an array for each stage: only then does the compiler see that reads of
+    // one need not wait for loads into another
+    __shared__ __align__(16) uint8_t s0[kTile > kStage ? kTile : kStage];
+    __shared__ __align__(16) uint8_t s1[kTile];
+    __shared__ __align__(16) uint8_t s2[S > 2 ? kTile : 16];
+    __shared__ __align__(16) uint8_t s3[S > 3 ? kTile : 16];
+    __shared__ __align__(16) uint8_t spans[S > 2 ? 16 : 2 * kScales];
+
+    int tile_m, tile_n;
+    if (!tile_of(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, &tile_m, &tile_n)) return;
+    const int64_t m0 = (int64_t)tile_m * BM;
+    const int n0 = tile_n * BN;
+    const int lane = lane_id(), wave = uniform(threadIdx.x >> 6);
+    const int lrow = lane / 8, chunk = (lane % 8 ^ swizzle(lrow)) * 16;
+    // A lane's loads by their offsets from the tile's first row (below 2^31:
+    // kMaxLd), so that their addresses take a register each and scalar steps in K.
+    const uint8_t *A = p.A + m0 * p.lda, *B = p.B + n0 * p.ldb, *SA = p.sa + m0 * p.ldsa, *SB = p.sb + n0 * p.ldsb;
+    const unsigned lda = (unsigned)p.lda, ldb = (unsigned)p.ldb;
+    const int last_a = p.M - m0 < BM ? (int)(p.M - m0) - 1 : BM - 1, last_b = p.N - n0 < BN ? p.N - n0 - 1 : BN - 1;
+    unsigned from[NA + NB], sfrom[NS];  // of codes, of scales (two lanes a row)
+#pragma unroll
+    for (int i = 0; i < NA; ++i) from[i] = min((wave * NA + i) * 8 + lrow, last_a) * lda + chunk;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) from[NA + i] = min((wave * NB + i) * 8 + lrow, last_b) * ldb + chunk;
+    // a wave's load of scales is of A's rows or of B's; past the last: again the
+    // first ones, the same bytes
+    auto s_load = [&](int i) __attribute__((always_inline)) { return (wave * NS + i) % kScaleLoads; };
+    auto of_a = [&](int i) __attribute__((always_inline)) { return s_load(i) * 32 < BM; };
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int r = s_load(i) * 32 + lane / 2;
+        sfrom[i] = of_a(i) ? min(r, last_a) * (unsigned)p.ldsa : min(r - BM, last_b) * (unsigned)p.ldsb;
+    }
+    const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+    const int r16 = lane & 15, g4 = lane >> 4;
+    v4f acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+
+    const int tiles = p.K / 256;
+    // one of a wave's NL loads of tile t; past the end the last tile's, not used
+    auto fetch_one = [&](uint8_t* s, int t, int l) __attribute__((always_inline)) {
+        t = t < tiles ? t : tiles - 1;
+        if (l < NA + NB) {
+            const int at = l < NA ? wave * NA + l : BM / 8 + wave * NB + l - NA;
+            to_lds16(l < NA ? A : B, from[l < NA + NB ? l : 0], t * kBK, s + at * 1024);
+        } else {
+            const int i = l < NA + NB ? 0 : l - NA - NB;
+            to_lds4(of_a(i) ? SA : SB, sfrom[i] + (lane & 1) * 4, t * kBlocks, s + kCodes + s_load(i) * 256);
+        }
+    };
+    auto fetch = [&](uint8_t* s, int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int l = 0; l < NL; ++l) fetch_one(s, t, l);
+    };
+    // The scales of tiles 4 n .. 4 n + 3: 16 bytes a lane; where there are fewer
+    // tiles, 4 bytes a lane, those past them the row's first again, not used.  (Of 8
+    // bytes of a row in every tile, a wave's load touched 32 lines for 256 bytes:
+    // 8192 x 8192 x 8192 took 276 us.)
+    auto fetch_span = [&](int n) __attribute__((always_inline)) {
+        uint8_t* to = spans + (n & 1) * kScales;
+        if ((n + 1) * kSpan <= tiles) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+                to_lds16(of_a(i) ? SA : SB, sfrom[i] + (lane & 1) * 16, n * kSpan * kBlocks, to + s_load(i) * 1024);
+        } else {
+            const int there = (tiles - n * kSpan) * 2, d = lane % 8 < there ? lane % 8 : 0;
+            for (int i = wave; i < (BM + BN) / 8; i += kW) {
+                const int r = i * 8 + lane / 8;
+                const bool a = i * 8 < BM;
+                to_lds4(a ? SA : SB, (a ? min(r, last_a) * (unsigned)p.ldsa : min(r - BM, last_b) * (unsigned)p.ldsb) + d * 4,
+                        n * kSpan * kBlocks, to + i * 256);
+            }
+        }
+    };
+    // Each group is one row fragment against all channel fragments; fragments are
+    // read two groups (channels: one k step) ahead.
+    constexpr int G = 2 * FM;
+    // Where a lane's fragments and scales start in a stage.  Opaque, so that every
+    // read is one of these registers and an immediate: the compiler else makes
+    // addresses of all of them, more than there are registers.
+    auto place = [&](int kk) __attribute__((always_inline)) { return ((g4 * 2 + kk) ^ swizzle(r16)) * 16; };
+    int oa[2] = {(wm + r16) * kBK + place(0), (wm + r16) * kBK + place(1)};
+    int ob[2] = {(BM + wn + r16) * kBK + place(0), (BM + wn + r16) * kBK + place(1)};
+    int osa = (wm + r16) * kRowScales + g4 * 2, osb = (BM + wn + r16) * kRowScales + g4 * 2;
+    asm volatile("" : "+v"(oa[0]), "+v"(oa[1]), "+v"(ob[0]), "+v"(ob[1]), "+v"(osa), "+v"(osb));
+    auto code_a = [&](const uint8_t* s, int g) __attribute__((always_inline)) {
+        return *reinterpret_cast<const v4i*>(s + oa[g / FM] + g % FM * 16 * kBK);
+    };
+    auto code_b = [&](const uint8_t* s, int kk, int j) __attribute__((always_inline)) {
+        return *reinterpret_cast<const v4i*>(s + ob[kk] + j * 16 * kBK);
+    };
+    auto scale_a = [&](const uint8_t* s, int i) __attribute__((always_inline)) {
+        return (int)*reinterpret_cast<const uint16_t*>(s + osa + i * 16 * kRowScales);
+    };
+    auto scale_b = [&](const uint8_t* s, int j) __attribute__((always_inline)) {
+        return (int)*reinterpret_cast<const uint16_t*>(s + osb + j * 16 * kRowScales);
+    };
+    // One tile multiplied, with the loads of tile t (to `next`) spread between: a
+    // wave that issues its loads in one go waits for the address unit, and its
+    // matrix instructions with it.
+    auto multiply = [&](auto with_loads, const uint8_t* s, const uint8_t* sc, uint8_t* next, int t)
+                        __attribute__((always_inline)) {
+        v4i fa[3], fb[2][FN];
+        int sa[FM], sb[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) sb[j] = scale_b(sc, j);
+        sa[0] = scale_a(sc, 0);
+        fa[0] = code_a(s, 0);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) fb[0][j] = code_b(s, 0, j);
+        if (FM > 1) sa[FM > 1 ? 1 : 0] = scale_a(sc, 1);
+        fa[1] = code_a(s, 1);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int kk = g / FM, i = g % FM;
+            if (g + 2 < G) fa[(g + 2) % 3] = code_a(s, g + 2);
+            if (g + 2 < FM) sa[g + 2 < FM ? g + 2 : 0] = scale_a(sc, g + 2);
+            if (kk == 0) {
+#pragma unroll
+                for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j) fb[1][j] = code_b(s, 1, j);
+            }
+            if constexpr (with_loads.value) {
+#pragma unroll
+                for (int l = 0; l < NL; ++l)
+                    if (l * G / NL == g) fetch_one(next, t, l);
+            }
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                acc[i][j] = kk == 0 ? mfma4<0>(fb[0][j], fa[g % 3], acc[i][j], sb[j], sa[i])
+                                    : mfma4<1>(fb[1][j], fa[g % 3], acc[i][j], sb[j], sa[i]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // Tile t is in s; the loads of tile t + S - 1 go to `next`, whose tile every
+    // wave has read before the barrier.  No branch between loads and waits, so the
+    // number in flight is known everywhere.
+    auto step = [&](const uint8_t* s, uint8_t* next, int t) __attribute__((always_inline)) {
+        wait_loads<(S - 2) * NL>();
+        barrier();
+        multiply(std::true_type{}, s, s + kCodes, next, t + S - 1);
+    };
+    if constexpr (S == 2) {
+        // Two stages, the barrier before a tile's last two groups: by then all its
+        // fragments are in registers, so the next tile's first ones are read, and
+        // the loads of the one after that are issued into its LDS, while the matrix
+        // instructions go on.
+        static_assert(G % 4 == 0 && FM >= 4, "the ring of fragments comes round with the tile");
+        v4i fa[4], fb[2][FN];
+        int sa[2][FM], sb[2][FN];
+        // Tile t's first fragments and all its scales, where no load is in flight (as
+        // one into `spans` may be later, the compiler would wait for it)
+        auto first = [&](auto turn, const uint8_t* s, int t) __attribute__((always_inline)) {
+            const uint8_t* sc = spans + (t / kSpan & 1) * kScales + t % kSpan * kBlocks;
+            fa[0] = code_a(s, 0);
+            sa[turn.value][0] = scale_a(sc, 0);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                fb[0][j] = code_b(s, 0, j);
+                sb[turn.value][j] = scale_b(sc, j);
+            }
+            fa[1] = code_a(s, 1);
+#pragma unroll
+            for (int i = 1; i < FM; ++i) sa[turn.value][i] = scale_a(sc, i);
+        };
+        // A tile's first kEarly loads go out behind the barrier that frees its LDS,
+        // the others between the first groups of the next tile: all at once they
+        // hold up the fragment reads.
+        constexpr int kEarly = MX4_EARLY, kPer = MX4_PER;
+        static_assert(kEarly + kPer * (G - 2) >= NL, "all loads go out");
+        auto run = [&](auto turn, uint8_t* s, uint8_t* next, int t) __attribute__((always_inline)) {
+            constexpr int kTurn = turn.value;
+            if (kTurn == 0 && t % kSpan == 0 && t + kSpan < tiles) fetch_span(t / kSpan + 1);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int kk = g / FM, i = g % FM;
+                if (g + 2 < G) fa[(g + 2) % 4] = code_a(s, g + 2);
+                if (kk == 0) {
+#pragma unroll
+                    for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j) fb[1][j] = code_b(s, 1, j);
+                }
+                if (g == G - 2) {
+                    wait_loads<0>();
+                    barrier();
+                    first(std::integral_constant<int, 1 - kTurn>{}, next, t + 1);
+                }
+                if (kEarly > 0 && g >= G - 2) fetch_one(s, t + 2, g - (G - 2));
+                else
+#pragma unroll
+                    for (int l = kEarly + g * kPer; l < kEarly + (g + 1) * kPer && l < NL; ++l)
+                        fetch_one(next, t + 1, l);
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    acc[i][j] = kk == 0 ? mfma4<0>(fb[0][j], fa[g % 4], acc[i][j], sb[kTurn][j], sa[kTurn][i])
+                                        : mfma4<1>(fb[1][j], fa[g % 4], acc[i][j], sb[kTurn][j], sa[kTurn][i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // at least two tiles (deep_ok)
+        fetch_span(0);
+        fetch(s0, 0);
+        wait_loads<0>();
+        barrier();
+        first(std::integral_constant<int, 0>{}, s0, 0);
+#pragma unroll
+        for (int l = 0; l < kEarly; ++l) fetch_one(s1, 1, l);
+        int t = 0;
+        for (; t + 2 <= tiles; t += 2) {
+            run(std::integral_constant<int, 0>{}, s0, s1, t);
+            run(std::integral_constant<int, 1>{}, s1, s0, t + 1);
+        }
+        if (t < tiles) run(std::integral_constant<int, 0>{}, s0, s1, t);
+    } else if (tiles == 1) {  // nothing to load ahead
+        fetch(s0, 0);
+        wait_loads<0>();
+        barrier();
+        multiply(std::false_type{}, s0, s0 + kCodes, s0, 0);
+    } else if (tiles > 1) {
+        fetch(s0, 0);
+        fetch(s1, 1);
+        if (S > 3) fetch(s2, 2);
+        int t = 0;
+        for (; t + S <= tiles; t += S) {
+            step(s0, S == 3 ? s2 : s3, t);
+            step(s1, s0, t + 1);
+            step(s2, s1, t + 2);
+            if (S > 3) step(s3, s2, t + 3);
+        }
+        // the last tiles % S are in flight
+        wait_loads<0>();
+        barrier();
+        if (t < tiles) multiply(std::false_type{}, s0, s0 + kCodes, s0, 0);
+        if (t + 1 < tiles) multiply(std::false_type{}, s1, s1 + kCodes, s1, 0);
+        if (S > 3 && t + 2 < tiles) multiply(std::false_type{}, s2, s2 + kCodes, s2, 0);
+    }
+    wait_loads<0>();  // also those past the end
+    if (p.K % 256) {
+        const int k0 = tiles * kBK, blocks = p.K / kMxBlock + (p.K % kMxBlock != 0);
+        uint8_t* sc = S > 2 ? s0 + kCodes : spans;
+        v4i end[NA + NB];
+        uint32_t ends[NS];
+#pragma unroll
+        for (int l = 0; l < NA + NB; ++l) end[l] = codes16((l < NA ? A : B) + (from[l] - chunk), k0 + chunk, p.K);
+#pragma unroll
+        for (int l = 0; l < NS; ++l)
+            ends[l] = scales4((of_a(l) ? SA : SB) + sfrom[l], k0 / 16 + (lane & 1) * 4, blocks);
+        __syncthreads();
+#pragma unroll
+        for (int l = 0; l < NA + NB; ++l)
+            *reinterpret_cast<v4i*>(s0 + (l < NA ? wave * NA + l : BM / 8 + wave * NB + l - NA) * 1024 + lane * 16) = end[l];
+#pragma unroll
+        for (int l = 0; l < NS; ++l)
+            *reinterpret_cast<uint32_t*>(sc + (s_load(l) * 32 + lane / 2) * kRowScales + (lane & 1) * 4) = ends[l];
+        __syncthreads();
+        multiply(std::false_type{}, s0, sc, s0, 0);
+    }
+    barrier();  // the stage takes the tiles' place
+    epilogue<FM, FN>(p, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(s0) + wave * (Stage<FN>::kBytes / 4));
+}
 
 template <int BM, int BN>
 int run_tile(vdttfs_ctx* ctx, const Mx4Args& a) {
@@ -232,18 +618,53 @@ int run_tile(vdttfs_ctx* ctx, const Mx4Args& a) {
 
 }  // namespace
 
+// Rows that loads to LDS can take.
+constexpr int64_t kMaxLd = 1 << 22;  // 256 rows of them below 2^31 bytes
+static bool aligned(const Mx4Args& a) {
+    return a.lda <= kMaxLd && a.ldb <= kMaxLd && a.ldsa <= kMaxLd && a.ldsb <= kMaxLd && (((uintptr_t)a.A | (uintptr_t)a.B | (uintptr_t)a.lda | (uintptr_t)a.ldb) & 15) == 0 &&
+           (((uintptr_t)a.sa | (uintptr_t)a.sb | (uintptr_t)a.ldsa | (uintptr_t)a.ldsb) & 3) == 0;
+}
+
+template <int BM, int BN, int WM, int WN, int S>
+static int run_big(vdttfs_ctx* ctx, const Mx4Args& a) {
+    const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
+    k_mx4_big<BM, BN, WM, WN, S><<<dim3((unsigned)(tm * tn)), WM * WN * 64, 0, ctx->stream>>>(a, (int)tm, (int)tn);
+    VD_HIP(hipGetLastError());
+    return VDTTFS_OK;
+}
+
+struct Mx4Tile {
+    int bm, bn;
+};
+static Mx4Tile tile_for(int64_t M, int N, int K, bool is_aligned) {
+    auto tiles = [&](int bm, int bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); };
+    if (!is_aligned) return tiles(64, 64) >= 192 ? Mx4Tile{64, 64} : Mx4Tile{32, 32};
+    const int64_t big = tiles(256, 256), rounds = (big + 255) / 256;
+    const bool deep = K >= 512;
+    if (deep && (rounds == 1 ? big >= 160 : big * 10 >= rounds * 256 * 7)) return Mx4Tile{256, 256};
+    if (deep && tiles(128, 128) >= 384) return Mx4Tile{128, 128};
+    return tiles(64, 64) >= 192 ? Mx4Tile{64, 64} : Mx4Tile{32, 32};
+}
+
+#ifndef MX4_BIG
+#define MX4_BIG 2, 4
+#endif
 int launch_mx4(vdttfs_ctx* ctx, const Mx4Args& a) {
     if (a.M <= 0 || a.N <= 0) return VDTTFS_OK;
-    const bool large = (a.M + 63) / 64 * ((a.N + 63) / 64) >= 192;
-    const int t = large ? 64 : 32;
-    const int64_t rows = max_blocks(256) / ((a.N + t - 1) / t) * t;  // as many a launch as its tiles allow
+    const bool fast = aligned(a);
+    const Mx4Tile t = tile_for(a.M, a.N, a.K, fast);
+    const int64_t rows = max_blocks(512) / ((a.N + t.bn - 1) / t.bn) * t.bm;  // as many a launch as its tiles allow
     for (int64_t m = 0; m < a.M; m += rows) {
         Mx4Args part = a;
         part.A += m * a.lda;
         part.sa += m * a.ldsa;
         part.out = static_cast<char*>(a.out) + m * a.ldo * (a.out_elem == VDTTFS_ELEM_F32 ? 4 : 2);
         part.M = a.M - m < rows ? a.M - m : rows;
-        const int rc = large ? run_tile<64, 64>(ctx, part) : run_tile<32, 32>(ctx, part);
+        int rc;
+        if (!fast) rc = t.bm == 64 ? run_tile<64, 64>(ctx, part) : run_tile<32, 32>(ctx, part);
+        else if (t.bm == 256) rc = run_big<256, 256, MX4_BIG, 2>(ctx, part);
+        else if (t.bm == 128) rc = run_big<128, 128, 2, 2, 2>(ctx, part);
+        else rc = t.bm == 64 ? run_big<64, 64, 2, 2, 4>(ctx, part) : run_big<32, 32, 2, 2, 4>(ctx, part);
         if (rc != VDTTFS_OK) return rc;
     }
     return VDTTFS_OK;
