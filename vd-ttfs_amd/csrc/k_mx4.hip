@@ -232,96 +232,61 @@ __global__ __launch_bounds__(WM* WN * 64) void k_mx4_tile(Mx4Args p, int tiles_n
     }
 }
 
-// p[0..3], the last of the first n_ok again past them (n_ok <= 0: p[0] .. is
-// not there, and p[n_ok - 1] is).
-struct __attribute__((packed, aligned(4))) Floats4 {
-    v4f v;
-};
-__device__ __forceinline__ v4f take4(const float* p, int n_ok, bool whole) {
-    if (whole) return reinterpret_cast<const Floats4*>(p)->v;
-    v4f r;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = p[e < n_ok ? e : n_ok - 1];
-    return r;
-}
-
 // A wave's sums to its outputs.  A lane has four neighbouring channels of a row;
 // stored from there, a wave would write 32 bytes of each of 16 rows at a time.  So
-// 16 rows at a time pass through the wave's own part of LDS (stage) and leave as 16
-// bytes a lane, a row's outputs together.  nw: the wave's first channel.
-template <int FN>
+// two fragments of rows at a time pass through the wave's own part of LDS (16-byte
+// chunk c of row r at chunk c ^ r), and leave eight neighbours a lane, a row's
+// outputs together.  The loop over rows is one piece of code for all types, ends and
+// activations: unrolled for each, a tile's end took 9.5 us, most of it instructions
+// on their way.  nw: the wave's first channel.
+template <int FM, int FN>
 struct Stage {
-    static constexpr int kCols = FN * 16, kRow = kCols + 4;  // floats from row to row
-    static constexpr int kBytes = 16 * kRow * 4;
+    static constexpr int kFrags = FM > 1 ? 2 : 1, kRows = kFrags * 16, kCols = FN * 16;
+    static constexpr int kBytes = kRows * kCols * 4;
 };
 template <int FM, int FN>
 __device__ __forceinline__ void epilogue(const Mx4Args& p, const v4f (&acc)[FM][FN], int64_t m0, int nw, float* stage) {
-    typedef Stage<FN> S;
-    const int lane = lane_id();
-    const int size = p.out_elem == VDTTFS_ELEM_F32 ? 4 : 2;
-    const bool bf16 = p.out_elem == VDTTFS_ELEM_BF16;
-    const bool whole = nw + S::kCols <= p.N;
-    const bool vec = ((p.ldo * size) & 15) == 0 && (((uintptr_t)p.out + (size_t)nw * size) & 15) == 0;
-    v4f b[FN];  // before the stores: a load between them would wait in line
+    typedef Stage<FM, FN> S;
+    constexpr int kChunks = S::kCols / 4, kLanes = S::kCols / 8, kPass = 64 / kLanes;  // lanes of a row, rows of a pass
+    const int lane = lane_id(), c = lane % kLanes * 8, left = p.N - nw - c;
+    float bias[8];
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-        const int n = nw + j * 16 + (lane >> 4) * 4;
-        b[j] = p.bias ? take4(p.bias + n, p.N - n, whole) : v4f{0, 0, 0, 0};
-    }
+    for (int e = 0; e < 8; ++e) bias[e] = p.bias && e < left ? p.bias[nw + c + e] : 0.0f;
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int64_t mi = m0 + i * 16;
-        if (mi >= p.M) break;
+    for (int i0 = 0; i0 < FM; i0 += S::kFrags) {
+        const int64_t mi = m0 + i0 * 16;
+        if (mi >= p.M) return;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            v4f v = acc[i][j];
-            if (p.bias) {
+        for (int i = 0; i < S::kFrags; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] += b[j][e];
+            for (int j = 0; j < FN; ++j) {
+                const int r = i * 16 + (lane & 15), at = (j * 4 + (lane >> 4)) ^ (r & (kChunks - 1));
+                *reinterpret_cast<v4f*>(stage + r * S::kCols + at * 4) = acc[i0 + i][j];
             }
+        wave_sync();
+#pragma unroll 1
+        for (int r = lane / kLanes; r < S::kRows; r += kPass) {
+            if (mi + r >= p.M || left <= 0) break;
+            const int x = r & (kChunks - 1);
+            const v4f lo = *reinterpret_cast<const v4f*>(stage + r * S::kCols + ((c / 4) ^ x) * 4);
+            const v4f hi = *reinterpret_cast<const v4f*>(stage + r * S::kCols + ((c / 4 + 1) ^ x) * 4);
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += bias[e];
             if (p.act == VDTTFS_ACT_RELU) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = apply_act(v[e], VDTTFS_ACT_RELU);
+                for (int e = 0; e < 8; ++e) v[e] = apply_act(v[e], VDTTFS_ACT_RELU);
             } else if (p.act == VDTTFS_ACT_SILU) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = apply_act(v[e], VDTTFS_ACT_SILU);
+                for (int e = 0; e < 8; ++e) v[e] = apply_act(v[e], VDTTFS_ACT_SILU);
             }
-            *reinterpret_cast<v4f*>(stage + (lane & 15) * S::kRow + j * 16 + (lane >> 4) * 4) = v;
-        }
-        wave_sync();
-        if (vec) {
-            // lanes of a row: eight columns each of two bytes, four of four
-            const int cols = size == 2 ? 8 : 4, lanes = S::kCols / cols, per = 64 / lanes;
+            const int64_t o = (mi + r) * p.ldo + nw + c;
+            if (left >= 8) {
+                put8(p.out, o, p.out_elem, v);
+            } else {
 #pragma unroll
-            for (int r0 = 0; r0 < 16; r0 += 64 / (S::kCols / 4)) {
-                // (16-bit rows take every second turn's rows too)
-                const int r = size == 2 ? 2 * r0 + lane / lanes : r0 + lane / lanes;
-                if (size == 2 && 2 * r0 >= 16) break;
-                const int c = lane % lanes * cols;
-                if (r >= 16 || r - (size == 2 ? 2 * r0 : r0) >= per || mi + r >= p.M) continue;
-                const float* f = stage + r * S::kRow + c;
-                const int64_t o = (mi + r) * p.ldo + nw + c;
-                if (nw + c + cols > p.N) {
-#pragma unroll 1
-                    for (int e = 0; e < p.N - nw - c; ++e) store_elem(p.out, o + e, f[e], p.out_elem);
-                    continue;
-                }
-                const v4f x = *reinterpret_cast<const v4f*>(f);
-                if (size == 4) {
-                    __builtin_nontemporal_store(x, reinterpret_cast<v4f*>(static_cast<float*>(p.out) + o));
-                } else {
-                    const v4f y = *reinterpret_cast<const v4f*>(f + 4);
-                    const v4i w = {(int)pack2(x[0], x[1], bf16), (int)pack2(x[2], x[3], bf16),
-                                   (int)pack2(y[0], y[1], bf16), (int)pack2(y[2], y[3], bf16)};
-                    __builtin_nontemporal_store(w, reinterpret_cast<v4i*>(static_cast<uint16_t*>(p.out) + o));
-                }
-            }
-        } else {
-#pragma unroll 1
-            for (int at = lane; at < 16 * S::kCols; at += 64) {
-                const int row = at / S::kCols, c = at % S::kCols;
-                if (mi + row >= p.M || nw + c >= p.N) continue;
-                store_elem(p.out, (mi + row) * p.ldo + nw + c, stage[row * S::kRow + c], p.out_elem);
+                for (int e = 0; e < 8; ++e)
+                    if (e < left) store_elem(p.out, o + e, v[e], p.out_elem);
             }
         }
         wave_sync();
@@ -345,7 +310,7 @@ __global__ __launch_bounds__(WM* WN * 64, WM* WN == 4 && BM == 256 ? 1 : 2) void
     constexpr int kSpan = 4, kRowScales = S > 2 ? kBlocks : kSpan * kBlocks, kScales = (BM + BN) * kRowScales;
     static_assert(NA * kW * 8 == BM && NB * kW * 8 == BN && BM % 32 == 0 && BN % 32 == 0, "loads divide");
     static_assert(S >= 2 && S <= 4 && (S - 2) * NL < 64, "stages");
-    constexpr int kStage = kW * Stage<FN>::kBytes;
+    constexpr int kStage = kW * Stage<FM, FN>::kBytes;
     // an array for each stage: only then does the compiler see that reads of
     // one need not wait for loads into another
     __shared__ __align__(16) uint8_t s0[kTile > kStage ? kTile : kStage];
@@ -605,7 +570,7 @@ __global__ __launch_bounds__(WM* WN * 64, WM* WN == 4 && BM == 256 ? 1 : 2) void
         multiply(std::false_type{}, s0, sc, s0, 0);
     }
     barrier();  // the stage takes the tiles' place
-    epilogue<FM, FN>(p, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(s0) + wave * (Stage<FN>::kBytes / 4));
+    epilogue<FM, FN>(p, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(s0) + wave * (Stage<FM, FN>::kBytes / 4));
 }
 
 template <int BM, int BN>

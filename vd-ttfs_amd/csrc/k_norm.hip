@@ -14,24 +14,9 @@ namespace {
 
 constexpr int kNoRes = -1;
 
-// Eight neighbouring values to a row of a float type; all there.
 struct __attribute__((packed, aligned(1))) AnyUint2 {
     uint32_t v[2];
 };
-__device__ __forceinline__ void put8(void* p, int64_t at, int elem, const float (&f)[8]) {
-    if (elem == VDTTFS_ELEM_F32) {
-        AnyUint4* to = reinterpret_cast<AnyUint4*>(static_cast<float*>(p) + at);
-        to[0].v = v4u{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
-        to[1].v = v4u{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])};
-        return;
-    }
-    AnyUint4* to = reinterpret_cast<AnyUint4*>(static_cast<uint16_t*>(p) + at);
-    if (elem == VDTTFS_ELEM_BF16)
-        to->v = v4u{pack2(f[0], f[1], true), pack2(f[2], f[3], true), pack2(f[4], f[5], true), pack2(f[6], f[7], true)};
-    else
-        to->v = v4u{pack2(f[0], f[1], false), pack2(f[2], f[3], false), pack2(f[4], f[5], false),
-                    pack2(f[6], f[7], false)};
-}
 __device__ __forceinline__ void store8(void* p, int64_t row, int c, int cols, int elem, const float (&f)[8]) {
     if (cols - c >= 8) {
         put8(p, row + c, elem, f);

@@ -40,6 +40,31 @@ __device__ __forceinline__ uint32_t mx4_codes8(const float (&x)[8], int scale) {
     return scale == kMxNan ? 0 : w;
 }
 
+// Eight neighbouring values to a row of a float type; all there.
+typedef v4u v4u_any __attribute__((aligned(1)));
+#ifndef PUTNT
+#define PUTNT 1
+#endif
+__device__ __forceinline__ void put16(void* p, v4u v) {
+    if (PUTNT) __builtin_nontemporal_store(v, static_cast<v4u_any*>(p));
+    else *static_cast<v4u_any*>(p) = v;
+}
+__device__ __forceinline__ void put8(void* p, int64_t at, int elem, const float (&f)[8]) {
+    if (elem == VDTTFS_ELEM_F32) {
+        float* to = static_cast<float*>(p) + at;
+        put16(to, v4u{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])});
+        put16(to + 4, v4u{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])});
+        return;
+    }
+    uint16_t* to = static_cast<uint16_t*>(p) + at;
+    if (elem == VDTTFS_ELEM_BF16)
+        put16(to, v4u{pack2(f[0], f[1], true), pack2(f[2], f[3], true), pack2(f[4], f[5], true),
+                      pack2(f[6], f[7], true)});
+    else
+        put16(to, v4u{pack2(f[0], f[1], false), pack2(f[2], f[3], false), pack2(f[4], f[5], false),
+                      pack2(f[6], f[7], false)});
+}
+
 struct __attribute__((packed, aligned(1))) AnyUint {
     uint32_t v;
 };
