@@ -140,6 +140,9 @@ struct Mx4Args {
     int act, out_elem;
 };
 int launch_mx4(vdttfs_ctx* ctx, const Mx4Args& a);
+// The product of few rows, quantised in the kernel (a.A and a.sa unused).
+bool mx4_small_linear_ok(int64_t M, int K);
+int launch_mx4_small_linear(vdttfs_ctx* ctx, const Mx4Args& a, const void* x, int elem, int64_t ldx);
 
 // Rows to the order of their experts: place[row * top_k + slot], start[0 .. E]
 // (nullable), and the rows themselves; hist: scratch of dispatch_place_bytes.
@@ -150,6 +153,10 @@ struct PlaceArgs {
     int64_t M;
     int top_k, E;
 };
+// Few pairs: all of it in one launch, without scratch.
+bool dispatch_few_ok(int64_t pairs);
+int launch_dispatch_few(vdttfs_ctx* ctx, const PlaceArgs& a, void* z, int64_t ldz, const void* x, int elem, int64_t ldx,
+                        int cols);
 size_t dispatch_place_bytes(int64_t pairs, int n_experts);
 int launch_place(vdttfs_ctx* ctx, const PlaceArgs& a, int* hist);
 int launch_dispatch_rows(vdttfs_ctx* ctx, const PlaceArgs& a, void* z, int64_t ldz, const void* x, int elem, int64_t ldx,

@@ -127,6 +127,8 @@ int vdttfs_mx4_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, c
     VD_TRY(check_out("mx4_linear", d_out, out_elem, ldo, N));
     VD_TRY(check_in("mx4_linear", d_x, x_elem, ldx, M, K));
     VD_TRY(check_mx4_product("mx4_linear", d_w, ldw, d_ws, ldws, d_bias, act, K));
+    Mx4Args a{nullptr, 0, nullptr, 0, d_w, ldw, d_ws, ldws, d_bias, d_out, ldo, M, N, K, act, out_elem};
+    if (mx4_small_linear_ok(M, K)) return launch_mx4_small_linear(ctx, a, d_x, x_elem, ldx);
     const int64_t ldq = (mx4_bytes(K) + 127) / 128 * 128, lds = ldq / 16;
     Layout l;
     const size_t at_q = l.take((size_t)M * ldq), at_s = l.take((size_t)M * lds);
@@ -134,7 +136,11 @@ int vdttfs_mx4_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, c
     VD_TRY(head_scratch(ctx, l.bytes, &buf));
     uint8_t *q = buf + at_q, *s = buf + at_s;
     VD_TRY(launch_mx4_quant_rows(ctx, d_x, x_elem, ldx, M, K, q, ldq, s, lds, K));
-    return launch_mx4(ctx, Mx4Args{q, ldq, s, lds, d_w, ldw, d_ws, ldws, d_bias, d_out, ldo, M, N, K, act, out_elem});
+    a.A = q;
+    a.lda = ldq;
+    a.sa = s;
+    a.ldsa = lds;
+    return launch_mx4(ctx, a);
 }
 
 int vdttfs_norm_rows(vdttfs_ctx* ctx, void* d_y, int y_elem, int64_t ldy, const void* d_x, int x_elem, int64_t ldx,
@@ -198,6 +204,7 @@ int vdttfs_dispatch(vdttfs_ctx* ctx, void* d_z, int64_t ldz, int32_t* d_place, i
         VD_TRY(check_matrix("dispatch", d_z, elem, ldz, cols));
     }
     const PlaceArgs a{d_place, d_start, d_idx, M, top_k, n_experts};
+    if (dispatch_few_ok(M * top_k)) return launch_dispatch_few(ctx, a, d_z, ldz, d_x, elem, ldx, cols);
     unsigned char* buf = nullptr;
     const size_t bytes = dispatch_place_bytes(M * top_k, n_experts);
     if (bytes) VD_TRY(head_scratch(ctx, bytes, &buf));

@@ -3,8 +3,11 @@
 // A pair is (row m, slot j), number m * top_k + j; its place is its rank among
 // the pairs with an expert, by expert and then by number.  Rows move as they are;
 // sums over slots are in 32 bits, in the order of the slots.
+#include <type_traits>
+
 #include "elem.h"
 #include "head.h"
+#include "mx4.h"
 #include "quant.h"
 #include "sort.h"
 #include "wave.h"
@@ -148,78 +151,226 @@ __global__ __launch_bounds__(kCopy) void k_dispatch_rows(PlaceArgs a, void* __re
                       a.place + m * a.top_k, a.top_k, a.M * a.top_k);
 }
 
-// A row of floats with its slots.  T threads a row, eight neighbours a thread and
-// turn.
-__device__ __forceinline__ bool placed(int p, int64_t rows) { return p >= 0 && p < rows; }
+// Up to kFewPairs pairs in one launch: a workgroup per row looks through all pairs
+// for the ranks of its own, and one more counts the experts' starts.  (The three
+// launches of the sort and the copy's take 13 us for one row, this 4.6.)
+constexpr int kFewPairs = 1024;
+__global__ __launch_bounds__(kCopy) void k_dispatch_few(PlaceArgs a, void* __restrict__ z, int64_t ldz,
+                                                        const void* __restrict__ x, int64_t ldx, int cols, int unit) {
+    __shared__ int e[kFewPairs];
+    __shared__ int hist[kMaxExperts];
+    __shared__ int mine[64];  // top_k <= 64
+    __shared__ int sums[kCopy / 64];
+    const int pairs = (int)(a.M * a.top_k), wave = threadIdx.x >> 6, lane = lane_id();
+    for (int q = threadIdx.x; q < kFewPairs; q += kCopy) e[q] = expert_of(a, q, pairs);
+    if (blockIdx.x == a.M) {  // the starts: four neighbouring experts a thread
+        for (int i = threadIdx.x; i < kMaxExperts; i += kCopy) hist[i] = 0;
+        __syncthreads();
+        for (int q = threadIdx.x; q < kFewPairs; q += kCopy)
+            if (e[q] >= 0) atomicAdd(&hist[e[q]], 1);
+        __syncthreads();
+        const int4 n = reinterpret_cast<const int4*>(hist)[threadIdx.x];
+        const int all = n.x + n.y + n.z + n.w, incl = wave_incl_scan(all);
+        if (lane == 63) sums[wave] = incl;
+        __syncthreads();
+        int at = incl - all;
+        for (int w = 0; w < wave; ++w) at += sums[w];
+        const int four[4] = {at, at + n.x, at + n.x + n.y, at + n.x + n.y + n.z};
+        for (int i = 0; i < 4; ++i)
+            if ((int)threadIdx.x * 4 + i < a.E) a.start[threadIdx.x * 4 + i] = four[i];
+        if (threadIdx.x == kCopy - 1) a.start[a.E] = at + all;
+        return;
+    }
+    __syncthreads();
+    const int m = blockIdx.x;
+    for (int j = wave; j < a.top_k; j += kCopy / 64) {
+        const int p = m * a.top_k + j, own = e[p];
+        int before = 0;
+        for (int q = lane; q < (pairs + 63) / 64 * 64; q += 64)
+            before += __popcll(__ballot(e[q] >= 0 && (e[q] < own || (e[q] == own && q < p))));
+        if (lane == 0) {
+            mine[j] = own >= 0 ? before : -1;
+            a.place[p] = mine[j];
+        }
+    }
+    __syncthreads();
+    copy_to_slots(z, ldz * unit, static_cast<const char*>(x) + m * ldx * unit, (int64_t)cols * unit, unit, mine, a.top_k,
+                  pairs);
+}
 
-template <int ZE>
-__global__ __launch_bounds__(256) void k_gather_sum(void* __restrict__ out, int out_elem, int64_t ldo,
-                                                    const void* __restrict__ z, int64_t ldz,
-                                                    const int32_t* __restrict__ place, const float* __restrict__ wt,
-                                                    int64_t M, int top_k, int cols, int log_t) {
-    const int T = 1 << log_t, rows = 256 >> log_t, lane = threadIdx.x & (T - 1);
-    const int64_t most = M * top_k;
-    for (int64_t m = (int64_t)blockIdx.x * rows + (threadIdx.x >> log_t); m < M; m += (int64_t)gridDim.x * rows) {
+// ---- sums over slots, and their gradients --------------------------------------------
+// T lanes share a row (a part of a wave, a wave, or the workgroup), eight neighbours a
+// lane and turn.  Up to eight slots' loads are in flight at a time; a wave that has a
+// row to itself finds its places by scalar loads.
+constexpr int kRow = 256, kSlots = 8;
+template <int T>
+__device__ __forceinline__ int64_t row_of(int64_t m) {
+    if constexpr (T >= 64) return (int64_t)__builtin_amdgcn_readfirstlane((int)m);
+    return m;
+}
+struct Slots {
+    int place[kSlots];
+    float w[kSlots];
+};
+// The slots j0 .. j0 + 7 of a row: places of -1 past the last.
+__device__ __forceinline__ Slots slots_of(const int32_t* place, const float* wt, int64_t q, int n, int64_t rows) {
+    Slots s;
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+        const int p = j < n ? place[q + j] : -1;
+        s.place[j] = p >= 0 && p < rows ? p : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) s.w[j] = wt && s.place[j] >= 0 ? wt[q + j] : 1.0f;
+    return s;
+}
+template <int ELEM>
+__device__ __forceinline__ void end8(const void* x, int64_t row, int c, int cols, float (&f)[8]) {
+    if (cols - c < 8) tail8<ELEM>(x, row, c, cols, f);
+}
+__device__ __forceinline__ void store8(void* p, int64_t row, int c, int cols, int elem, const float (&f)[8]) {
+    if (cols - c >= 8) {
+        put8(p, row + c, elem, f);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < cols - c) store_elem(p, row + c + i, f[i], elem);
+}
+
+template <int ZE, int T>
+__global__ __launch_bounds__(kRow) void k_gather_sum(void* __restrict__ out, int out_elem, int64_t ldo,
+                                                     const void* __restrict__ z, int64_t ldz,
+                                                     const int32_t* __restrict__ place, const float* __restrict__ wt,
+                                                     int64_t M, int top_k, int cols) {
+    constexpr int kRows = kRow / T;
+    const int lane = threadIdx.x % T;
+    const int64_t rows = M * top_k;
+    for (int64_t at = (int64_t)blockIdx.x * kRows + threadIdx.x / T; at < M; at += (int64_t)gridDim.x * kRows) {
+        const int64_t m = row_of<T>(at);
         for (unsigned c = lane * 8; c < (unsigned)cols; c += T * 8) {
+            const bool whole = cols - (int)c >= 8;
             float sum[8] = {};
-            for (int j = 0; j < top_k; ++j) {
-                const int p = place[m * top_k + j];
-                if (!placed(p, most)) continue;
-                const float w = wt ? wt[m * top_k + j] : 1.0f;
-                float f[8];
-                load8<ZE>(z, (int64_t)p * ldz, (int)c, cols, f);
+            for (int j0 = 0; j0 < top_k; j0 += kSlots) {
+                const Slots s = slots_of(place, wt, m * top_k + j0, top_k - j0, rows);
+                Raw8<ZE> raw[kSlots];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum[i] += w * f[i];
+                for (int j = 0; j < kSlots; ++j) {
+                    raw[j] = nothing8<ZE>();
+                    if (s.place[j] >= 0 && whole) raw[j] = raw8<ZE>(z, s.place[j] * ldz + c);
+                }
+#pragma unroll
+                for (int j = 0; j < kSlots; ++j) {
+                    if (s.place[j] < 0) continue;
+                    float f[8];
+                    unpack8<ZE>(raw[j], f);
+                    end8<ZE>(z, s.place[j] * ldz, (int)c, cols, f);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum[i] += s.w[j] * f[i];
+                }
             }
-            const int64_t o = m * ldo + c;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < cols - (int)c) store_elem(out, o + i, sum[i], out_elem);
+            store8(out, m * ldo, (int)c, cols, out_elem, sum);
         }
     }
 }
 
-// A workgroup per row: dout is read for each group of slots, and every slot's z
-// once.
-template <int ZE, int OE>
-__global__ __launch_bounds__(256) void k_combine_grad(void* __restrict__ dz, int64_t lddz, float* __restrict__ dw,
-                                                      const void* __restrict__ z, int64_t ldz,
-                                                      const void* __restrict__ dout, int64_t ldo,
-                                                      const int32_t* __restrict__ place, const float* __restrict__ wt,
-                                                      int64_t M, int top_k, int cols) {
-    __shared__ float part[4];
-    const int64_t most = M * top_k;
-    for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
-        for (int j = 0; j < top_k; ++j) {
-            const int64_t q = m * top_k + j;
-            const int p = place[q];
-            const bool on = placed(p, most);  // the same for the workgroup
-            float dot = 0.0f;
-            if (on) {
-                const float w = wt ? wt[q] : 1.0f;
-                for (unsigned c = threadIdx.x * 8; c < (unsigned)cols; c += 256 * 8) {
-                    float d[8];
-                    load8<OE>(dout, m * ldo, (int)c, cols, d);
-                    if (dw) {
-                        float f[8];
-                        load8<ZE>(z, (int64_t)p * ldz, (int)c, cols, f);
+// Eight sums over T lanes at once: lanes exchange halves of the values they hold until
+// each has one, so ten moves do for eight sums of a wave.  Lane l has that of slot
+// slot_of(l) in the end.
+template <int T>
+__device__ __forceinline__ int slot_of(int lane) {
+    return (lane >> 5 & 1) * 4 + (lane >> 4 & 1) * 2 + (lane >> 3 & 1);
+}
+__device__ __forceinline__ float wave_sum8(float (&v)[kSlots]) {
+    const int lane = lane_id();
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) dot = __builtin_fmaf(d[i], f[i], dot);
+    for (int o = 32, n = 4; o >= 8; o /= 2, n /= 2) {
+        const bool up = (lane & o) != 0;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+            v[i] = keep + __shfl_xor(give, o, 64);
+        }
+    }
+    float s = v[0];
+#pragma unroll
+    for (int o = 4; o > 0; o /= 2) s += __shfl_xor(s, o, 64);
+    return s;
+}
+
+// dout is read once for eight slots, every slot's z once, and dz written once.
+template <int ZE, int OE, int T>
+__global__ __launch_bounds__(kRow) void k_combine_grad(void* __restrict__ dz, int64_t lddz, float* __restrict__ dw,
+                                                       const void* __restrict__ z, int64_t ldz,
+                                                       const void* __restrict__ dout, int64_t ldo,
+                                                       const int32_t* __restrict__ place, const float* __restrict__ wt,
+                                                       int64_t M, int top_k, int cols) {
+    constexpr int kRows = kRow / T;
+    __shared__ float part[2][kRow / 64][kSlots];
+    const int lane = threadIdx.x % T, wave = threadIdx.x >> 6;
+    const int64_t rows = M * top_k;
+    int turn = 0;
+    for (int64_t at = (int64_t)blockIdx.x * kRows + threadIdx.x / T; at < M; at += (int64_t)gridDim.x * kRows) {
+        const int64_t m = row_of<T>(at);
+        for (int j0 = 0; j0 < top_k; j0 += kSlots) {
+            const Slots s = slots_of(place, wt, m * top_k + j0, top_k - j0, rows);
+            float dot[kSlots] = {};
+            for (unsigned c = lane * 8; c < (unsigned)cols; c += T * 8) {
+                const bool whole = cols - (int)c >= 8;
+                Raw8<ZE> raw[kSlots];
+                float d[8];
+                if (dw) {
+#pragma unroll
+                    for (int j = 0; j < kSlots; ++j) {
+                        raw[j] = nothing8<ZE>();
+                        if (s.place[j] >= 0 && whole) raw[j] = raw8<ZE>(z, s.place[j] * ldz + c);
                     }
-                    if (dz) {
+                }
+                load8<OE>(dout, m * ldo, (int)c, cols, d);
+                if (dz) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (i < cols - (int)c) store_elem(dz, (int64_t)p * lddz + c + i, w * d[i], ZE);
+                    for (int j = 0; j < kSlots; ++j) {
+                        if (s.place[j] < 0) continue;
+                        float f[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) f[i] = s.w[j] * d[i];
+                        store8(dz, s.place[j] * lddz, (int)c, cols, ZE, f);
+                    }
+                }
+                if (dw) {
+#pragma unroll
+                    for (int j = 0; j < kSlots; ++j) {
+                        if (s.place[j] < 0) continue;
+                        float f[8];
+                        unpack8<ZE>(raw[j], f);
+                        end8<ZE>(z, s.place[j] * ldz, (int)c, cols, f);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) dot[j] = __builtin_fmaf(d[i], f[i], dot[j]);
                     }
                 }
             }
             if (!dw) continue;
+            const int64_t q = m * top_k + j0;
+            if constexpr (T < 64) {
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-            if (lane_id() == 0) part[threadIdx.x >> 6] = dot;
-            __syncthreads();
-            if (threadIdx.x == 0) dw[q] = part[0] + part[1] + part[2] + part[3];
-            __syncthreads();
+                for (int j = 0; j < kSlots; ++j) {
+#pragma unroll
+                    for (int o = T / 2; o > 0; o /= 2) dot[j] += __shfl_xor(dot[j], o, 64);
+                    if (lane == 0 && j < top_k - j0) dw[q + j] = dot[j];
+                }
+            } else {
+                const int l = lane_id(), j = slot_of<T>(l);
+                float sum = wave_sum8(dot);
+                if constexpr (T > 64) {
+                    if ((l & 7) == 0) part[turn][wave][j] = sum;
+                    __syncthreads();
+                    sum = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < T / 64; ++w) sum += part[turn][w][j];
+                    turn ^= 1;
+                }
+                if ((T == 64 || wave == 0) && (l & 7) == 0 && j < top_k - j0) dw[q + j] = sum;
+            }
         }
     }
 }
@@ -250,6 +401,15 @@ int launch_place(vdttfs_ctx* ctx, const PlaceArgs& a, int* hist) {
     return VDTTFS_OK;
 }
 
+bool dispatch_few_ok(int64_t pairs) { return pairs > 0 && pairs <= kFewPairs; }
+int launch_dispatch_few(vdttfs_ctx* ctx, const PlaceArgs& a, void* z, int64_t ldz, const void* x, int elem, int64_t ldx,
+                        int cols) {
+    k_dispatch_few<<<dim3((unsigned)(a.M + (a.start ? 1 : 0))), kCopy, 0, ctx->stream>>>(
+        a, z, ldz, x, ldx, cols, elem == VDTTFS_ELEM_F32 ? 4 : 2);
+    VD_HIP(hipGetLastError());
+    return VDTTFS_OK;
+}
+
 int launch_dispatch_rows(vdttfs_ctx* ctx, const PlaceArgs& a, void* z, int64_t ldz, const void* x, int elem, int64_t ldx,
                          int cols) {
     if (a.M <= 0 || cols <= 0) return VDTTFS_OK;
@@ -259,50 +419,51 @@ int launch_dispatch_rows(vdttfs_ctx* ctx, const PlaceArgs& a, void* z, int64_t l
     return VDTTFS_OK;
 }
 
+namespace {
+
+// Lanes of a row: as many as have a run of eight, up to a wave; past that the
+// workgroup.
+template <class F>
+void by_lanes(int cols, const F& f) {
+    if (cols <= 64) f(std::integral_constant<int, 8>{});
+    else if (cols <= 128) f(std::integral_constant<int, 16>{});
+    else if (cols <= 256) f(std::integral_constant<int, 32>{});
+    else if (cols <= 512) f(std::integral_constant<int, 64>{});
+    else f(std::integral_constant<int, kRow>{});
+}
+template <class F>
+void by_elem(int elem, const F& f) {
+    if (elem == VDTTFS_ELEM_F32) f(std::integral_constant<int, VDTTFS_ELEM_F32>{});
+    else if (elem == VDTTFS_ELEM_BF16) f(std::integral_constant<int, VDTTFS_ELEM_BF16>{});
+    else f(std::integral_constant<int, VDTTFS_ELEM_F16>{});
+}
+dim3 grid_rows(int64_t M, int lanes) { return dim3(grid_of((M + kRow / lanes - 1) / (kRow / lanes), 1 << 20)); }
+
+}  // namespace
+
 int launch_gather_sum(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem, int64_t ldz,
                       const int32_t* place, const float* wt, int64_t M, int top_k, int cols) {
-    int log_t = 2;
-    while (log_t < 8 && (8 << log_t) < cols) ++log_t;
-    const int64_t rows = 256 >> log_t;
-    const dim3 grid(grid_of((M + rows - 1) / rows, 1 << 20));
-    if (z_elem == VDTTFS_ELEM_F32)
-        k_gather_sum<VDTTFS_ELEM_F32><<<grid, 256, 0, ctx->stream>>>(out, out_elem, ldo, z, ldz, place, wt, M, top_k,
-                                                                     cols, log_t);
-    else if (z_elem == VDTTFS_ELEM_BF16)
-        k_gather_sum<VDTTFS_ELEM_BF16><<<grid, 256, 0, ctx->stream>>>(out, out_elem, ldo, z, ldz, place, wt, M, top_k,
-                                                                      cols, log_t);
-    else
-        k_gather_sum<VDTTFS_ELEM_F16><<<grid, 256, 0, ctx->stream>>>(out, out_elem, ldo, z, ldz, place, wt, M, top_k,
-                                                                     cols, log_t);
+    by_lanes(cols, [&](auto t) {
+        by_elem(z_elem, [&](auto ze) {
+            k_gather_sum<ze.value, t.value><<<grid_rows(M, t.value), kRow, 0, ctx->stream>>>(out, out_elem, ldo, z, ldz,
+                                                                                             place, wt, M, top_k, cols);
+        });
+    });
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
-}
-
-template <int ZE>
-static void combine_grad_z(vdttfs_ctx* ctx, void* dz, int64_t lddz, float* dw, const void* z, int64_t ldz,
-                           const void* dout, int out_elem, int64_t ldo, const int32_t* place, const float* wt, int64_t M,
-                           int top_k, int cols) {
-    const dim3 grid(grid_of(M, 1 << 20));
-    if (out_elem == VDTTFS_ELEM_F32)
-        k_combine_grad<ZE, VDTTFS_ELEM_F32><<<grid, 256, 0, ctx->stream>>>(dz, lddz, dw, z, ldz, dout, ldo, place, wt,
-                                                                           M, top_k, cols);
-    else if (out_elem == VDTTFS_ELEM_BF16)
-        k_combine_grad<ZE, VDTTFS_ELEM_BF16><<<grid, 256, 0, ctx->stream>>>(dz, lddz, dw, z, ldz, dout, ldo, place, wt,
-                                                                            M, top_k, cols);
-    else
-        k_combine_grad<ZE, VDTTFS_ELEM_F16><<<grid, 256, 0, ctx->stream>>>(dz, lddz, dw, z, ldz, dout, ldo, place, wt,
-                                                                           M, top_k, cols);
 }
 
 int launch_combine_grad(vdttfs_ctx* ctx, void* dz, int64_t lddz, float* dw, const void* z, int z_elem, int64_t ldz,
                         const void* dout, int out_elem, int64_t ldo, const int32_t* place, const float* wt, int64_t M,
                         int top_k, int cols) {
-    if (z_elem == VDTTFS_ELEM_F32)
-        combine_grad_z<VDTTFS_ELEM_F32>(ctx, dz, lddz, dw, z, ldz, dout, out_elem, ldo, place, wt, M, top_k, cols);
-    else if (z_elem == VDTTFS_ELEM_BF16)
-        combine_grad_z<VDTTFS_ELEM_BF16>(ctx, dz, lddz, dw, z, ldz, dout, out_elem, ldo, place, wt, M, top_k, cols);
-    else
-        combine_grad_z<VDTTFS_ELEM_F16>(ctx, dz, lddz, dw, z, ldz, dout, out_elem, ldo, place, wt, M, top_k, cols);
+    by_lanes(cols, [&](auto t) {
+        by_elem(z_elem, [&](auto ze) {
+            by_elem(out_elem, [&](auto oe) {
+                k_combine_grad<ze.value, oe.value, t.value><<<grid_rows(M, t.value), kRow, 0, ctx->stream>>>(
+                    dz, lddz, dw, z, ldz, dout, ldo, place, wt, M, top_k, cols);
+            });
+        });
+    });
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }

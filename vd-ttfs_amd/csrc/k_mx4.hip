@@ -23,6 +23,12 @@ namespace vdttfs {
 namespace {
 
 // ---- quantisation -----------------------------------------------------------------
+// The value of a spike time: its linear encoding's pixel.
+__device__ __forceinline__ float time_value(float t, float tfs, int T) {
+    const int b = arrival_bin(t, tfs, T);
+    return b < 0 ? 0.0f : (float)(T - b) / (float)T;
+}
+
 // Eight values a thread, four neighbouring threads a block of 32.
 template <int ELEM>
 __global__ __launch_bounds__(256) void k_mx4_quant(const void* __restrict__ x, int64_t ldx, int64_t rows, int cols,
@@ -36,10 +42,7 @@ __global__ __launch_bounds__(256) void k_mx4_quant(const void* __restrict__ x, i
         load8<ELEM>(x, m * ldx, c, cols, f);
         if constexpr (ELEM == VDTTFS_ELEM_TIMES) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int b = arrival_bin(f[i], tfs, T);
-                f[i] = b < 0 ? 0.0f : (float)(T - b) / (float)T;
-            }
+            for (int i = 0; i < 8; ++i) f[i] = time_value(f[i], tfs, T);
         }
         uint32_t most = 0;
 #pragma unroll
@@ -573,6 +576,112 @@ __global__ __launch_bounds__(WM* WN * 64, WM* WN == 4 && BM == 256 ? 1 : 2) void
     epilogue<FM, FN>(p, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(s0) + wave * (Stage<FM, FN>::kBytes / 4));
 }
 
+// ---- few rows -------------------------------------------------------------------------
+// A workgroup has 16 channels, its eight waves share K in spans of 512 elements, and
+// the sums meet in LDS: bound by the weights, which are read once, straight to
+// registers.  Of a span a lane takes 64 neighbouring bytes of a channel (blocks 4 g ..
+// 4 g + 3, g = lane / 16) and their four scales.  Activations: up to 16 rows of codes
+// in memory (ELEM kElemCodes), read alike (of 17 rows the smallest tiles take as long,
+// of 64 x 8192 x 8192 16 us for 28); or of floats or spike times, quantised by every
+// workgroup into LDS while its weights are on their way, where that is no more than
+// eight runs of eight a thread (4 x 4096 x 4096 from BF16 5.5 us, 8.0 with a launch of
+// its own for that; 8 x 4096 x 4096 7.4 and 7.9).
+constexpr int kSpanBlocks = 16, kSmallWaves = 8, kSmallRows = 16, kSmallRuns = 8;
+struct Span {
+    v4i c[4];
+    int s;
+};
+__device__ __forceinline__ Span load_span(const uint8_t* codes, const uint8_t* scales, int span, int g, int K) {
+    Span r;
+    const int b = span * kSpanBlocks + g * 4;
+    if (K - span * 512 >= 512) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.c[i] = reinterpret_cast<const Bytes16*>(codes + (b + i) * 16)->v;
+        r.s = (int)reinterpret_cast<const AnyUint*>(scales + b)->v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.c[i] = codes16(codes, (b + i) * 16, K);
+        r.s = (int)scales4(scales, b, K / kMxBlock + (K % kMxBlock != 0));
+    }
+    return r;
+}
+template <int ELEM>
+__global__ __launch_bounds__(kSmallWaves * 64) void k_mx4_small(Mx4Args p, const void* __restrict__ x, int64_t ldx,
+                                                                float tfs, int T) {
+    constexpr bool kCodesIn = ELEM == kElemCodes;
+    constexpr int kQuant = kCodesIn ? 16 : kSmallRuns * kSmallWaves * 64 * 4;  // bytes of codes
+    __shared__ float part[kSmallWaves][kSmallRows][16 + 1];
+    __shared__ __align__(16) uint8_t q[kQuant];
+    __shared__ __align__(4) uint8_t qs[kCodesIn ? 16 : kQuant / 16];
+    const int lane = lane_id(), wave = uniform(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16, n = n0 + r16 < p.N ? n0 + r16 : p.N - 1;
+    const uint8_t *wc = p.B + (int64_t)n * p.ldb, *ws = p.sb + (int64_t)n * p.ldsb;
+    const int spans = p.K / 512 + (p.K % 512 != 0), M = (int)p.M;
+    Span w{};
+    if (wave < spans) w = load_span(wc, ws, wave, g, p.K);
+    if constexpr (!kCodesIn) {
+        // runs of eight to codes; blocks past the row's end to codes of 0
+        const int per = spans * kSpanBlocks * 4;
+        for (int at = threadIdx.x; at < M * per; at += kSmallWaves * 64) {
+            const int m = at / per, c = (at - m * per) * 8, b = c / kMxBlock;
+            float f[8];
+            load8<ELEM>(x, m * ldx, c, p.K, f);
+            if constexpr (ELEM == VDTTFS_ELEM_TIMES) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = time_value(f[i], tfs, T);
+            }
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = max(most, magnitude(f[i]));
+            const int scale = mx4_scale(quad_max(most));
+            // a span's 16 chunks at 16 places by the row, for the fragments' reads
+            const int to = m * spans * kSpanBlocks + (b ^ m);
+            *reinterpret_cast<uint32_t*>(q + to * 16 + c % kMxBlock / 2) = mx4_codes8(f, scale);
+            if (c % kMxBlock == 0) qs[m * spans * kSpanBlocks + b] = (uint8_t)scale;
+        }
+        __syncthreads();
+    }
+    v4f acc = {0, 0, 0, 0};
+    const int row = r16 < M ? r16 : M - 1;
+    for (int span = wave; span < spans; span += kSmallWaves) {
+        Span a;
+        if constexpr (kCodesIn) {
+            a = load_span(p.A + row * p.lda, p.sa + row * p.ldsa, span, g, p.K);
+        } else {
+            const int b = row * spans * kSpanBlocks;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                a.c[i] = *reinterpret_cast<const v4i*>(q + (b + ((span * kSpanBlocks + g * 4 + i) ^ row)) * 16);
+            a.s = *reinterpret_cast<const int*>(qs + b + span * kSpanBlocks + g * 4);
+        }
+        Span next{};
+        if (span + kSmallWaves < spans) next = load_span(wc, ws, span + kSmallWaves, g, p.K);
+        acc = mfma4<0>(w.c[0], a.c[0], acc, w.s, a.s);
+        acc = mfma4<1>(w.c[1], a.c[1], acc, w.s, a.s);
+        acc = mfma4<2>(w.c[2], a.c[2], acc, w.s, a.s);
+        acc = mfma4<3>(w.c[3], a.c[3], acc, w.s, a.s);
+        w = next;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[wave][r16][g * 4 + e] = acc[e];
+    __syncthreads();
+    const int m = threadIdx.x / 16, c = threadIdx.x % 16;
+    if (m >= M || n0 + c >= p.N) return;
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSmallWaves; ++i) v += part[i][m][c];
+    if (p.bias) v += p.bias[n0 + c];
+    store_elem(p.out, (int64_t)m * p.ldo + n0 + c, apply_act(v, p.act), p.out_elem);
+}
+
+template <int ELEM>
+int run_small(vdttfs_ctx* ctx, const Mx4Args& a, const void* x, int64_t ldx) {
+    k_mx4_small<ELEM><<<dim3((unsigned)((a.N + 15) / 16)), kSmallWaves * 64, 0, ctx->stream>>>(a, x, ldx, ctx->c.tfs,
+                                                                                               ctx->c.T);
+    VD_HIP(hipGetLastError());
+    return VDTTFS_OK;
+}
+
 template <int BM, int BN>
 int run_tile(vdttfs_ctx* ctx, const Mx4Args& a) {
     const int64_t tn = (a.N + BN - 1) / BN, blocks = (a.M + BM - 1) / BM * tn;
@@ -614,8 +723,21 @@ static Mx4Tile tile_for(int64_t M, int N, int K, bool is_aligned) {
 #ifndef MX4_BIG
 #define MX4_BIG 2, 4
 #endif
+// Whether rows of floats or spike times are quantised by their product.
+bool mx4_small_linear_ok(int64_t M, int K) {
+    const int64_t per = ((int64_t)K + 511) / 512 * 64;  // runs of eight of a row, whole spans
+    return M <= kSmallRows && K > 0 && M * per <= kSmallRuns * kSmallWaves * 64;
+}
+int launch_mx4_small_linear(vdttfs_ctx* ctx, const Mx4Args& a, const void* x, int elem, int64_t ldx) {
+    if (elem == VDTTFS_ELEM_F32) return run_small<VDTTFS_ELEM_F32>(ctx, a, x, ldx);
+    if (elem == VDTTFS_ELEM_BF16) return run_small<VDTTFS_ELEM_BF16>(ctx, a, x, ldx);
+    if (elem == VDTTFS_ELEM_F16) return run_small<VDTTFS_ELEM_F16>(ctx, a, x, ldx);
+    return run_small<VDTTFS_ELEM_TIMES>(ctx, a, x, ldx);
+}
+
 int launch_mx4(vdttfs_ctx* ctx, const Mx4Args& a) {
     if (a.M <= 0 || a.N <= 0) return VDTTFS_OK;
+    if (a.M <= kSmallRows) return run_small<kElemCodes>(ctx, a, nullptr, 0);
     const bool fast = aligned(a);
     const Mx4Tile t = tile_for(a.M, a.N, a.K, fast);
     const int64_t rows = max_blocks(512) / ((a.N + t.bn - 1) / t.bn) * t.bm;  // as many a launch as its tiles allow
