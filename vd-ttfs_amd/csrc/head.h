@@ -139,7 +139,18 @@ struct Mx4Args {
     int N, K;
     int act, out_elem;
 };
-int launch_mx4(vdttfs_ctx* ctx, const Mx4Args& a);
+// The kernels of a product: fragments of 16 x 16 whose waves share K, tiles through
+// registers, tiles loaded to LDS; and which operands (codes, scales) are copied first to
+// rows on 16 bytes with zeros behind them.
+enum Mx4Path { kMx4Few, kMx4Tile32, kMx4Tile64, kMx4Lds32, kMx4Lds64, kMx4Lds128, kMx4Lds256 };
+struct Mx4Plan {
+    Mx4Path path;
+    bool a, sa, b, sb;
+};
+Mx4Plan mx4_plan(const Mx4Args& a);
+int launch_mx4_realign(vdttfs_ctx* ctx, const uint8_t* q, int64_t ldq, const uint8_t* s, int64_t lds, int64_t rows,
+                       int K, uint8_t* to_q, int64_t ldq_to, uint8_t* to_s, int64_t lds_to);
+int launch_mx4(vdttfs_ctx* ctx, const Mx4Args& a, Mx4Path path);
 // The product of few rows, quantised in the kernel (a.A and a.sa unused).
 bool mx4_small_linear_ok(int64_t M, int K);
 int launch_mx4_small_linear(vdttfs_ctx* ctx, const Mx4Args& a, const void* x, int elem, int64_t ldx);

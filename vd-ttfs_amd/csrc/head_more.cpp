@@ -29,6 +29,39 @@ int check_mx4_product(const char* what, const void* w, int64_t ldw, const void* 
     return VDTTFS_OK;
 }
 
+// Rows of copies and of scratch: whole cache lines of codes.
+int64_t mx4_ld(int K) { return (mx4_bytes(K) + 127) / 128 * 128; }
+int64_t mx4_lds(int K) { return (mx4_ld(K) / 16 + 15) / 16 * 16; }
+
+size_t mx4_copy_bytes(const Mx4Args& a, const Mx4Plan& p) {
+    Layout l;
+    if (p.a) l.take((size_t)a.M * mx4_ld(a.K));
+    if (p.sa) l.take((size_t)a.M * mx4_lds(a.K));
+    if (p.b) l.take((size_t)a.N * mx4_ld(a.K));
+    if (p.sb) l.take((size_t)a.N * mx4_lds(a.K));
+    return l.bytes;
+}
+
+// The product, its operands copied first where the plan says so.
+int mx4_product(vdttfs_ctx* ctx, Mx4Args a, const Mx4Plan& p, unsigned char* buf) {
+    const int64_t ld = mx4_ld(a.K), lds = mx4_lds(a.K);
+    auto copy = [&](bool codes, bool scales, const uint8_t*& q, int64_t& ldq, const uint8_t*& s, int64_t& ls,
+                    int64_t rows) -> int {
+        if (!codes && !scales) return VDTTFS_OK;
+        uint8_t* to_q = codes ? buf : nullptr;
+        if (codes) buf += ((size_t)rows * ld + 255) & ~size_t(255);
+        uint8_t* to_s = scales ? buf : nullptr;
+        if (scales) buf += ((size_t)rows * lds + 255) & ~size_t(255);
+        VD_TRY(launch_mx4_realign(ctx, q, ldq, s, ls, rows, a.K, to_q, ld, to_s, lds));
+        if (codes) q = to_q, ldq = ld;
+        if (scales) s = to_s, ls = lds;
+        return VDTTFS_OK;
+    };
+    VD_TRY(copy(p.a, p.sa, a.A, a.lda, a.sa, a.ldsa, a.M));
+    VD_TRY(copy(p.b, p.sb, a.B, a.ldb, a.sb, a.ldsb, a.N));
+    return launch_mx4(ctx, a, p.path);
+}
+
 int check_elem(const char* what, int elem) {
     return elem < VDTTFS_ELEM_F32 || elem > VDTTFS_ELEM_F16 ? bad(what, "unknown element type") : VDTTFS_OK;
 }
@@ -115,7 +148,12 @@ int vdttfs_mx4_matmul(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, c
     VD_TRY(check_out("mx4_matmul", d_out, out_elem, ldo, N));
     VD_TRY(check_mx4("mx4_matmul", d_q, ldq, d_s, lds, K));
     VD_TRY(check_mx4_product("mx4_matmul", d_w, ldw, d_ws, ldws, d_bias, act, K));
-    return launch_mx4(ctx, Mx4Args{d_q, ldq, d_s, lds, d_w, ldw, d_ws, ldws, d_bias, d_out, ldo, M, N, K, act, out_elem});
+    const Mx4Args a{d_q, ldq, d_s, lds, d_w, ldw, d_ws, ldws, d_bias, d_out, ldo, M, N, K, act, out_elem};
+    const Mx4Plan p = mx4_plan(a);
+    unsigned char* buf = nullptr;
+    const size_t bytes = mx4_copy_bytes(a, p);
+    if (bytes) VD_TRY(head_scratch(ctx, bytes, &buf));
+    return mx4_product(ctx, a, p, buf);
 }
 
 int vdttfs_mx4_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, const void* d_x, int x_elem,
@@ -129,18 +167,20 @@ int vdttfs_mx4_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, c
     VD_TRY(check_mx4_product("mx4_linear", d_w, ldw, d_ws, ldws, d_bias, act, K));
     Mx4Args a{nullptr, 0, nullptr, 0, d_w, ldw, d_ws, ldws, d_bias, d_out, ldo, M, N, K, act, out_elem};
     if (mx4_small_linear_ok(M, K)) return launch_mx4_small_linear(ctx, a, d_x, x_elem, ldx);
-    const int64_t ldq = (mx4_bytes(K) + 127) / 128 * 128, lds = ldq / 16;
+    a.lda = mx4_ld(K);
+    a.ldsa = mx4_lds(K);
+    const Mx4Plan p = mx4_plan(a);  // of the strides: the rows in scratch are aligned
     Layout l;
-    const size_t at_q = l.take((size_t)M * ldq), at_s = l.take((size_t)M * lds);
+    const size_t at_q = l.take((size_t)M * a.lda), at_s = l.take((size_t)M * a.ldsa);
+    const size_t own = l.bytes;
+    l.take(mx4_copy_bytes(a, p));
     unsigned char* buf;
     VD_TRY(head_scratch(ctx, l.bytes, &buf));
     uint8_t *q = buf + at_q, *s = buf + at_s;
-    VD_TRY(launch_mx4_quant_rows(ctx, d_x, x_elem, ldx, M, K, q, ldq, s, lds, K));
+    VD_TRY(launch_mx4_quant_rows(ctx, d_x, x_elem, ldx, M, K, q, a.lda, s, a.ldsa, K));
     a.A = q;
-    a.lda = ldq;
     a.sa = s;
-    a.ldsa = lds;
-    return launch_mx4(ctx, a);
+    return mx4_product(ctx, a, p, buf + own);
 }
 
 int vdttfs_norm_rows(vdttfs_ctx* ctx, void* d_y, int y_elem, int64_t ldy, const void* d_x, int x_elem, int64_t ldx,

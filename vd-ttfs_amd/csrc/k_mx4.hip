@@ -15,10 +15,6 @@
 #include "tiles.h"
 #include "wave.h"
 
-#ifndef MX4_EARLY
-#define MX4_EARLY 0
-#define MX4_PER 2
-#endif
 namespace vdttfs {
 namespace {
 
@@ -104,6 +100,15 @@ __device__ __forceinline__ uint32_t scales4(const uint8_t* row, int b, int block
     return v;
 }
 
+// The scales of blocks b and b + 1.
+struct __attribute__((packed, aligned(1))) AnyShort {
+    uint16_t v;
+};
+__device__ __forceinline__ int scales2(const uint8_t* row, int b, int blocks) {
+    if (blocks - b >= 2) return reinterpret_cast<const AnyShort*>(row + b)->v;
+    return b < blocks ? row[b] | kOne << 8 : kOne * 0x101;
+}
+
 // 16 codes' bytes from byte k of a row of K elements, those past its end 0, also
 // the upper half of a last byte.
 __device__ __forceinline__ v4i codes16(const uint8_t* row, int k, int K) {
@@ -128,112 +133,6 @@ constexpr int kBlocks = kBK / 16;
 // different banks (with r & 7 in their place every other one collided: 26 M cycles
 // of conflicts in 8192 x 8192 x 8192, and 300 us).
 __device__ __forceinline__ int swizzle(int r) { return (r >> 1 & 1) | (r & 4); }
-
-// A workgroup of WM x WN waves computes BM rows x BN channels.  Operands at any
-// alignment pass through registers to LDS.
-template <int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM* WN * 64) void k_mx4_tile(Mx4Args p, int tiles_n) {
-    constexpr int kT = WM * WN * 64;
-    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-    constexpr int R = BM + BN, N16 = R * 8 / kT, NS = (R * 2 + kT - 1) / kT;
-    static_assert(N16 * kT == R * 8, "chunks divide");
-    __shared__ __align__(16) uint8_t lds[R * kBK];
-    __shared__ __align__(16) uint8_t scales[R * kBlocks];
-    const int tile_m = blockIdx.x / tiles_n, tile_n = blockIdx.x % tiles_n;
-    const int64_t m0 = (int64_t)tile_m * BM;
-    const int n0 = tile_n * BN;
-    const int tid = threadIdx.x, lane = lane_id(), wave = uniform(tid >> 6);
-    const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
-    const int blocks = p.K / kMxBlock + (p.K % kMxBlock != 0);
-    const int bytes = p.K / 2 + (p.K & 1);
-    // row r of the tile: an activation row, or a channel
-    auto codes_of = [&](int r) -> const uint8_t* {
-        if (r < BM) {
-            const int64_t m = m0 + r < p.M ? m0 + r : p.M - 1;
-            return p.A + m * p.lda;
-        }
-        const int n = n0 + r - BM < p.N ? n0 + r - BM : p.N - 1;
-        return p.B + n * p.ldb;
-    };
-    auto scales_of = [&](int r) -> const uint8_t* {
-        if (r < BM) {
-            const int64_t m = m0 + r < p.M ? m0 + r : p.M - 1;
-            return p.sa + m * p.ldsa;
-        }
-        const int n = n0 + r - BM < p.N ? n0 + r - BM : p.N - 1;
-        return p.sb + n * p.ldsb;
-    };
-    v4f acc[FM][FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
-    for (int k0 = 0; k0 < bytes; k0 += kBK) {
-        v4i raw[N16];
-        uint32_t sc[NS];
-#pragma unroll
-        for (int i = 0; i < N16; ++i) {
-            const int at = tid + i * kT;
-            raw[i] = codes16(codes_of(at / 8), k0 + at % 8 * 16, p.K);
-        }
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const int at = tid + i * kT;
-            sc[i] = at < R * 2 ? scales4(scales_of(at / 2), k0 / 16 + at % 2 * 4, blocks) : 0;
-        }
-        __syncthreads();  // the previous tile is read
-#pragma unroll
-        for (int i = 0; i < N16; ++i) {
-            const int at = tid + i * kT, r = at / 8;
-            *reinterpret_cast<v4i*>(lds + r * kBK + (at % 8 ^ swizzle(r)) * 16) = raw[i];
-        }
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const int at = tid + i * kT;
-            if (at < R * 2) *reinterpret_cast<uint32_t*>(scales + at * 4) = sc[i];
-        }
-        __syncthreads();
-        const int r16 = lane & 15, g = lane >> 4;
-        int sa[FM], sb[FN];
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-            sa[i] = *reinterpret_cast<const uint16_t*>(scales + (wm + i * 16 + r16) * kBlocks + g * 2);
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-            sb[j] = *reinterpret_cast<const uint16_t*>(scales + (BM + wn + j * 16 + r16) * kBlocks + g * 2);
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const int c = ((g * 2 + kk) ^ swizzle(r16)) * 16;
-            v4i fa[FM], fb[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const v4i*>(lds + (wm + i * 16 + r16) * kBK + c);
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-                fb[j] = *reinterpret_cast<const v4i*>(lds + (BM + wn + j * 16 + r16) * kBK + c);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    acc[i][j] = kk == 0 ? mfma4<0>(fb[j], fa[i], acc[i][j], sb[j], sa[i])
-                                        : mfma4<1>(fb[j], fa[i], acc[i][j], sb[j], sa[i]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int64_t m = m0 + wm + i * 16 + (lane & 15);
-        if (m >= p.M) continue;
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int n = n0 + wn + j * 16 + (lane >> 4) * 4 + e;
-                if (n >= p.N) continue;
-                float v = acc[i][j][e];
-                if (p.bias) v += p.bias[n];
-                store_elem(p.out, m * p.ldo + n, apply_act(v, p.act), p.out_elem);
-            }
-    }
-}
 
 // A wave's sums to its outputs.  A lane has four neighbouring channels of a row;
 // stored from there, a wave would write 32 bytes of each of 16 rows at a time.  So
@@ -296,21 +195,107 @@ __device__ __forceinline__ void epilogue(const Mx4Args& p, const v4f (&acc)[FM][
     }
 }
 
-// The large product: tiles of 128 bytes a row and the 8 scales of their blocks go
-// from memory to LDS directly (16 and 4 bytes a lane, no registers between).  Rows
-// of codes on 16 bytes, of scales on 4.  The last K % 256 elements come through
-// registers with zeros behind them.
+// A workgroup of WM x WN waves computes BM rows x BN channels, operands at any
+// alignment: codes pass through registers to LDS, the next tile's on their way while
+// one is multiplied; a lane loads its fragments' scales itself.
+template <int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM* WN * 64) void k_mx4_tile(Mx4Args p, int tiles_n) {
+    constexpr int kT = WM * WN * 64;
+    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+    constexpr int R = BM + BN, NL = R * 8 / kT;
+    static_assert(NL * kT == R * 8, "chunks divide");
+    constexpr int kStage = WM * WN * Stage<FM, FN>::kBytes;
+    __shared__ __align__(16) uint8_t lds[R * kBK > kStage ? R * kBK : kStage];
+    const int tile_m = blockIdx.x / tiles_n, tile_n = blockIdx.x % tiles_n;
+    const int64_t m0 = (int64_t)tile_m * BM;
+    const int n0 = tile_n * BN;
+    const int tid = threadIdx.x, lane = lane_id(), wave = uniform(tid >> 6), r16 = lane & 15, g = lane >> 4;
+    const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+    const int blocks = p.K / kMxBlock + (p.K % kMxBlock != 0);
+    const int bytes = p.K / 2 + (p.K & 1);
+    auto a_row = [&](int r) { return m0 + r < p.M ? m0 + r : p.M - 1; };
+    auto b_row = [&](int r) { return (int64_t)(n0 + r < p.N ? n0 + r : p.N - 1); };
+    const uint8_t* from[NL];  // row r of the tile: an activation row, or a channel
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+        const int r = (tid + i * kT) / 8;
+        from[i] = r < BM ? p.A + a_row(r) * p.lda : p.B + b_row(r - BM) * p.ldb;
+    }
+    const uint8_t *sfa[FM], *sfb[FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sfa[i] = p.sa + a_row(wm + i * 16 + r16) * p.ldsa;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) sfb[j] = p.sb + b_row(wn + j * 16 + r16) * p.ldsb;
+    v4f acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+    v4i raw[NL];
+    int na[FM], nb[FN];
+    auto fetch = [&](int k0) {
+        if (p.K - k0 * 2 >= 2 * kBK) {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) raw[i] = reinterpret_cast<const Bytes16*>(from[i] + k0 + (tid & 7) * 16)->v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) raw[i] = codes16(from[i], k0 + (tid & 7) * 16, p.K);
+        }
+#pragma unroll
+        for (int i = 0; i < FM; ++i) na[i] = scales2(sfa[i], k0 / 16 + g * 2, blocks);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) nb[j] = scales2(sfb[j], k0 / 16 + g * 2, blocks);
+    };
+    if (bytes > 0) fetch(0);
+    for (int k0 = 0; k0 < bytes; k0 += kBK) {
+        __syncthreads();  // the previous tile is read
+        int sa[FM], sb[FN];
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int r = (tid + i * kT) / 8;
+            *reinterpret_cast<v4i*>(lds + r * kBK + ((tid & 7) ^ swizzle(r)) * 16) = raw[i];
+        }
+#pragma unroll
+        for (int i = 0; i < FM; ++i) sa[i] = na[i];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) sb[j] = nb[j];
+        __syncthreads();
+        if (k0 + kBK < bytes) fetch(k0 + kBK);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const int c = ((g * 2 + kk) ^ swizzle(r16)) * 16;
+            v4i fa[FM], fb[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const v4i*>(lds + (wm + i * 16 + r16) * kBK + c);
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                fb[j] = *reinterpret_cast<const v4i*>(lds + (BM + wn + j * 16 + r16) * kBK + c);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    acc[i][j] = kk == 0 ? mfma4<0>(fb[j], fa[i], acc[i][j], sb[j], sa[i])
+                                        : mfma4<1>(fb[j], fa[i], acc[i][j], sb[j], sa[i]);
+        }
+    }
+    __syncthreads();
+    epilogue<FM, FN>(p, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(lds) + wave * (Stage<FM, FN>::kBytes / 4));
+}
+
+// The large product: tiles of 128 bytes a row go from memory to LDS directly (16
+// bytes a lane, no registers between), S deep.  Rows of codes on 16 bytes.  Of two
+// stages the scales go to LDS too, those of four tiles at a time, of rows on 4 bytes;
+// of more a lane loads those of its fragments, of any alignment, and holds them until
+// their tile.  The last K % 256 elements come through registers with zeros behind them.
 template <int BM, int BN, int WM, int WN, int S>
-__global__ __launch_bounds__(WM* WN * 64, WM* WN == 4 && BM == 256 ? 1 : 2) void k_mx4_big(Mx4Args p, int tiles_m,
-                                                                                          int tiles_n) {
+__global__ __launch_bounds__(WM* WN * 64, 2) void k_mx4_big(Mx4Args p, int tiles_m, int tiles_n) {
     constexpr int kW = WM * WN;
     constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
     constexpr int NA = BM / 8 / kW, NB = BN / 8 / kW;  // loads of codes of a wave and tile, 8 rows each
     constexpr int kScaleLoads = (BM + BN) / 32, NS = (kScaleLoads + kW - 1) / kW;
-    constexpr int NL = NA + NB + (S > 2 ? NS : 0);
-    constexpr int kCodes = (BM + BN) * kBK, kTile = kCodes + (S > 2 ? (BM + BN) * kBlocks : 0);
-    // two stages: the scales of four tiles at a time, 32 bytes a row, two deep
-    constexpr int kSpan = 4, kRowScales = S > 2 ? kBlocks : kSpan * kBlocks, kScales = (BM + BN) * kRowScales;
+    constexpr int NL = NA + NB + (S > 2 ? FM + FN : 0);  // loads of a wave and tile
+    constexpr int kCodes = (BM + BN) * kBK, kTile = kCodes;
+    constexpr int kSpan = 4, kRowScales = kSpan * kBlocks, kScales = (BM + BN) * kRowScales;
     static_assert(NA * kW * 8 == BM && NB * kW * 8 == BN && BM % 32 == 0 && BN % 32 == 0, "loads divide");
     static_assert(S >= 2 && S <= 4 && (S - 2) * NL < 64, "stages");
     constexpr int kStage = kW * Stage<FM, FN>::kBytes;
@@ -333,20 +318,11 @@ __global__ __launch_bounds__(WM* WN * 64, WM* WN == 4 && BM == 256 ? 1 : 2) void
     const uint8_t *A = p.A + m0 * p.lda, *B = p.B + n0 * p.ldb, *SA = p.sa + m0 * p.ldsa, *SB = p.sb + n0 * p.ldsb;
     const unsigned lda = (unsigned)p.lda, ldb = (unsigned)p.ldb;
     const int last_a = p.M - m0 < BM ? (int)(p.M - m0) - 1 : BM - 1, last_b = p.N - n0 < BN ? p.N - n0 - 1 : BN - 1;
-    unsigned from[NA + NB], sfrom[NS];  // of codes, of scales (two lanes a row)
+    unsigned from[NA + NB];
 #pragma unroll
     for (int i = 0; i < NA; ++i) from[i] = min((wave * NA + i) * 8 + lrow, last_a) * lda + chunk;
 #pragma unroll
     for (int i = 0; i < NB; ++i) from[NA + i] = min((wave * NB + i) * 8 + lrow, last_b) * ldb + chunk;
-    // a wave's load of scales is of A's rows or of B's; past the last: again the
-    // first ones, the same bytes
-    auto s_load = [&](int i) __attribute__((always_inline)) { return (wave * NS + i) % kScaleLoads; };
-    auto of_a = [&](int i) __attribute__((always_inline)) { return s_load(i) * 32 < BM; };
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        const int r = s_load(i) * 32 + lane / 2;
-        sfrom[i] = of_a(i) ? min(r, last_a) * (unsigned)p.ldsa : min(r - BM, last_b) * (unsigned)p.ldsb;
-    }
     const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
     const int r16 = lane & 15, g4 = lane >> 4;
     v4f acc[FM][FN];
@@ -356,40 +332,31 @@ __global__ __launch_bounds__(WM* WN * 64, WM* WN == 4 && BM == 256 ? 1 : 2) void
         for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
 
     const int tiles = p.K / 256;
-    // one of a wave's NL loads of tile t; past the end the last tile's, not used
-    auto fetch_one = [&](uint8_t* s, int t, int l) __attribute__((always_inline)) {
+    // The scales of a lane's fragments: two bytes of each row and channel.
+    struct Scales {
+        int a[FM], b[FN];
+    };
+    unsigned sfa[FM], sfb[FN];  // where they start
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sfa[i] = min(wm + i * 16 + r16, last_a) * (unsigned)p.ldsa + g4 * 2;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) sfb[j] = min(wn + j * 16 + r16, last_b) * (unsigned)p.ldsb + g4 * 2;
+    // one of a wave's NL loads of tile t, of scales to sc; past the end the last
+    // tile's, not used
+    auto fetch_one = [&](uint8_t* s, Scales& sc, int t, int l) __attribute__((always_inline)) {
         t = t < tiles ? t : tiles - 1;
         if (l < NA + NB) {
             const int at = l < NA ? wave * NA + l : BM / 8 + wave * NB + l - NA;
             to_lds16(l < NA ? A : B, from[l < NA + NB ? l : 0], t * kBK, s + at * 1024);
         } else {
             const int i = l < NA + NB ? 0 : l - NA - NB;
-            to_lds4(of_a(i) ? SA : SB, sfrom[i] + (lane & 1) * 4, t * kBlocks, s + kCodes + s_load(i) * 256);
+            if (i < FM) sc.a[i < FM ? i : 0] = reinterpret_cast<const AnyShort*>(SA + t * kBlocks + sfa[i < FM ? i : 0])->v;
+            else sc.b[i < FM ? 0 : i - FM] = reinterpret_cast<const AnyShort*>(SB + t * kBlocks + sfb[i < FM ? 0 : i - FM])->v;
         }
     };
-    auto fetch = [&](uint8_t* s, int t) __attribute__((always_inline)) {
+    auto fetch = [&](uint8_t* s, Scales& sc, int t) __attribute__((always_inline)) {
 #pragma unroll
-        for (int l = 0; l < NL; ++l) fetch_one(s, t, l);
-    };
-    // The scales of tiles 4 n .. 4 n + 3: 16 bytes a lane; where there are fewer
-    // tiles, 4 bytes a lane, those past them the row's first again, not used.  (Of 8
-    // bytes of a row in every tile, a wave's load touched 32 lines for 256 bytes:
-    // 8192 x 8192 x 8192 took 276 us.)
-    auto fetch_span = [&](int n) __attribute__((always_inline)) {
-        uint8_t* to = spans + (n & 1) * kScales;
-        if ((n + 1) * kSpan <= tiles) {
-#pragma unroll
-            for (int i = 0; i < NS; ++i)
-                to_lds16(of_a(i) ? SA : SB, sfrom[i] + (lane & 1) * 16, n * kSpan * kBlocks, to + s_load(i) * 1024);
-        } else {
-            const int there = (tiles - n * kSpan) * 2, d = lane % 8 < there ? lane % 8 : 0;
-            for (int i = wave; i < (BM + BN) / 8; i += kW) {
-                const int r = i * 8 + lane / 8;
-                const bool a = i * 8 < BM;
-                to_lds4(a ? SA : SB, (a ? min(r, last_a) * (unsigned)p.ldsa : min(r - BM, last_b) * (unsigned)p.ldsb) + d * 4,
-                        n * kSpan * kBlocks, to + i * 256);
-            }
-        }
+        for (int l = 0; l < NL; ++l) fetch_one(s, sc, t, l);
     };
     // Each group is one row fragment against all channel fragments; fragments are
     // read two groups (channels: one k step) ahead.
@@ -400,40 +367,27 @@ __global__ __launch_bounds__(WM* WN * 64, WM* WN == 4 && BM == 256 ? 1 : 2) void
     auto place = [&](int kk) __attribute__((always_inline)) { return ((g4 * 2 + kk) ^ swizzle(r16)) * 16; };
     int oa[2] = {(wm + r16) * kBK + place(0), (wm + r16) * kBK + place(1)};
     int ob[2] = {(BM + wn + r16) * kBK + place(0), (BM + wn + r16) * kBK + place(1)};
-    int osa = (wm + r16) * kRowScales + g4 * 2, osb = (BM + wn + r16) * kRowScales + g4 * 2;
-    asm volatile("" : "+v"(oa[0]), "+v"(oa[1]), "+v"(ob[0]), "+v"(ob[1]), "+v"(osa), "+v"(osb));
+    asm volatile("" : "+v"(oa[0]), "+v"(oa[1]), "+v"(ob[0]), "+v"(ob[1]));
     auto code_a = [&](const uint8_t* s, int g) __attribute__((always_inline)) {
         return *reinterpret_cast<const v4i*>(s + oa[g / FM] + g % FM * 16 * kBK);
     };
     auto code_b = [&](const uint8_t* s, int kk, int j) __attribute__((always_inline)) {
         return *reinterpret_cast<const v4i*>(s + ob[kk] + j * 16 * kBK);
     };
-    auto scale_a = [&](const uint8_t* s, int i) __attribute__((always_inline)) {
-        return (int)*reinterpret_cast<const uint16_t*>(s + osa + i * 16 * kRowScales);
-    };
-    auto scale_b = [&](const uint8_t* s, int j) __attribute__((always_inline)) {
-        return (int)*reinterpret_cast<const uint16_t*>(s + osb + j * 16 * kRowScales);
-    };
     // One tile multiplied, with the loads of tile t (to `next`) spread between: a
     // wave that issues its loads in one go waits for the address unit, and its
     // matrix instructions with it.
-    auto multiply = [&](auto with_loads, const uint8_t* s, const uint8_t* sc, uint8_t* next, int t)
+    auto multiply = [&](auto with_loads, const uint8_t* s, const Scales& sc, uint8_t* next, Scales& next_sc, int t)
                         __attribute__((always_inline)) {
         v4i fa[3], fb[2][FN];
-        int sa[FM], sb[FN];
-#pragma unroll
-        for (int j = 0; j < FN; ++j) sb[j] = scale_b(sc, j);
-        sa[0] = scale_a(sc, 0);
         fa[0] = code_a(s, 0);
 #pragma unroll
         for (int j = 0; j < FN; ++j) fb[0][j] = code_b(s, 0, j);
-        if (FM > 1) sa[FM > 1 ? 1 : 0] = scale_a(sc, 1);
         fa[1] = code_a(s, 1);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             const int kk = g / FM, i = g % FM;
             if (g + 2 < G) fa[(g + 2) % 3] = code_a(s, g + 2);
-            if (g + 2 < FM) sa[g + 2 < FM ? g + 2 : 0] = scale_a(sc, g + 2);
             if (kk == 0) {
 #pragma unroll
                 for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j) fb[1][j] = code_b(s, 1, j);
@@ -441,51 +395,83 @@ __global__ __launch_bounds__(WM* WN * 64, WM* WN == 4 && BM == 256 ? 1 : 2) void
             if constexpr (with_loads.value) {
 #pragma unroll
                 for (int l = 0; l < NL; ++l)
-                    if (l * G / NL == g) fetch_one(next, t, l);
+                    if (l * G / NL == g) fetch_one(next, next_sc, t, l);
             }
 #pragma unroll
             for (int j = 0; j < FN; ++j)
-                acc[i][j] = kk == 0 ? mfma4<0>(fb[0][j], fa[g % 3], acc[i][j], sb[j], sa[i])
-                                    : mfma4<1>(fb[1][j], fa[g % 3], acc[i][j], sb[j], sa[i]);
+                acc[i][j] = kk == 0 ? mfma4<0>(fb[0][j], fa[g % 3], acc[i][j], sc.b[j], sc.a[i])
+                                    : mfma4<1>(fb[1][j], fa[g % 3], acc[i][j], sc.b[j], sc.a[i]);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     // Tile t is in s; the loads of tile t + S - 1 go to `next`, whose tile every
     // wave has read before the barrier.  No branch between loads and waits, so the
     // number in flight is known everywhere.
-    auto step = [&](const uint8_t* s, uint8_t* next, int t) __attribute__((always_inline)) {
+    Scales sc[S];
+    auto step = [&](const uint8_t* s, const Scales& from_sc, uint8_t* next, Scales& next_sc, int t)
+                    __attribute__((always_inline)) {
         wait_loads<(S - 2) * NL>();
         barrier();
-        multiply(std::true_type{}, s, s + kCodes, next, t + S - 1);
+        multiply(std::true_type{}, s, from_sc, next, next_sc, t + S - 1);
     };
     if constexpr (S == 2) {
+        // The scales of tiles 4 n .. 4 n + 3, 32 bytes a row: 16 bytes a lane; where
+        // there are fewer tiles, 4 bytes a lane, those past them the row's first again,
+        // not used.  (Of 8 bytes of a row in every tile, a wave's load touched 32 lines
+        // for 256 bytes: 8192 x 8192 x 8192 took 276 us in place of 259.)
+        static_assert(kScaleLoads % kW == 0, "each wave has as many");
+        // a wave's load of scales is of A's rows or of B's
+        auto s_load = [&](int i) __attribute__((always_inline)) { return wave * NS + i; };
+        auto row_at = [&](int r) __attribute__((always_inline)) {
+            return r < BM ? min(r, last_a) * (unsigned)p.ldsa : min(r - BM, last_b) * (unsigned)p.ldsb;
+        };
+        unsigned sfrom[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) sfrom[i] = row_at(s_load(i) * 32 + lane / 2);
+        auto fetch_span = [&](int n) __attribute__((always_inline)) {
+            uint8_t* to = spans + (n & 1) * kScales;
+            if ((n + 1) * kSpan <= tiles) {
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+                    to_lds16(s_load(i) * 32 < BM ? SA : SB, sfrom[i] + (lane & 1) * 16, n * kSpan * kBlocks,
+                             to + s_load(i) * 1024);
+            } else {
+                const int there = (tiles - n * kSpan) * 2, d = lane % 8 < there ? lane % 8 : 0;
+                for (int i = wave; i < (BM + BN) / 8; i += kW)
+                    to_lds4(i * 8 < BM ? SA : SB, row_at(i * 8 + lane / 8) + d * 4, n * kSpan * kBlocks, to + i * 256);
+            }
+        };
+        int osa = (wm + r16) * kRowScales + g4 * 2, osb = (BM + wn + r16) * kRowScales + g4 * 2;
+        asm volatile("" : "+v"(osa), "+v"(osb));
         // Two stages, the barrier before a tile's last two groups: by then all its
         // fragments are in registers, so the next tile's first ones are read, and
         // the loads of the one after that are issued into its LDS, while the matrix
         // instructions go on.
         static_assert(G % 4 == 0 && FM >= 4, "the ring of fragments comes round with the tile");
         v4i fa[4], fb[2][FN];
-        int sa[2][FM], sb[2][FN];
         // Tile t's first fragments and all its scales, where no load is in flight (as
         // one into `spans` may be later, the compiler would wait for it)
         auto first = [&](auto turn, const uint8_t* s, int t) __attribute__((always_inline)) {
-            const uint8_t* sc = spans + (t / kSpan & 1) * kScales + t % kSpan * kBlocks;
+            const uint8_t* at = spans + (t / kSpan & 1) * kScales + t % kSpan * kBlocks;
+            auto scale = [&](int o) __attribute__((always_inline)) {
+                return (int)*reinterpret_cast<const uint16_t*>(at + o);
+            };
+            Scales& x = sc[turn.value];
             fa[0] = code_a(s, 0);
-            sa[turn.value][0] = scale_a(sc, 0);
+            x.a[0] = scale(osa);
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
                 fb[0][j] = code_b(s, 0, j);
-                sb[turn.value][j] = scale_b(sc, j);
+                x.b[j] = scale(osb + j * 16 * kRowScales);
             }
             fa[1] = code_a(s, 1);
 #pragma unroll
-            for (int i = 1; i < FM; ++i) sa[turn.value][i] = scale_a(sc, i);
+            for (int i = 1; i < FM; ++i) x.a[i] = scale(osa + i * 16 * kRowScales);
         };
-        // A tile's first kEarly loads go out behind the barrier that frees its LDS,
-        // the others between the first groups of the next tile: all at once they
+        // The next tile's loads go out between the first groups: all at once they
         // hold up the fragment reads.
-        constexpr int kEarly = MX4_EARLY, kPer = MX4_PER;
-        static_assert(kEarly + kPer * (G - 2) >= NL, "all loads go out");
+        constexpr int kPer = 2;
+        static_assert(kPer * (G - 2) >= NL, "all loads go out");
         auto run = [&](auto turn, uint8_t* s, uint8_t* next, int t) __attribute__((always_inline)) {
             constexpr int kTurn = turn.value;
             if (kTurn == 0 && t % kSpan == 0 && t + kSpan < tiles) fetch_span(t / kSpan + 1);
@@ -502,26 +488,21 @@ __global__ __launch_bounds__(WM* WN * 64, WM* WN == 4 && BM == 256 ? 1 : 2) void
                     barrier();
                     first(std::integral_constant<int, 1 - kTurn>{}, next, t + 1);
                 }
-                if (kEarly > 0 && g >= G - 2) fetch_one(s, t + 2, g - (G - 2));
-                else
 #pragma unroll
-                    for (int l = kEarly + g * kPer; l < kEarly + (g + 1) * kPer && l < NL; ++l)
-                        fetch_one(next, t + 1, l);
+                for (int l = g * kPer; l < (g + 1) * kPer && l < NL; ++l) fetch_one(next, sc[0], t + 1, l);
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
-                    acc[i][j] = kk == 0 ? mfma4<0>(fb[0][j], fa[g % 4], acc[i][j], sb[kTurn][j], sa[kTurn][i])
-                                        : mfma4<1>(fb[1][j], fa[g % 4], acc[i][j], sb[kTurn][j], sa[kTurn][i]);
+                    acc[i][j] = kk == 0 ? mfma4<0>(fb[0][j], fa[g % 4], acc[i][j], sc[kTurn].b[j], sc[kTurn].a[i])
+                                        : mfma4<1>(fb[1][j], fa[g % 4], acc[i][j], sc[kTurn].b[j], sc[kTurn].a[i]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
         // at least two tiles (deep_ok)
         fetch_span(0);
-        fetch(s0, 0);
+        fetch(s0, sc[0], 0);
         wait_loads<0>();
         barrier();
         first(std::integral_constant<int, 0>{}, s0, 0);
-#pragma unroll
-        for (int l = 0; l < kEarly; ++l) fetch_one(s1, 1, l);
         int t = 0;
         for (; t + 2 <= tiles; t += 2) {
             run(std::integral_constant<int, 0>{}, s0, s1, t);
@@ -529,63 +510,67 @@ __global__ __launch_bounds__(WM* WN * 64, WM* WN == 4 && BM == 256 ? 1 : 2) void
         }
         if (t < tiles) run(std::integral_constant<int, 0>{}, s0, s1, t);
     } else if (tiles == 1) {  // nothing to load ahead
-        fetch(s0, 0);
+        fetch(s0, sc[0], 0);
         wait_loads<0>();
         barrier();
-        multiply(std::false_type{}, s0, s0 + kCodes, s0, 0);
+        multiply(std::false_type{}, s0, sc[0], s0, sc[0], 0);
     } else if (tiles > 1) {
-        fetch(s0, 0);
-        fetch(s1, 1);
-        if (S > 3) fetch(s2, 2);
+        constexpr int k3 = S > 3 ? 3 : 2;
+        uint8_t* last = S > 3 ? s3 : s2;
+        // (in this order: else the compiler waits, in every turn of the loop, for scales
+        // that it has put behind later loads here)
+        fetch(s0, sc[0], 0);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(s1, sc[1], 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (S > 3) fetch(s2, sc[2], 2);
+        __builtin_amdgcn_sched_barrier(0);
         int t = 0;
         for (; t + S <= tiles; t += S) {
-            step(s0, S == 3 ? s2 : s3, t);
-            step(s1, s0, t + 1);
-            step(s2, s1, t + 2);
-            if (S > 3) step(s3, s2, t + 3);
+            step(s0, sc[0], last, sc[k3], t);
+            step(s1, sc[1], s0, sc[0], t + 1);
+            step(s2, sc[2], s1, sc[1], t + 2);
+            if (S > 3) step(s3, sc[k3], s2, sc[2], t + 3);
         }
         // the last tiles % S are in flight
         wait_loads<0>();
         barrier();
-        if (t < tiles) multiply(std::false_type{}, s0, s0 + kCodes, s0, 0);
-        if (t + 1 < tiles) multiply(std::false_type{}, s1, s1 + kCodes, s1, 0);
-        if (S > 3 && t + 2 < tiles) multiply(std::false_type{}, s2, s2 + kCodes, s2, 0);
+        if (t < tiles) multiply(std::false_type{}, s0, sc[0], s0, sc[0], 0);
+        if (t + 1 < tiles) multiply(std::false_type{}, s1, sc[1], s1, sc[1], 0);
+        if (S > 3 && t + 2 < tiles) multiply(std::false_type{}, s2, sc[2], s2, sc[2], 0);
     }
     wait_loads<0>();  // also those past the end
     if (p.K % 256) {
         const int k0 = tiles * kBK, blocks = p.K / kMxBlock + (p.K % kMxBlock != 0);
-        uint8_t* sc = S > 2 ? s0 + kCodes : spans;
         v4i end[NA + NB];
-        uint32_t ends[NS];
 #pragma unroll
         for (int l = 0; l < NA + NB; ++l) end[l] = codes16((l < NA ? A : B) + (from[l] - chunk), k0 + chunk, p.K);
+        Scales ends;
 #pragma unroll
-        for (int l = 0; l < NS; ++l)
-            ends[l] = scales4((of_a(l) ? SA : SB) + sfrom[l], k0 / 16 + (lane & 1) * 4, blocks);
+        for (int i = 0; i < FM; ++i) ends.a[i] = scales2(SA + (sfa[i] - g4 * 2), k0 / 16 + g4 * 2, blocks);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) ends.b[j] = scales2(SB + (sfb[j] - g4 * 2), k0 / 16 + g4 * 2, blocks);
         __syncthreads();
 #pragma unroll
         for (int l = 0; l < NA + NB; ++l)
             *reinterpret_cast<v4i*>(s0 + (l < NA ? wave * NA + l : BM / 8 + wave * NB + l - NA) * 1024 + lane * 16) = end[l];
-#pragma unroll
-        for (int l = 0; l < NS; ++l)
-            *reinterpret_cast<uint32_t*>(sc + (s_load(l) * 32 + lane / 2) * kRowScales + (lane & 1) * 4) = ends[l];
         __syncthreads();
-        multiply(std::false_type{}, s0, sc, s0, 0);
+        multiply(std::false_type{}, s0, ends, s0, ends, 0);
     }
     barrier();  // the stage takes the tiles' place
     epilogue<FM, FN>(p, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(s0) + wave * (Stage<FM, FN>::kBytes / 4));
 }
 
 // ---- few rows -------------------------------------------------------------------------
-// A workgroup has 16 channels, its eight waves share K in spans of 512 elements, and
-// the sums meet in LDS: bound by the weights, which are read once, straight to
-// registers.  Of a span a lane takes 64 neighbouring bytes of a channel (blocks 4 g ..
-// 4 g + 3, g = lane / 16) and their four scales.  Activations: up to 16 rows of codes
-// in memory (ELEM kElemCodes), read alike (of 17 rows the smallest tiles take as long,
-// of 64 x 8192 x 8192 16 us for 28); or of floats or spike times, quantised by every
-// workgroup into LDS while its weights are on their way, where that is no more than
-// eight runs of eight a thread (4 x 4096 x 4096 from BF16 5.5 us, 8.0 with a launch of
-// its own for that; 8 x 4096 x 4096 7.4 and 7.9).
+// A workgroup has 16 rows and 16 channels, its eight waves share K in spans of 512
+// elements, and the sums meet in LDS: operands straight to registers, at any
+// alignment.  For a row or a few the weights' bytes bound it, for few tiles of long
+// rows it has eight times the waves.  Of a span a lane takes 64 neighbouring bytes of a
+// channel (blocks 4 g .. 4 g + 3, g = lane / 16) and their four scales.  Activations:
+// codes in memory (ELEM kElemCodes), read alike; or up to 16 rows of floats or spike
+// times, quantised by every workgroup into LDS while its weights are on their way, where
+// that is no more than eight runs of eight a thread (4 x 4096 x 4096 from BF16 5.5 us,
+// 8.0 with a launch of its own for that; 8 x 4096 x 4096 7.4 and 7.9).
 constexpr int kSpanBlocks = 16, kSmallWaves = 8, kSmallRows = 16, kSmallRuns = 8;
 struct Span {
     v4i c[4];
@@ -614,9 +599,11 @@ __global__ __launch_bounds__(kSmallWaves * 64) void k_mx4_small(Mx4Args p, const
     __shared__ __align__(16) uint8_t q[kQuant];
     __shared__ __align__(4) uint8_t qs[kCodesIn ? 16 : kQuant / 16];
     const int lane = lane_id(), wave = uniform(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16, n = n0 + r16 < p.N ? n0 + r16 : p.N - 1;
+    const int tiles_n = (p.N + 15) / 16;
+    const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * kSmallRows;
+    const int n0 = blockIdx.x % tiles_n * 16, n = n0 + r16 < p.N ? n0 + r16 : p.N - 1;
     const uint8_t *wc = p.B + (int64_t)n * p.ldb, *ws = p.sb + (int64_t)n * p.ldsb;
-    const int spans = p.K / 512 + (p.K % 512 != 0), M = (int)p.M;
+    const int spans = p.K / 512 + (p.K % 512 != 0), M = p.M - m0 < kSmallRows ? (int)(p.M - m0) : kSmallRows;
     Span w{};
     if (wave < spans) w = load_span(wc, ws, wave, g, p.K);
     if constexpr (!kCodesIn) {
@@ -646,7 +633,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void k_mx4_small(Mx4Args p, const
     for (int span = wave; span < spans; span += kSmallWaves) {
         Span a;
         if constexpr (kCodesIn) {
-            a = load_span(p.A + row * p.lda, p.sa + row * p.ldsa, span, g, p.K);
+            a = load_span(p.A + (m0 + row) * p.lda, p.sa + (m0 + row) * p.ldsa, span, g, p.K);
         } else {
             const int b = row * spans * kSpanBlocks;
 #pragma unroll
@@ -671,13 +658,41 @@ __global__ __launch_bounds__(kSmallWaves * 64) void k_mx4_small(Mx4Args p, const
 #pragma unroll
     for (int i = 0; i < kSmallWaves; ++i) v += part[i][m][c];
     if (p.bias) v += p.bias[n0 + c];
-    store_elem(p.out, (int64_t)m * p.ldo + n0 + c, apply_act(v, p.act), p.out_elem);
+    store_elem(p.out, (m0 + m) * p.ldo + n0 + c, apply_act(v, p.act), p.out_elem);
+}
+
+// Rows at any alignment to rows on `ld_to` bytes, a multiple of 16, `fill` behind
+// them: codes (K elements; the upper half of an odd row's last byte is cleared) or
+// scales (K bytes), 16 bytes a thread.
+template <bool CODES>
+__device__ __forceinline__ void realign(const uint8_t* __restrict__ from, int64_t ld, int64_t rows, int K,
+                                        uint8_t* __restrict__ to, int64_t ld_to) {
+    const int64_t per = ld_to / 16, n = rows * per;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (int64_t)gridDim.x * 256) {
+        const int64_t r = at / per;
+        const int k = (int)(at - r * per) * 16;
+        v4i v;
+        if constexpr (CODES) {
+            v = codes16(from + r * ld, k, K);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = (int)scales4(from + r * ld, k + 4 * i, K);
+        }
+        *reinterpret_cast<v4i*>(to + r * ld_to + k) = v;
+    }
+}
+__global__ __launch_bounds__(256) void k_mx4_realign(const uint8_t* __restrict__ q, int64_t ldq,
+                                                     const uint8_t* __restrict__ s, int64_t lds, int64_t rows, int K,
+                                                     uint8_t* __restrict__ to_q, int64_t ldq_to,
+                                                     uint8_t* __restrict__ to_s, int64_t lds_to) {
+    if (to_q) realign<true>(q, ldq, rows, K, to_q, ldq_to);
+    if (to_s) realign<false>(s, lds, rows, K / kMxBlock + (K % kMxBlock != 0), to_s, lds_to);
 }
 
 template <int ELEM>
 int run_small(vdttfs_ctx* ctx, const Mx4Args& a, const void* x, int64_t ldx) {
-    k_mx4_small<ELEM><<<dim3((unsigned)((a.N + 15) / 16)), kSmallWaves * 64, 0, ctx->stream>>>(a, x, ldx, ctx->c.tfs,
-                                                                                               ctx->c.T);
+    const int64_t blocks = (a.M + kSmallRows - 1) / kSmallRows * ((a.N + 15) / 16);
+    k_mx4_small<ELEM><<<dim3((unsigned)blocks), kSmallWaves * 64, 0, ctx->stream>>>(a, x, ldx, ctx->c.tfs, ctx->c.T);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
@@ -692,13 +707,10 @@ int run_tile(vdttfs_ctx* ctx, const Mx4Args& a) {
 
 }  // namespace
 
-// Rows that loads to LDS can take.
+// Rows that loads to LDS can take: of codes on 16 bytes, and where scales go that way
+// too (large tiles), of scales on 4.
 constexpr int64_t kMaxLd = 1 << 22;  // 256 rows of them below 2^31 bytes
-static bool aligned(const Mx4Args& a) {
-    return a.lda <= kMaxLd && a.ldb <= kMaxLd && a.ldsa <= kMaxLd && a.ldsb <= kMaxLd && (((uintptr_t)a.A | (uintptr_t)a.B | (uintptr_t)a.lda | (uintptr_t)a.ldb) & 15) == 0 &&
-           (((uintptr_t)a.sa | (uintptr_t)a.sb | (uintptr_t)a.ldsa | (uintptr_t)a.ldsb) & 3) == 0;
-}
-
+static bool off(const uint8_t* p, int64_t ld, int to) { return (((uintptr_t)p | (uintptr_t)ld) & (to - 1)) != 0 || ld > kMaxLd; }
 template <int BM, int BN, int WM, int WN, int S>
 static int run_big(vdttfs_ctx* ctx, const Mx4Args& a) {
     const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
@@ -707,22 +719,6 @@ static int run_big(vdttfs_ctx* ctx, const Mx4Args& a) {
     return VDTTFS_OK;
 }
 
-struct Mx4Tile {
-    int bm, bn;
-};
-static Mx4Tile tile_for(int64_t M, int N, int K, bool is_aligned) {
-    auto tiles = [&](int bm, int bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); };
-    if (!is_aligned) return tiles(64, 64) >= 192 ? Mx4Tile{64, 64} : Mx4Tile{32, 32};
-    const int64_t big = tiles(256, 256), rounds = (big + 255) / 256;
-    const bool deep = K >= 512;
-    if (deep && (rounds == 1 ? big >= 160 : big * 10 >= rounds * 256 * 7)) return Mx4Tile{256, 256};
-    if (deep && tiles(128, 128) >= 384) return Mx4Tile{128, 128};
-    return tiles(64, 64) >= 192 ? Mx4Tile{64, 64} : Mx4Tile{32, 32};
-}
-
-#ifndef MX4_BIG
-#define MX4_BIG 2, 4
-#endif
 // Whether rows of floats or spike times are quantised by their product.
 bool mx4_small_linear_ok(int64_t M, int K) {
     const int64_t per = ((int64_t)K + 511) / 512 * 64;  // runs of eight of a row, whole spans
@@ -735,23 +731,83 @@ int launch_mx4_small_linear(vdttfs_ctx* ctx, const Mx4Args& a, const void* x, in
     return run_small<VDTTFS_ELEM_TIMES>(ctx, a, x, ldx);
 }
 
-int launch_mx4(vdttfs_ctx* ctx, const Mx4Args& a) {
+// The kernel of a product and what it wants copied first.  Measured (us; K last,
+// "odd": rows off 16 bytes, LDS tiles with their copies):
+//   few tiles, long rows: 256x256x8192 16x16 7.2, LDS 32 12.4, 64 22; 235x34x3873 odd
+//   8.4, through registers 32 11.6; 128x1024x1024 5.0 and 4.8; 64x4096x4096 (256 tiles
+//   of 32) 11.7 and 8.2
+//   short rows: 7150x2496x128 through registers 64 20.5, LDS 64 28; 2000x2000x512 8.7,
+//   LDS 64 9.6, LDS 128 8.2
+//   8192x4096x4096 LDS 256 75; 3000x3000x3000 (144 tiles of 256) 45, 128 51;
+//   2560x8192x2048 (320, so a second round a quarter full) 41.5 and 37
+//   2048x2048x2048 (256 tiles of 128) LDS 128 11, 64 28; 512x4096x4096 (128) 18, 25;
+//   256x4096x4096 (64) 14.3, 13.7; 4225x192x4864 (68) 21, 11.3, through registers 20
+//   odd: 3000x3000x3000 copied 45, through registers 83; 2048x2048x2048 21 and 25;
+//   4225x192x4864 23 and 24, one operand alone some 16; 2000x2000x512 14 and 9.7
+Mx4Plan mx4_plan(const Mx4Args& a) {
+    Mx4Plan p{};
+    auto tiles = [&](int t) { return (a.M + t - 1) / t * ((a.N + t - 1) / t); };
+    const bool many = tiles(64) >= 192;
+    const Mx4Path registers = many ? kMx4Tile64 : kMx4Tile32;
+    if (a.M <= kSmallRows || (a.K >= 1024 && tiles(32) <= 128)) return p.path = kMx4Few, p;
+    if (a.K < 512) return p.path = registers, p;
+    const int64_t big = tiles(256), rounds = (big + 255) / 256;
+    const double work = (double)a.M * a.N * a.K;
+    p.path = many ? kMx4Lds64 : kMx4Lds32;
+    if (rounds == 1 ? big >= 160 : big * 10 >= rounds * 256 * 7) p.path = kMx4Lds256;
+    else if (tiles(128) >= 110) p.path = kMx4Lds128;
+    p.a = off(a.A, a.lda, 16);
+    p.b = off(a.B, a.ldb, 16);
+    p.sa = a.ldsa > kMaxLd;
+    p.sb = a.ldsb > kMaxLd;
+    if (p.a || p.b || p.sa || p.sb) {
+        const bool both = (p.a || p.sa) && (p.b || p.sb);
+        if (work < (both ? 6e9 : 3e9)) return Mx4Plan{registers, false, false, false, false};
+    }
+    if (p.path == kMx4Lds256 || p.path == kMx4Lds128) {  // whose scales go to LDS in fours
+        const bool sa = off(a.sa, a.ldsa, 4), sb = off(a.sb, a.ldsb, 4);
+        if (work < 2e9 && ((sa && !p.a) || (sb && !p.b))) {
+            p.path = many ? kMx4Lds64 : kMx4Lds32;
+        } else {
+            p.sa |= sa;
+            p.sb |= sb;
+        }
+    }
+    return p;
+}
+
+int launch_mx4_realign(vdttfs_ctx* ctx, const uint8_t* q, int64_t ldq, const uint8_t* s, int64_t lds, int64_t rows,
+                       int K, uint8_t* to_q, int64_t ldq_to, uint8_t* to_s, int64_t lds_to) {
+    const int64_t n = rows * (to_q ? ldq_to : lds_to) / 16, blocks = (n + 255) / 256;
+    k_mx4_realign<<<dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), 256, 0, ctx->stream>>>(
+        q, ldq, s, lds, rows, K, to_q, ldq_to, to_s, lds_to);
+    VD_HIP(hipGetLastError());
+    return VDTTFS_OK;
+}
+
+int launch_mx4(vdttfs_ctx* ctx, const Mx4Args& a, Mx4Path path) {
     if (a.M <= 0 || a.N <= 0) return VDTTFS_OK;
-    if (a.M <= kSmallRows) return run_small<kElemCodes>(ctx, a, nullptr, 0);
-    const bool fast = aligned(a);
-    const Mx4Tile t = tile_for(a.M, a.N, a.K, fast);
-    const int64_t rows = max_blocks(512) / ((a.N + t.bn - 1) / t.bn) * t.bm;  // as many a launch as its tiles allow
+    static constexpr struct {
+        int bm, bn;
+    } kTiles[] = {{16, 16}, {32, 32}, {64, 64}, {32, 32}, {64, 64}, {128, 128}, {256, 256}};
+    const int bm = kTiles[path].bm, bn = kTiles[path].bn;
+    const int64_t rows = max_blocks(512) / ((a.N + bn - 1) / bn) * bm;  // as many a launch as its tiles allow
     for (int64_t m = 0; m < a.M; m += rows) {
         Mx4Args part = a;
         part.A += m * a.lda;
         part.sa += m * a.ldsa;
         part.out = static_cast<char*>(a.out) + m * a.ldo * (a.out_elem == VDTTFS_ELEM_F32 ? 4 : 2);
         part.M = a.M - m < rows ? a.M - m : rows;
-        int rc;
-        if (!fast) rc = t.bm == 64 ? run_tile<64, 64>(ctx, part) : run_tile<32, 32>(ctx, part);
-        else if (t.bm == 256) rc = run_big<256, 256, MX4_BIG, 2>(ctx, part);
-        else if (t.bm == 128) rc = run_big<128, 128, 2, 2, 2>(ctx, part);
-        else rc = t.bm == 64 ? run_big<64, 64, 2, 2, 4>(ctx, part) : run_big<32, 32, 2, 2, 4>(ctx, part);
+        int rc = VDTTFS_OK;
+        switch (path) {
+            case kMx4Few: rc = run_small<kElemCodes>(ctx, part, nullptr, 0); break;
+            case kMx4Tile32: rc = run_tile<32, 32>(ctx, part); break;
+            case kMx4Tile64: rc = run_tile<64, 64>(ctx, part); break;
+            case kMx4Lds32: rc = run_big<32, 32, 2, 2, 4>(ctx, part); break;
+            case kMx4Lds64: rc = run_big<64, 64, 2, 2, 4>(ctx, part); break;
+            case kMx4Lds128: rc = run_big<128, 128, 2, 2, 2>(ctx, part); break;
+            case kMx4Lds256: rc = run_big<256, 256, 2, 4, 2>(ctx, part); break;
+        }
         if (rc != VDTTFS_OK) return rc;
     }
     return VDTTFS_OK;
