@@ -52,7 +52,8 @@ def run_dispatch(ctx, idx, E, bits, elem, pad=0):
 SIZES = [  # M, k, E, D
     (1, 1, 1, 1), (1, 6, 64, 128), (2, 3, 4, 33), (5, 64, 1024, 7), (40, 8, 8, 130), (257, 2, 8, 512), (300, 1, 100, 64),
     (1000, 4, 60, 96), (700, 3, 1000, 40), (3000, 8, 64, 257), (9001, 2, 256, 33), (70000, 1, 16, 8), (20000, 6, 1024, 16),
-    (128, 16, 16, 1000), (129, 16, 17, 1001), (4, 2, 3, 20000), (512, 4, 7, 24), (2048, 1, 2, 10), (2049, 1, 2, 10)]
+    (128, 16, 16, 1000), (129, 16, 17, 1001), (4, 2, 3, 20000), (512, 4, 7, 24), (2048, 1, 2, 10), (2049, 1, 2, 10),
+    (256, 4, 5, 12), (205, 5, 1024, 4), (4096, 1, 9, 2), (4097, 1, 9, 2), (1366, 3, 1024, 2), (262200, 4, 5, 2)]
 
 
 @pytest.mark.parametrize("M,k,E,D", SIZES)
@@ -316,7 +317,7 @@ def test_route_dispatch_products_combine(gpu_ctx_factory):
 
 def test_large_sort_in_a_graph(gpu_ctx_factory):
     c = gpu_ctx_factory(vdttfs.TaskConsts(T=64, delta=16))
-    M, k, E, D = 5000, 3, 50, 8
+    M, k, E, D = 9000, 3, 50, 8
     x = np.random.default_rng(0).standard_normal((M, D)).astype(np.float32)
     dx, idx, place, start = c.to_device(x), c.empty((M, k), np.int32), c.empty((M, k), np.int32), c.empty(E + 1, np.int32)
     z = c.empty((M * k, D))

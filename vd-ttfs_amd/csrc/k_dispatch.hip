@@ -17,6 +17,8 @@ namespace {
 
 constexpr int kPairs = 2048;  // pairs of a workgroup of the sort
 constexpr int kWaves = 16;    // of such a workgroup
+constexpr int kOnePairs = 4096;  // pairs that one workgroup places by itself
+constexpr int kSumBlocks = 512;  // workgroups that sum the counts by themselves
 
 __device__ __forceinline__ int expert_of(const PlaceArgs& a, int64_t q, int64_t pairs) {
     const int e = q < pairs ? a.idx[q] : -1;
@@ -84,33 +86,34 @@ __global__ __launch_bounds__(1024) void k_place_scan(PlaceArgs a, int* __restric
     }
 }
 
-// Each pair's place: a wave has 128 neighbouring pairs, counts them by expert,
-// adds what the waves before it have, and ranks 64 at a time among themselves.
-__global__ __launch_bounds__(1024) void k_place(PlaceArgs a, const int* __restrict__ hist, int bits) {
-    extern __shared__ int at[];  // [kWaves][E]
+// The places of a workgroup's pairs: each wave has N runs of 64 neighbouring ones,
+// counts them by expert, adds what the waves before it have, and ranks a run's lanes
+// among themselves.  first(), called by all threads: the place of the workgroup's first
+// pair of expert threadIdx.x (unused from E on).
+template <int N, class F>
+__device__ __forceinline__ void place_block(const PlaceArgs& a, int64_t q0, int* at, int bits, const F& first) {
     const int64_t pairs = a.M * a.top_k;
     const int wave = threadIdx.x >> 6, lane = lane_id();
-    const int64_t q0 = (int64_t)blockIdx.x * kPairs + wave * (kPairs / kWaves) + lane;
-    int e[2];
+    q0 += wave * (N * 64) + lane;
+    int e[N];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) e[i] = expert_of(a, q0 + 64 * i, pairs);
+    for (int i = 0; i < N; ++i) e[i] = expert_of(a, q0 + 64 * i, pairs);
     for (int i = threadIdx.x; i < kWaves * a.E; i += 1024) at[i] = 0;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < N; ++i)
         if (e[i] >= 0) atomicAdd(&at[wave * a.E + e[i]], 1);
     __syncthreads();
-    if ((int)threadIdx.x < a.E) {
-        int sum = hist[(int64_t)blockIdx.x * a.E + threadIdx.x];
+    int sum = first();
+    if ((int)threadIdx.x < a.E)
         for (int w = 0; w < kWaves; ++w) {
             const int n = at[w * a.E + threadIdx.x];
             at[w * a.E + threadIdx.x] = sum;
             sum += n;
         }
-    }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < N; ++i) {
         const uint64_t same = lanes_like(e[i], bits);
         const int rank = __popcll(same & lanemask_lt());
         int to = -1;
@@ -120,6 +123,66 @@ __global__ __launch_bounds__(1024) void k_place(PlaceArgs a, const int* __restri
         wave_sync();
         if (q0 + 64 * i < pairs) a.place[q0 + 64 * i] = to;
     }
+}
+
+// ... from the scanned counts.
+__global__ __launch_bounds__(1024) void k_place(PlaceArgs a, const int* __restrict__ hist, int bits) {
+    extern __shared__ int at[];  // [kWaves][E]
+    place_block<kPairs / 1024>(a, (int64_t)blockIdx.x * kPairs, at, bits, [&] {
+        return (int)threadIdx.x < a.E ? hist[(int64_t)blockIdx.x * a.E + threadIdx.x] : 0;
+    });
+}
+
+// ... from the counts, which every workgroup sums by itself: one launch less.  2^bits
+// threads go over the experts, and share the blocks.
+__global__ __launch_bounds__(1024) void k_place_sum(PlaceArgs a, const int* __restrict__ hist, int blocks, int bits) {
+    extern __shared__ int at[];
+    __shared__ int before[1024], total[1024];
+    __shared__ int lds[16];
+    place_block<kPairs / 1024>(a, (int64_t)blockIdx.x * kPairs, at, bits, [&] {
+        const int e = threadIdx.x & ((1 << bits) - 1), run = threadIdx.x >> bits, runs = 1024 >> bits;
+        int mine = 0, all = 0;
+        if (e < a.E)
+#pragma unroll 4
+            for (int b = run; b < blocks; b += runs) {
+                const int n = hist[b * a.E + e];
+                all += n;
+                mine += b < (int)blockIdx.x ? n : 0;
+            }
+        before[threadIdx.x] = mine;
+        total[threadIdx.x] = all;
+        __syncthreads();
+        mine = all = 0;
+        if (run == 0)
+            for (int r = 0; r < runs; ++r) {
+                mine += before[(r << bits) + e];
+                all += total[(r << bits) + e];
+            }
+        int used;
+        const int start = block_excl_scan(all, lds, &used);
+        if (blockIdx.x == 0 && a.start) {
+            if ((int)threadIdx.x < a.E) a.start[threadIdx.x] = start;
+            if (threadIdx.x == 0) a.start[a.E] = used;
+        }
+        return start + mine;
+    });
+}
+
+// ... of all pairs, by one workgroup.
+__global__ __launch_bounds__(1024) void k_place_one(PlaceArgs a, int bits) {
+    extern __shared__ int at[];
+    __shared__ int lds[16];
+    place_block<kOnePairs / 1024>(a, 0, at, bits, [&] {
+        int n = 0, used;
+        if ((int)threadIdx.x < a.E)
+            for (int w = 0; w < kWaves; ++w) n += at[w * a.E + threadIdx.x];
+        const int start = block_excl_scan(n, lds, &used);
+        if (a.start) {
+            if ((int)threadIdx.x < a.E) a.start[threadIdx.x] = start;
+            if (threadIdx.x == 0) a.start[a.E] = used;
+        }
+        return start;
+    });
 }
 
 // A row's bytes to another; both may start anywhere that their type allows.
@@ -132,7 +195,7 @@ __device__ __forceinline__ void copy_to_slots(void* z, int64_t ld_bytes, const v
         const v4u v = reinterpret_cast<const AnyUint4*>(from + b)->v;
         for (int j = 0; j < n; ++j) {
             const int p = place[j];
-            if (p >= 0 && p < rows) reinterpret_cast<AnyUint4*>(static_cast<char*>(z) + p * ld_bytes + b)->v = v;
+            if (p >= 0 && p < rows) put16(static_cast<char*>(z) + p * ld_bytes + b, v);
         }
     }
     for (int64_t b = whole + (int64_t)threadIdx.x * unit; b < bytes; b += kCopy * unit)
@@ -380,24 +443,37 @@ unsigned grid_of(int64_t blocks, unsigned most) { return (unsigned)(blocks < mos
 }  // namespace
 
 size_t dispatch_place_bytes(int64_t pairs, int n_experts) {
-    return (size_t)((pairs + kPairs - 1) / kPairs) * n_experts * 4;
+    return pairs <= kOnePairs ? 0 : (size_t)((pairs + kPairs - 1) / kPairs) * n_experts * 4;
 }
 
+// By pairs (rows of 16 bytes sorted and moved, of 60 experts):
+//   to kOnePairs  one workgroup (4014: 9.3 us; counting first 10.8)
+//   beyond        count, place (8028: 11.3 us; one workgroup 14.8; with a scan 13.4),
+//                 and a scan between from kSumBlocks workgroups on, whose counts would
+//                 be read by too many (1048576 of 1024 experts 158 us, with a scan 180;
+//                 2097152 422 and 358; of 60 experts 100 and 103, 197 and 194)
 int launch_place(vdttfs_ctx* ctx, const PlaceArgs& a, int* hist) {
     const int64_t pairs = a.M * a.top_k;
     const int blocks = (int)((pairs + kPairs - 1) / kPairs);
-    int log = 0;
-    while ((1 << log) < a.E) ++log;
-    if (blocks > 0) {
-        k_place_count<<<dim3((unsigned)blocks), 1024, 0, ctx->stream>>>(a, hist);
+    const size_t lds = (size_t)kWaves * a.E * 4;
+    int bits = 0;
+    while ((1 << bits) < a.E) ++bits;
+    if (pairs <= kOnePairs) {
+        k_place_one<<<dim3(1), 1024, lds, ctx->stream>>>(a, bits);
         VD_HIP(hipGetLastError());
+        return VDTTFS_OK;
     }
-    k_place_scan<<<dim3(1), 1024, 0, ctx->stream>>>(a, hist, blocks, log);
+    k_place_count<<<dim3((unsigned)blocks), 1024, 0, ctx->stream>>>(a, hist);
     VD_HIP(hipGetLastError());
-    if (blocks > 0) {
-        k_place<<<dim3((unsigned)blocks), 1024, (size_t)kWaves * a.E * 4, ctx->stream>>>(a, hist, log);
+    if (blocks <= kSumBlocks) {
+        k_place_sum<<<dim3((unsigned)blocks), 1024, lds, ctx->stream>>>(a, hist, blocks, bits);
         VD_HIP(hipGetLastError());
+        return VDTTFS_OK;
     }
+    k_place_scan<<<dim3(1), 1024, 0, ctx->stream>>>(a, hist, blocks, bits);
+    VD_HIP(hipGetLastError());
+    k_place<<<dim3((unsigned)blocks), 1024, lds, ctx->stream>>>(a, hist, bits);
+    VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
 
