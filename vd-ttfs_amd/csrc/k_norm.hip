@@ -39,18 +39,19 @@ __device__ __forceinline__ void store_codes8(int8_t* q, int64_t row, int c, int 
         if (i < cols - c) q[row + c + i] = (int8_t)k[i];
 }
 
-// Sums and largest magnitudes over the LANES lanes that share a row, in every
-// one of them.  `turn` alternates between rows, so that one barrier a row does.
+// Sums and largest magnitudes (as bits: those of a NaN are above all others, so it
+// wins) over the LANES lanes that share a row, in every one of them.  `turn` alternates between rows, so that one barrier a row does.
 template <int LANES>
 struct Shared {
-    float sum[2][LANES > 64 ? LANES / 64 : 1], top[2][LANES > 64 ? LANES / 64 : 1];
+    float sum[2][LANES > 64 ? LANES / 64 : 1];
+    uint32_t top[2][LANES > 64 ? LANES / 64 : 1];
 };
 template <int LANES, bool TOP>
-__device__ __forceinline__ void over_row(float& sum, float& top, Shared<LANES>& s, int turn) {
+__device__ __forceinline__ void over_row(float& sum, uint32_t& top, Shared<LANES>& s, int turn) {
 #pragma unroll
     for (int o = 1; o < LANES && o < 64; o *= 2) {
         sum += __shfl_xor(sum, o, 64);
-        if (TOP) top = nan_max(top, __shfl_xor(top, o, 64));
+        if (TOP) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
     }
     if constexpr (LANES > 64) {
         const int wave = threadIdx.x >> 6;
@@ -64,7 +65,7 @@ __device__ __forceinline__ void over_row(float& sum, float& top, Shared<LANES>& 
 #pragma unroll
         for (int i = 1; i < LANES / 64; ++i) {
             sum += s.sum[turn][i];
-            if (TOP) top = nan_max(top, s.top[turn][i]);
+            if (TOP) top = max(top, s.top[turn][i]);
         }
     }
 }
@@ -82,8 +83,8 @@ __device__ __forceinline__ bool in_range(float sum) { return sum >= kFewest && s
 __device__ __forceinline__ Root plain_root(float sum, int cols, float eps) {
     return Root{1.0f, 1.0f / sqrtf(sum / (float)cols + eps)};
 }
-__device__ __forceinline__ float factor_of(float top) {
-    int e = (int)(magnitude(top) >> 23) - 127;
+__device__ __forceinline__ float factor_of(uint32_t top) {
+    int e = (int)(top >> 23) - 127;
     e = e < -126 ? -126 : e > 126 ? 126 : e;
     return __uint_as_float((uint32_t)(127 - e) << 23);
 }
@@ -138,7 +139,8 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
                 if (c < a.cols && from >= 0) rr[v] = raw8<RE>(a.res, m * a.ldr + from);
             }
         }
-        float sum = 0.0f, top = 0.0f;
+        float sum = 0.0f;
+        uint32_t top = 0;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int c = (v * LANES + lane) * 8;
@@ -165,7 +167,7 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = nan_max(top, fabsf(u[v][i]));
+                for (int i = 0; i < 8; ++i) top = max(top, magnitude(u[v][i]));
             over_row<LANES, true>(sum, top, lds, turn);
         } else {
             over_row<LANES, false>(sum, top, lds, turn);
@@ -179,11 +181,12 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
         }
         Root root = plain_root(sum, a.cols, a.eps);
         if (!in_range(sum)) {  // the same in all lanes of the row
-            float most = 0.0f, none = 0.0f, again = 0.0f;
+            float none = 0.0f, again = 0.0f;
+            uint32_t most = 0;
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) most = nan_max(most, fabsf(h[v][i]));
+                for (int i = 0; i < 8; ++i) most = max(most, magnitude(h[v][i]));
             over_row<LANES, true>(none, most, lds, turn);
             turn ^= 1;
             const float f = factor_of(most);
@@ -191,13 +194,13 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
             for (int v = 0; v < NV; ++v)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) again += (h[v][i] * f) * (h[v][i] * f);
-            over_row<LANES, false>(again, none, lds, turn);
+            over_row<LANES, false>(again, most, lds, turn);
             turn ^= 1;
-            root = far_root(again, most, f, a.cols, a.eps);
+            root = far_root(again, __uint_as_float(most), f, a.cols, a.eps);
         }
         if (a.kind == kCodes8) {
             // codes are those of u: a row's codes do not change with a factor of all of it
-            const float s = scale_of(top);
+            const float s = scale_of(__uint_as_float(top));
             if (lane == 0) a.scale[m] = (float)((double)s * root.f * root.r);
             const Coder coder = coder_of(s);
 #pragma unroll
@@ -255,7 +258,7 @@ __global__ __launch_bounds__(kLong) void k_norm_long(NormArgs a) {
     // unsigned: a thread's column goes past the row's end, and past 2^31
     const unsigned cols = (unsigned)a.cols, ends = (cols + kMxBlock - 1) / kMxBlock * kMxBlock;
     for (int64_t m = blockIdx.x; m < a.rows; m += gridDim.x) {
-        float top = 0.0f;
+        uint32_t top = 0;
         double total = 0.0;  // a thread has up to 2^18 runs
         for (unsigned c = threadIdx.x * 8; c < cols; c += kLong * 8) {
             float h[8], part = 0.0f;
@@ -265,19 +268,20 @@ __global__ __launch_bounds__(kLong) void k_norm_long(NormArgs a) {
             total += part;
             times_gain(a, (int)c, h);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = nan_max(top, fabsf(h[i]));
+            for (int i = 0; i < 8; ++i) top = max(top, magnitude(h[i]));
         }
         float sum = (float)total;
         over_row<kLong, true>(sum, top, lds, turn);
         turn ^= 1;
         Root root = plain_root(sum, a.cols, a.eps);
         if (!in_range(sum)) {
-            float most = 0.0f, none = 0.0f, again = 0.0f;
+            float none = 0.0f, again = 0.0f;
+            uint32_t most = 0;
             for (unsigned c = threadIdx.x * 8; c < cols; c += kLong * 8) {
                 float h[8];
                 load_h<XE, RE>(a, m, (int)c, h);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) most = nan_max(most, fabsf(h[i]));
+                for (int i = 0; i < 8; ++i) most = max(most, magnitude(h[i]));
             }
             over_row<kLong, true>(none, most, lds, turn);
             turn ^= 1;
@@ -290,11 +294,11 @@ __global__ __launch_bounds__(kLong) void k_norm_long(NormArgs a) {
                 for (int i = 0; i < 8; ++i) total_f += (double)((h[i] * f) * (h[i] * f));
             }
             again = (float)total_f;
-            over_row<kLong, false>(again, none, lds, turn);
+            over_row<kLong, false>(again, most, lds, turn);
             turn ^= 1;
-            root = far_root(again, most, f, a.cols, a.eps);
+            root = far_root(again, __uint_as_float(most), f, a.cols, a.eps);
         }
-        const float s8 = scale_of(top);
+        const float s8 = scale_of(__uint_as_float(top));
         const Coder coder = coder_of(s8);
         if (a.kind == kCodes8 && threadIdx.x == 0) a.scale[m] = (float)((double)s8 * root.f * root.r);
         for (unsigned c = threadIdx.x * 8; c < ends; c += kLong * 8) {
@@ -341,6 +345,7 @@ void norm_types(vdttfs_ctx* ctx, const NormArgs& a) {
     else if (a.cols <= 256) norm_nv<XE, RE, 1, 32, 256>(ctx, a);
     else if (a.cols <= 512) norm_nv<XE, RE, 1, 64, 256>(ctx, a);
     else if (a.cols <= 1024 && a.rows >= 1024) norm_nv<XE, RE, 2, 64, 256>(ctx, a);
+    else if (a.cols <= 1536) norm_nv<XE, RE, 1, 192, 192>(ctx, a);
     else if (a.cols <= 2048) norm_nv<XE, RE, 1, 256, 256>(ctx, a);
     else if (a.cols <= 4096) norm_nv<XE, RE, 2, 256, 256>(ctx, a);
     else if (a.cols <= 8192) norm_nv<XE, RE, 4, 256, 256>(ctx, a);
