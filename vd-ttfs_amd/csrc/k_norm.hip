@@ -112,7 +112,7 @@ enum { kFloats, kCodes8, kCodes4 };
 // with a residual 21.0 us; loaded one by one behind the others 30.9).  The sum, which may take the residual's place,
 // is stored behind the barrier that all loads come before.
 template <int XE, int RE, int NV, int LANES, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
+__global__ __launch_bounds__(THREADS, NV == 2 ? 4 : 1) void k_norm(NormArgs a) {
     static_assert(LANES <= 64 || LANES == THREADS, "a row has a part of a wave, a wave or the workgroup");
     __shared__ Shared<LANES> lds;
     constexpr int kRows = THREADS / LANES;
@@ -339,6 +339,12 @@ void norm_nv(vdttfs_ctx* ctx, const NormArgs& a) {
         <<<dim3((unsigned)(blocks < most ? blocks : most)), THREADS, 0, ctx->stream>>>(a);
 }
 
+// By columns: as many lanes as a row has runs of eight, to a wave; with rows enough to
+// fill the CUs a wave takes two, so that no barrier is needed; then three waves or four,
+// one run a lane, then four or eight of two.  Four runs in 256 lanes instead of two in 512: 3973 x 5632 to 8
+// bits 47.2 us and 40.6, 2000 x 4100 24.3 and 18.2, 4096 x 8192 to 4 bits 48.0 and 41.7;
+// the other way round 4000 x 6144 of 32-bit floats throughout, 76.7 and 82.4.  One run in
+// 1024 lanes 52.1, 23.1, 49.9 and 75.1.
 template <int XE, int RE>
 void norm_types(vdttfs_ctx* ctx, const NormArgs& a) {
     if (a.cols <= 128) norm_nv<XE, RE, 1, 16, 256>(ctx, a);
@@ -348,7 +354,7 @@ void norm_types(vdttfs_ctx* ctx, const NormArgs& a) {
     else if (a.cols <= 1536) norm_nv<XE, RE, 1, 192, 192>(ctx, a);
     else if (a.cols <= 2048) norm_nv<XE, RE, 1, 256, 256>(ctx, a);
     else if (a.cols <= 4096) norm_nv<XE, RE, 2, 256, 256>(ctx, a);
-    else if (a.cols <= 8192) norm_nv<XE, RE, 4, 256, 256>(ctx, a);
+    else if (a.cols <= 8192) norm_nv<XE, RE, 2, 512, 512>(ctx, a);
     else if (a.cols <= 16384) norm_nv<XE, RE, 2, 1024, 1024>(ctx, a);
     else
         k_norm_long<XE, RE><<<dim3((unsigned)(a.rows < 512 ? a.rows : 512)), kLong, 0, ctx->stream>>>(a);
