@@ -148,8 +148,16 @@ struct Mx4Plan {
     bool a, sa, b, sb;
 };
 Mx4Plan mx4_plan(const Mx4Args& a);
-int launch_mx4_realign(vdttfs_ctx* ctx, const uint8_t* q, int64_t ldq, const uint8_t* s, int64_t lds, int64_t rows,
-                       int K, uint8_t* to_q, int64_t ldq_to, uint8_t* to_s, int64_t lds_to);
+struct Mx4Copies {
+    struct {
+        const uint8_t* q;
+        int64_t ldq;
+        const uint8_t* s;
+        int64_t lds, rows;
+        uint8_t *to_q, *to_s;  // NULL: stays
+    } of[2];
+};
+int launch_mx4_realign(vdttfs_ctx* ctx, const Mx4Copies& c, int K, int64_t ldq_to, int64_t lds_to);
 int launch_mx4(vdttfs_ctx* ctx, const Mx4Args& a, Mx4Path path);
 // The product of few rows, quantised in the kernel (a.A and a.sa unused).
 bool mx4_small_linear_ok(int64_t M, int K);

@@ -45,20 +45,15 @@ size_t mx4_copy_bytes(const Mx4Args& a, const Mx4Plan& p) {
 // The product, its operands copied first where the plan says so.
 int mx4_product(vdttfs_ctx* ctx, Mx4Args a, const Mx4Plan& p, unsigned char* buf) {
     const int64_t ld = mx4_ld(a.K), lds = mx4_lds(a.K);
-    auto copy = [&](bool codes, bool scales, const uint8_t*& q, int64_t& ldq, const uint8_t*& s, int64_t& ls,
-                    int64_t rows) -> int {
-        if (!codes && !scales) return VDTTFS_OK;
-        uint8_t* to_q = codes ? buf : nullptr;
-        if (codes) buf += ((size_t)rows * ld + 255) & ~size_t(255);
-        uint8_t* to_s = scales ? buf : nullptr;
-        if (scales) buf += ((size_t)rows * lds + 255) & ~size_t(255);
-        VD_TRY(launch_mx4_realign(ctx, q, ldq, s, ls, rows, a.K, to_q, ld, to_s, lds));
-        if (codes) q = to_q, ldq = ld;
-        if (scales) s = to_s, ls = lds;
-        return VDTTFS_OK;
-    };
-    VD_TRY(copy(p.a, p.sa, a.A, a.lda, a.sa, a.ldsa, a.M));
-    VD_TRY(copy(p.b, p.sb, a.B, a.ldb, a.sb, a.ldsb, a.N));
+    Layout l;
+    Mx4Copies c{};
+    c.of[0] = {a.A, a.lda, a.sa, a.ldsa, a.M, nullptr, nullptr};
+    c.of[1] = {a.B, a.ldb, a.sb, a.ldsb, a.N, nullptr, nullptr};
+    if (p.a) a.A = c.of[0].to_q = buf + l.take((size_t)a.M * ld), a.lda = ld;
+    if (p.sa) a.sa = c.of[0].to_s = buf + l.take((size_t)a.M * lds), a.ldsa = lds;
+    if (p.b) a.B = c.of[1].to_q = buf + l.take((size_t)a.N * ld), a.ldb = ld;
+    if (p.sb) a.sb = c.of[1].to_s = buf + l.take((size_t)a.N * lds), a.ldsb = lds;
+    VD_TRY(launch_mx4_realign(ctx, c, a.K, ld, lds));
     return launch_mx4(ctx, a, p.path);
 }
 

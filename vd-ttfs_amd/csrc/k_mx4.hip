@@ -6,6 +6,7 @@
 // lane, so the scales cost no instruction of their own.  Products of two elements
 // are multiples of a quarter up to 36, so a block's sum is exact; the sum over
 // blocks is in 32-bit floats.
+#include <algorithm>
 #include <type_traits>
 
 #include "codes.h"
@@ -669,7 +670,7 @@ __device__ __forceinline__ void realign(const uint8_t* __restrict__ from, int64_
                                         uint8_t* __restrict__ to, int64_t ld_to) {
     const int64_t per = ld_to / 16, n = rows * per;
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (int64_t)gridDim.x * 256) {
-        const int64_t r = at / per;
+        const int64_t r = n < (int64_t(1) << 32) ? (uint32_t)at / (uint32_t)per : at / per;
         const int k = (int)(at - r * per) * 16;
         v4i v;
         if constexpr (CODES) {
@@ -681,12 +682,10 @@ __device__ __forceinline__ void realign(const uint8_t* __restrict__ from, int64_
         *reinterpret_cast<v4i*>(to + r * ld_to + k) = v;
     }
 }
-__global__ __launch_bounds__(256) void k_mx4_realign(const uint8_t* __restrict__ q, int64_t ldq,
-                                                     const uint8_t* __restrict__ s, int64_t lds, int64_t rows, int K,
-                                                     uint8_t* __restrict__ to_q, int64_t ldq_to,
-                                                     uint8_t* __restrict__ to_s, int64_t lds_to) {
-    if (to_q) realign<true>(q, ldq, rows, K, to_q, ldq_to);
-    if (to_s) realign<false>(s, lds, rows, K / kMxBlock + (K % kMxBlock != 0), to_s, lds_to);
+__global__ __launch_bounds__(256) void k_mx4_realign(Mx4Copies c, int K, int64_t ldq_to, int64_t lds_to) {
+    const auto& o = c.of[blockIdx.y];
+    if (o.to_q) realign<true>(o.q, o.ldq, o.rows, K, o.to_q, ldq_to);
+    if (o.to_s) realign<false>(o.s, o.lds, o.rows, K / kMxBlock + (K % kMxBlock != 0), o.to_s, lds_to);
 }
 
 template <int ELEM>
@@ -776,11 +775,14 @@ Mx4Plan mx4_plan(const Mx4Args& a) {
     return p;
 }
 
-int launch_mx4_realign(vdttfs_ctx* ctx, const uint8_t* q, int64_t ldq, const uint8_t* s, int64_t lds, int64_t rows,
-                       int K, uint8_t* to_q, int64_t ldq_to, uint8_t* to_s, int64_t lds_to) {
-    const int64_t n = rows * (to_q ? ldq_to : lds_to) / 16, blocks = (n + 255) / 256;
-    k_mx4_realign<<<dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), 256, 0, ctx->stream>>>(
-        q, ldq, s, lds, rows, K, to_q, ldq_to, to_s, lds_to);
+int launch_mx4_realign(vdttfs_ctx* ctx, const Mx4Copies& c, int K, int64_t ldq_to, int64_t lds_to) {
+    int64_t blocks = 0;
+    for (const auto& o : c.of) {
+        const int64_t n = o.rows * (o.to_q ? ldq_to : o.to_s ? lds_to : 0) / 16;
+        blocks = std::max(blocks, (n + 255) / 256);
+    }
+    if (!blocks) return VDTTFS_OK;
+    k_mx4_realign<<<dim3((unsigned)std::min(blocks, int64_t(1) << 20), 2), 256, 0, ctx->stream>>>(c, K, ldq_to, lds_to);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
