@@ -200,6 +200,69 @@ def test_matmul_of_no_terms_is_the_bias(ctx, M, N):
     np.testing.assert_array_equal(out.get(), np.broadcast_to(b, (M, N)))
 
 
+def operand_at(ctx, rng, rows, cols, off_q, off_s):
+    """operand with rows of codes off 16 bytes by off_q and of scales off 4 by off_s, first rows too."""
+    c = rng.integers(0, 16, (rows, cols)).astype(np.uint8)
+    s = rng.integers(120, 127, (rows, blocks_of(cols))).astype(np.uint8)
+    ld, lds = -(-bytes_of(cols) // 16) * 16 + off_q, -(-blocks_of(cols) // 4) * 4 + off_s
+    at = lambda a, ld, off: View(ctx.to_device(np.concatenate([np.full(off, 255, np.uint8), strided(a, ld).ravel()])), off)  # noqa: E731
+    return at(Q.mx4_pack(c), ld, off_q), at(s, lds, off_s), ld, lds, Q.mx4_values(c, s)
+
+
+@pytest.mark.parametrize("M,N,K", [(2561, 4200, 512), (3329, 3001, 545), (1400, 1500, 3001), (4097, 200, 2050),
+                                   (70, 8200, 1025), (513, 769, 4100)])
+@pytest.mark.parametrize("off", [(0, 0, 0, 0), (3, 0, 0, 0), (0, 1, 0, 0), (0, 0, 8, 0), (0, 0, 0, 2), (0, 3, 4, 0),
+                                 (5, 0, 0, 1), (0, 1, 0, 3), (2, 1, 7, 2)])
+def test_large_matmul_at_any_alignment(ctx, M, N, K, off):
+    """off: bytes by which codes and scales of the rows, then of the channels, miss 16 and 4."""
+    rng = np.random.default_rng(M + N + K)
+    q, s, ld, lds, x = operand_at(ctx, rng, M, K, *off[:2])
+    w, ws, ldw, ldws, wv = operand_at(ctx, rng, N, K, *off[2:])
+    b = rng.standard_normal(N).astype(np.float32)
+    out = Out(ctx, M, N, N + 1, np.float32)
+    ctx.mx4_matmul(out, R.F32, N + 1, q, ld, s, lds, w, ldw, ws, ldws, ctx.to_device(b), R.NONE, M, N, K)
+    check(out.get(), R.F32, *Q.mx4_product(x, wv, b, R.NONE))
+
+
+def test_matmul_that_copies_in_a_graph(gpu_ctx_factory):
+    """Rows off 16 bytes are copied to scratch: a capture before any call is refused, and goes on."""
+    c = gpu_ctx_factory(vdttfs.TaskConsts(T=64, delta=16))
+    M, N, K = 1200, 1300, 5001
+    rng = np.random.default_rng(4)
+    n, b = bytes_of(K), blocks_of(K)
+    w, ws, ldw, ldws, _ = operand_at(c, rng, N, K, 5, 1)
+    q, s, out = c.empty((M, n), np.uint8), c.empty((M, b), np.uint8), c.empty((M, N), np.float32)
+    s.fill(127)
+    f = c.empty(32)
+    seen = []
+
+    def call():
+        c.mx4_matmul(out, R.F32, N, q, n, s, b, w, ldw, ws, ldws, None, R.NONE, M, N, K)
+
+    def refused_call():
+        with pytest.raises(vdttfs.VdttfsError) as e:
+            call()
+        seen.append(e.value.code)
+        c.mx4_quant_rows(f, R.F32, 32, 1, 32, q, n, s, b)  # the capture goes on
+
+    Captured(c, refused_call).close()
+    assert seen == [_lib.E_UNSUPPORTED]
+    call()
+    c.synchronize()
+    g = Captured(c, call)
+    for seed in range(4):
+        q.upload(np.random.default_rng(seed).integers(0, 256, (M, n)).astype(np.uint8))
+        out.fill(0xFF)
+        g.replay()
+        c.synchronize()
+        got = out.download()
+        call()
+        c.synchronize()
+        np.testing.assert_array_equal(got, out.download())
+        assert np.isfinite(got).all() and got.any()
+    g.close()
+
+
 def test_matmul_past_32_bit_offsets(ctx):
     """Rows of codes 2.4 GB apart from first to last, and rows of outputs."""
     M, N, K, ld = 8192, 96, 400, 300032

@@ -741,8 +741,8 @@ int launch_mx4_small_linear(vdttfs_ctx* ctx, const Mx4Args& a, const void* x, in
 //   2560x8192x2048 (320, so a second round a quarter full) 41.5 and 37
 //   2048x2048x2048 (256 tiles of 128) LDS 128 11, 64 28; 512x4096x4096 (128) 18, 25;
 //   256x4096x4096 (64) 14.3, 13.7; 4225x192x4864 (68) 21, 11.3, through registers 20
-//   odd: 3000x3000x3000 copied 45, through registers 83; 2048x2048x2048 21 and 25;
-//   4225x192x4864 23 and 24, one operand alone some 16; 2000x2000x512 14 and 9.7
+//   odd: 3000x3000x3000 copied 47, through registers 83; 2048x2048x2048 19 and 25;
+//   4225x192x4864 24 and 24, one operand alone some 16; 2000x2000x512 14 and 9.7
 Mx4Plan mx4_plan(const Mx4Args& a) {
     Mx4Plan p{};
     auto tiles = [&](int t) { return (a.M + t - 1) / t * ((a.N + t - 1) / t); };
