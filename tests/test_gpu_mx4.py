@@ -277,6 +277,21 @@ def test_matmul_past_32_bit_offsets(ctx):
     q.free()
 
 
+def test_matmul_of_rows_longer_than_offsets(ctx):
+    """128 rows of codes span 2^31 bytes: ones in the upper half of the rows, twos in the lower."""
+    M, K = 1408, 33554432 + 160
+    n, b = K // 2, K // 32
+    q, s, out = ctx.empty(M * n, np.uint8), ctx.empty(M * b, np.uint8), Out(ctx, M, M, M, np.float32)
+    q.fill(0x22)
+    _lib.check(_lib.lib().vdttfs_memset(ctx.handle, View(q, M // 2 * n).ptr, 0x44, M // 2 * n))
+    s.fill(127)
+    ctx.mx4_matmul(out, R.F32, M, q, n, s, b, q, n, s, b, None, R.NONE, M, M, K)
+    half = np.where(np.arange(M) < M // 2, 1.0, 2.0)
+    np.testing.assert_array_equal(out.get(), np.outer(half, half) * K)  # sums of 32s: exact
+    q.free()
+    s.free()
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 70, 333), (3, 70, 333), (16, 70, 333), (20, 70, 333), (150, 70, 333), (1, 4096, 4096),
                                    (5, 1000, 2048), (16, 300, 8192), (700, 600, 512), (33, 40, 1)])
 @pytest.mark.parametrize("x_elem", [R.F32, R.BF16, R.F16, R.TIMES])

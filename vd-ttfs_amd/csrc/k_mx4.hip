@@ -498,7 +498,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_mx4_big(Mx4Args p, int tiles
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        // at least two tiles (deep_ok)
+        // at least two tiles: from 512 elements on (mx4_plan)
         fetch_span(0);
         fetch(s0, sc[0], 0);
         wait_loads<0>();
@@ -749,7 +749,7 @@ Mx4Plan mx4_plan(const Mx4Args& a) {
     const bool many = tiles(64) >= 192;
     const Mx4Path registers = many ? kMx4Tile64 : kMx4Tile32;
     if (a.M <= kSmallRows || (a.K >= 1024 && tiles(32) <= 128)) return p.path = kMx4Few, p;
-    if (a.K < 512) return p.path = registers, p;
+    if (a.K < 512 || a.K / 2 > kMaxLd - 128) return p.path = registers, p;  // or rows too long for copies too
     const int64_t big = tiles(256), rounds = (big + 255) / 256;
     const double work = (double)a.M * a.N * a.K;
     p.path = many ? kMx4Lds64 : kMx4Lds32;
