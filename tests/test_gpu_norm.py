@@ -127,6 +127,21 @@ def test_norms_in_place_and_unaligned(ctx, K):
         np.testing.assert_array_equal(dr.arr.download()[1:].reshape(M, K), R.to_bits(h, elem))
 
 
+@pytest.mark.parametrize("M,K", [(9, 7), (40, 9), (1100, 513), (700, 1025), (900, 1541), (300, 2049), (200, 4099),
+                                 (150, 8191), (60, 8195), (20, 16385)])
+def test_row_ends_in_place(ctx, M, K):
+    """A row's last values are read with its neighbours', which the sum replaces."""
+    x, r, g = inputs(M, K, K)
+    for elem in (R.F32, R.F16):
+        xb, rb = R.to_bits(x, elem), R.to_bits(r, elem)
+        dx, dr = ctx.to_device(xb), ctx.to_device(rb)
+        out = Out(ctx, M, K, K + 1, np.float32)
+        ctx.norm_rows(out, R.F32, K + 1, dx, elem, K, dr, elem, K, dr, K, ctx.to_device(g), 1e-6, M, K)
+        h, _, _, y = Q.norm(R.from_bits(xb, elem), R.from_bits(rb, elem), g, 1e-6)
+        check(out.get(), R.F32, y, Q.NORM_U * np.abs(y) + 2.0 ** -148)
+        np.testing.assert_array_equal(dr.download(), R.to_bits(h, elem))
+
+
 @pytest.mark.parametrize("K", [40, 300, 2000, 20000])
 def test_norms_of_the_largest_and_smallest_rows(ctx, K):
     """Squares past either end of 32 bits, zeros, and rows that are not finite."""
