@@ -173,7 +173,7 @@ struct PlaceArgs {
     int top_k, E;
 };
 // Few pairs: all of it in one launch, without scratch.
-bool dispatch_few_ok(int64_t pairs);
+bool dispatch_few_ok(int64_t pairs, int top_k);
 int launch_dispatch_few(vdttfs_ctx* ctx, const PlaceArgs& a, void* z, int64_t ldz, const void* x, int elem, int64_t ldx,
                         int cols);
 size_t dispatch_place_bytes(int64_t pairs, int n_experts);

@@ -239,7 +239,7 @@ int vdttfs_dispatch(vdttfs_ctx* ctx, void* d_z, int64_t ldz, int32_t* d_place, i
         VD_TRY(check_matrix("dispatch", d_z, elem, ldz, cols));
     }
     const PlaceArgs a{d_place, d_start, d_idx, M, top_k, n_experts};
-    if (dispatch_few_ok(M * top_k)) return launch_dispatch_few(ctx, a, d_z, ldz, d_x, elem, ldx, cols);
+    if (dispatch_few_ok(M * top_k, top_k)) return launch_dispatch_few(ctx, a, d_z, ldz, d_x, elem, ldx, cols);
     unsigned char* buf = nullptr;
     const size_t bytes = dispatch_place_bytes(M * top_k, n_experts);
     if (bytes) VD_TRY(head_scratch(ctx, bytes, &buf));

@@ -26,7 +26,8 @@ __device__ __forceinline__ float time_value(float t, float tfs, int T) {
     return b < 0 ? 0.0f : (float)(T - b) / (float)T;
 }
 
-// Eight values a thread, four neighbouring threads a block of 32.
+// Eight values a thread, four neighbouring threads a block of 32.  Bound by memory: 8192
+// x 4096 BF16 17 us, 85 MB at 5.0 TB/s.
 template <int ELEM>
 __global__ __launch_bounds__(256) void k_mx4_quant(const void* __restrict__ x, int64_t ldx, int64_t rows, int cols,
                                                    uint8_t* __restrict__ q, int64_t ldq, uint8_t* __restrict__ s,
@@ -198,7 +199,9 @@ __device__ __forceinline__ void epilogue(const Mx4Args& p, const v4f (&acc)[FM][
 
 // A workgroup of WM x WN waves computes BM rows x BN channels, operands at any
 // alignment: codes pass through registers to LDS, the next tile's on their way while
-// one is multiplied; a lane loads its fragments' scales itself.
+// one is multiplied; a lane loads its fragments' scales itself.  Two barriers a step, so
+// for what is not worth a copy or has few steps: 333 x 1111 x 1003 7 us, of which a
+// launch is 4.5 (mx4_plan has what it takes beside the others).
 template <int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN * 64) void k_mx4_tile(Mx4Args p, int tiles_n) {
     constexpr int kT = WM * WN * 64;
@@ -288,6 +291,12 @@ __global__ __launch_bounds__(WM* WN * 64) void k_mx4_tile(Mx4Args p, int tiles_n
 // stages the scales go to LDS too, those of four tiles at a time, of rows on 4 bytes;
 // of more a lane loads those of its fragments, of any alignment, and holds them until
 // their tile.  The last K % 256 elements come through registers with zeros behind them.
+//
+// 8192 x 4096 x 4096 from BF16's codes 73 to 75 us (3.7 POP/s), 8192 x 8192 x 8192 260.
+// A tile of 256 x 256 takes 2 us to its first step, 1.75 a step of 256, and 6 to its
+// outputs.  A step's matrix instructions alone take 1.24 us on random codes and 1.0 on
+// zeros: the chip's power bounds them, at 1.74 GHz in place of 2.37.  Halves of the waves
+// in turn, one multiplying while the other loads: 80 and 267 us.
 template <int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_mx4_big(Mx4Args p, int tiles_m, int tiles_n) {
     constexpr int kW = WM * WN;

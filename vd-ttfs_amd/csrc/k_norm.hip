@@ -3,7 +3,8 @@
 //
 // h = x + r, u = h g, y = u / sqrt(mean(h^2) + eps).  Bound by memory: a row is
 // held in registers between the two, so x and r are read once and the sum and y
-// written once.
+// written once (16384 x 4096 BF16 with a residual 96 us, 0.54 GB at 5.6 TB/s).  Codes
+// of 8 bits cost as many instructions again: 8192 x 2048 24 us, 4.9 TB/s.
 #include "elem.h"
 #include "head.h"
 #include "mx4.h"
@@ -109,8 +110,8 @@ enum { kFloats, kCodes8, kCodes4 };
 // LANES lanes hold a row, eight values a lane and turn (NV turns).  Gains stay in
 // registers over the workgroup's rows.  Where fewer than eight are left, a lane loads
 // the row's last eight with the others' loads and moves them (7552 x 1165 to 8 bits
-// with a residual 21.0 us; loaded one by one behind the others 30.9).  The sum, which may take the residual's place,
-// is stored behind the barrier that all loads come before.
+// with a residual 21.0 us; loaded one by one behind the others 30.9).  The sum, which
+// may take the residual's place, is stored behind the barrier that all loads come before.
 template <int XE, int RE, int NV, int LANES, int THREADS>
 __global__ __launch_bounds__(THREADS, NV == 2 ? 4 : 1) void k_norm(NormArgs a) {
     static_assert(LANES <= 64 || LANES == THREADS, "a row has a part of a wave, a wave or the workgroup");
