@@ -322,7 +322,7 @@ __global__ __launch_bounds__(kRow) void k_gather_sum(void* __restrict__ out, int
     const int64_t rows = M * top_k;
     for (int64_t at = (int64_t)blockIdx.x * kRows + threadIdx.x / T; at < M; at += (int64_t)gridDim.x * kRows) {
         const int64_t m = row_of<T>(at);
-        for (unsigned run = lane * 8; run < (unsigned)cols; run += T * 8) {
+        for (unsigned run = (blockIdx.y * T + lane) * 8; run < (unsigned)cols; run += gridDim.y * T * 8) {
             const int c = from_column((int)run, cols);
             float sum[8] = {};
             for (int j0 = 0; j0 < top_k; j0 += kSlots) {
@@ -534,9 +534,14 @@ dim3 grid_rows(int64_t M, int lanes) { return dim3(grid_of((M + kRow / lanes - 1
 int launch_gather_sum(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem, int64_t ldz,
                       const int32_t* place, const float* wt, int64_t M, int top_k, int cols) {
     by_lanes(cols, [&](auto t) {
+        dim3 grid = grid_rows(M, t.value);
+        // few long rows: their columns over several workgroups (1 x 8 rows of 8192 BF16 4.2
+        // us, by one 7.5; 100 x 8 4.1 and 7.8)
+        if (t.value == kRow && M < 256)
+            grid.y = grid_of(((int64_t)cols + kRow * 8 - 1) / (kRow * 8), 512 / (unsigned)M);
         by_elem(z_elem, [&](auto ze) {
-            k_gather_sum<ze.value, t.value><<<grid_rows(M, t.value), kRow, 0, ctx->stream>>>(out, out_elem, ldo, z, ldz,
-                                                                                             place, wt, M, top_k, cols);
+            k_gather_sum<ze.value, t.value>
+                <<<grid, kRow, 0, ctx->stream>>>(out, out_elem, ldo, z, ldz, place, wt, M, top_k, cols);
         });
     });
     VD_HIP(hipGetLastError());
