@@ -527,7 +527,8 @@ int vdttfs_stepnet_create_culif(vdttfs_ctx* ctx, const vdttfs_culif_layer* layer
  * call that needs more than an earlier one made fails with
  * VDTTFS_E_UNSUPPORTED, so run it once before capturing it.  A graph of such a
  * call holds the scratch, so it runs in turn with the context's other calls;
- * routing has none, and its graphs may run beside them. */
+ * routing, norms, combine and the gradients have none, and their graphs may run
+ * beside them. */
 /* Element types.  TIMES, an input only: float spike times as the engine's maps
  * hold them, under the context's T and tfs. */
 #define VDTTFS_ELEM_F32   0
