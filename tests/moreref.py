@@ -126,7 +126,7 @@ def combine(z, place, wt):
 
 
 def combine_grad(z, place, wt, dout):
-    """(dz, dw, bound of dw): a thread adds 8 (cols / 2048 + 1) terms, 12 levels add the threads."""
+    """(dz, dw, bound of dw): a lane adds up to 8 (cols / 512 + 1) terms, 12 levels add lanes and waves."""
     M, k = place.shape
     d = dout.astype(np.float64)
     dz, dw, mag = np.zeros(z.shape), np.zeros((M, k)), np.zeros((M, k))
@@ -136,4 +136,4 @@ def combine_grad(z, place, wt, dout):
         dz[at] = d[on] if wt is None else wt[on, j].astype(np.float64)[:, None] * d[on]
         t = d[on] * z[at].astype(np.float64)
         dw[on, j], mag[on, j] = t.sum(axis=1), np.abs(t).sum(axis=1)
-    return dz, dw, (8 * (z.shape[1] / 2048 + 1) + 12) * U * 1.01 * mag + 2.0 ** -148
+    return dz, dw, (8 * (z.shape[1] / 512 + 1) + 12) * U * 1.01 * mag + 2.0 ** -148

@@ -3,6 +3,7 @@
 // A pair is (row m, slot j), number m * top_k + j; its place is its rank among
 // the pairs with an expert, by expert and then by number.  Rows move as they are;
 // sums over slots are in 32 bits, in the order of the slots.
+#include <algorithm>
 #include <type_traits>
 
 #include "elem.h"
@@ -511,14 +512,23 @@ int launch_dispatch_rows(vdttfs_ctx* ctx, const PlaceArgs& a, void* z, int64_t l
 
 namespace {
 
-// Lanes of a row: as many as have a run of eight, up to a wave; past that the
-// workgroup.
+// Lanes of a row: as many as have a run of eight, up to a wave; past that a wave where
+// rows are many and each has no more than `few` values in its slots (its barrier and its
+// sum over lanes are then most of its time), else the workgroup.  BF16, us, a wave and a
+// workgroup a row:
+//   sums       10450 x 1 x 1024 10.5 and 14.6, 16384 x 2 x 1024 17.4 and 21.9, 9039 x 4 x
+//              1792 26.7 and 25.6, 500 x 8 x 1024 5.1 and 4.7
+//   gradients  10450 x 1 x 1024 18 and 47, 16384 x 1 x 4096 67 and 95, 9039 x 4 x 1792 49
+//              and 56, 16384 x 8 x 1024 99 and 113, x 2048 251 and 233, 500 x 8 x 1024 8.3
+//              and 7.3
+constexpr int kFewOfSum = 4096, kFewOfGrad = 8192;
 template <class F>
-void by_lanes(int cols, const F& f) {
+void by_lanes(int64_t M, int top_k, int cols, int few, const F& f) {
     if (cols <= 64) f(std::integral_constant<int, 8>{});
     else if (cols <= 128) f(std::integral_constant<int, 16>{});
     else if (cols <= 256) f(std::integral_constant<int, 32>{});
-    else if (cols <= 512) f(std::integral_constant<int, 64>{});
+    else if (cols <= 512 || (M >= 2048 && (int64_t)cols * std::min(top_k, kSlots) <= few))
+        f(std::integral_constant<int, 64>{});
     else f(std::integral_constant<int, kRow>{});
 }
 template <class F>
@@ -533,7 +543,7 @@ dim3 grid_rows(int64_t M, int lanes) { return dim3(grid_of((M + kRow / lanes - 1
 
 int launch_gather_sum(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, const void* z, int z_elem, int64_t ldz,
                       const int32_t* place, const float* wt, int64_t M, int top_k, int cols) {
-    by_lanes(cols, [&](auto t) {
+    by_lanes(M, top_k, cols, kFewOfSum, [&](auto t) {
         dim3 grid = grid_rows(M, t.value);
         // few long rows: their columns over several workgroups (1 x 8 rows of 8192 BF16 4.2
         // us, by one 7.5; 100 x 8 4.1 and 7.8)
@@ -551,7 +561,7 @@ int launch_gather_sum(vdttfs_ctx* ctx, void* out, int out_elem, int64_t ldo, con
 int launch_combine_grad(vdttfs_ctx* ctx, void* dz, int64_t lddz, float* dw, const void* z, int z_elem, int64_t ldz,
                         const void* dout, int out_elem, int64_t ldo, const int32_t* place, const float* wt, int64_t M,
                         int top_k, int cols) {
-    by_lanes(cols, [&](auto t) {
+    by_lanes(M, top_k, cols, kFewOfGrad, [&](auto t) {
         by_elem(z_elem, [&](auto ze) {
             by_elem(out_elem, [&](auto oe) {
                 k_combine_grad<ze.value, oe.value, t.value><<<grid_rows(M, t.value), kRow, 0, ctx->stream>>>(
