@@ -356,6 +356,46 @@ def test_large_sort_in_a_graph(gpu_ctx_factory):
     g.close()
 
 
+@pytest.mark.parametrize("M,k,E,D", [(1, 6, 64, 1024), (100, 8, 16, 130), (1200, 3, 9, 77)])
+def test_a_training_step_in_a_graph(gpu_ctx_factory, M, k, E, D):
+    """There, back and both gradients, replayed between eager calls of the same."""
+    c = gpu_ctx_factory(vdttfs.TaskConsts(T=64, delta=16))
+    x, idx, wt, dout = (c.empty(s, t) for s, t in (((M, D), np.float32), ((M, k), np.int32), ((M, k), np.float32),
+                                                   ((M, D), np.float32)))
+    z, place, start = c.empty((M * k, D)), c.empty((M, k), np.int32), c.empty(E + 1, np.int32)
+    out, dz, dw, dx = c.empty((M, D)), c.empty((M * k, D)), c.empty((M, k)), c.empty((M, D))
+    results = (z, place, start, out, dz, dw, dx)
+
+    def call():
+        c.dispatch(z, D, place, start, x, R.F32, D, idx, M, k, E, D)
+        c.combine(out, R.F32, D, z, R.F32, D, place, wt, M, k, D)
+        c.combine_grad(dz, D, dw, z, R.F32, D, dout, R.F32, D, place, wt, M, k, D)
+        c.dispatch_grad(dx, R.F32, D, dz, D, place, M, k, D)
+
+    idx.fill(0)
+    call()
+    c.synchronize()
+    g = Captured(c, call)
+    for seed in range(4):
+        rng = np.random.default_rng(seed)
+        i = rng.integers(-1, E, (M, k)).astype(np.int32)
+        idx.upload(i)
+        for a in (x, wt, dout):
+            a.upload(rng.standard_normal(a.shape).astype(np.float32))
+        seen = []
+        for run in (g.replay, call, g.replay):
+            for r in results:
+                r.fill(0)
+            c.synchronize()
+            run()
+            c.synchronize()
+            seen.append([r.download() for r in results])
+        for a, b in zip(seen[0] + seen[2], seen[1] + seen[1]):
+            np.testing.assert_array_equal(a, b)
+        np.testing.assert_array_equal(seen[0][1], Q.places(i, E)[0])
+    g.close()
+
+
 def test_refusals(ctx):
     f, i = ctx.empty(4096, np.float32), ctx.empty(4096, np.int32)
     odd, INV, UNS = View(f, 2), _lib.E_INVALID, _lib.E_UNSUPPORTED
