@@ -55,7 +55,8 @@ SIZES = [  # M, k, E, D
     (128, 16, 16, 1000), (129, 16, 17, 1001), (4, 2, 3, 20000), (512, 4, 7, 24), (2048, 1, 2, 10), (2049, 1, 2, 10),
     (256, 4, 5, 12), (205, 5, 1024, 4), (4096, 1, 9, 2), (4097, 1, 9, 2), (1366, 3, 1024, 2), (262200, 4, 5, 2),
     (16, 64, 60, 40), (2, 64, 60, 40), (128, 8, 60, 9), (128, 8, 1024, 9), (3, 2, 4, 4099), (200, 3, 8, 2051),
-    (2050, 1, 8, 2051), (2100, 3, 8, 700), (2048, 8, 9, 1024), (2049, 8, 9, 1025)]
+    (2050, 1, 8, 2051), (2100, 3, 8, 700), (2048, 8, 9, 1024), (2049, 8, 9, 1025),
+    (16384, 1, 5, 2), (16385, 1, 1024, 2)]
 
 
 @pytest.mark.parametrize("M,k,E,D", SIZES)

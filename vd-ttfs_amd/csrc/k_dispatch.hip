@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kPairs = 2048;  // pairs of a workgroup of the sort
 constexpr int kWaves = 16;    // of such a workgroup
-constexpr int kOnePairs = 4096;  // pairs that one workgroup places by itself
+constexpr int kEachPairs = 16384;  // pairs of which every workgroup counts all
 constexpr int kSumBlocks = 512;  // workgroups that sum the counts by themselves
 
 __device__ __forceinline__ int expert_of(const PlaceArgs& a, int64_t q, int64_t pairs) {
@@ -169,20 +169,34 @@ __global__ __launch_bounds__(1024) void k_place_sum(PlaceArgs a, const int* __re
     });
 }
 
-// ... of all pairs, by one workgroup.
-__global__ __launch_bounds__(1024) void k_place_one(PlaceArgs a, int bits) {
+// ... from all pairs, which every workgroup counts by itself: no launch before it, and
+// no scratch.
+__global__ __launch_bounds__(1024) void k_place_each(PlaceArgs a, int bits) {
     extern __shared__ int at[];
+    __shared__ int before[kMaxExperts], total[kMaxExperts];
     __shared__ int lds[16];
-    place_block<kOnePairs / 1024>(a, 0, at, bits, [&] {
-        int n = 0, used;
-        if ((int)threadIdx.x < a.E)
-            for (int w = 0; w < kWaves; ++w) n += at[w * a.E + threadIdx.x];
-        const int start = block_excl_scan(n, lds, &used);
-        if (a.start) {
+    const int64_t q0 = (int64_t)blockIdx.x * kPairs;
+    place_block<kPairs / 1024>(a, q0, at, bits, [&] {
+        const int pairs = (int)(a.M * a.top_k);
+        before[threadIdx.x] = total[threadIdx.x] = 0;
+        __syncthreads();
+        for (int q = threadIdx.x; q < pairs; q += 4 * 1024) {
+            int e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = expert_of(a, q + i * 1024, pairs);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (e[i] >= 0) atomicAdd(q + i * 1024 < q0 ? &before[e[i]] : &total[e[i]], 1);
+        }
+        __syncthreads();
+        const int mine = before[threadIdx.x];
+        int used;
+        const int start = block_excl_scan(mine + total[threadIdx.x], lds, &used);
+        if (blockIdx.x == 0 && a.start) {
             if ((int)threadIdx.x < a.E) a.start[threadIdx.x] = start;
             if (threadIdx.x == 0) a.start[a.E] = used;
         }
-        return start;
+        return start + mine;
     });
 }
 
@@ -456,23 +470,24 @@ unsigned grid_of(int64_t blocks, unsigned most) { return (unsigned)(blocks < mos
 }  // namespace
 
 size_t dispatch_place_bytes(int64_t pairs, int n_experts) {
-    return pairs <= kOnePairs ? 0 : (size_t)((pairs + kPairs - 1) / kPairs) * n_experts * 4;
+    return pairs <= kEachPairs ? 0 : (size_t)((pairs + kPairs - 1) / kPairs) * n_experts * 4;
 }
 
-// By pairs (rows of 16 bytes sorted and moved, of 60 experts):
-//   to kOnePairs  one workgroup (4014: 9.3 us; counting first 10.8)
-//   beyond        count, place (8028: 11.3 us; one workgroup 14.8; with a scan 13.4),
-//                 and a scan between from kSumBlocks workgroups on, whose counts would
-//                 be read by too many (1048576 of 1024 experts 158 us, with a scan 180;
-//                 2097152 422 and 358; of 60 experts 100 and 103, 197 and 194)
+// By pairs (rows of 16 bytes sorted and moved, us, of 60 experts unless said):
+//   to kEachPairs  place at once (8028: 9.7, counting first 11.3; 16056: 10.9 and 11.7, of
+//                  4 experts 13.7 and 14.7; 32768: 14.1 and 13.3)
+//   beyond         count, place (32768: with a scan 15.4)
+//   beyond         kSumBlocks workgroups a scan between, as too many would read the counts
+//                  (1048576 of 1024 experts 158, with a scan 180; 2097152 422 and 358; of
+//                  60 experts 100 and 103, 197 and 194)
 int launch_place(vdttfs_ctx* ctx, const PlaceArgs& a, int* hist) {
     const int64_t pairs = a.M * a.top_k;
     const int blocks = (int)((pairs + kPairs - 1) / kPairs);
     const size_t lds = (size_t)kWaves * a.E * 4;
     int bits = 0;
     while ((1 << bits) < a.E) ++bits;
-    if (pairs <= kOnePairs) {
-        k_place_one<<<dim3(1), 1024, lds, ctx->stream>>>(a, bits);
+    if (pairs <= kEachPairs) {
+        k_place_each<<<dim3((unsigned)std::max(blocks, 1)), 1024, lds, ctx->stream>>>(a, bits);
         VD_HIP(hipGetLastError());
         return VDTTFS_OK;
     }
