@@ -202,8 +202,11 @@ __global__ __launch_bounds__(1024) void k_place_each(PlaceArgs a, int bits) {
 
 // A row's bytes to another; both may start anywhere that their type allows.
 // A workgroup reads a row once and writes it to its slots.  Bound by memory: 16384 x 8
-// rows of 2048 BF16 109 us, 0.6 GB at 5.5 TB/s.
+// rows of 2048 BF16 109 us, 0.6 GB at 5.5 TB/s.  Rows off 16 bytes keep to the caches,
+// where neighbours' parts of a line meet (16384 x 8 of 2047 with their places 145 us,
+// past them 161; 4412 x 6 of 2427 46 and 45).
 constexpr int kCopy = 256;
+template <bool PAST>
 __device__ __forceinline__ void copy_to_slots(void* z, int64_t ld_bytes, const void* x_row, int64_t bytes, int unit,
                                               const int* place, int n, int64_t rows) {
     const char* from = static_cast<const char*>(x_row);
@@ -212,7 +215,10 @@ __device__ __forceinline__ void copy_to_slots(void* z, int64_t ld_bytes, const v
         const v4u v = reinterpret_cast<const AnyUint4*>(from + b)->v;
         for (int j = 0; j < n; ++j) {
             const int p = place[j];
-            if (p >= 0 && p < rows) put16(static_cast<char*>(z) + p * ld_bytes + b, v);
+            if (p < 0 || p >= rows) continue;
+            char* to = static_cast<char*>(z) + p * ld_bytes + b;
+            if (PAST) put16(to, v);
+            else reinterpret_cast<AnyUint4*>(to)->v = v;
         }
     }
     for (int64_t b = whole + (int64_t)threadIdx.x * unit; b < bytes; b += kCopy * unit)
@@ -224,11 +230,12 @@ __device__ __forceinline__ void copy_to_slots(void* z, int64_t ld_bytes, const v
             else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from + b);
         }
 }
+template <bool PAST>
 __global__ __launch_bounds__(kCopy) void k_dispatch_rows(PlaceArgs a, void* __restrict__ z, int64_t ldz,
                                                          const void* __restrict__ x, int64_t ldx, int cols, int unit) {
     for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x)
-        copy_to_slots(z, ldz * unit, static_cast<const char*>(x) + m * ldx * unit, (int64_t)cols * unit, unit,
-                      a.place + m * a.top_k, a.top_k, a.M * a.top_k);
+        copy_to_slots<PAST>(z, ldz * unit, static_cast<const char*>(x) + m * ldx * unit, (int64_t)cols * unit, unit,
+                            a.place + m * a.top_k, a.top_k, a.M * a.top_k);
 }
 
 // Up to kFewPairs pairs in one launch: a workgroup per row looks through all pairs
@@ -276,8 +283,8 @@ __global__ __launch_bounds__(kCopy) void k_dispatch_few(PlaceArgs a, void* __res
         }
     }
     __syncthreads();
-    copy_to_slots(z, ldz * unit, static_cast<const char*>(x) + m * ldx * unit, (int64_t)cols * unit, unit, mine, a.top_k,
-                  pairs);
+    copy_to_slots<true>(z, ldz * unit, static_cast<const char*>(x) + m * ldx * unit, (int64_t)cols * unit, unit, mine,
+                        a.top_k, pairs);
 }
 
 // ---- sums over slots, and their gradients --------------------------------------------
@@ -519,8 +526,10 @@ int launch_dispatch_few(vdttfs_ctx* ctx, const PlaceArgs& a, void* z, int64_t ld
 int launch_dispatch_rows(vdttfs_ctx* ctx, const PlaceArgs& a, void* z, int64_t ldz, const void* x, int elem, int64_t ldx,
                          int cols) {
     if (a.M <= 0 || cols <= 0) return VDTTFS_OK;
-    k_dispatch_rows<<<dim3(grid_of(a.M, 1 << 20)), kCopy, 0, ctx->stream>>>(a, z, ldz, x, ldx, cols,
-                                                                            elem == VDTTFS_ELEM_F32 ? 4 : 2);
+    const int unit = elem == VDTTFS_ELEM_F32 ? 4 : 2;
+    const dim3 grid(grid_of(a.M, 1 << 20));
+    if (ldz * unit % 16) k_dispatch_rows<false><<<grid, kCopy, 0, ctx->stream>>>(a, z, ldz, x, ldx, cols, unit);
+    else k_dispatch_rows<true><<<grid, kCopy, 0, ctx->stream>>>(a, z, ldz, x, ldx, cols, unit);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
