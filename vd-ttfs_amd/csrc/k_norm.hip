@@ -110,7 +110,7 @@ enum { kFloats, kCodes8, kCodes4 };
 // LANES lanes hold a row, eight values a lane and turn (NV turns).  Gains stay in
 // registers over the workgroup's rows.  Where fewer than eight are left, a lane loads
 // the row's last eight with the others' loads and moves them (7552 x 1165 to 8 bits
-// with a residual 21.0 us; loaded one by one behind the others 30.9).  The sum, which
+// with a residual 17 us; loaded one by one behind the others 10 more).  The sum, which
 // may take the residual's place, is stored behind the barrier that all loads come before.
 template <int XE, int RE, int NV, int LANES, int THREADS>
 __global__ __launch_bounds__(THREADS, NV == 2 ? 4 : 1) void k_norm(NormArgs a) {
