@@ -202,6 +202,37 @@ def test_rows_do_not_depend_on_the_batch(ctx, M):
         np.testing.assert_array_equal(first, one)
 
 
+@pytest.mark.parametrize("K", [5, 100, 250, 500, 1000, 1500, 2000, 4100, 9000, 20000])
+@pytest.mark.parametrize("res_elem", [None, R.F32])
+def test_gains_that_carry_large_rows_past_the_largest_float(ctx, K, res_elem):
+    """Finite rows give finite results: h * gain leaves the range of 32 bits, y does not."""
+    rng = np.random.default_rng(K)
+    M = 11
+    v = rng.uniform(0.5, 1, (M, K)) * rng.choice([-1, 1], (M, K))
+    top = np.array([3e38, 3.4e38, 1e30, 2.0 ** 65, 1.0, 1e37, 3e38, 1e35, 1e25, 3.4e38, 1e-30])
+    x = (v * top[:, None]).astype(np.float32)
+    r = None if res_elem is None else (x * np.float32(-0.25)).astype(np.float32)
+    g = (rng.uniform(1, 2, K) * np.exp2(rng.integers(0, 28, K))).astype(np.float32)
+    for eps in (0.0, 1e-6):
+        c = Case(ctx, x, R.F32, r, res_elem or 0, g, eps)
+        h, g64 = c.h.astype(np.float64), g.astype(np.float64)
+        c.y = h * g64 * c.inv
+        assert np.isfinite(c.y).all() and (K < 100 or not np.isfinite(c.u).all())
+        c.floats(R.F32)
+        c.floats(R.BF16)
+        c.codes4()
+        # the 8-bit codes are those of u times any power of two
+        q, sc, s = Out(ctx, M, K, K, np.int8), Out(ctx, 1, M, M, np.float32), c.sums()
+        ctx.norm_quant(q, K, sc, *c.rows(s, K))
+        far = np.where(top > 1e20, 2.0 ** -64, 1.0)[:, None]
+        rq, rs = R.quant_rows((h * far).astype(np.float32) * g)
+        np.testing.assert_array_equal(q.get(), rq)
+        want = rs.astype(np.float64) / far[:, 0] * c.inv[:, 0]
+        assert (np.abs(sc.get()[0] - want) <= Q.NORM_U * want + 2.0 ** -148).all()
+        c.check_sum(s)
+
+
+
 def test_norm_then_products_in_a_graph(gpu_ctx_factory):
     """The run of them together: residual and norm, a product in 8 bits, a norm, a product in 4, captured and replayed."""
     c = gpu_ctx_factory(vdttfs.TaskConsts(T=64, delta=16))

@@ -41,7 +41,8 @@ __device__ __forceinline__ void store_codes8(int8_t* q, int64_t row, int c, int 
 }
 
 // Sums and largest magnitudes (as bits: those of a NaN are above all others, so it
-// wins) over the LANES lanes that share a row, in every one of them.  `turn` alternates between rows, so that one barrier a row does.
+// wins) over the LANES lanes that share a row, in every one of them.  `turn` alternates
+// between calls, so that one barrier a call does.
 template <int LANES>
 struct Shared {
     float sum[2][LANES > 64 ? LANES / 64 : 1];
@@ -73,9 +74,11 @@ __device__ __forceinline__ void over_row(float& sum, uint32_t& top, Shared<LANES
 
 // 1 / sqrt(mean + eps) of a row as f * r, f a power of two.  Squares of values
 // past 2^63 or below 2^-60 or so leave the range of 32 bits: such a row is summed
-// again with its largest value brought near 1 (`scaled_sum` of the factor f, the
-// sum of (h f)^2), and its root taken in 64 bits.  Zeros alone with an eps of 0
-// give 0.
+// again with its largest value brought near 1 (the sum of (h f)^2), and its root
+// taken in 64 bits.  Where that makes it smaller the gain is taken of h f too, as
+// h g may pass the largest float where y is of ordinary size; where it makes it
+// larger, u stays the 32-bit product that its 8-bit codes are defined by.  Zeros
+// alone with an eps of 0 give 0.
 constexpr float kFewest = 0x1p-100f, kMost = 0x1p120f;
 struct Root {
     float f, r;
@@ -191,13 +194,20 @@ __global__ __launch_bounds__(THREADS, NV == 2 ? 4 : 1) void k_norm(NormArgs a) {
             over_row<LANES, true>(none, most, lds, turn);
             turn ^= 1;
             const float f = factor_of(most);
+            const float before = f < 1.0f ? f : 1.0f;  // the factor taken before the gain
+            top = 0;
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) again += (h[v][i] * f) * (h[v][i] * f);
-            over_row<LANES, false>(again, most, lds, turn);
+                for (int i = 0; i < 8; ++i) {
+                    again += (h[v][i] * f) * (h[v][i] * f);
+                    u[v][i] = a.gain ? (h[v][i] * before) * g[v][i] : h[v][i] * before;
+                    top = max(top, magnitude(u[v][i]));
+                }
+            over_row<LANES, true>(again, top, lds, turn);
             turn ^= 1;
             root = far_root(again, __uint_as_float(most), f, a.cols, a.eps);
+            if (before < 1.0f) root.f = 1.0f;
         }
         if (a.kind == kCodes8) {
             // codes are those of u: a row's codes do not change with a factor of all of it
@@ -244,7 +254,9 @@ __device__ __forceinline__ void load_h(const NormArgs& a, int64_t m, int c, floa
         for (int i = 0; i < 8; ++i) h[i] += r[i];
     }
 }
-__device__ __forceinline__ void times_gain(const NormArgs& a, int c, float (&h)[8]) {
+__device__ __forceinline__ void times_gain(const NormArgs& a, int c, float f, float (&h)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] *= f;
     if (!a.gain) return;
     float g[8];
     load8<VDTTFS_ELEM_F32>(a.gain, 0, c, a.cols, g);
@@ -267,7 +279,7 @@ __global__ __launch_bounds__(kLong) void k_norm_long(NormArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) part = __builtin_fmaf(h[i], h[i], part);
             total += part;
-            times_gain(a, (int)c, h);
+            times_gain(a, (int)c, 1.0f, h);
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = max(top, magnitude(h[i]));
         }
@@ -275,6 +287,7 @@ __global__ __launch_bounds__(kLong) void k_norm_long(NormArgs a) {
         over_row<kLong, true>(sum, top, lds, turn);
         turn ^= 1;
         Root root = plain_root(sum, a.cols, a.eps);
+        float before = 1.0f;  // the factor taken before the gain
         if (!in_range(sum)) {
             float none = 0.0f, again = 0.0f;
             uint32_t most = 0;
@@ -287,17 +300,23 @@ __global__ __launch_bounds__(kLong) void k_norm_long(NormArgs a) {
             over_row<kLong, true>(none, most, lds, turn);
             turn ^= 1;
             const float f = factor_of(most);
+            before = f < 1.0f ? f : 1.0f;
             double total_f = 0.0;
+            top = 0;
             for (unsigned c = threadIdx.x * 8; c < cols; c += kLong * 8) {
                 float h[8];
                 load_h<XE, RE>(a, m, (int)c, h);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) total_f += (double)((h[i] * f) * (h[i] * f));
+                times_gain(a, (int)c, before, h);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = max(top, magnitude(h[i]));
             }
             again = (float)total_f;
-            over_row<kLong, false>(again, most, lds, turn);
+            over_row<kLong, true>(again, top, lds, turn);
             turn ^= 1;
             root = far_root(again, __uint_as_float(most), f, a.cols, a.eps);
+            if (before < 1.0f) root.f = 1.0f;
         }
         const float s8 = scale_of(__uint_as_float(top));
         const Coder coder = coder_of(s8);
@@ -308,7 +327,7 @@ __global__ __launch_bounds__(kLong) void k_norm_long(NormArgs a) {
             if constexpr (RE != kNoRes) {
                 if (a.sum && c < cols) store8(a.sum, m * a.lds, (int)c, a.cols, RE, h);
             }
-            times_gain(a, (int)c, h);
+            times_gain(a, (int)c, before, h);
             if (a.kind == kCodes8) {
                 int k[8];
                 codes8(h, coder, k);
