@@ -232,6 +232,18 @@ def test_gains_that_carry_large_rows_past_the_largest_float(ctx, K, res_elem):
         c.check_sum(s)
 
 
+@pytest.mark.parametrize("K", [40, 700, 2000, 20000])
+def test_the_largest_eps(ctx, K):
+    """mean + eps past the largest float: the root is not."""
+    x = np.random.default_rng(K).standard_normal((6, K)).astype(np.float32)
+    x *= np.array([1e18, 1e17, 1.0, 0.0, 1e-3, 3e37], np.float32)[:, None] * np.float32(0.2)
+    for eps in (np.finfo(np.float32).max, np.float32(1.7e38)):
+        c = Case(ctx, x, R.F32, None, 0, None, eps)
+        assert (c.y[0] != 0).all()
+        c.floats(R.F32)
+        c.codes8()
+
+
 
 def test_norm_then_products_in_a_graph(gpu_ctx_factory):
     """The run of them together: residual and norm, a product in 8 bits, a norm, a product in 4, captured and replayed."""

@@ -83,7 +83,10 @@ constexpr float kFewest = 0x1p-100f, kMost = 0x1p120f;
 struct Root {
     float f, r;
 };
-__device__ __forceinline__ bool in_range(float sum) { return sum >= kFewest && sum <= kMost; }
+// mean + eps too: with an eps at the largest float a mean of 2^103 passes it
+__device__ __forceinline__ bool in_range(float sum, float eps) {
+    return sum >= kFewest && sum <= kMost && eps < 0x1p127f;
+}
 __device__ __forceinline__ Root plain_root(float sum, int cols, float eps) {
     return Root{1.0f, 1.0f / sqrtf(sum / (float)cols + eps)};
 }
@@ -184,7 +187,7 @@ __global__ __launch_bounds__(THREADS, NV == 2 ? 4 : 1) void k_norm(NormArgs a) {
             }
         }
         Root root = plain_root(sum, a.cols, a.eps);
-        if (!in_range(sum)) {  // the same in all lanes of the row
+        if (!in_range(sum, a.eps)) {  // the same in all lanes of the row
             float none = 0.0f, again = 0.0f;
             uint32_t most = 0;
 #pragma unroll
@@ -288,7 +291,7 @@ __global__ __launch_bounds__(kLong) void k_norm_long(NormArgs a) {
         turn ^= 1;
         Root root = plain_root(sum, a.cols, a.eps);
         float before = 1.0f;  // the factor taken before the gain
-        if (!in_range(sum)) {
+        if (!in_range(sum, a.eps)) {
             float none = 0.0f, again = 0.0f;
             uint32_t most = 0;
             for (unsigned c = threadIdx.x * 8; c < cols; c += kLong * 8) {
