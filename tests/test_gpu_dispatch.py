@@ -75,6 +75,20 @@ def test_dispatch(ctx, M, k, E, D, elem, pad):
     np.testing.assert_array_equal(z, want)
 
 
+@pytest.mark.parametrize("E", [1, 2, 3, 4, 5, 255, 256, 257, 1021, 1022, 1023, 1024])
+def test_starts_of_few_pairs(ctx, E):
+    """The starts in one launch with the rows, four experts a thread: any number of experts, and none past them written."""
+    rng = np.random.default_rng(E)
+    for M, k in ((1, 1), (3, 5), (200, 3), (1024, 1)):
+        idx = choose(rng, M, k, E)
+        idx[0, 0] = E - 1  # the last expert has a pair
+        bits = np.zeros((M, 4), np.float32)
+        _, place, start = run_dispatch(ctx, idx, E, bits, R.F32)
+        rp, rs = Q.places(idx, E)
+        np.testing.assert_array_equal(start, rs)
+        np.testing.assert_array_equal(place, rp)
+
+
 def test_dispatch_keeps_the_order_of_one_expert(ctx):
     """All on one expert, all on none, and the same experts over and over: places are in the pairs' order."""
     for M, k, E in ((5000, 2, 40), (300, 3, 40)):

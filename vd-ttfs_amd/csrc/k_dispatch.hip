@@ -247,7 +247,7 @@ constexpr int kFewPairs = 1024, kFewWork = 8 * kFewPairs;
 __global__ __launch_bounds__(kCopy) void k_dispatch_few(PlaceArgs a, void* __restrict__ z, int64_t ldz,
                                                         const void* __restrict__ x, int64_t ldx, int cols, int unit) {
     __shared__ int e[kFewPairs];
-    __shared__ int hist[kMaxExperts];
+    __shared__ __align__(16) int hist[kMaxExperts];  // read in fours
     __shared__ int mine[64];  // top_k <= 64
     __shared__ int sums[kCopy / 64];
     const int pairs = (int)(a.M * a.top_k), wave = threadIdx.x >> 6, lane = lane_id();
