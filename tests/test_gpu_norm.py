@@ -244,6 +244,55 @@ def test_the_largest_eps(ctx, K):
         c.codes8()
 
 
+# More rows than the workgroups of one launch take at once, so each goes on to a
+# second row or group of rows: lanes of a row 16, 32, 64 (one and two runs), 192, 256
+# (one and two), 512, 1024, and rows past those.
+@pytest.mark.parametrize("M,K,first", [(32801, 90, 32768), (16391, 250, 16384), (8201, 500, 8192), (8203, 1000, 8192),
+                                       (6001, 1025, 2730), (4199, 1541, 2048), (4301, 2049, 2048), (2500, 4099, 1024),
+                                       (1101, 8195, 512), (1030, 16385, 512)])
+def test_workgroups_of_several_rows(ctx, M, K, first):
+    """Rows that are summed again between rows that are not, and the sum in the residual's place."""
+    assert M > first
+    rng = np.random.default_rng(M + K)
+    x, r, g = inputs(M, K, M + K)
+    m = np.arange(M)
+    kind = rng.integers(0, 8, M)  # most rows are ordinary
+    kind[[0, first % M, M - 1]] = 1, 0, 2
+    scale = np.select([kind == 1, kind == 2, kind == 3], [1e30, 1e-30, 0.0], 1.0).astype(np.float32)[:, None]
+    x, r = x * scale, r * scale
+    c = Case(ctx, x, R.F32, r, R.F32, g, 0.0)
+    c.codes8()
+    c.codes4()
+    want = Out(ctx, M, K, K, np.float32)
+    ctx.norm_rows(want, R.F32, K, *c.rows())
+    c.check_y(want.get(), R.F32)
+    # in place
+    out = Out(ctx, M, K, K, np.float32)
+    ctx.norm_rows(out, R.F32, K, c.dx, R.F32, K, c.dr, R.F32, K, c.dr, K, c.dg, 0.0, M, K)
+    np.testing.assert_array_equal(c.dr.download(), c.h)
+    np.testing.assert_array_equal(out.get(), want.get())
+    assert (want.get()[m[kind == 3]] == 0).all()
+
+
+@pytest.mark.parametrize("K", [600, 1000, 1024, 2050])
+def test_what_of_a_row_does_not_depend_on_the_batch(ctx, K):
+    """Sums and 8-bit codes are the same bits in any batch; floats and scales, whose sum may be taken in another
+    order (513 to 1024 columns, from 1024 rows on), keep to the same bounds."""
+    M = 1100
+    x, r, g = inputs(M, K, K)
+    seen = []
+    for n in (1, 2, 1023, 1024, M):
+        c = Case(ctx, x[:n], R.F32, r[:n], R.F32, g)
+        q, sc, s = Out(ctx, n, K, K, np.int8), Out(ctx, 1, n, n, np.float32), Out(ctx, n, K, K, np.float32)
+        ctx.norm_quant(q, K, sc, *c.rows(s, K))
+        c.check_sum(s)
+        c.floats(R.F32)
+        c.codes4()
+        seen.append((q.get(), s.get()))
+    for q, s in seen[:-1]:
+        np.testing.assert_array_equal(q, seen[-1][0][:len(q)])
+        np.testing.assert_array_equal(s, seen[-1][1][:len(s)])
+
 
 def test_norm_then_products_in_a_graph(gpu_ctx_factory):
     """The run of them together: residual and norm, a product in 8 bits, a norm, a product in 4, captured and replayed."""
