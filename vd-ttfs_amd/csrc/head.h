@@ -116,10 +116,9 @@ struct NormArgs {
 };
 int launch_norm(vdttfs_ctx* ctx, NormArgs a, int x_elem, int res_elem);
 
-// Rows to microscaled codes of 4 bits; columns [cols, cols_zero) of each row get
-// codes and scales of 0 (cols_zero: cols itself, or a multiple of 32).
+// Rows to microscaled codes of 4 bits.
 int launch_mx4_quant_rows(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int64_t rows, int cols, uint8_t* q,
-                          int64_t ldq, uint8_t* s, int64_t lds, int cols_zero);
+                          int64_t ldq, uint8_t* s, int64_t lds);
 int launch_mx4_quant_kernel(vdttfs_ctx* ctx, const float* kernel, int c_in, int c_out, uint8_t* w, int64_t ldw,
                             uint8_t* s, int64_t lds);
 // A product of microscaled rows: activations A [M], weights B [N].

@@ -120,7 +120,7 @@ int vdttfs_mx4_quant_rows(vdttfs_ctx* ctx, const void* d_x, int elem, int64_t ld
     VD_TRY(check_in("mx4_quant_rows", d_x, elem, ldx, rows, cols));
     if (rows == 0 || cols == 0) return VDTTFS_OK;
     VD_TRY(check_mx4("mx4_quant_rows", d_q, ldq, d_s, lds, cols));
-    return launch_mx4_quant_rows(ctx, d_x, elem, ldx, rows, cols, d_q, ldq, d_s, lds, cols);
+    return launch_mx4_quant_rows(ctx, d_x, elem, ldx, rows, cols, d_q, ldq, d_s, lds);
 }
 
 int vdttfs_mx4_quant_kernel(vdttfs_ctx* ctx, const float* d_kernel, int C_in, int C_out, uint8_t* d_w, int64_t ldw,
@@ -172,7 +172,7 @@ int vdttfs_mx4_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, c
     unsigned char* buf;
     VD_TRY(head_scratch(ctx, l.bytes, &buf));
     uint8_t *q = buf + at_q, *s = buf + at_s;
-    VD_TRY(launch_mx4_quant_rows(ctx, d_x, x_elem, ldx, M, K, q, a.lda, s, a.ldsa, K));
+    VD_TRY(launch_mx4_quant_rows(ctx, d_x, x_elem, ldx, M, K, q, a.lda, s, a.ldsa));
     a.A = q;
     a.sa = s;
     return mx4_product(ctx, a, p, buf + own);

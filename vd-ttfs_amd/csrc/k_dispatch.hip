@@ -372,7 +372,6 @@ __global__ __launch_bounds__(kRow) void k_gather_sum(void* __restrict__ out, int
 // Eight sums over T lanes at once: lanes exchange halves of the values they hold until
 // each has one, so ten moves do for eight sums of a wave.  Lane l has that of slot
 // slot_of(l) in the end.
-template <int T>
 __device__ __forceinline__ int slot_of(int lane) {
     return (lane >> 5 & 1) * 4 + (lane >> 4 & 1) * 2 + (lane >> 3 & 1);
 }
@@ -456,7 +455,7 @@ __global__ __launch_bounds__(kRow) void k_combine_grad(void* __restrict__ dz, in
                     if (lane == 0 && j < top_k - j0) dw[q + j] = dot[j];
                 }
             } else {
-                const int l = lane_id(), j = slot_of<T>(l);
+                const int l = lane_id(), j = slot_of(l);
                 float sum = wave_sum8(dot);
                 if constexpr (T > 64) {
                     if ((l & 7) == 0) part[turn][wave][j] = sum;

@@ -31,8 +31,8 @@ __device__ __forceinline__ float time_value(float t, float tfs, int T) {
 template <int ELEM>
 __global__ __launch_bounds__(256) void k_mx4_quant(const void* __restrict__ x, int64_t ldx, int64_t rows, int cols,
                                                    uint8_t* __restrict__ q, int64_t ldq, uint8_t* __restrict__ s,
-                                                   int64_t lds, int cols_zero, float tfs, int T) {
-    const int64_t per = ((int64_t)cols_zero + kMxBlock - 1) / kMxBlock * 4;  // runs of eight in a row
+                                                   int64_t lds, float tfs, int T) {
+    const int64_t per = ((int64_t)cols + kMxBlock - 1) / kMxBlock * 4;  // runs of eight in a row
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < rows * per; at += (int64_t)gridDim.x * 256) {
         const int64_t m = at / per;
         const int c = (int)(at - m * per) * 8;
@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void k_mx4_quant(const void* __restrict__ x, i
 #pragma unroll
         for (int i = 0; i < 8; ++i) most = max(most, magnitude(f[i]));
         const int scale = mx4_scale(quad_max(most));
-        mx4_store8(q + m * ldq, s + m * lds, c, cols_zero, mx4_codes8(f, scale), scale);
+        mx4_store8(q + m * ldq, s + m * lds, c, cols, mx4_codes8(f, scale), scale);
     }
 }
 
@@ -307,14 +307,14 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_mx4_big(Mx4Args p, int tiles
     constexpr int kCodes = (BM + BN) * kBK, kTile = kCodes;
     constexpr int kSpan = 4, kRowScales = kSpan * kBlocks, kScales = (BM + BN) * kRowScales;
     static_assert(NA * kW * 8 == BM && NB * kW * 8 == BN && BM % 32 == 0 && BN % 32 == 0, "loads divide");
-    static_assert(S >= 2 && S <= 4 && (S - 2) * NL < 64, "stages");
+    static_assert((S == 2 || S == 4) && (S - 2) * NL < 64, "stages");
     constexpr int kStage = kW * Stage<FM, FN>::kBytes;
     // an array for each stage: only then does the compiler see that reads of
     // one need not wait for loads into another
     __shared__ __align__(16) uint8_t s0[kTile > kStage ? kTile : kStage];
     __shared__ __align__(16) uint8_t s1[kTile];
     __shared__ __align__(16) uint8_t s2[S > 2 ? kTile : 16];
-    __shared__ __align__(16) uint8_t s3[S > 3 ? kTile : 16];
+    __shared__ __align__(16) uint8_t s3[S > 2 ? kTile : 16];
     __shared__ __align__(16) uint8_t spans[S > 2 ? 16 : 2 * kScales];
 
     int tile_m, tile_n;
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_mx4_big(Mx4Args p, int tiles
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
 
-    const int tiles = p.K / 256;
+    const int tiles = p.K / 256;  // at least two: from 512 elements on (mx4_plan)
     // The scales of a lane's fragments: two bytes of each row and channel.
     struct Scales {
         int a[FM], b[FN];
@@ -507,7 +507,6 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_mx4_big(Mx4Args p, int tiles
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        // at least two tiles: from 512 elements on (mx4_plan)
         fetch_span(0);
         fetch(s0, sc[0], 0);
         wait_loads<0>();
@@ -519,35 +518,28 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_mx4_big(Mx4Args p, int tiles
             run(std::integral_constant<int, 1>{}, s1, s0, t + 1);
         }
         if (t < tiles) run(std::integral_constant<int, 0>{}, s0, s1, t);
-    } else if (tiles == 1) {  // nothing to load ahead
-        fetch(s0, sc[0], 0);
-        wait_loads<0>();
-        barrier();
-        multiply(std::false_type{}, s0, sc[0], s0, sc[0], 0);
-    } else if (tiles > 1) {
-        constexpr int k3 = S > 3 ? 3 : 2;
-        uint8_t* last = S > 3 ? s3 : s2;
+    } else {
         // (in this order: else the compiler waits, in every turn of the loop, for scales
         // that it has put behind later loads here)
         fetch(s0, sc[0], 0);
         __builtin_amdgcn_sched_barrier(0);
         fetch(s1, sc[1], 1);
         __builtin_amdgcn_sched_barrier(0);
-        if (S > 3) fetch(s2, sc[2], 2);
+        fetch(s2, sc[2], 2);
         __builtin_amdgcn_sched_barrier(0);
         int t = 0;
         for (; t + S <= tiles; t += S) {
-            step(s0, sc[0], last, sc[k3], t);
+            step(s0, sc[0], s3, sc[3], t);
             step(s1, sc[1], s0, sc[0], t + 1);
             step(s2, sc[2], s1, sc[1], t + 2);
-            if (S > 3) step(s3, sc[k3], s2, sc[2], t + 3);
+            step(s3, sc[3], s2, sc[2], t + 3);
         }
         // the last tiles % S are in flight
         wait_loads<0>();
         barrier();
         if (t < tiles) multiply(std::false_type{}, s0, sc[0], s0, sc[0], 0);
         if (t + 1 < tiles) multiply(std::false_type{}, s1, sc[1], s1, sc[1], 0);
-        if (S > 3 && t + 2 < tiles) multiply(std::false_type{}, s2, sc[2], s2, sc[2], 0);
+        if (t + 2 < tiles) multiply(std::false_type{}, s2, sc[2], s2, sc[2], 0);
     }
     wait_loads<0>();  // also those past the end
     if (p.K % 256) {
@@ -825,20 +817,20 @@ int launch_mx4(vdttfs_ctx* ctx, const Mx4Args& a, Mx4Path path) {
 }
 
 int launch_mx4_quant_rows(vdttfs_ctx* ctx, const void* x, int elem, int64_t ldx, int64_t rows, int cols, uint8_t* q,
-                          int64_t ldq, uint8_t* s, int64_t lds, int cols_zero) {
-    if (rows <= 0 || cols_zero <= 0) return VDTTFS_OK;
-    const int64_t per = ((int64_t)cols_zero + kMxBlock - 1) / kMxBlock * 4, blocks = (rows * per + 255) / 256;
+                          int64_t ldq, uint8_t* s, int64_t lds) {
+    if (rows <= 0 || cols <= 0) return VDTTFS_OK;
+    const int64_t per = ((int64_t)cols + kMxBlock - 1) / kMxBlock * 4, blocks = (rows * per + 255) / 256;
     const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20));
     const float tfs = ctx->c.tfs;
     const int T = ctx->c.T;
     if (elem == VDTTFS_ELEM_F32)
-        k_mx4_quant<VDTTFS_ELEM_F32><<<grid, 256, 0, ctx->stream>>>(x, ldx, rows, cols, q, ldq, s, lds, cols_zero, tfs, T);
+        k_mx4_quant<VDTTFS_ELEM_F32><<<grid, 256, 0, ctx->stream>>>(x, ldx, rows, cols, q, ldq, s, lds, tfs, T);
     else if (elem == VDTTFS_ELEM_BF16)
-        k_mx4_quant<VDTTFS_ELEM_BF16><<<grid, 256, 0, ctx->stream>>>(x, ldx, rows, cols, q, ldq, s, lds, cols_zero, tfs, T);
+        k_mx4_quant<VDTTFS_ELEM_BF16><<<grid, 256, 0, ctx->stream>>>(x, ldx, rows, cols, q, ldq, s, lds, tfs, T);
     else if (elem == VDTTFS_ELEM_F16)
-        k_mx4_quant<VDTTFS_ELEM_F16><<<grid, 256, 0, ctx->stream>>>(x, ldx, rows, cols, q, ldq, s, lds, cols_zero, tfs, T);
+        k_mx4_quant<VDTTFS_ELEM_F16><<<grid, 256, 0, ctx->stream>>>(x, ldx, rows, cols, q, ldq, s, lds, tfs, T);
     else
-        k_mx4_quant<VDTTFS_ELEM_TIMES><<<grid, 256, 0, ctx->stream>>>(x, ldx, rows, cols, q, ldq, s, lds, cols_zero, tfs, T);
+        k_mx4_quant<VDTTFS_ELEM_TIMES><<<grid, 256, 0, ctx->stream>>>(x, ldx, rows, cols, q, ldq, s, lds, tfs, T);
     VD_HIP(hipGetLastError());
     return VDTTFS_OK;
 }
