@@ -200,6 +200,48 @@ def test_matmul_of_no_terms_is_the_bias(ctx, M, N):
     np.testing.assert_array_equal(out.get(), np.broadcast_to(b, (M, N)))
 
 
+@pytest.mark.parametrize("M,N,K", [(3, 70, 700), (40, 70, 160), (300, 333, 500), (200, 300, 1024), (900, 1100, 1280),
+                                   (1500, 1300, 1024)])
+def test_matmul_of_scales_at_both_ends(ctx, M, N, K):
+    """Scales from 2^-127 to 2^127 whose products are near 1: sums of them are exact; elements of 0 under the largest."""
+    rng = np.random.default_rng(M + K)
+    b = blocks_of(K)
+    c, w = rng.integers(0, 16, (M, K)).astype(np.uint8), rng.integers(0, 16, (N, K)).astype(np.uint8)
+    a = rng.integers(0, 255, b)
+    a[:3] = 0, 254, 127
+    s = np.tile(a.astype(np.uint8), (M, 1))
+    ws = np.clip(254 - a + rng.integers(-2, 3, (N, b)), 0, 254).astype(np.uint8)
+    s[:, 3], ws[:, 3] = 254, 254
+    c[:, 96:128] &= 8  # zeros of both signs
+    n = bytes_of(K)
+    out = Out(ctx, M, N, N, np.float32)
+    dev = [ctx.to_device(v) for v in (Q.mx4_pack(c), s, Q.mx4_pack(w), ws)]
+    ctx.mx4_matmul(out, R.F32, N, dev[0], n, dev[1], b, dev[2], n, dev[3], b, None, R.NONE, M, N, K)
+    # multiples of 2^-4 below 2^18: exact in every order
+    np.testing.assert_array_equal(out.get(), Q.mx4_values(c, s) @ Q.mx4_values(w, ws).T)
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 70, 64), (40, 70, 64), (300, 333, 500), (200, 300, 512)])
+def test_matmul_of_sums_below_the_normal_range(ctx, M, N, K):
+    rng = np.random.default_rng(M)
+    b, n = blocks_of(K), bytes_of(K)
+    c, w = rng.integers(0, 16, (M, K)).astype(np.uint8), rng.integers(0, 16, (N, K)).astype(np.uint8)
+    s, ws = np.full((M, b), 60, np.uint8), np.full((N, b), 127 - 60 - 10, np.uint8)  # products of 2^-137
+    out = Out(ctx, M, N, N, np.float32)
+    dev = [ctx.to_device(v) for v in (Q.mx4_pack(c), s, Q.mx4_pack(w), ws)]
+    ctx.mx4_matmul(out, R.F32, N, dev[0], n, dev[1], b, dev[2], n, dev[3], b, None, R.NONE, M, N, K)
+    np.testing.assert_array_equal(out.get(), Q.mx4_values(c, s) @ Q.mx4_values(w, ws).T)
+
+
+@pytest.mark.parametrize("M", [1, 20, 300])
+def test_linear_of_no_terms_is_the_bias(ctx, M):
+    N = 50
+    b = np.random.default_rng(1).standard_normal(N).astype(np.float32)
+    out = Out(ctx, M, N, N, np.float32)
+    ctx.mx4_linear(out, R.F32, N, Null, R.F32, 0, Null, 0, Null, 0, ctx.to_device(b), R.NONE, M, N, 0)
+    np.testing.assert_array_equal(out.get(), np.broadcast_to(b, (M, N)))
+
+
 def operand_at(ctx, rng, rows, cols, off_q, off_s):
     """operand with rows of codes off 16 bytes by off_q and of scales off 4 by off_s, first rows too."""
     c = rng.integers(0, 16, (rows, cols)).astype(np.uint8)
