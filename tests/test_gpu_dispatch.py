@@ -261,6 +261,35 @@ def test_not_finite_values_pass_where_they_belong(ctx):
     assert np.isnan(got[7, 3]) and np.isinf(got[9]).all() and (~np.isfinite(got)).sum() == N + 1
 
 
+@pytest.mark.parametrize("elem", [R.F32, R.BF16])
+@pytest.mark.parametrize("N", [300, 1000, 1100])
+def test_what_of_a_row_does_not_depend_on_the_batch(ctx, N, elem):
+    """Sums over slots and dz are the same bits in any batch; the weights' gradients, summed over columns by a wave from
+    2048 rows on and by a workgroup below, keep to the same bound."""
+    rng = np.random.default_rng(N)
+    M, k, few = 2300, 3, 7
+    place = np.concatenate([rng.permutation(few * k), few * k + rng.permutation((M - few) * k)]).astype(np.int32)
+    place = place.reshape(M, k)  # the first rows' pairs are the first rows of z in every batch
+    (bits, z), (dbits, d) = values(rng, M * k, N, elem), values(rng, M, N, elem)
+    wt = rng.standard_normal((M, k)).astype(np.float32)
+    dev = [ctx.to_device(a) for a in (bits, dbits, wt)]
+    seen = []
+    for n in (few, 2047, 2048, M):
+        p = place[:n].copy()
+        p[few:] = np.where(p[few:] < n * k, p[few:], -1)
+        dp = ctx.to_device(p)
+        outs = [Out(ctx, n, N, N, R.np_type(elem)), Out(ctx, n, N, N, R.np_type(elem)),
+                Out(ctx, n * k, N, N, R.np_type(elem)), Out(ctx, n, k, k, np.float32)]
+        ctx.combine(outs[0], elem, N, dev[0], elem, N, dp, dev[2], n, k, N)
+        ctx.dispatch_grad(outs[1], elem, N, dev[0], N, dp, n, k, N)
+        ctx.combine_grad(outs[2], N, outs[3], dev[0], elem, N, dev[1], elem, N, dp, dev[2], n, k, N)
+        check(outs[3].get(), R.F32, *Q.combine_grad(z[:n * k], p, wt[:n], d[:n])[1:])
+        seen.append([outs[0].get()[:few], outs[1].get()[:few], outs[2].get()[:few * k]])
+    for other in seen[:-1]:
+        for a, b in zip(other, seen[-1]):
+            np.testing.assert_array_equal(a, b)
+
+
 def test_route_dispatch_products_combine(gpu_ctx_factory):
     """The run of them together: route, rows by expert, a 4-bit product for each expert, and back; then replayed from a
     graph, where the products take all the rows (their starts are the device's)."""
