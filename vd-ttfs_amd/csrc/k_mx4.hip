@@ -200,7 +200,7 @@ __device__ __forceinline__ void epilogue(const Mx4Args& p, const v4f (&acc)[FM][
 // A workgroup of WM x WN waves computes BM rows x BN channels, operands at any
 // alignment: codes pass through registers to LDS, the next tile's on their way while
 // one is multiplied; a lane loads its fragments' scales itself.  Two barriers a step, so
-// for what is not worth a copy or has few steps: 333 x 1111 x 1003 7 us, of which a
+// for what is not worth a copy or has few steps: 333 x 1111 x 1003 6.4 us, of which a
 // launch is 4.5 (mx4_plan has what it takes beside the others).
 template <int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN * 64) void k_mx4_tile(Mx4Args p, int tiles_n) {
@@ -292,11 +292,12 @@ __global__ __launch_bounds__(WM* WN * 64) void k_mx4_tile(Mx4Args p, int tiles_n
 // of more a lane loads those of its fragments, of any alignment, and holds them until
 // their tile.  The last K % 256 elements come through registers with zeros behind them.
 //
-// 8192 x 4096 x 4096 from BF16's codes 73 to 75 us (3.7 POP/s), 8192 x 8192 x 8192 260.
-// A tile of 256 x 256 takes 2 us to its first step, 1.75 a step of 256, and 6 to its
-// outputs.  A step's matrix instructions alone take 1.24 us on random codes and 1.0 on
-// zeros: the chip's power bounds them, at 1.74 GHz in place of 2.37.  Halves of the waves
-// in turn, one multiplying while the other loads: 80 and 267 us.
+// 8192 x 4096 x 4096 from BF16's codes 71 to 77 us by the card (3.6 to 3.9 POP/s), 8192 x
+// 8192 x 8192 249 to 262.  A tile of 256 x 256 takes 2 us to its first step, 1.75 a step
+// of 256, and 6 to its outputs.  A step's matrix instructions alone take 1.24 us on random
+// codes and 1.0 on zeros, as their power takes the clock from 2.37 GHz to 1.74; a step's
+// 192 KB of reads and 64 KB of writes of LDS take it as many cycles, not all beside them.
+// Halves of the waves in turn, one multiplying while the other loads: 80 and 267 us.
 template <int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_mx4_big(Mx4Args p, int tiles_m, int tiles_n) {
     constexpr int kW = WM * WN;

@@ -4,7 +4,7 @@
 // h = x + r, u = h g, y = u / sqrt(mean(h^2) + eps).  Bound by memory: a row is
 // held in registers between the two, so x and r are read once and the sum and y
 // written once (16384 x 4096 BF16 with a residual 96 us, 0.54 GB at 5.6 TB/s).  Codes
-// of 8 bits cost as many instructions again: 8192 x 2048 24 us, 4.9 TB/s.
+// of 8 bits cost as many instructions again: 8192 x 2048 24 to 25 us, 4.8 TB/s.
 #include "elem.h"
 #include "head.h"
 #include "mx4.h"
@@ -245,7 +245,9 @@ __global__ __launch_bounds__(THREADS, NV == 2 ? 4 : 1) void k_norm(NormArgs a) {
 }
 
 // Rows past what a workgroup holds: a workgroup each, which reads its row twice
-// (the second time from the caches).  The sum is written in the second reading, as
+// (the second time from the caches), and four times where its squares leave the range.
+// F32 with a residual, its sum and floats out: 1 and 64 rows of 20000 8.8 and 9.9 us, of
+// 65536 22 and 32, where the bytes of 64 take 12.  The sum is written in the second reading, as
 // it may take the residual's place; a thread has the same columns in both.
 template <int XE, int RE>
 __device__ __forceinline__ void load_h(const NormArgs& a, int64_t m, int c, float (&h)[8]) {

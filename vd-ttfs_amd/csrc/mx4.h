@@ -44,7 +44,7 @@ typedef v4u v4u_any __attribute__((aligned(1)));
 // 16 bytes to any address, past the caches: what is written here is read by another
 // launch, and large outputs push out what this one still reads (16384 x 4096 normed
 // 99.5 us with ordinary stores, 96.3 so; 16384 x 8 rows of 2048 to their experts and
-// back 240 and 218).
+// back 240 and 218; each call by itself, not a chain whose rows the caches would hold).
 __device__ __forceinline__ void put16(void* p, v4u v) { __builtin_nontemporal_store(v, static_cast<v4u_any*>(p)); }
 // Eight neighbouring values to a row of a float type; all there.
 __device__ __forceinline__ void put8(void* p, int64_t at, int elem, const float (&f)[8]) {
