@@ -616,9 +616,9 @@ int vdttfs_mx4_linear(vdttfs_ctx* ctx, void* d_out, int out_elem, int64_t ldo, c
  * place.  The mean is of h before that rounding.  x, res: F32, BF16 or F16, each of
  * its own type.  eps >= 0; a row of zeros gives zeros, with an eps of 0 too.  Rows
  * of any finite values: a row whose squares leave the range of 32 bits is scaled by
- * a power of two, a large one before its gain, so its u may pass the largest float
- * where its y does not.  (Other rows, of values up to 2^60, take gains up to 2^67.)
- * cols >= 1.
+ * a power of two, before its gain if its u would pass the largest float, so that y
+ * and the codes come out where they are finite.  (Other rows, of values up to 2^60,
+ * take gains up to 2^67.)  cols >= 1.
  *   norm_rows:  y rounded to y_elem
  *   norm_quant: 8-bit codes of a row and their scale, for i8_matmul: the codes that
  *     quant_rows gives of the row u (a factor of all of a row does not change its

@@ -232,6 +232,19 @@ def test_gains_that_carry_large_rows_past_the_largest_float(ctx, K, res_elem):
         c.check_sum(s)
 
 
+@pytest.mark.parametrize("K", [5, 250, 1000, 2000, 4100, 20000])
+def test_small_gains_leave_large_rows_their_codes(ctx, K):
+    """h * gain of ordinary size, with gains next to the smallest normal float: u is that product, to the bit."""
+    rng = np.random.default_rng(K)
+    M = 6
+    x = (rng.standard_normal((M, K)) * np.array([1e37, 1e30, 2.0 ** 70, 1e38 / 8, 1e20, 2.0 ** 66])[:, None]).astype(np.float32)
+    g = np.ldexp(rng.uniform(1, 2, K), -125).astype(np.float32)
+    for eps in (0.0, 1e-6):
+        c = Case(ctx, x, R.F32, None, 0, g, eps)
+        c.codes8()
+        c.floats(R.F32)
+
+
 @pytest.mark.parametrize("K", [40, 700, 2000, 20000])
 def test_the_largest_eps(ctx, K):
     """mean + eps past the largest float: the root is not."""

@@ -75,10 +75,9 @@ __device__ __forceinline__ void over_row(float& sum, uint32_t& top, Shared<LANES
 // 1 / sqrt(mean + eps) of a row as f * r, f a power of two.  Squares of values
 // past 2^63 or below 2^-60 or so leave the range of 32 bits: such a row is summed
 // again with its largest value brought near 1 (the sum of (h f)^2), and its root
-// taken in 64 bits.  Where that makes it smaller the gain is taken of h f too, as
-// h g may pass the largest float where y is of ordinary size; where it makes it
-// larger, u stays the 32-bit product that its 8-bit codes are defined by.  Zeros
-// alone with an eps of 0 give 0.
+// taken in 64 bits.  Where h g passes the largest float, though y does not, the gain
+// is taken of h f; else u stays the 32-bit product that its 8-bit codes are defined
+// by.  Zeros alone with an eps of 0 give 0.
 constexpr float kFewest = 0x1p-100f, kMost = 0x1p120f;
 struct Root {
     float f, r;
@@ -101,6 +100,12 @@ __device__ __forceinline__ Root far_root(float sum, float top, float f, int cols
     // mean(h^2) + eps = (mean((h f)^2) + eps f^2) / f^2
     const double v = (double)sum / cols + (double)eps * f * f;
     return Root{f, (float)(1.0 / sqrt(v))};
+}
+
+// The factor taken before the gain: of a row of finite values, the largest `most`, of
+// whose u some, `lost` of them, are not.
+__device__ __forceinline__ float before_gain(float lost, uint32_t most, float f) {
+    return lost > 0.0f && most < 0x7f800000u ? f : 1.0f;
 }
 
 // Eight values, `by` of them further on, then zeros.
@@ -188,16 +193,19 @@ __global__ __launch_bounds__(THREADS, NV == 2 ? 4 : 1) void k_norm(NormArgs a) {
         }
         Root root = plain_root(sum, a.cols, a.eps);
         if (!in_range(sum, a.eps)) {  // the same in all lanes of the row
-            float none = 0.0f, again = 0.0f;
+            float lost = 0.0f, again = 0.0f;
             uint32_t most = 0;
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) most = max(most, magnitude(h[v][i]));
-            over_row<LANES, true>(none, most, lds, turn);
+                for (int i = 0; i < 8; ++i) {
+                    most = max(most, magnitude(h[v][i]));
+                    // of half of h, whose products with the gain need not be kept
+                    if (fabsf(a.gain ? (h[v][i] * 0.5f) * g[v][i] : h[v][i] * 0.5f) >= 0x1p127f) lost = 1.0f;
+                }
+            over_row<LANES, true>(lost, most, lds, turn);
             turn ^= 1;
-            const float f = factor_of(most);
-            const float before = f < 1.0f ? f : 1.0f;  // the factor taken before the gain
+            const float f = factor_of(most), before = before_gain(lost, most, f);
             top = 0;
 #pragma unroll
             for (int v = 0; v < NV; ++v)
@@ -210,7 +218,7 @@ __global__ __launch_bounds__(THREADS, NV == 2 ? 4 : 1) void k_norm(NormArgs a) {
             over_row<LANES, true>(again, top, lds, turn);
             turn ^= 1;
             root = far_root(again, __uint_as_float(most), f, a.cols, a.eps);
-            if (before < 1.0f) root.f = 1.0f;
+            if (before != 1.0f) root.f = 1.0f;
         }
         if (a.kind == kCodes8) {
             // codes are those of u: a row's codes do not change with a factor of all of it
@@ -294,7 +302,7 @@ __global__ __launch_bounds__(kLong) void k_norm_long(NormArgs a) {
         Root root = plain_root(sum, a.cols, a.eps);
         float before = 1.0f;  // the factor taken before the gain
         if (!in_range(sum, a.eps)) {
-            float none = 0.0f, again = 0.0f;
+            float lost = 0.0f, again = 0.0f;
             uint32_t most = 0;
             for (unsigned c = threadIdx.x * 8; c < cols; c += kLong * 8) {
                 float h[8];
@@ -302,10 +310,11 @@ __global__ __launch_bounds__(kLong) void k_norm_long(NormArgs a) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) most = max(most, magnitude(h[i]));
             }
-            over_row<kLong, true>(none, most, lds, turn);
+            if (top >= 0x7f800000u) lost = 1.0f;
+            over_row<kLong, true>(lost, most, lds, turn);
             turn ^= 1;
             const float f = factor_of(most);
-            before = f < 1.0f ? f : 1.0f;
+            before = before_gain(lost, most, f);
             double total_f = 0.0;
             top = 0;
             for (unsigned c = threadIdx.x * 8; c < cols; c += kLong * 8) {
@@ -321,7 +330,7 @@ __global__ __launch_bounds__(kLong) void k_norm_long(NormArgs a) {
             over_row<kLong, true>(again, top, lds, turn);
             turn ^= 1;
             root = far_root(again, __uint_as_float(most), f, a.cols, a.eps);
-            if (before < 1.0f) root.f = 1.0f;
+            if (before != 1.0f) root.f = 1.0f;
         }
         const float s8 = scale_of(__uint_as_float(top));
         const Coder coder = coder_of(s8);
